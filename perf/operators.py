@@ -308,7 +308,7 @@ def _run_own(s):
         return s.bounds
     if k == "select":
         ctx.select_pages(p(s.q), p(s.bounds), s.total, p(s.table), s.width, p(s.lens), p(s.selected), n, nh, nkv, HD,
-                         c["max_len"], c["top"], 1, 1, stream=stream)
+                         s.width * PAGE, c["top"], 1, 1, stream=stream)
         return s.selected
     if k == "selected":
         ctx.decode_selected(p(s.q), p(s.kp), p(s.vp), s.total, p(s.table), s.width, p(s.lens), p(s.selected), c["top"],
