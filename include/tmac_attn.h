@@ -336,6 +336,83 @@ int tmac_layer_attention_paged(tmac_context* ctx, tmac_stream stream, int kv_dty
                                const int32_t* positions, float* out, int n_seq, int n_head, int n_kv_head,
                                int head_dim, int max_len, float base);
 
+/* ---- serving on paged caches (extensions; no counterpart in the reference, whose engine holds one
+ *      sequence) ----
+ * Pools, pages, block tables and kv_dtype as above; head_dim 64, any n_kv_head, at most 16 query
+ * heads per kv head (more: TMAC_ERR_UNSUPPORTED).  Row, length and position arrays are DEVICE arrays,
+ * so a captured call replays with new ones.  n_seq = 0 does nothing.  Which workgroup sums what
+ * depends on the call's host arguments only: the same call gives the same bits.
+ *
+ * Append: a ragged batch of new rows (prompt chunks and single tokens mixed).  Rows
+ * row_starts[s] .. row_starts[s + 1] - 1 of q / k / v (row_starts [n_seq + 1], ascending) belong to
+ * sequence s, the first at position positions[s].  q and k are rotated at their positions as
+ * tmac_rope_op does (same table, same bits), q to q_out [n_rows][n_head][64], k and v to their rows
+ * of the pools in the cache's type as the layer step stores them (same bits).  q and q_out may both
+ * be null (only k, v).  Strides are floats between rows (multiples of 4), so a fused projection's
+ * [q | k | v] rows serve as they are; q_out may be q itself where q_stride is n_head * 64, otherwise
+ * it overlaps none of the inputs.  n_head only shapes q: any multiple of n_kv_head.
+ *   Rows before row_starts[0] or at or past row_starts[n_seq] (padding) are not read, and their
+ * q_out rows keep what they held.  A row whose position is outside [0, max_len) is skipped and sets
+ * bit 0 of the device error word; max_len <= 16 * max_pages.  A row whose block-table entry is outside
+ * the pool is rotated but not stored (bit 2; unlike a read, a write is never clamped onto another
+ * page).  No two rows of a call may fall on the same pool row. */
+int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q, int64_t q_stride,
+                         float* q_out, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                         void* k_pages, void* v_pages, int n_pages, const int32_t* block_table, int max_pages,
+                         const int32_t* row_starts, const int32_t* positions, int n_seq, int n_rows, int n_head,
+                         int n_kv_head, int head_dim, int max_len, float base);
+/* Page-sparse decode: bounds of the stored keys per page, the pages a query selects by them, and
+ * attention over the selected pages only.
+ *   tmac_kv_page_bounds: bounds is a pool beside the page pools, bf16 [n_pages][n_kv_head][2][64]: the
+ *     largest stored key of every dim over the page's rows, then the smallest, rounded outward (an
+ *     infinite bound to the largest finite bf16; a dim that holds a NaN gets the whole finite range).
+ *     For each sequence, the pages that hold rows first_rows[s] .. lengths[s] - 1 (null first_rows: 0)
+ *     are computed from all of their rows before lengths[s]; other pages keep their bounds.
+ *     lengths[s] - first_rows[s] <= max_new (it sizes the grid): a longer range, or a length above
+ *     16 * max_pages, is skipped and sets bit 1; an entry outside the pool is skipped and sets bit 2.
+ *     A page needs its bounds again only when a row of it was written and it may be scored: not while
+ *     tmac_select_pages takes it anyway (its `last`).
+ *   tmac_select_pages: q [n_seq][n_head][64] (rotated, as the attention gets it).  The score of a page
+ *     for kv head h is the largest over the group's query heads of sum_d max(q_d hi_d, q_d lo_d), an
+ *     upper bound of q . k over the page's keys; summed in 64 bits and rounded once to fp32.  selected
+ *     [n_seq][n_kv_head][top]: the logical pages of the sequence's first `first` and last `last` pages
+ *     and, up to `top` in all, those with the highest scores (ties: the lower page), ascending, then
+ *     -1; all pages where there are no more than top.  first + last <= top.  Bounds of the first and
+ *     last pages are not read.  A length above max_len gives an empty list (all -1) and sets bit 1; an
+ *     entry outside the pool is clamped and sets bit 2.  With a query that is not finite the list holds
+ *     valid, distinct pages, which ones is not defined.
+ *   tmac_attention_decode_selected: one query token per sequence over the rows 16 j .. 16 j + 15 below
+ *     lengths[s] of the listed pages j of its kv head (any order; a page listed twice counts twice).
+ *     -1 entries are empty; another entry outside [0, max_pages) is skipped and sets bit 2; a
+ *     block-table entry outside the pool is clamped and sets bit 2.  No row at all gives a zero output.
+ *     A list of every page gives tmac_attention_decode_paged up to rounding. */
+int tmac_kv_page_bounds(tmac_context* ctx, tmac_stream stream, int kv_dtype, const void* k_pages, int n_pages,
+                        const int32_t* block_table, int max_pages, const int32_t* first_rows, const int32_t* lengths,
+                        void* bounds, int n_seq, int n_kv_head, int head_dim, int max_new);
+int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, const void* bounds, int n_pages,
+                      const int32_t* block_table, int max_pages, const int32_t* lengths, int32_t* selected, int n_seq,
+                      int n_head, int n_kv_head, int head_dim, int max_len, int top, int first, int last);
+int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
+                                   const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
+                                   int max_pages, const int32_t* lengths, const int32_t* selected, int top, float* out,
+                                   int n_seq, int n_head, int n_kv_head, int head_dim);
+/* Decode of a batch whose sequences share long prefixes: group g = sequences group_starts[g] ..
+ * group_starts[g + 1] - 1 (group_starts [n_groups + 1], ascending) shares its first prefix_lens[g]
+ * rows, which are read, once for all of them, through the block table of the group's first sequence;
+ * a sequence's rows from there to lengths[s] - 1 are its own, through its own table.  (The entries of
+ * the other sequences' tables for pages wholly inside the prefix are not read.)  A sequence in no
+ * group has no prefix.  The result is tmac_attention_decode_paged's, up to rounding, where the tables
+ * agree on the prefix.  Length 0 gives a zero output.  prefix_lens[g] <= max_prefix and lengths[s] -
+ * prefix <= max_tail (both size the grid; each <= 16 * max_pages), and a length above 0 is at least
+ * its prefix and at most 16 * max_pages: otherwise the sequence's output is NaN and bit 1 is set.  A
+ * block-table entry outside the pool is clamped and sets bit 2.  n_groups = 0: group_starts and
+ * prefix_lens may be null. */
+int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
+                                 const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
+                                 int max_pages, const int32_t* lengths, const int32_t* group_starts,
+                                 const int32_t* prefix_lens, int n_groups, float* out, int n_seq, int n_head,
+                                 int n_kv_head, int head_dim, int max_prefix, int max_tail);
+
 /* ---- chunked causal prefill (extension; the reference feeds prompts one token at a time,
  *      tmac_gguf.cpp:1621-1658, so its oracle is attention_op per query row) ----
  * Query i of sequence s sits at position prefix_len + i and attends rows

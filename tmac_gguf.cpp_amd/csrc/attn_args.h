@@ -183,6 +183,87 @@ struct KqArgs {
     int cols;
 };
 
+// Append of a ragged batch of rows to a paged cache: row t of q / k / v belongs
+// to the last sequence s with row_starts[s] <= t and sits at position
+// positions[s] + t - row_starts[s].
+struct AppendArgs {
+    const float* q;          // rows of [n_head][64] at q_stride floats; null: no queries
+    float* q_out;            // [n_rows][n_head][64]
+    const float* k;          // rows of [n_kv_head][64] at k_stride floats
+    const float* v;
+    char* k_pages;
+    char* v_pages;
+    const int32_t* block_table;  // [n_seq][max_pages]
+    const int32_t* row_starts;   // [n_seq + 1]
+    const int32_t* positions;    // [n_seq]
+    const float2* rope_cs;       // [rows][32], at least `capacity` rows
+    int* err;
+    int64_t q_stride, k_stride, v_stride;
+    int n_pages, max_pages, n_seq, n_rows, n_head, n_kv_head;
+    int capacity;            // positions lie below it: min(max_len, 16 * max_pages)
+    int rows_per_group;      // rows per workgroup, at most kAppendRows
+};
+constexpr int kAppendRows = 16;
+
+// Per (page, kv head) bounds of the stored keys: bf16 [n_pages][n_kv_head][2][64],
+// the largest value of every dim, then the smallest, rounded outward.
+struct BoundsArgs {
+    const char* k_pages;
+    const int32_t* block_table;
+    const int32_t* first_rows;  // [n_seq] first row whose page is computed; null: 0
+    const int32_t* lengths;
+    uint16_t* bounds;
+    int* err;
+    int n_pages, max_pages, n_seq, n_kv_head;
+    int max_new;             // rows first_rows[s] .. lengths[s] - 1, at most
+    int n_grid;              // pages per sequence this launch covers
+};
+constexpr int kBoundsBytes = 2 * kHeadDim * 2;  // per (page, kv head)
+
+struct SelectArgs {
+    const float* q;          // [n_seq][n_head][64]
+    const uint16_t* bounds;
+    const int32_t* block_table;
+    const int32_t* lengths;
+    int32_t* selected;       // [n_seq][n_kv_head][top]
+    uint32_t* keys;          // workspace [n_seq][n_kv_head][key_stride]: order-preserving score bits
+    int* err;
+    int n_pages, max_pages, n_seq, n_head, n_kv_head;
+    int max_len, key_stride;
+    int top, first, last;
+    int chunks;              // score kernel: workgroups per (sequence, kv head)
+};
+constexpr int kScorePages = 128;  // score kernel: pages per workgroup
+
+// Decode attention by (sequence or group, kv head, run of pages): over the
+// pages of a list, or over shared prefixes and each sequence's own rows.
+struct PagedAttnArgs {
+    const float* q;          // [n_seq][n_head][64]
+    const char* k_pages;
+    const char* v_pages;
+    const int32_t* block_table;
+    const int32_t* lengths;
+    float* out;
+    float* ws;               // partials [n_seq][n_head][n_slots][kPartialStride]
+    int* err;
+    int n_pages, max_pages, n_seq, n_head, n_kv_head;
+    float qscale;
+    int n_slots;             // partials per (sequence, query head)
+    // list
+    const int32_t* selected; // [n_seq][n_kv_head][top]
+    int top, per_split;      // list entries; entries per workgroup
+    // shared prefixes
+    const int32_t* group_starts;  // [n_groups + 1]
+    const int32_t* prefix_lens;   // [n_groups]
+    int n_groups, max_prefix, max_tail;
+    int prefix_splits;       // slots 0 .. prefix_splits - 1: runs of the prefix
+    int prefix_blocks;       // blocks of kSharedCols (sequence, query head) columns, at most
+    int tail_splits, tail_rows;  // slots behind them: runs of tail_rows own rows
+};
+constexpr int kPagedWaves = 4;    // waves per workgroup
+constexpr int kMaxGroupHeads = 16;  // query heads per kv head, at most (MFMA columns)
+constexpr int kSharedCols = 64;   // prefix workgroup: (sequence, query head) columns
+
 struct PosArgs {
     int* pos;
     int value;

@@ -1,0 +1,879 @@
+// paged_kernels.hip -- gfx950 kernels of the serving operators on 16-row paged
+// caches: appending rotated rows, per-page key bounds, page selection, and
+// decode attention over selected pages or over shared prefixes.
+//
+// All take head_dim 64, any number of kv heads and up to kMaxGroupHeads query
+// heads per kv head at run time; a kernel is built per cache element type.
+#include <hip/hip_runtime.h>
+
+#include "attn_args.h"
+#include "attn_device.h"
+
+using namespace tmac;
+
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// ---------------------------------------------------------------------------
+// Append.  A workgroup takes rows_per_group consecutive rows.  Every thread
+// looks at its share of row_starts once: an entry at or before the first row
+// raises the sequence of that row, an entry inside raises that row's, so a
+// running maximum over the rows gives each its sequence (the last one that
+// starts at or before it; empty sequences never win).  The rows' positions and
+// pages go to LDS, then slots of 8 lanes (8 dims a lane) take the rows' heads:
+// n_head query heads (rotated to q_out), n_kv_head keys (rotated, to the
+// cache) and n_kv_head values.  Rotation and storage are the layer step's
+// (rope8, put_row), so a row's bytes do not depend on which call wrote it.
+template <typename T>
+__device__ __forceinline__ void append_body(const AppendArgs& a) {
+    __shared__ int s_seq[kAppendRows];
+    __shared__ int s_pos[kAppendRows];
+    __shared__ int64_t s_row[kAppendRows];  // pool row, -1: not stored
+    const int R = a.rows_per_group;
+    const int t0 = blockIdx.x * R, n = min(R, a.n_rows - t0);
+    const int tid = threadIdx.x;
+    if (tid < kAppendRows) s_seq[tid] = -1;
+    __syncthreads();
+    for (int i = tid; i <= a.n_seq; i += 256) {
+        const int at = a.row_starts[i];
+        if (at <= t0)
+            atomicMax(&s_seq[0], i);
+        else if (at < t0 + n)
+            atomicMax(&s_seq[at - t0], i);
+    }
+    __syncthreads();
+    if (tid < n) {
+        int s = -1;
+        for (int i = 0; i <= tid; ++i) s = max(s, s_seq[i]);
+        int pos = -1;
+        int64_t row = -1;
+        if (s >= 0 && s < a.n_seq) {  // entry n_seq: rows behind the last sequence
+            const int64_t p = (int64_t)a.positions[s] + (t0 + tid - a.row_starts[s]);
+            if (p >= 0 && p < a.capacity) {
+                pos = (int)p;
+                const int page = a.block_table[(size_t)s * a.max_pages + (pos >> kPageShift)];
+                if (page >= 0 && page < a.n_pages)
+                    row = (int64_t)page * kPageRows + (pos & (kPageRows - 1));
+                else
+                    atomicOr(a.err, 4);
+            } else {
+                atomicOr(a.err, 1);
+            }
+        }
+        s_pos[tid] = pos;
+        s_row[tid] = row;
+    }
+    __syncthreads();
+    const int c = tid & 7, slot = tid >> 3;
+    const int nh = a.q ? a.n_head : 0, kv = a.n_kv_head, per = nh + 2 * kv;
+    constexpr int HB = CacheFmt<T>::kHeadBytes, DB = CacheFmt<T>::kDimBytes;
+    for (int it = slot; it < n * per; it += 32) {
+        const int r = it / per, h = it - r * per, pos = s_pos[r];
+        if (pos < 0) continue;
+        const int64_t t = t0 + r, row = s_row[r];
+        float x[8];
+        if (h < nh) {
+            load8(x, a.q + t * a.q_stride + h * kHeadDim + 4 * c);
+            rope8(x, a.rope_cs + (size_t)pos * (kHeadDim / 2), c);
+            store8(a.q_out + (t * nh + h) * kHeadDim + 4 * c, x);
+        } else if (row >= 0) {
+            const bool key = h < nh + kv;
+            const int hk = key ? h - nh : h - nh - kv;
+            load8(x, (key ? a.k + t * a.k_stride : a.v + t * a.v_stride) + hk * kHeadDim + 4 * c);
+            if (key) rope8(x, a.rope_cs + (size_t)pos * (kHeadDim / 2), c);
+            char* p = (key ? a.k_pages : a.v_pages) + (row * kv + hk) * HB + 4 * c * DB;
+            put_row<T>(x, p, c, true);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Page bounds.  One wave per (sequence, page, kv head): a slot of 8 lanes reads
+// a row, 8 dims a lane, rows slot and slot + 8; the running max and min go
+// over the slots with three lane exchanges.
+//
+// bf16 rounded outward: the fp32 value with its low half cut is the bf16 next
+// to it toward zero, and adding one to the cut word steps away from zero.  A
+// value beyond the largest finite bf16 becomes that, a NaN makes the dim's
+// bounds the whole range: bounds are always finite.
+__device__ __forceinline__ unsigned bf16_above(float x, bool up) {
+    const unsigned u = __float_as_uint(x);
+    const bool neg = u >> 31;
+    unsigned t = (u & 0x7FFFFFFFu) >> 16;
+    if ((u & 0xFFFFu) && neg != up) t++;
+    return min(t, 0x7F7Fu) | (neg ? 0x8000u : 0u);
+}
+
+template <typename T>
+__device__ __forceinline__ void bounds_body(const BoundsArgs& a) {
+    const int lane = threadIdx.x & 63, c = lane & 7, slot = lane >> 3;
+    const int64_t item = (int64_t)blockIdx.x * kPagedWaves + (threadIdx.x >> 6);
+    const int kv = a.n_kv_head;
+    const int64_t per_seq = (int64_t)a.n_grid * kv;
+    if (item >= per_seq * a.n_seq) return;
+    const int s = (int)(item / per_seq), rest = (int)(item - s * per_seq), i = rest / kv, h = rest - i * kv;
+    const int len = a.lengths[s], first = a.first_rows ? max(a.first_rows[s], 0) : 0;
+    if (first >= len) return;
+    if (len - first > a.max_new || len > (int64_t)a.max_pages * kPageRows) {
+        if (rest == 0 && lane == 0) atomicOr(a.err, 2);
+        return;
+    }
+    const int j = (first >> kPageShift) + i;
+    const int n = min(kPageRows, len - j * kPageRows);
+    if (n <= 0) return;
+    const int page = a.block_table[(size_t)s * a.max_pages + j];
+    if (page < 0 || page >= a.n_pages) {
+        if (lane == 0) atomicOr(a.err, 4);
+        return;
+    }
+    constexpr int HB = CacheFmt<T>::kHeadBytes, DB = CacheFmt<T>::kDimBytes;
+    const char* base = a.k_pages + ((size_t)page * kPageRows * kv + h) * HB + 4 * c * DB;
+    float hi[8], lo[8];
+    unsigned bad = 0;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        hi[t] = kNegInf;
+        lo[t] = -kNegInf;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int r = slot + 8 * u;
+        float x[8];
+        load_row<T, false>(x, base + (size_t)min(r, n - 1) * kv * HB, c);  // a row beyond the last repeats it
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            hi[t] = fmaxf(hi[t], x[t]);
+            lo[t] = fminf(lo[t], x[t]);
+            bad |= (x[t] == x[t] ? 0u : 1u) << t;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        hi[t] = xor_max<8>(hi[t]);
+        lo[t] = -xor_max<8>(-lo[t]);
+    }
+    bad |= __shfl_xor(bad, 8);
+    bad |= __shfl_xor(bad, 16);
+    bad |= __shfl_xor(bad, 32);
+    if (slot < 2) {  // slot 0 writes the largest values, slot 1 the smallest
+        uint16_t b[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+            b[t] = (uint16_t)((bad >> t & 1) ? (slot ? 0xFF7Fu : 0x7F7Fu) : bf16_above(slot ? lo[t] : hi[t], slot == 0));
+        uint16_t* o = a.bounds + ((size_t)page * kv + h) * (kBoundsBytes / 2) + slot * kHeadDim + 4 * c;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            *reinterpret_cast<u32x2*>(o + 32 * t) = u32x2{(unsigned)b[4 * t] | (unsigned)b[4 * t + 1] << 16,
+                                                         (unsigned)b[4 * t + 2] | (unsigned)b[4 * t + 3] << 16};
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Page selection.  A page's score for a kv head is the largest, over the
+// group's query heads, of sum_d max(q_d hi_d, q_d lo_d): no key of the page
+// has a larger q . k.  The sum runs in 64 bits and is rounded once, so scores,
+// and with them the selection, do not depend on the order of the sum (up to
+// 2^-53).  max(q hi, q lo) is q times hi where q >= 0 and times lo elsewhere; a
+// bf16 value as a double has a low word of zero, so one bit select of the high
+// words picks the factor.
+//
+// Slot of 8 lanes = one page, 8 dims a lane; the queries' 8 dims of every head
+// stay in registers over the workgroup's kScorePages pages.
+__device__ __forceinline__ double slot_sum64(double x) {
+#pragma unroll
+    for (int m = 1; m < 8; m *= 2) x += __shfl_xor(x, m);
+    return x;
+}
+
+// fp32 -> unsigned of the same order; NaN as +infinity.
+__device__ __forceinline__ unsigned order_key(float x) {
+    const unsigned u = x == x ? __float_as_uint(x) : 0x7F800000u;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int select_pages_of(const SelectArgs& a, int s) {  // -1: a bad length
+    const int len = max(a.lengths[s], 0);
+    return len > a.max_len ? -1 : (len + kPageRows - 1) >> kPageShift;
+}
+
+template <int GT>
+__device__ __forceinline__ void score_body(const SelectArgs& a) {
+    const int lane = threadIdx.x & 63, c = lane & 7, slot = threadIdx.x >> 3;
+    const int kv = a.n_kv_head, G = a.n_head / kv;
+    const int chunk = blockIdx.x % a.chunks, sk = blockIdx.x / a.chunks, s = sk / kv, h = sk - s * kv;
+    const int n = select_pages_of(a, s);
+    const int j0 = chunk * kScorePages, j1 = min(n, j0 + kScorePages);
+    if (n <= a.top || j0 >= j1) return;  // every page is taken, or none left
+    for (int g0 = 0; g0 < G; g0 += GT) {
+        double q[GT][8];
+        unsigned up[GT][8];  // all ones where the query value is not negative
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            float x[8];
+            const float* p = a.q + ((size_t)s * a.n_head + h * G + min(g0 + g, G - 1)) * kHeadDim + 8 * c;
+            const float4 u = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
+            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+            x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                q[g][t] = (double)x[t];
+                up[g][t] = x[t] < 0.f ? 0u : ~0u;
+            }
+        }
+        for (int j = j0 + slot; j < j1; j += 32) {
+            int page = a.block_table[(size_t)s * a.max_pages + j];
+            if (page < 0 || page >= a.n_pages) {
+                if (c == 0) atomicOr(a.err, 4);
+                page = min(max(page, 0), a.n_pages - 1);
+            }
+            const uint16_t* b = a.bounds + ((size_t)page * kv + h) * (kBoundsBytes / 2) + 8 * c;
+            const u32x4 uh = *reinterpret_cast<const u32x4*>(b), ul = *reinterpret_cast<const u32x4*>(b + kHeadDim);
+            double sum[GT];
+#pragma unroll
+            for (int g = 0; g < GT; ++g) sum[g] = 0.0;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const unsigned hi = __double2hiint(__uint_as_float(t & 1 ? uh[t / 2] & 0xFFFF0000u : uh[t / 2] << 16));
+                const unsigned lo = __double2hiint(__uint_as_float(t & 1 ? ul[t / 2] & 0xFFFF0000u : ul[t / 2] << 16));
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                    const unsigned x = (hi & up[g][t]) | (lo & ~up[g][t]);
+                    sum[g] = __builtin_fma(q[g][t], __hiloint2double((int)x, 0), sum[g]);
+                }
+            }
+            unsigned best = 0;
+#pragma unroll
+            for (int g = 0; g < GT; ++g) best = max(best, order_key((float)slot_sum64(sum[g])));
+            if (c == 0) {
+                unsigned* key = a.keys + (size_t)sk * a.key_stride + j;
+                *key = g0 ? max(*key, best) : best;
+            }
+        }
+    }
+}
+
+// The top pages of one (sequence, kv head), ascending.  Digit by digit from the
+// top, a histogram of the keys that agree with the digits found so far gives
+// the digit of the top-th largest key; then one pass in page order takes the
+// keys above it and the first of those equal to it.
+constexpr int kSelectThreads = 256;
+__device__ __forceinline__ unsigned key_of(const SelectArgs& a, const unsigned* keys, int j, int n) {
+    return j < a.first || j >= n - a.last ? 0xFFFFFFFFu : keys[j];
+}
+
+__device__ __forceinline__ void select_body(const SelectArgs& a) {
+    __shared__ unsigned s_hist[256];
+    __shared__ unsigned s_prefix, s_left;
+    __shared__ int s_gt[kSelectThreads / 64], s_eq[kSelectThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int sk = blockIdx.x, s = sk / a.n_kv_head;
+    const int n = select_pages_of(a, s);
+    int32_t* out = a.selected + (size_t)sk * a.top;
+    if (n < 0 && tid == 0) atomicOr(a.err, 2);
+    if (n <= a.top) {
+        for (int i = tid; i < a.top; i += kSelectThreads) out[i] = i < n ? i : -1;
+        return;
+    }
+    const unsigned* keys = a.keys + (size_t)sk * a.key_stride;
+    unsigned prefix = 0, left = (unsigned)a.top;  // keys still to take among those that agree with prefix
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        s_hist[tid] = 0;
+        __syncthreads();
+        for (int j = tid; j < n; j += kSelectThreads) {
+            const unsigned k = key_of(a, keys, j, n);
+            if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[k >> shift & 255], 1u);
+        }
+        __syncthreads();
+        if (tid < 64) {  // lane l: digits 255 - 4 l .. 252 - 4 l, from the top
+            unsigned cnt[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += cnt[i] = s_hist[255 - 4 * lane - i];
+            unsigned incl = sum;
+#pragma unroll
+            for (int m = 1; m < 64; m *= 2) {
+                const unsigned o = __shfl_up(incl, m);
+                if (lane >= m) incl += o;
+            }
+            unsigned above = incl - sum;
+            if (above < left && incl >= left) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (above < left && above + cnt[i] >= left) {
+                        s_prefix = prefix | (unsigned)(255 - 4 * lane - i) << shift;
+                        s_left = left - above;
+                    }
+                    above += cnt[i];
+                }
+            }
+        }
+        __syncthreads();
+        prefix = s_prefix;
+        left = s_left;
+    }
+    int n_gt = 0, n_eq = 0;  // taken so far, equal keys seen so far
+    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
+        const int j = j0 + tid;
+        const unsigned k = j < n ? key_of(a, keys, j, n) : 0;
+        const bool gt = j < n && k > prefix, eq = j < n && k == prefix;
+        const uint64_t bg = __ballot(gt), be = __ballot(eq), below = (1ull << lane) - 1;
+        __syncthreads();
+        if (lane == 0) {
+            s_gt[wave] = __popcll(bg);
+            s_eq[wave] = __popcll(be);
+        }
+        __syncthreads();
+        int g = n_gt, e = n_eq;  // before this thread's page
+        for (int w = 0; w < kSelectThreads / 64; ++w) {
+            if (w < wave) g += s_gt[w], e += s_eq[w];
+            n_gt += s_gt[w], n_eq += s_eq[w];
+        }
+        g += __popcll(bg & below);
+        e += __popcll(be & below);
+        if (gt || (eq && e < (int)left)) out[g + min(e, (int)left)] = j;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Decode attention by (columns, kv head, run of pages) on fp32 MFMA
+// (v_mfma_f32_16x16x4_f32, products and sums of fp32: the cache rows are
+// widened exactly, so every cache type gets the fp32 result).  A tile is one
+// page, 16 keys x up to NC blocks of 16 columns; a column is a query head of
+// one sequence.
+//   S^T (16 keys x 16 columns) = K (keys x dims) . Q^T.   Lane (i = l % 16,
+//     g = l / 16) holds key i's dims 32 m + 8 g + e of K and column i's of Q:
+//     step (m, e) contracts the four dims 32 m + 8 g + e, g = 0..3.
+//   P^T = exp2(S^T - m), online per column with a lazy maximum.
+//   O^T (64 dims x 16 columns) += V^T . P^T.  The accumulator S^T leaves keys
+//     4 g + r, r = 0..3, in lane group g, so step r contracts the keys 4 g + r
+//     straight from the same registers; row i of block b is dim 4 i + b, so
+//     lane (i, g) reads V of key 4 g + r as the four dims 4 i + 0..3.
+// No operand passes through LDS or another lane.
+template <typename T>
+struct Tile {};
+template <>
+struct Tile<float> {
+    f32x4 k[4], v[4];
+};
+template <>
+struct Tile<__bf16> {
+    u32x4 k[2];
+    u32x2 v[4];
+};
+template <>
+struct Tile<_Float16> {
+    u32x4 k[2];
+    u32x2 v[4];
+};
+template <>
+struct Tile<q8_0_t> {
+    unsigned k[4], kd, v[4], vd[4];
+};
+
+// kp / vp: row 0 of the page's head; stride: bytes between rows.
+template <typename T>
+__device__ __forceinline__ void tile_load(Tile<T>& t, const char* kp, const char* vp, int stride, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    const char* kr = kp + i * stride;
+    constexpr int DB = CacheFmt<T>::kDimBytes;
+    if constexpr (__is_same(T, float)) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            t.k[2 * m] = *reinterpret_cast<const f32x4*>(kr + (32 * m + 8 * g) * DB);
+            t.k[2 * m + 1] = *reinterpret_cast<const f32x4*>(kr + (32 * m + 8 * g + 4) * DB);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t.v[r] = *reinterpret_cast<const f32x4*>(vp + (4 * g + r) * stride + 4 * i * DB);
+    } else if constexpr (__is_same(T, q8_0_t)) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            t.k[2 * m] = *reinterpret_cast<const unsigned*>(kr + 32 * m + 8 * g);
+            t.k[2 * m + 1] = *reinterpret_cast<const unsigned*>(kr + 32 * m + 8 * g + 4);
+        }
+        t.kd = *reinterpret_cast<const unsigned*>(kr + 64);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            t.v[r] = *reinterpret_cast<const unsigned*>(vp + (4 * g + r) * stride + 4 * i);
+            t.vd[r] = *reinterpret_cast<const unsigned*>(vp + (4 * g + r) * stride + 64);
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) t.k[m] = *reinterpret_cast<const u32x4*>(kr + (32 * m + 8 * g) * DB);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t.v[r] = *reinterpret_cast<const u32x2*>(vp + (4 * g + r) * stride + 4 * i * DB);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float half16(unsigned w, int e) {  // element e (0, 1) of a word of 16-bit values
+    if constexpr (__is_same(T, __bf16))
+        return __uint_as_float(e ? w & 0xFFFF0000u : w << 16);
+    else
+        return half_bits_to_float(e ? w >> 16 : w & 0xFFFFu);
+}
+
+// Element (m, e) of the K operand; element b of the V operand of step r.
+template <typename T>
+__device__ __forceinline__ float tile_k(const Tile<T>& t, int m, int e) {
+    if constexpr (__is_same(T, float))
+        return t.k[2 * m + e / 4][e % 4];
+    else if constexpr (__is_same(T, q8_0_t))
+        return (float)(signed char)(t.k[2 * m + e / 4] >> (8 * (e % 4))) *
+               half_bits_to_float(m ? t.kd >> 16 : t.kd & 0xFFFFu);
+    else
+        return half16<T>(t.k[m][e / 2], e % 2);
+}
+template <typename T>
+__device__ __forceinline__ float tile_v(const Tile<T>& t, int r, int b, int i) {
+    if constexpr (__is_same(T, float))
+        return t.v[r][b];
+    else if constexpr (__is_same(T, q8_0_t))
+        return (float)(signed char)(t.v[r] >> (8 * b)) * half_bits_to_float(i < 8 ? t.vd[r] & 0xFFFFu : t.vd[r] >> 16);
+    else
+        return half16<T>(t.v[r][b / 2], b % 2);
+}
+
+constexpr float kNoMax = -__FLT_MAX__;  // running maximum of a column that has met no key
+
+// One wave's state for NC blocks of 16 columns.
+template <int NC>
+struct Cols {
+    float q[NC][16];
+    f32x4 o[NC][4];  // block b, row r: dim 16 g + 4 r + b
+    float m[NC], l[NC];  // m: the column's (equal in the four lane groups); l: this lane's keys
+};
+
+// One tile: keys lo .. hi - 1 of the page take part.
+template <typename T, int NC>
+__device__ __forceinline__ void attend_tile(Cols<NC>& st, const Tile<T>& t, int lo, int hi, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    const bool full = lo <= 0 && hi >= kPageRows;
+    f32x4 s[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float kx = tile_k<T>(t, m, e);
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+                s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx, st.q[n][8 * m + e], s[n], 0, 0, 0);
+        }
+    if (!full) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool in = 4 * g + r >= lo && 4 * g + r < hi;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) s[n][r] = in ? s[n][r] : kNegInf;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const float top = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3]));
+        if (__any(top > st.m[n] + kTau || st.m[n] == kNoMax)) {
+            const float m1 = fmaxf(st.m[n], max4_rows(top));
+            const float w = fast_exp2(st.m[n] - m1);
+            st.m[n] = m1;
+            st.l[n] *= w;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) st.o[n][b] *= w;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[n][r] = fast_exp2(s[n][r] - st.m[n]);
+        st.l[n] += (s[n][0] + s[n][1]) + (s[n][2] + s[n][3]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const bool in = full || (4 * g + r >= lo && 4 * g + r < hi);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float vx = in ? tile_v<T>(t, r, b, i) : 0.f;  // a row outside may hold anything
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+                st.o[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx, s[n][r], st.o[n][b], 0, 0, 0);
+        }
+    }
+}
+
+// A run of tiles.  Entry e (0 <= e < n) is page pages(e) of the pool (checked,
+// in range) with logical page index logical(e); rows row_lo .. row_hi - 1 of
+// the sequence take part.  The workgroup's waves take the entries in turn; a
+// wave looks up 64 of its entries at a time, one a lane.
+template <typename T, int NC, typename Look>
+__device__ __forceinline__ void attend_run(Cols<NC>& st, const PagedAttnArgs& a, int h, int n, int64_t row_lo,
+                                           int64_t row_hi, int wave, int lane, Look look) {
+    constexpr int HB = CacheFmt<T>::kHeadBytes;
+    const int stride = a.n_kv_head * HB;
+    const size_t page_bytes = (size_t)kPageRows * stride;
+    const int mine = (n - wave + kPagedWaves - 1) / kPagedWaves;  // this wave's entries
+    for (int c0 = 0; c0 < mine; c0 += 64) {
+        const int cnt = min(64, mine - c0);
+        int logical = -1, page = 0;
+        if (lane < cnt) look((c0 + lane) * kPagedWaves + wave, logical, page);
+        Tile<T> t[2];
+        auto fetch = [&](Tile<T>& x, int e) {
+            const size_t at = (size_t)__builtin_amdgcn_readlane(page, e) * page_bytes + (size_t)h * HB;
+            tile_load<T>(x, a.k_pages + at, a.v_pages + at, stride, lane);
+        };
+        fetch(t[0], 0);
+        for (int e = 0; e < cnt; e += 2) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (e + u < cnt) {
+                    fetch(t[1 - u], min(e + u + 1, cnt - 1));
+                    const int j = __builtin_amdgcn_readlane(logical, e + u);
+                    const int64_t r0 = (int64_t)j * kPageRows;
+                    const int lo = (int)max((int64_t)0, min(row_lo - r0, (int64_t)kPageRows));
+                    const int hi = j < 0 ? 0 : (int)max((int64_t)0, min(row_hi - r0, (int64_t)kPageRows));
+                    if (hi > lo) attend_tile<T, NC>(st, t[u], lo, hi, lane);
+                }
+            }
+        }
+    }
+}
+
+template <int NC>
+__device__ __forceinline__ void cols_init(Cols<NC>& st) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        st.m[n] = kNoMax;
+        st.l[n] = 0.f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) st.o[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+}
+
+// Column q row pointer (null: an unused column) -> pre-scaled operand.
+__device__ __forceinline__ void load_q(float (&q)[16], const float* p, float scale, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (p) {
+            x = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g);
+            y = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g + 4);
+        }
+        float* o = q + 8 * m;
+        o[0] = x.x * scale; o[1] = x.y * scale; o[2] = x.z * scale; o[3] = x.w * scale;
+        o[4] = y.x * scale; o[5] = y.y * scale; o[6] = y.z * scale; o[7] = y.w * scale;
+    }
+}
+
+// Merges the waves of the workgroup through LDS and hands every column's (m, l,
+// acc[dim]) to `put`, which runs once per (column, dim).
+template <int NC>
+struct MergeLds {
+    float o[kPagedWaves][NC * 16][kHeadDim + 1];
+    float m[kPagedWaves][NC * 16], l[kPagedWaves][NC * 16];
+};
+template <int NC, typename Put>
+__device__ __forceinline__ void merge_waves(Cols<NC>& st, MergeLds<NC>& lds, int wave, int lane, Put put) {
+    const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const float l = sum4_rows(st.l[n]);
+        if (g == 0) {
+            lds.m[wave][16 * n + i] = st.m[n];
+            lds.l[wave][16 * n + i] = l;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds.o[wave][16 * n + i][16 * g + 4 * r + b] = st.o[n][b][r];
+    }
+    __syncthreads();
+    for (int c = wave; c < NC * 16; c += kPagedWaves) {
+        float M = lds.m[0][c];
+#pragma unroll
+        for (int w = 1; w < kPagedWaves; ++w) M = fmaxf(M, lds.m[w][c]);
+        float L = 0.f, A = 0.f;
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; ++w) {
+            const float x = fast_exp2(lds.m[w][c] - M);
+            L += x * lds.l[w][c];
+            A += x * lds.o[w][c][lane];
+        }
+        put(c, lane, M, L, A);
+    }
+}
+
+__device__ __forceinline__ float finish_row(float acc, float l) { return l == 0.f ? 0.f : acc / l; }
+
+// Stores one (column, dim) of a partial.
+__device__ __forceinline__ void put_partial(const PagedAttnArgs& a, int s, int head, int slot, int d, float M, float L,
+                                            float A) {
+    float* w = a.ws + (((size_t)s * a.n_head + head) * a.n_slots + slot) * kPartialStride;
+    w[d] = A;
+    if (d == 0) {
+        w[kHeadDim] = M;
+        w[kHeadDim + 1] = L;
+    }
+}
+
+// Over a list: workgroup (split, kv head, sequence).
+template <typename T>
+__device__ __forceinline__ void selected_body(const PagedAttnArgs& a) {
+    __shared__ MergeLds<1> lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kv = a.n_kv_head, G = a.n_head / kv;
+    const int split = blockIdx.x % a.n_slots, sk = blockIdx.x / a.n_slots, s = sk / kv, h = sk - s * kv;
+    const int len = a.lengths[s];
+    const int e0 = split * a.per_split, n = min(a.per_split, a.top - e0);
+    const int32_t* list = a.selected + (size_t)sk * a.top + e0;
+    const int32_t* table = a.block_table + (size_t)s * a.max_pages;
+    Cols<1> st;
+    cols_init(st);
+    const int col = lane & 15;
+    load_q(st.q[0], col < G ? a.q + ((size_t)s * a.n_head + h * G + col) * kHeadDim : nullptr, a.qscale, lane);
+    attend_run<T, 1>(st, a, h, n, 0, len, wave, lane, [&](int e, int& logical, int& page) {
+        const int j = list[e];
+        if (j == -1) return;
+        if (j < 0 || j >= a.max_pages) {
+            atomicOr(a.err, 4);
+            return;
+        }
+        if ((int64_t)j * kPageRows >= len) return;  // behind the last row
+        page = table[j];
+        if (page < 0 || page >= a.n_pages) {
+            atomicOr(a.err, 4);
+            page = min(max(page, 0), a.n_pages - 1);
+        }
+        logical = j;
+    });
+    merge_waves<1>(st, lds, wave, lane, [&](int c, int d, float M, float L, float A) {
+        if (c >= G) return;
+        if (a.n_slots == 1)
+            a.out[((size_t)s * a.n_head + h * G + c) * kHeadDim + d] = finish_row(A, L);
+        else
+            put_partial(a, s, h * G + c, split, d, M, L, A);
+    });
+}
+
+// Merge of `n` partials of one (sequence, query head): one wave, a dim a lane.
+__device__ __forceinline__ void merge_slots(const float* w, int n0, int skip_to, int n1, int lane, float& M, float& L,
+                                            float& A) {
+    // slots 0 .. n0 - 1 and skip_to .. skip_to + n1 - 1
+    const int n = n0 + n1;
+    M = kNoMax, L = 0.f, A = 0.f;
+    for (int c0 = 0; c0 < n; c0 += 64) {
+        const int e = c0 + lane, cnt = min(64, n - c0);
+        float m = kNoMax, l = 0.f;
+        if (e < n) {
+            const float* p = w + (size_t)(e < n0 ? e : skip_to + e - n0) * kPartialStride;
+            m = p[kHeadDim];
+            l = p[kHeadDim + 1];
+        }
+        const float m1 = fmaxf(M, xor_max<1>(m));
+        const float f = fast_exp2(M - m1);
+        const float x = fast_exp2(m - m1);
+        L = L * f + xor_sum<1>(l * x);
+        A *= f;
+        for (int i = 0; i < cnt; ++i) {
+            const int ei = c0 + i;
+            const float* p = w + (size_t)(ei < n0 ? ei : skip_to + ei - n0) * kPartialStride;
+            A += __shfl(x, i) * p[lane];
+        }
+        M = m1;
+    }
+}
+
+__device__ __forceinline__ void selected_merge_body(const PagedAttnArgs& a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * kPagedWaves + (threadIdx.x >> 6);
+    if (row >= (int64_t)a.n_seq * a.n_head) return;
+    float M, L, A;
+    merge_slots(a.ws + (size_t)row * a.n_slots * kPartialStride, a.n_slots, a.n_slots, 0, lane, M, L, A);
+    a.out[(size_t)row * kHeadDim + lane] = finish_row(A, L);
+}
+
+// Group g's sequences [first, end), clamped into the batch.
+__device__ __forceinline__ void group_range(const PagedAttnArgs& a, int g, int& first, int& end) {
+    first = min(max(a.group_starts[g], 0), a.n_seq);
+    end = min(max(a.group_starts[g + 1], first), a.n_seq);
+}
+
+// The group of a sequence: the last one that starts at or before it and ends
+// behind it; -1: none.  Wave-wide.
+__device__ __forceinline__ int group_of(const PagedAttnArgs& a, int s, int lane) {
+    int found = -1;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
+        const int g = g0 + lane;
+        bool in = false;
+        if (g < a.n_groups) {
+            int first, end;
+            group_range(a, g, first, end);
+            in = s >= first && s < end;
+        }
+        const uint64_t b = __ballot(in);
+        if (b) found = g0 + 63 - __clzll(b);
+    }
+    return found;
+}
+
+// A sequence's rows: [0, prefix) through its group's first sequence, [prefix,
+// len) through its own pages.
+struct SharedSeq {
+    int64_t prefix, len;
+    bool bad;  // a length or prefix outside what the launch covers
+};
+__device__ __forceinline__ SharedSeq shared_seq(const PagedAttnArgs& a, int s, int g) {
+    SharedSeq r;
+    r.len = max(a.lengths[s], 0);
+    r.prefix = g >= 0 ? max(a.prefix_lens[g], 0) : 0;
+    r.bad = r.len > 0 && (r.prefix > a.max_prefix || r.len < r.prefix || r.len - r.prefix > a.max_tail ||
+                          r.len > (int64_t)a.max_pages * kPageRows);
+    return r;
+}
+
+// Pages of one run of a prefix of `prefix` rows cut into prefix_splits runs.
+__device__ __forceinline__ int prefix_run_pages(const PagedAttnArgs& a, int64_t prefix) {
+    const int n = (int)((prefix + kPageRows - 1) >> kPageShift);
+    return max(1, (n + a.prefix_splits - 1) / a.prefix_splits);
+}
+
+// Shared prefixes and own rows: the first prefix_blocks * n_kv_head *
+// prefix_splits workgroups take (64 columns of a group, kv head, run of its
+// prefix), the rest (own rows of a sequence, kv head, run).
+template <typename T>
+__device__ __forceinline__ void shared_body(const PagedAttnArgs& a) {
+    constexpr int NC = kSharedCols / 16;
+    __shared__ union {
+        MergeLds<NC> p;
+        MergeLds<1> t;
+    } lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kv = a.n_kv_head, G = a.n_head / kv;
+    const int n_prefix = a.prefix_blocks * kv * a.prefix_splits;
+    const int col = lane & 15;
+    if ((int)blockIdx.x < n_prefix) {
+        const int split = blockIdx.x % a.prefix_splits, bh = blockIdx.x / a.prefix_splits, h = bh % kv, block = bh / kv;
+        // the group whose column blocks hold this one
+        int g = -1, first = 0, end = 0, left = block;
+        for (int g0 = 0; g0 < a.n_groups && g < 0; g0 += 64) {
+            int f = 0, e = 0;
+            if (g0 + lane < a.n_groups) group_range(a, g0 + lane, f, e);
+            const int nb = (int)(((int64_t)(e - f) * G + kSharedCols - 1) / kSharedCols);
+            int incl = nb;
+#pragma unroll
+            for (int m = 1; m < 64; m *= 2) {
+                const int o = __shfl_up(incl, m);
+                if (lane >= m) incl += o;
+            }
+            const uint64_t b = __ballot(incl > left);
+            if (b) {
+                const int at = __ffsll((unsigned long long)b) - 1;
+                g = g0 + at;
+                first = __shfl(f, at);
+                end = __shfl(e, at);
+                left -= __shfl(incl - nb, at);
+            } else {
+                left -= __shfl(incl, 63);
+            }
+        }
+        g = __builtin_amdgcn_readfirstlane(g);
+        first = __builtin_amdgcn_readfirstlane(first);
+        end = __builtin_amdgcn_readfirstlane(end);
+        left = __builtin_amdgcn_readfirstlane(left);
+        if (g < 0) return;
+        const int64_t prefix = max(a.prefix_lens[g], 0);
+        if (prefix == 0 || prefix > a.max_prefix || prefix > (int64_t)a.max_pages * kPageRows) return;
+        const int per = prefix_run_pages(a, prefix), j0 = split * per;
+        const int n_all = (int)((prefix + kPageRows - 1) >> kPageShift);
+        const int n = min(per, n_all - j0);
+        if (n <= 0) return;
+        Cols<NC> st;
+        cols_init(st);
+        const int rows = (end - first) * G;  // (sequence, head of the group) columns of the group
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            const int c = left * kSharedCols + 16 * t + col;
+            load_q(st.q[t],
+                   c < rows ? a.q + ((size_t)(first + c / G) * a.n_head + h * G + c % G) * kHeadDim : nullptr,
+                   a.qscale, lane);
+        }
+        const int32_t* table = a.block_table + (size_t)first * a.max_pages;
+        attend_run<T, NC>(st, a, h, n, 0, prefix, wave, lane, [&](int e, int& logical, int& page) {
+            logical = j0 + e;
+            page = table[logical];
+            if (page < 0 || page >= a.n_pages) {
+                atomicOr(a.err, 4);
+                page = min(max(page, 0), a.n_pages - 1);
+            }
+        });
+        merge_waves<NC>(st, lds.p, wave, lane, [&](int c, int d, float M, float L, float A) {
+            const int r = left * kSharedCols + c;
+            if (r < rows) put_partial(a, first + r / G, h * G + r % G, split, d, M, L, A);
+        });
+    } else {
+        const int id = blockIdx.x - n_prefix;
+        const int split = id % a.tail_splits, sk = id / a.tail_splits, s = sk / kv, h = sk - s * kv;
+        const SharedSeq q = shared_seq(a, s, group_of(a, s, lane));
+        if (q.bad) return;
+        const int64_t lo = q.prefix + (int64_t)split * a.tail_rows, hi = min(q.len, lo + a.tail_rows);
+        if (lo >= hi) return;
+        const int j0 = (int)(lo >> kPageShift), n = (int)((hi - 1) >> kPageShift) - j0 + 1;
+        Cols<1> st;
+        cols_init(st);
+        load_q(st.q[0], col < G ? a.q + ((size_t)s * a.n_head + h * G + col) * kHeadDim : nullptr, a.qscale, lane);
+        const int32_t* table = a.block_table + (size_t)s * a.max_pages;
+        attend_run<T, 1>(st, a, h, n, lo, hi, wave, lane, [&](int e, int& logical, int& page) {
+            logical = j0 + e;
+            page = table[logical];
+            if (page < 0 || page >= a.n_pages) {
+                atomicOr(a.err, 4);
+                page = min(max(page, 0), a.n_pages - 1);
+            }
+        });
+        merge_waves<1>(st, lds.t, wave, lane, [&](int c, int d, float M, float L, float A) {
+            if (c < G) put_partial(a, s, h * G + c, a.prefix_splits + split, d, M, L, A);
+        });
+    }
+}
+
+__device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * kPagedWaves + (threadIdx.x >> 6);
+    if (row >= (int64_t)a.n_seq * a.n_head) return;
+    const int s = (int)(row / a.n_head);
+    const SharedSeq q = shared_seq(a, s, group_of(a, s, lane));
+    float y = 0.f;
+    if (q.bad) {
+        if (lane == 0) atomicOr(a.err, 2);
+        y = __builtin_nanf("");
+    } else if (q.len > 0) {
+        const int64_t per = q.prefix ? (int64_t)prefix_run_pages(a, q.prefix) * kPageRows : 1;
+        const int n0 = (int)((q.prefix + per - 1) / per);
+        const int n1 = (int)((q.len - q.prefix + a.tail_rows - 1) / a.tail_rows);
+        float M, L, A;
+        merge_slots(a.ws + (size_t)row * a.n_slots * kPartialStride, n0, a.prefix_splits, n1, lane, M, L, A);
+        y = finish_row(A, L);
+    }
+    a.out[(size_t)row * kHeadDim + lane] = y;
+}
+
+}  // namespace
+
+#define TMAC_PAGED_KERNELS(NAME, T)                                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void tmac_append_##NAME(AppendArgs a) { append_body<T>(a); }          \
+    extern "C" __global__ __launch_bounds__(256) void tmac_page_bounds_##NAME(BoundsArgs a) { bounds_body<T>(a); }     \
+    extern "C" __global__ __launch_bounds__(256) void tmac_selected_##NAME(PagedAttnArgs a) { selected_body<T>(a); }   \
+    extern "C" __global__ __launch_bounds__(256) void tmac_shared_##NAME(PagedAttnArgs a) { shared_body<T>(a); }
+TMAC_PAGED_KERNELS(f32, float)
+TMAC_PAGED_KERNELS(bf16, __bf16)
+TMAC_PAGED_KERNELS(f16, _Float16)
+TMAC_PAGED_KERNELS(q8, q8_0_t)
+
+#define TMAC_SCORE_KERNEL(GT) \
+    extern "C" __global__ __launch_bounds__(256) void tmac_page_scores_g##GT(SelectArgs a) { score_body<GT>(a); }
+TMAC_SCORE_KERNEL(1)
+TMAC_SCORE_KERNEL(2)
+TMAC_SCORE_KERNEL(3)
+TMAC_SCORE_KERNEL(4)
+TMAC_SCORE_KERNEL(5)
+TMAC_SCORE_KERNEL(6)
+TMAC_SCORE_KERNEL(7)
+TMAC_SCORE_KERNEL(8)
+extern "C" __global__ __launch_bounds__(kSelectThreads) void tmac_select_pages(SelectArgs a) { select_body(a); }
+extern "C" __global__ __launch_bounds__(256) void tmac_selected_merge(PagedAttnArgs a) { selected_merge_body(a); }
+extern "C" __global__ __launch_bounds__(256) void tmac_shared_merge(PagedAttnArgs a) { shared_merge_body(a); }

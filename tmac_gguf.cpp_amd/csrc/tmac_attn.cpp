@@ -30,12 +30,14 @@
 #include "attn_args.h"
 
 // The gfx950 code objects, one per kernel part (code_object.S).
-constexpr int kCodeParts = 4;
+constexpr int kCodeParts = 5;
 extern "C" const unsigned char* const tmac_attn_code_objects[kCodeParts];
 extern "C" const uint64_t tmac_attn_code_object_sizes[kCodeParts];
 // tmac_scratch.hip: the device address of the fixed scratch array on `device` (the current device).
 extern "C" int tmac_scratch_setup(int device, void** ptr);
 
+using tmac::AppendArgs;
+using tmac::BoundsArgs;
 using tmac::CopyArgs;
 using tmac::CvtArgs;
 using tmac::DecodeArgs;
@@ -47,6 +49,8 @@ using tmac::kPrefillTileElems;
 using tmac::kPrefillWaves;
 using tmac::PosArgs;
 using tmac::KqArgs;
+using tmac::PagedAttnArgs;
+using tmac::SelectArgs;
 using tmac::QkvArgs;
 using tmac::kQkvWaves;
 using tmac::RopeArgs;
@@ -133,6 +137,9 @@ struct tmac_context {
     hipFunction_t any_combine[3] = {};
     hipFunction_t k_rope = nullptr, k_copy = nullptr, k_pos = nullptr, k_qkv = nullptr, k_cvt16 = nullptr,
                   k_cvt_q8 = nullptr;
+    // serving operators on paged caches, by kv_dtype; page scores by query heads per pass - 1
+    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_shared[4] = {}, k_scores[8] = {};
+    hipFunction_t k_select = nullptr, k_selected_merge = nullptr, k_shared_merge = nullptr;
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
     float* ws = nullptr;
@@ -1042,6 +1049,28 @@ int tmac_init(tmac_context** out, int device) {
         (e = get_function(ctx, &ctx->k_kq[1][1], "tmac_gemv_rows_q6_k")) != hipSuccess ||
         (e = get_function(ctx, &ctx->k_cvt_q8, "tmac_cvt_q8")) != hipSuccess)
         return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
+    {
+        char name[64];
+        for (int dt = 0; dt < 4; dt++) {
+            const std::pair<const char*, hipFunction_t*> by_type[] = {{"tmac_append", &ctx->k_append[dt]},
+                                                                      {"tmac_page_bounds", &ctx->k_bounds[dt]},
+                                                                      {"tmac_selected", &ctx->k_selected[dt]},
+                                                                      {"tmac_shared", &ctx->k_shared[dt]}};
+            for (auto& k : by_type) {
+                std::snprintf(name, sizeof(name), "%s_%s", k.first, kTypeName[dt]);
+                if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
+            }
+        }
+        for (int g = 1; g <= 8; g++) {
+            std::snprintf(name, sizeof(name), "tmac_page_scores_g%d", g);
+            if ((e = get_function(ctx, &ctx->k_scores[g - 1], name)) != hipSuccess)
+                return bail(hip_fail(ctx, e, name));
+        }
+        if ((e = get_function(ctx, &ctx->k_select, "tmac_select_pages")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_selected_merge, "tmac_selected_merge")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_shared_merge, "tmac_shared_merge")) != hipSuccess)
+            return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
+    }
     if ((e = hipStreamCreateWithFlags(&ctx->aux, hipStreamNonBlocking)) != hipSuccess)
         return bail(hip_fail(ctx, e, "hipStreamCreateWithFlags"));
     if ((e = hipMalloc(&ctx->err, sizeof(int))) != hipSuccess) return bail(hip_fail(ctx, e, "hipMalloc"));
@@ -1398,6 +1427,295 @@ int tmac_layer_attention_paged(tmac_context* ctx, tmac_stream stream, int kv_dty
                              n_seq, max_len);
     }
     return run_decode(ctx, (hipStream_t)stream, kern, a, n_seq, max_len, n_kv_head);
+}
+
+// ---- serving operators on paged caches ----
+
+// Shared checks: cache type and head layout (head_dim 64, any number of kv heads, at most kMaxGroupHeads query heads
+// per kv head), and the block table's geometry.
+static int check_serving(tmac_context* ctx, const char* what, int kv_dtype, int n_pages, const int32_t* block_table,
+                         int max_pages, int n_seq, int n_head, int n_kv_head, int head_dim) {
+    if (kv_dtype != TMAC_KV_F32 && kv_dtype != TMAC_KV_BF16 && kv_dtype != TMAC_KV_F16 && kv_dtype != TMAC_KV_Q8_0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG,
+                    std::string(what) + ": kv_dtype must be TMAC_KV_F32, _BF16, _F16 or _Q8_0");
+    if (n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG,
+                    std::string(what) + ": n_head must be a positive multiple of n_kv_head");
+    if (head_dim != kHeadDim) return fail(ctx, TMAC_ERR_UNSUPPORTED, std::string(what) + ": head_dim must be 64");
+    if (n_head / n_kv_head > tmac::kMaxGroupHeads)
+        return fail(ctx, TMAC_ERR_UNSUPPORTED, std::string(what) + ": more than 16 query heads per kv head");
+    if (!block_table) return fail(ctx, TMAC_ERR_NULL_POINTER, std::string(what) + ": null block_table");
+    if ((uintptr_t)block_table % 4) return fail(ctx, TMAC_ERR_MISALIGNED, std::string(what) + ": block_table");
+    if (n_pages < 1 || max_pages < 1 || n_seq < 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, std::string(what) + ": need n_pages, max_pages >= 1 and n_seq >= 0");
+    return TMAC_OK;
+}
+
+// A grid of `units` workgroups, refused where its index would not fit.
+static int check_units(tmac_context* ctx, const char* what, int64_t units) {
+    if (units > INT_MAX) return fail(ctx, TMAC_ERR_INVALID_ARG, std::string(what) + ": too many units of work");
+    return TMAC_OK;
+}
+
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q, int64_t q_stride,
+                         float* q_out, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                         void* k_pages, void* v_pages, int n_pages, const int32_t* block_table, int max_pages,
+                         const int32_t* row_starts, const int32_t* positions, int n_seq, int n_rows, int n_head,
+                         int n_kv_head, int head_dim, int max_len, float base) {
+    const char* what = "kv_append_paged";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    if (!k || !v || !k_pages || !v_pages || !row_starts || !positions || !q != !q_out)
+        return fail(ctx, TMAC_ERR_NULL_POINTER, "kv_append_paged: null buffer");
+    if (n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: n_head must be a positive multiple of n_kv_head");
+    // rows are stored per kv head: the number of query heads per kv head does not matter here
+    if ((rc = check_serving(ctx, what, kv_dtype, n_pages, block_table, max_pages, n_seq, n_kv_head, n_kv_head,
+                            head_dim)))
+        return rc;
+    if (!aligned16(q) || !aligned16(q_out) || !aligned16(k) || !aligned16(v) || !aligned16(k_pages) ||
+        !aligned16(v_pages) || q_stride % 4 || k_stride % 4 || v_stride % 4 || (uintptr_t)row_starts % 4 ||
+        (uintptr_t)positions % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "kv_append_paged: rows and pools must be 16-byte aligned");
+    if (n_rows < 0 || max_len < 1 || max_len > (int64_t)max_pages * kPageRows)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: need n_rows >= 0 and 1 <= max_len <= 16 * max_pages");
+    const int64_t q_row = (int64_t)n_head * kHeadDim, kv_row = (int64_t)n_kv_head * kHeadDim;
+    if (n_rows > 1 && ((q && q_stride < q_row) || k_stride < kv_row || v_stride < kv_row))
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: a row stride is shorter than its row");
+    if (!(base > 0.f) || !std::isfinite(base)) return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: bad base");
+    if (n_seq == 0 || n_rows == 0) return TMAC_OK;
+    // q_out may be q itself (same rows); any other overlap would let a row be overwritten before it is read
+    if (q && !(q == q_out && (q_stride == q_row || n_rows == 1))) {
+        const uintptr_t q0 = (uintptr_t)q, q1 = (uintptr_t)(q + (n_rows - 1) * q_stride + q_row);
+        const uintptr_t o0 = (uintptr_t)q_out, o1 = (uintptr_t)(q_out + n_rows * q_row);
+        if (q0 < o1 && o0 < q1)
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: q_out overlaps q without being it");
+    }
+    if ((rc = set_device(ctx))) return rc;
+    const RopeTable* rt = nullptr;
+    if ((rc = rope_table(ctx, (hipStream_t)stream, head_dim, base, max_len, &rt))) return rc;
+    AppendArgs a{};
+    a.q = q;
+    a.q_out = q_out;
+    a.k = k;
+    a.v = v;
+    a.k_pages = static_cast<char*>(k_pages);
+    a.v_pages = static_cast<char*>(v_pages);
+    a.block_table = block_table;
+    a.row_starts = row_starts;
+    a.positions = positions;
+    a.rope_cs = rt->dev;
+    a.err = ctx->err;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.n_pages = n_pages;
+    a.max_pages = max_pages;
+    a.n_seq = n_seq;
+    a.n_rows = n_rows;
+    a.n_head = n_head;
+    a.n_kv_head = n_kv_head;
+    a.capacity = max_len;
+    a.rows_per_group = (int)std::min<int64_t>(tmac::kAppendRows, std::max<int64_t>(1, n_rows / (8 * ctx->n_cu)));
+    return launch(ctx, ctx->k_append[kv_dtype], (unsigned)cdiv(n_rows, a.rows_per_group), 1, 256, (hipStream_t)stream,
+                  &a);
+}
+
+int tmac_kv_page_bounds(tmac_context* ctx, tmac_stream stream, int kv_dtype, const void* k_pages, int n_pages,
+                        const int32_t* block_table, int max_pages, const int32_t* first_rows, const int32_t* lengths,
+                        void* bounds, int n_seq, int n_kv_head, int head_dim, int max_new) {
+    const char* what = "kv_page_bounds";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    if (!k_pages || !lengths || !bounds) return fail(ctx, TMAC_ERR_NULL_POINTER, "kv_page_bounds: null buffer");
+    if ((rc = check_serving(ctx, what, kv_dtype, n_pages, block_table, max_pages, n_seq, n_kv_head, n_kv_head,
+                            head_dim)))
+        return rc;
+    if (!aligned16(k_pages) || !aligned16(bounds) || (uintptr_t)lengths % 4 || (uintptr_t)first_rows % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "kv_page_bounds: pool and bounds must be 16-byte aligned");
+    if (max_new < 0) return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_page_bounds: max_new >= 0");
+    if (n_seq == 0 || max_new == 0) return TMAC_OK;
+    // pages that max_new consecutive rows touch: from the last row of a page on, one more than they fill
+    const int64_t n_grid = std::min<int64_t>(max_pages, first_rows ? ((int64_t)max_new + kPageRows - 2) / kPageRows + 1
+                                                                   : cdiv(max_new, kPageRows));
+    BoundsArgs a{static_cast<const char*>(k_pages), block_table, first_rows, lengths, static_cast<uint16_t*>(bounds),
+                 ctx->err, n_pages, max_pages, n_seq, n_kv_head, max_new, (int)n_grid};
+    if (n_grid * n_kv_head > INT_MAX) return check_units(ctx, what, n_grid * n_kv_head);
+    const int64_t blocks = cdiv(n_grid * n_kv_head * n_seq, tmac::kPagedWaves);
+    if ((rc = check_units(ctx, what, blocks)) || (rc = set_device(ctx))) return rc;
+    return launch(ctx, ctx->k_bounds[kv_dtype], (unsigned)blocks, 1, 64 * tmac::kPagedWaves, (hipStream_t)stream, &a);
+}
+
+int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, const void* bounds, int n_pages,
+                      const int32_t* block_table, int max_pages, const int32_t* lengths, int32_t* selected, int n_seq,
+                      int n_head, int n_kv_head, int head_dim, int max_len, int top, int first, int last) {
+    const char* what = "select_pages";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    if (!q || !bounds || !lengths || !selected)
+        return fail(ctx, TMAC_ERR_NULL_POINTER, "select_pages: null buffer");
+    if ((rc = check_serving(ctx, what, TMAC_KV_F32, n_pages, block_table, max_pages, n_seq, n_head, n_kv_head,
+                            head_dim)))
+        return rc;
+    if (!aligned16(q) || !aligned16(bounds) || (uintptr_t)lengths % 4 || (uintptr_t)selected % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "select_pages: q and bounds must be 16-byte aligned");
+    if (max_len < 1 || max_len > (int64_t)max_pages * kPageRows)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: need 1 <= max_len <= 16 * max_pages");
+    if (top < 1 || first < 0 || last < 0 || (int64_t)first + last > top)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: need top >= 1, first, last >= 0, first + last <= top");
+    if (n_seq == 0) return TMAC_OK;
+    const int64_t n_sk = (int64_t)n_seq * n_kv_head, pages = cdiv(max_len, kPageRows);
+    const int64_t chunks = cdiv(pages, tmac::kScorePages);
+    if ((rc = check_units(ctx, what, n_sk * chunks)) || (rc = set_device(ctx))) return rc;
+    SelectArgs a{};
+    a.q = q;
+    a.bounds = static_cast<const uint16_t*>(bounds);
+    a.block_table = block_table;
+    a.lengths = lengths;
+    a.selected = selected;
+    a.err = ctx->err;
+    a.n_pages = n_pages;
+    a.max_pages = max_pages;
+    a.n_seq = n_seq;
+    a.n_head = n_head;
+    a.n_kv_head = n_kv_head;
+    a.max_len = max_len;
+    a.key_stride = (int)pages;
+    a.top = top;
+    a.first = first;
+    a.last = last;
+    a.chunks = (int)chunks;
+    if (pages > top) {  // otherwise every list holds all of its sequence's pages
+        if ((rc = ensure_workspace(ctx, (hipStream_t)stream, (size_t)(n_sk * pages)))) return rc;
+        a.keys = reinterpret_cast<uint32_t*>(workspace(ctx));
+        const int group = n_head / n_kv_head, passes = group > 8 ? 2 : 1;
+        if ((rc = launch(ctx, ctx->k_scores[cdiv(group, passes) - 1], (unsigned)(n_sk * chunks), 1, 256,
+                         (hipStream_t)stream, &a)))
+            return rc;
+    }
+    return launch(ctx, ctx->k_select, (unsigned)n_sk, 1, 256, (hipStream_t)stream, &a);
+}
+
+// Checks and arguments that both attentions over paged caches share.
+static int paged_attn_args(tmac_context* ctx, const char* what, int kv_dtype, const float* q, const void* k_pages,
+                           const void* v_pages, int n_pages, const int32_t* block_table, int max_pages,
+                           const int32_t* lengths, float* out, int n_seq, int n_head, int n_kv_head, int head_dim,
+                           PagedAttnArgs* a) {
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    if (!q || !k_pages || !v_pages || !lengths || !out)
+        return fail(ctx, TMAC_ERR_NULL_POINTER, std::string(what) + ": null buffer");
+    if ((rc = check_serving(ctx, what, kv_dtype, n_pages, block_table, max_pages, n_seq, n_head, n_kv_head, head_dim)))
+        return rc;
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || (uintptr_t)lengths % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, std::string(what) + ": q, out and pools must be 16-byte aligned");
+    if ((rc = check_units(ctx, what, cdiv((int64_t)n_seq * n_head, tmac::kPagedWaves)))) return rc;
+    a->q = q;
+    a->k_pages = static_cast<const char*>(k_pages);
+    a->v_pages = static_cast<const char*>(v_pages);
+    a->block_table = block_table;
+    a->lengths = lengths;
+    a->out = out;
+    a->err = ctx->err;
+    a->n_pages = n_pages;
+    a->max_pages = max_pages;
+    a->n_seq = n_seq;
+    a->n_head = n_head;
+    a->n_kv_head = n_kv_head;
+    a->qscale = kQScale;
+    return TMAC_OK;
+}
+
+static int paged_partials(tmac_context* ctx, tmac_stream stream, PagedAttnArgs* a) {
+    const size_t floats = (size_t)a->n_seq * a->n_head * a->n_slots * kPartialStride;
+    int rc = ensure_workspace(ctx, (hipStream_t)stream, floats);
+    if (rc == TMAC_OK) a->ws = workspace(ctx);
+    return rc;
+}
+
+int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
+                                   const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
+                                   int max_pages, const int32_t* lengths, const int32_t* selected, int top, float* out,
+                                   int n_seq, int n_head, int n_kv_head, int head_dim) {
+    const char* what = "decode_selected";
+    PagedAttnArgs a{};
+    int rc = paged_attn_args(ctx, what, kv_dtype, q, k_pages, v_pages, n_pages, block_table, max_pages, lengths, out,
+                             n_seq, n_head, n_kv_head, head_dim, &a);
+    if (rc) return rc;
+    if (!selected) return fail(ctx, TMAC_ERR_NULL_POINTER, "decode_selected: null selected");
+    if ((uintptr_t)selected % 4) return fail(ctx, TMAC_ERR_MISALIGNED, "decode_selected: selected");
+    if (top < 1) return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_selected: top >= 1");
+    if (n_seq == 0) return TMAC_OK;
+    a.selected = selected;
+    a.top = top;
+    const int64_t n_sk = (int64_t)n_seq * n_kv_head;
+    int64_t splits = std::min<int64_t>(cdiv(2 * ctx->n_cu, n_sk), cdiv(top, tmac::kPagedWaves));
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
+    a.per_split = (int)cdiv(top, splits);
+    a.n_slots = (int)cdiv(top, a.per_split);
+    if ((rc = check_units(ctx, what, n_sk * a.n_slots)) || (rc = set_device(ctx))) return rc;
+    if (a.n_slots > 1 && (rc = paged_partials(ctx, stream, &a))) return rc;
+    if ((rc = launch(ctx, ctx->k_selected[kv_dtype], (unsigned)(n_sk * a.n_slots), 1, 64 * tmac::kPagedWaves,
+                     (hipStream_t)stream, &a)) ||
+        a.n_slots == 1)
+        return rc;
+    return launch(ctx, ctx->k_selected_merge, (unsigned)cdiv((int64_t)n_seq * n_head, tmac::kPagedWaves), 1,
+                  64 * tmac::kPagedWaves, (hipStream_t)stream, &a);
+}
+
+int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
+                                 const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
+                                 int max_pages, const int32_t* lengths, const int32_t* group_starts,
+                                 const int32_t* prefix_lens, int n_groups, float* out, int n_seq, int n_head,
+                                 int n_kv_head, int head_dim, int max_prefix, int max_tail) {
+    const char* what = "decode_shared";
+    PagedAttnArgs a{};
+    int rc = paged_attn_args(ctx, what, kv_dtype, q, k_pages, v_pages, n_pages, block_table, max_pages, lengths, out,
+                             n_seq, n_head, n_kv_head, head_dim, &a);
+    if (rc) return rc;
+    if (n_groups < 0 || max_prefix < 0 || max_tail < 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_shared: n_groups, max_prefix, max_tail >= 0");
+    if (n_groups > 0 && (!group_starts || !prefix_lens))
+        return fail(ctx, TMAC_ERR_NULL_POINTER, "decode_shared: null group_starts or prefix_lens");
+    if ((uintptr_t)group_starts % 4 || (uintptr_t)prefix_lens % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "decode_shared: group_starts, prefix_lens");
+    if (max_prefix > (int64_t)max_pages * kPageRows || max_tail > (int64_t)max_pages * kPageRows)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_shared: max_prefix, max_tail <= 16 * max_pages");
+    if (n_seq == 0) return TMAC_OK;
+    a.group_starts = group_starts;
+    a.prefix_lens = prefix_lens;
+    a.n_groups = n_groups;
+    a.max_prefix = max_prefix;
+    a.max_tail = max_tail;
+    const int64_t group = n_head / n_kv_head, n_sk = (int64_t)n_seq * n_kv_head;
+    // blocks of columns: every group's last one may be partly filled
+    const int64_t blocks =
+        n_groups && max_prefix ? std::min<int64_t>(n_seq, n_seq * group / tmac::kSharedCols + n_groups) : 0;
+    a.prefix_blocks = (int)blocks;
+    a.prefix_splits = 0;
+    if (blocks) {
+        const int64_t pages = cdiv(max_prefix, kPageRows);
+        const int64_t splits = std::min<int64_t>(cdiv(ctx->n_cu, blocks * n_kv_head), cdiv(pages, 2 * tmac::kPagedWaves));
+        a.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
+    }
+    a.tail_rows = kPageRows;
+    if (max_tail) {
+        const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(2 * ctx->n_cu, n_sk), kMaxSplits));
+        a.tail_rows = (int)std::max<int64_t>(cdiv(cdiv(max_tail, splits), kPageRows) * kPageRows,
+                                             kPageRows * tmac::kPagedWaves);
+        a.tail_splits = (int)cdiv(max_tail, a.tail_rows);
+    }
+    a.n_slots = a.prefix_splits + a.tail_splits;
+    const int64_t units = blocks * n_kv_head * a.prefix_splits + n_sk * a.tail_splits;
+    if ((rc = check_units(ctx, what, units)) || (rc = set_device(ctx))) return rc;
+    if (a.n_slots && (rc = paged_partials(ctx, stream, &a))) return rc;
+    if (units && (rc = launch(ctx, ctx->k_shared[kv_dtype], (unsigned)units, 1, 64 * tmac::kPagedWaves,
+                              (hipStream_t)stream, &a)))
+        return rc;
+    return launch(ctx, ctx->k_shared_merge, (unsigned)cdiv((int64_t)n_seq * n_head, tmac::kPagedWaves), 1,
+                  64 * tmac::kPagedWaves, (hipStream_t)stream, &a);
 }
 
 int tmac_kv_convert(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* src, void* dst, int64_t n) {

@@ -90,6 +90,14 @@ SIGNATURES = {
                                          _i64]),
     "tmac_layer_attention_paged": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i,
                                         _i, _i, _f]),
+    "tmac_kv_append_paged": (_i, [_vp, _vp, _i, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp,
+                                  _i, _i, _i, _i, _i, _i, _f]),
+    "tmac_kv_page_bounds": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i]),
+    "tmac_select_pages": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "tmac_attention_decode_selected": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i,
+                                            _i]),
+    "tmac_attention_decode_shared": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i,
+                                          _i, _i, _i]),
     "tmac_matmul_q8_0": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp]),
     "tmac_matmul_q5_0": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp]),
     "tmac_matmul_add": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
@@ -529,6 +537,61 @@ class Context:
                                                  max_len, base)
         if check:
             self._check(rc, "layer_attention_paged")
+        return rc
+
+    # -- serving on paged caches -------------------------------------------------
+    def kv_append_paged(self, q, q_stride, q_out, k, k_stride, v, v_stride, k_pages, v_pages, n_pages, block_table,
+                        max_pages, row_starts, positions, n_seq, n_rows, n_head, n_kv_head, head_dim, max_len,
+                        base=1e6, stream=None, check=True, kv_dtype=TMAC_KV_F32) -> int:
+        """q (or None) rotated to q_out, k rotated and v to their pages (tmac_kv_append_paged)."""
+        rc = self.lib.tmac_kv_append_paged(self.handle, stream, kv_dtype, _p(q), q_stride, _p(q_out), _p(k), k_stride,
+                                           _p(v), v_stride, _p(k_pages), _p(v_pages), n_pages, _p(block_table),
+                                           max_pages, _p(row_starts), _p(positions), n_seq, n_rows, n_head, n_kv_head,
+                                           head_dim, max_len, base)
+        if check:
+            self._check(rc, "kv_append_paged")
+        return rc
+
+    def kv_page_bounds(self, k_pages, n_pages, block_table, max_pages, first_rows, lengths, bounds, n_seq, n_kv_head,
+                       head_dim, max_new, stream=None, check=True, kv_dtype=TMAC_KV_F32) -> int:
+        """bounds [n_pages][n_kv_head][2][64] bf16 of the pages that hold rows first_rows[s] .. lengths[s] - 1."""
+        rc = self.lib.tmac_kv_page_bounds(self.handle, stream, kv_dtype, _p(k_pages), n_pages, _p(block_table),
+                                          max_pages, _p(first_rows), _p(lengths), _p(bounds), n_seq, n_kv_head,
+                                          head_dim, max_new)
+        if check:
+            self._check(rc, "kv_page_bounds")
+        return rc
+
+    def select_pages(self, q, bounds, n_pages, block_table, max_pages, lengths, selected, n_seq, n_head, n_kv_head,
+                     head_dim, max_len, top, first=1, last=1, stream=None, check=True) -> int:
+        """selected [n_seq][n_kv_head][top]: the pages with the highest bounds of q . k, ascending, then -1."""
+        rc = self.lib.tmac_select_pages(self.handle, stream, _p(q), _p(bounds), n_pages, _p(block_table), max_pages,
+                                        _p(lengths), _p(selected), n_seq, n_head, n_kv_head, head_dim, max_len, top,
+                                        first, last)
+        if check:
+            self._check(rc, "select_pages")
+        return rc
+
+    def decode_selected(self, q, k_pages, v_pages, n_pages, block_table, max_pages, lengths, selected, top, out, n_seq,
+                        n_head, n_kv_head, head_dim, stream=None, check=True, kv_dtype=TMAC_KV_F32) -> int:
+        """decode_paged over the listed pages only."""
+        rc = self.lib.tmac_attention_decode_selected(self.handle, stream, kv_dtype, _p(q), _p(k_pages), _p(v_pages),
+                                                     n_pages, _p(block_table), max_pages, _p(lengths), _p(selected),
+                                                     top, _p(out), n_seq, n_head, n_kv_head, head_dim)
+        if check:
+            self._check(rc, "decode_selected")
+        return rc
+
+    def decode_shared(self, q, k_pages, v_pages, n_pages, block_table, max_pages, lengths, group_starts, prefix_lens,
+                      n_groups, out, n_seq, n_head, n_kv_head, head_dim, max_prefix, max_tail, stream=None, check=True,
+                      kv_dtype=TMAC_KV_F32) -> int:
+        """decode_paged of groups of sequences that share a prefix, read once per group."""
+        rc = self.lib.tmac_attention_decode_shared(self.handle, stream, kv_dtype, _p(q), _p(k_pages), _p(v_pages),
+                                                   n_pages, _p(block_table), max_pages, _p(lengths), _p(group_starts),
+                                                   _p(prefix_lens), n_groups, _p(out), n_seq, n_head, n_kv_head,
+                                                   head_dim, max_prefix, max_tail)
+        if check:
+            self._check(rc, "decode_shared")
         return rc
 
     def prefill(self, q, k, v, out, n_seq, n_q, prefix_len, seq_stride, n_head, n_kv_head, head_dim,
