@@ -336,4 +336,80 @@ __device__ __forceinline__ float sum4_rows(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+typedef __attribute__((address_space(4))) const int32_t* const_i32_ptr;
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 bf16x4_v;
+typedef __attribute__((address_space(3))) bf16x4_v* lds_bf16x4_ptr;
+typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 f16x4_v;
+typedef __attribute__((address_space(3))) f16x4_v* lds_f16x4_ptr;
+
+// The 16-bit element types of the MFMA decode: operand types, the matching
+// MFMAs and transposed LDS read, and packing of fp32 pairs (nearest even).
+//   bf16: fp32's exponent range, so q and P are split as they are.
+//   fp16: q is scaled per column by a power of two (its largest |value| to
+//   [2^14, 2^15)) and P by 2^7 before splitting, so the split parts stay in
+//   fp16's normal range; both scales are undone exactly after the MFMAs.
+template <typename T>
+struct MMath;
+template <>
+struct MMath<__bf16> {
+    typedef bf16x8 v8;
+    typedef i16x4 v4;
+    static constexpr bool kScaleQ = false;
+    static constexpr int kQParts = 3;  // 16-bit parts of an fp32 query element
+    static constexpr float kPScale = 1.0f;
+    __device__ static unsigned pack2(float a, float b) { return bf16_pair(a, b); }
+    __device__ static float lo(unsigned w) { return __uint_as_float(w << 16); }
+    __device__ static float hi(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
+    __device__ static f32x4 mfma32(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    __device__ static v8 cat(v4 a, v4 b) { return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)); }
+    __device__ static v4 read_tr(char* p) {
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_ptr)p));
+    }
+};
+template <>
+struct MMath<_Float16> {
+    typedef f16x8 v8;
+    typedef f16x4 v4;
+    static constexpr bool kScaleQ = true;
+    static constexpr int kQParts = 2;
+    static constexpr float kPScale = 128.0f;
+    __device__ static unsigned pack2(float a, float b) {
+        const f16x2 v = {(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(unsigned, v);
+    }
+    __device__ static float lo(unsigned w) { return half_bits_to_float(w & 0xffffu); }
+    __device__ static float hi(unsigned w) { return half_bits_to_float(w >> 16); }
+    __device__ static f32x4 mfma32(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    __device__ static v8 cat(v4 a, v4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+    __device__ static v4 read_tr(char* p) {
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_f16x4_ptr)p));
+    }
+};
+
+// Four int8 (one word) -> four bf16 (two words, element 2i in the low half), exactly.
+__device__ __forceinline__ u32x2 i8x4_to_bf16(unsigned w) {
+    const float f0 = (float)(signed char)w, f1 = (float)(signed char)(w >> 8);
+    const float f2 = (float)(signed char)(w >> 16), f3 = (float)(signed char)(w >> 24);
+    return u32x2{__builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u),
+                 __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u)};
+}
+
+// Four int8 (one word) -> four fp16 (two words, element 2i in the low half),
+// exactly: byte b becomes u = b ^ 0x80 = b + 128, the fp16 with bits
+// 0x6400 | u is 1024 + u, and subtracting 1152 (packed) leaves b.
+__device__ __forceinline__ u32x2 i8x4_to_f16(unsigned w) {
+    const unsigned x = w ^ 0x80808080u;
+    const unsigned a = __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u);  // bytes u0, 0x64, u1, 0x64
+    const unsigned b = __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u);  // bytes u2, 0x64, u3, 0x64
+    const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    return u32x2{__builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, a) - bias),
+                 __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, b) - bias)};
+}
+
 }  // namespace

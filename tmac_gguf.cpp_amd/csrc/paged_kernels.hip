@@ -13,8 +13,6 @@ using namespace tmac;
 
 namespace {
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-
 // ---------------------------------------------------------------------------
 // Append.  A workgroup takes rows_per_group consecutive rows.  Every thread
 // looks at its share of row_starts once: an entry at or before the first row
@@ -732,14 +730,446 @@ __device__ __forceinline__ int prefix_run_pages(const PagedAttnArgs& a, int64_t 
     return max(1, (n + a.prefix_splits - 1) / a.prefix_splits);
 }
 
+// ---------------------------------------------------------------------------
+// Shared prefix on 16-bit MFMA (v_mfma_f32_16x16x32).  A workgroup takes 64
+// columns, (sequence, query head) pairs of one group and kv head, over a run of
+// the prefix: wave (kg, cw) the columns 32 cw .. 32 cw + 31 and, of every
+// stage, the keys of half kg.  What bounds it is the products: every fp32
+// operand is carried by 16-bit parts that together hold its 24 bits, so fp32
+// accuracy costs a multiple of the plain product,
+//   cache   K, V        q            P            products, Q.K and P.V
+//   bf16    exact       3 bf16       3 bf16       3, 3
+//   fp16    exact       2 fp16       2 fp16       2, 2
+//   Q8_0    int8 exact  2 fp16       3 bf16 x 2   2, 3 (scales on S and on P)
+//   fp32    3 bf16      3 bf16       3 bf16       6, 6 (parts i + j <= 2; the rest is below 2^-24)
+// against fp32 MFMA at 1/16 of the 16-bit rate.  (Two bf16 parts of P, 2^-18,
+// left 2e-6 of the output's norm.)
+//
+// A stage's K and V rows go through registers (fetched one stage ahead) to LDS
+// once, converted there, and feed both column waves; V is read back transposed
+// (ds_read_b64_tr_b16).  16-byte chunks of a 128-byte LDS row are XORed with
+// the row, K by row & 7, V by 2 row & 7, so that both reads touch all banks.
+template <typename T>
+struct Px;
+template <>
+struct Px<__bf16> {
+    using KOps = MMath<__bf16>;
+    using VOps = MMath<__bf16>;
+    static constexpr int kParts = 1, kQ = 3, kP = 3, kSets = 1, kKeys = 64;
+};
+template <>
+struct Px<_Float16> {
+    using KOps = MMath<_Float16>;
+    using VOps = MMath<_Float16>;
+    static constexpr int kParts = 1, kQ = 2, kP = 2, kSets = 1, kKeys = 64;
+};
+template <>
+struct Px<q8_0_t> {
+    using KOps = MMath<_Float16>;
+    using VOps = MMath<__bf16>;
+    static constexpr int kParts = 1, kQ = 2, kP = 3, kSets = 2, kKeys = 64;
+};
+template <>
+struct Px<float> {
+    using KOps = MMath<__bf16>;
+    using VOps = MMath<__bf16>;
+    static constexpr int kParts = 3, kQ = 3, kP = 3, kSets = 1, kKeys = 32;
+};
+
+// One stage in LDS: rows of both key halves, `kParts` 16-bit images of K and V.
+template <typename T>
+struct PxStage {
+    static constexpr int kRows = 2 * Px<T>::kKeys;
+    char k[Px<T>::kParts][kRows][128];
+    char v[Px<T>::kParts][kRows][128];
+    float kd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];  // Q8_0 scales by dim half
+    float vd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];
+};
+
+__device__ __forceinline__ int px_k_at(int row, int chunk) { return (chunk ^ (row & 7)) << 4; }
+__device__ __forceinline__ int px_v_at(int row, int chunk) { return (chunk ^ ((2 * row) & 7)) << 4; }
+
+// This thread's share of a stage as fetched.
+template <typename T>
+struct PxRaw {
+    static constexpr int N = __is_same(T, q8_0_t) ? 2 : 4;  // 16-byte chunks per tensor
+    u32x4 k[N], v[N];
+    unsigned kd, vd;  // Q8_0: threads 0 .. 127 the scale words of their row
+};
+template <typename T>
+struct PxGeom {
+    static constexpr int kPerRow = __is_same(T, float) ? 16 : __is_same(T, q8_0_t) ? 4 : 8;  // chunks per row
+    static constexpr int kStep = 256 / kPerRow;                                              // rows per fetch
+    static constexpr int kPages = PxStage<T>::kRows / kPageRows;                             // pages per stage
+};
+
+typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+template <typename T>
+__device__ __forceinline__ void px_fetch(PxRaw<T>& r, const PagedAttnArgs& a, int h, const const_i32_ptr table, int j0,
+                                         int j_last, int tid, unsigned& bad) {
+    using G = PxGeom<T>;
+    constexpr int HB = CacheFmt<T>::kHeadBytes;
+    const int stride = a.n_kv_head * HB;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    auto base_of = [&](int row0) {  // of the page that holds stage row row0 (wave-uniform)
+        const int pg = table[min(j0 + row0 / kPageRows, j_last)];
+        bad |= (unsigned)pg >= (unsigned)a.n_pages;
+        return (size_t)min(max(pg, 0), a.n_pages - 1) * ((size_t)kPageRows * stride) + (size_t)h * HB;
+    };
+#pragma unroll
+    for (int i = 0; i < PxRaw<T>::N; ++i) {
+        const size_t base = base_of(i * G::kStep + wave * 64 / G::kPerRow);
+        const int row = (tid / G::kPerRow) % kPageRows;  // kStep is a multiple of a page's rows
+        const size_t at = base + (size_t)row * stride + (tid % G::kPerRow) * 16;
+        if constexpr (__is_same(T, q8_0_t)) {  // head rows are 4-byte aligned
+            r.k[i] = *reinterpret_cast<const u32x4_a4*>(a.k_pages + at);
+            r.v[i] = *reinterpret_cast<const u32x4_a4*>(a.v_pages + at);
+        } else {
+            r.k[i] = *reinterpret_cast<const u32x4*>(a.k_pages + at);
+            r.v[i] = *reinterpret_cast<const u32x4*>(a.v_pages + at);
+        }
+    }
+    if constexpr (__is_same(T, q8_0_t)) {
+        // lanes of waves 0 and 1: rows 64 wave + lane, four pages a wave
+        const int row = tid & 127;
+        size_t base = 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const size_t b = base_of(64 * (wave & 1) + 16 * p);
+            base = (row & 63) / kPageRows == p ? b : base;
+        }
+        const size_t at = base + (size_t)(row % kPageRows) * stride + 64;
+        r.kd = *reinterpret_cast<const unsigned*>(a.k_pages + at);
+        r.vd = *reinterpret_cast<const unsigned*>(a.v_pages + at);
+    }
+}
+
+// Three bf16 parts of two fp32 values (element 0 in the low half), cut bits: exact.
+__device__ __forceinline__ void split3(float x, float y, unsigned (&w)[3]) {
+    auto top = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); };
+    auto pair = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); };
+    w[0] = pair(x, y);
+    const float x1 = x - top(x), y1 = y - top(y);
+    w[1] = pair(x1, y1);
+    w[2] = pair(x1 - top(x1), y1 - top(y1));
+}
+// Two fp16 parts (nearest, then the nearest to what is left).
+__device__ __forceinline__ void split2(float x, float y, unsigned (&w)[3]) {
+    w[0] = MMath<_Float16>::pack2(x, y);
+    w[1] = MMath<_Float16>::pack2(x - MMath<_Float16>::lo(w[0]), y - MMath<_Float16>::hi(w[0]));
+}
+
+// Rows at or past `valid` of the stage: V is written as zeros (P is 0 there, and the row may hold anything).
+template <typename T>
+__device__ __forceinline__ void px_store(PxStage<T>& s, const PxRaw<T>& r, int valid, int tid) {
+    using G = PxGeom<T>;
+    const u32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < PxRaw<T>::N; ++i) {
+        const int row = i * G::kStep + tid / G::kPerRow, q = tid % G::kPerRow;
+        const u32x4 v = row < valid ? r.v[i] : zero;
+        if constexpr (__is_same(T, float)) {
+            const int half = 8 * (q & 1);
+            unsigned k0[3], k1[3], v0[3], v1[3];
+            split3(__uint_as_float(r.k[i][0]), __uint_as_float(r.k[i][1]), k0);
+            split3(__uint_as_float(r.k[i][2]), __uint_as_float(r.k[i][3]), k1);
+            split3(__uint_as_float(v[0]), __uint_as_float(v[1]), v0);
+            split3(__uint_as_float(v[2]), __uint_as_float(v[3]), v1);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                *reinterpret_cast<u32x2*>(&s.k[p][row][px_k_at(row, q / 2) + half]) = u32x2{k0[p], k1[p]};
+                *reinterpret_cast<u32x2*>(&s.v[p][row][px_v_at(row, q / 2) + half]) = u32x2{v0[p], v1[p]};
+            }
+        } else if constexpr (__is_same(T, q8_0_t)) {  // 16 values: chunks 2 q, 2 q + 1
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const u32x2 ka = i8x4_to_f16(r.k[i][2 * c]), kb = i8x4_to_f16(r.k[i][2 * c + 1]);
+                const u32x2 va = i8x4_to_bf16(v[2 * c]), vb = i8x4_to_bf16(v[2 * c + 1]);
+                *reinterpret_cast<u32x4*>(&s.k[0][row][px_k_at(row, 2 * q + c)]) = u32x4{ka[0], ka[1], kb[0], kb[1]};
+                *reinterpret_cast<u32x4*>(&s.v[0][row][px_v_at(row, 2 * q + c)]) = u32x4{va[0], va[1], vb[0], vb[1]};
+            }
+        } else {
+            *reinterpret_cast<u32x4*>(&s.k[0][row][px_k_at(row, q)]) = r.k[i];
+            *reinterpret_cast<u32x4*>(&s.v[0][row][px_v_at(row, q)]) = v;
+        }
+    }
+    if constexpr (__is_same(T, q8_0_t)) {
+        if (tid < PxStage<T>::kRows) {
+            s.kd[0][tid] = half_bits_to_float(r.kd & 0xFFFFu);
+            s.kd[1][tid] = half_bits_to_float(r.kd >> 16);
+            const unsigned vd = tid < valid ? r.vd : 0u;
+            s.vd[0][tid] = half_bits_to_float(vd & 0xFFFFu);
+            s.vd[1][tid] = half_bits_to_float(vd >> 16);
+        }
+    }
+}
+
+// Whether part i of one operand meets part j of the other.
+template <int NA, int NB>
+constexpr bool px_pair(int i, int j) {
+    return NA == 1 || NB == 1 || i + j <= 2;
+}
+
+// One wave's columns.
+template <typename T>
+struct PxCols {
+    typename Px<T>::KOps::v8 q[2][2][Px<T>::kQ];  // [column block][dim half][part]
+    float unscale[2];                             // fp16 operands: undoes the column's power of two
+    f32x4 o[2][4];                                // block b, row r: dim 16 b + 4 g + r
+    float m[2], l[2];
+};
+
+template <typename T>
+__device__ __forceinline__ void px_load_q(PxCols<T>& c, int t, const float* p, float scale, int lane) {
+    using X = Px<T>;
+    const int g = lane >> 4;
+    float x[2][8];
+    float top = 0.f;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
+        if (p) {
+            u = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g);
+            w = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g + 4);
+        }
+        const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[m][e] = y[e] * scale;
+            top = fmaxf(top, fabsf(x[m][e]));
+        }
+    }
+    c.unscale[t] = 1.f;
+    if constexpr (X::KOps::kScaleQ) {  // the column's largest value to [2^14, 2^15)
+        top = max4_rows(top);
+        const int e = min(max(14 - ((int)(__float_as_uint(top) >> 23) - 127), -126), 126);
+        const float up = __uint_as_float((unsigned)(127 + e) << 23);
+        c.unscale[t] = __uint_as_float((unsigned)(127 - e) << 23);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[m][i] *= up;
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        u32x4 w[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unsigned y[3] = {0, 0, 0};
+            if constexpr (X::KOps::kScaleQ)
+                split2(x[m][2 * i], x[m][2 * i + 1], y);
+            else
+                split3(x[m][2 * i], x[m][2 * i + 1], y);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) w[k][i] = y[k];
+        }
+#pragma unroll
+        for (int k = 0; k < X::kQ; ++k) c.q[t][m][k] = __builtin_bit_cast(typename X::KOps::v8, w[k]);
+    }
+}
+
+// The wave's keys of one stage (rows row0 .. row0 + kKeys - 1, of which `valid` take part).
+template <typename T>
+__device__ __forceinline__ void px_attend(PxCols<T>& c, PxStage<T>& s, int row0, int valid, int lane) {
+    using X = Px<T>;
+    using KO = typename X::KOps;
+    using VO = typename X::VOps;
+    constexpr int KT = X::kKeys / 16;  // 16-key tiles
+    constexpr bool Q8 = __is_same(T, q8_0_t);
+    const int i = lane & 15, g = lane >> 4;
+    f32x4 st[2][KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        const int row = row0 + 16 * kt + i;
+        f32x4 acc[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kp = 0; kp < X::kParts; ++kp) {
+                const auto kx = *reinterpret_cast<const typename KO::v8*>(&s.k[kp][row][px_k_at(row, 4 * m + g)]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int qp = 0; qp < X::kQ; ++qp)
+                        if (px_pair<X::kParts, X::kQ>(kp, qp))
+                            acc[t][Q8 ? m : 0] = KO::mfma32(kx, c.q[t][m][qp], acc[t][Q8 ? m : 0]);
+            }
+        if constexpr (Q8) {
+            const f32x4 d0 = *reinterpret_cast<const f32x4*>(&s.kd[0][row0 + 16 * kt + 4 * g]);
+            const f32x4 d1 = *reinterpret_cast<const f32x4*>(&s.kd[1][row0 + 16 * kt + 4 * g]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) st[t][kt] = (acc[t][0] * d0 + acc[t][1] * d1) * c.unscale[t];
+        } else {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                st[t][kt] = acc[t][0];
+                if constexpr (KO::kScaleQ) st[t][kt] *= c.unscale[t];
+            }
+        }
+    }
+    if (valid < X::kKeys) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) st[t][kt][r] = 16 * kt + 4 * g + r < valid ? st[t][kt][r] : kNegInf;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        float top = kNegInf;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+            top = fmaxf(top, fmaxf(fmaxf(st[t][kt][0], st[t][kt][1]), fmaxf(st[t][kt][2], st[t][kt][3])));
+        if (__any(top > c.m[t] + kTau || c.m[t] == kNoMax)) {
+            const float m1 = fmaxf(c.m[t], max4_rows(top));
+            const float w = fast_exp2(c.m[t] - m1);
+            c.m[t] = m1;
+            c.l[t] *= w;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) c.o[t][b] *= w;
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st[t][kt][r] = fast_exp2(st[t][kt][r] - c.m[t]);
+            c.l[t] += (st[t][kt][0] + st[t][kt][1]) + (st[t][kt][2] + st[t][kt][3]);
+        }
+    }
+    // 32 keys at a time: slots 8 g + e hold key 4 g + e of the first tile (e < 4) and of the second
+#pragma unroll
+    for (int ks = 0; ks < KT / 2; ++ks) {
+        typename VO::v8 px[2][X::kSets][X::kP];
+#pragma unroll
+        for (int set = 0; set < X::kSets; ++set) {
+            u32x4 w[2][3];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x4 d = {VO::kPScale, VO::kPScale, VO::kPScale, VO::kPScale};
+                if constexpr (Q8)
+                    d = *reinterpret_cast<const f32x4*>(&s.vd[set][row0 + 32 * ks + 16 * half + 4 * g]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float x = st[t][2 * ks + half][2 * r], y = st[t][2 * ks + half][2 * r + 1];
+                        if constexpr (Q8 || VO::kPScale != 1.0f) x *= d[2 * r], y *= d[2 * r + 1];
+                        unsigned z[3] = {0, 0, 0};
+                        if constexpr (X::kP == 2)
+                            split2(x, y, z);
+                        else
+                            split3(x, y, z);
+#pragma unroll
+                        for (int p = 0; p < X::kP; ++p) w[t][p][2 * half + r] = z[p];
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int p = 0; p < X::kP; ++p) px[t][set][p] = __builtin_bit_cast(typename VO::v8, w[t][p]);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int vp = 0; vp < X::kParts; ++vp) {
+                const int r0 = row0 + 32 * ks + 4 * g + (i >> 2), r1 = r0 + 16, chunk = 2 * b + ((i & 3) >> 1);
+                const auto v0 = VO::read_tr(&s.v[vp][r0][px_v_at(r0, chunk) + 8 * (i & 1)]);
+                const auto v1 = VO::read_tr(&s.v[vp][r1][px_v_at(r1, chunk) + 8 * (i & 1)]);
+                const auto vx = VO::cat(v0, v1);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int p = 0; p < X::kP; ++p)
+                        if (px_pair<X::kParts, X::kP>(vp, p))
+                            c.o[t][b] = VO::mfma32(vx, px[t][X::kSets == 2 ? b / 2 : 0][p], c.o[t][b]);
+            }
+    }
+}
+
+// Both key halves' columns through LDS; put(column, dim, m, l, acc).
+struct PxMerge {
+    float o[2][kSharedCols][kHeadDim + 4];
+    float m[2][kSharedCols], l[2][kSharedCols];
+};
+template <typename T>
+union PxLds {
+    PxStage<T> stage[__is_same(T, float) ? 1 : 2];
+    PxMerge merge;
+};
+
+template <typename T, typename ColPtr, typename Put>
+__device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, const int32_t* table_, int h, int j0,
+                                       int n_pages, int64_t rows, int n_cols, int tid, ColPtr col_ptr, Put put) {
+    using X = Px<T>;
+    using G = PxGeom<T>;
+    constexpr int NB = __is_same(T, float) ? 1 : 2;
+    const const_i32_ptr table = (const_i32_ptr)table_;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave >> 1, cw = wave & 1;
+    const int i = lane & 15, g = lane >> 4;
+    const int n_stage = (n_pages + G::kPages - 1) / G::kPages, j_last = j0 + n_pages - 1;
+    const int n_rows = (int)min((int64_t)n_pages * kPageRows, rows - (int64_t)j0 * kPageRows);  // of this run
+    const bool busy = 32 * cw < n_cols;
+    unsigned bad = 0;
+    PxRaw<T> raw;
+    px_fetch<T>(raw, a, h, table, j0, j_last, tid, bad);
+    PxCols<T> c;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        px_load_q<T>(c, t, col_ptr(32 * cw + 16 * t + i), a.qscale, lane);
+        c.m[t] = kNoMax;
+        c.l[t] = 0.f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) c.o[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    px_store<T>(lds.stage[0], raw, n_rows, tid);
+    __syncthreads();
+    for (int st = 0; st < n_stage; ++st) {
+        PxStage<T>& cur = lds.stage[NB == 2 ? st & 1 : 0];
+        const bool more = st + 1 < n_stage;
+        if (more) px_fetch<T>(raw, a, h, table, j0 + (st + 1) * G::kPages, j_last, tid, bad);
+        const int valid = min(n_rows - st * PxStage<T>::kRows - kg * X::kKeys, X::kKeys);
+        if (busy && valid > 0) px_attend<T>(c, cur, kg * X::kKeys, valid, lane);
+        if (more) {
+            if constexpr (NB == 1) __syncthreads();
+            px_store<T>(lds.stage[NB == 2 ? (st + 1) & 1 : 0], raw, n_rows - (st + 1) * PxStage<T>::kRows, tid);
+        }
+        __syncthreads();
+    }
+    if (bad && lane == 0) atomicOr(a.err, 4);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int col = 32 * cw + 16 * t + i;
+        const float l = sum4_rows(c.l[t]);
+        if (g == 0) {
+            lds.merge.m[kg][col] = c.m[t];
+            lds.merge.l[kg][col] = l;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            f32x4 o = c.o[t][b];
+            if constexpr (X::VOps::kPScale != 1.0f) o *= 1.0f / X::VOps::kPScale;
+            *reinterpret_cast<f32x4*>(&lds.merge.o[kg][col][16 * b + 4 * g]) = o;
+        }
+    }
+    __syncthreads();
+    for (int col = wave; col < min(n_cols, kSharedCols); col += kPagedWaves) {
+        const float m0 = lds.merge.m[0][col], m1 = lds.merge.m[1][col], M = fmaxf(m0, m1);
+        const float x0 = fast_exp2(m0 - M), x1 = fast_exp2(m1 - M);
+        put(col, lane, M, x0 * lds.merge.l[0][col] + x1 * lds.merge.l[1][col],
+            x0 * lds.merge.o[0][col][lane] + x1 * lds.merge.o[1][col][lane]);
+    }
+}
+
 // Shared prefixes and own rows: the first prefix_blocks * n_kv_head *
 // prefix_splits workgroups take (64 columns of a group, kv head, run of its
 // prefix), the rest (own rows of a sequence, kv head, run).
 template <typename T>
 __device__ __forceinline__ void shared_body(const PagedAttnArgs& a) {
-    constexpr int NC = kSharedCols / 16;
     __shared__ union {
-        MergeLds<NC> p;
+        PxLds<T> p;
         MergeLds<1> t;
     } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -782,29 +1212,15 @@ __device__ __forceinline__ void shared_body(const PagedAttnArgs& a) {
         const int n_all = (int)((prefix + kPageRows - 1) >> kPageShift);
         const int n = min(per, n_all - j0);
         if (n <= 0) return;
-        Cols<NC> st;
-        cols_init(st);
-        const int rows = (end - first) * G;  // (sequence, head of the group) columns of the group
-#pragma unroll
-        for (int t = 0; t < NC; ++t) {
-            const int c = left * kSharedCols + 16 * t + col;
-            load_q(st.q[t],
-                   c < rows ? a.q + ((size_t)(first + c / G) * a.n_head + h * G + c % G) * kHeadDim : nullptr,
-                   a.qscale, lane);
-        }
-        const int32_t* table = a.block_table + (size_t)first * a.max_pages;
-        attend_run<T, NC>(st, a, h, n, 0, prefix, wave, lane, [&](int e, int& logical, int& page) {
-            logical = j0 + e;
-            page = table[logical];
-            if (page < 0 || page >= a.n_pages) {
-                atomicOr(a.err, 4);
-                page = min(max(page, 0), a.n_pages - 1);
-            }
-        });
-        merge_waves<NC>(st, lds.p, wave, lane, [&](int c, int d, float M, float L, float A) {
-            const int r = left * kSharedCols + c;
-            if (r < rows) put_partial(a, first + r / G, h * G + r % G, split, d, M, L, A);
-        });
+        const int cols = (end - first) * G - left * kSharedCols;  // of the group, from this block's first on
+        auto seq_of = [&](int c) { return first + (left * kSharedCols + c) / G; };
+        auto head_of = [&](int c) { return h * G + (left * kSharedCols + c) % G; };
+        px_run<T>(
+            a, lds.p, a.block_table + (size_t)first * a.max_pages, h, j0, n, prefix, cols, threadIdx.x,
+            [&](int c) -> const float* {
+                return c < cols ? a.q + ((size_t)seq_of(c) * a.n_head + head_of(c)) * kHeadDim : nullptr;
+            },
+            [&](int c, int d, float M, float L, float A) { put_partial(a, seq_of(c), head_of(c), split, d, M, L, A); });
     } else {
         const int id = blockIdx.x - n_prefix;
         const int split = id % a.tail_splits, sk = id / a.tail_splits, s = sk / kv, h = sk - s * kv;
@@ -858,7 +1274,7 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     extern "C" __global__ __launch_bounds__(256) void tmac_append_##NAME(AppendArgs a) { append_body<T>(a); }          \
     extern "C" __global__ __launch_bounds__(256) void tmac_page_bounds_##NAME(BoundsArgs a) { bounds_body<T>(a); }     \
     extern "C" __global__ __launch_bounds__(256) void tmac_selected_##NAME(PagedAttnArgs a) { selected_body<T>(a); }   \
-    extern "C" __global__ __launch_bounds__(256) void tmac_shared_##NAME(PagedAttnArgs a) { shared_body<T>(a); }
+    extern "C" __global__ __launch_bounds__(256, 2) void tmac_shared_##NAME(PagedAttnArgs a) { shared_body<T>(a); }
 TMAC_PAGED_KERNELS(f32, float)
 TMAC_PAGED_KERNELS(bf16, __bf16)
 TMAC_PAGED_KERNELS(f16, _Float16)
