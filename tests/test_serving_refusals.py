@@ -157,7 +157,7 @@ def test_legal_edges(fake):
     assert ok("tmac_attention_decode_shared", n_groups=0, group_starts=None, prefix_lens=None)
     # no rows possible: the merge alone writes the zero outputs
     rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=0, max_tail=0)
-    assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_shared_merge"]
+    assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_shared_merge_w1"]
     # every list holds all pages: no scores
     rc, launches = fake.call("tmac_select_pages", top=40)
     assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_select_pages"]

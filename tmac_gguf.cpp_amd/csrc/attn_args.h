@@ -244,9 +244,10 @@ struct PagedAttnArgs {
     const int32_t* block_table;
     const int32_t* lengths;
     float* out;
-    float* ws;               // partials [n_seq][n_head][n_slots][kPartialStride]
+    float* ws;               // partials [n_seq][n_head][n_slots]: acc[64] each, then (m, l) each
     int* err;
     int n_pages, max_pages, n_seq, n_head, n_kv_head;
+    int group;               // n_head / n_kv_head
     float qscale;
     int n_slots;             // partials per (sequence, query head)
     // list
@@ -260,7 +261,8 @@ struct PagedAttnArgs {
     int prefix_blocks;       // blocks of kSharedCols (sequence, query head) columns, at most
     int tail_splits, tail_rows;  // slots behind them: runs of tail_rows own rows
 };
-constexpr int kPagedWaves = 4;    // waves per workgroup
+constexpr int kPagedWaves = 4;    // waves per workgroup: bounds, list, merges
+constexpr int kSharedWaves = 8;   // shared prefixes and own rows
 constexpr int kMaxGroupHeads = 16;  // query heads per kv head, at most (MFMA columns)
 constexpr int kSharedCols = 64;   // prefix workgroup: (sequence, query head) columns
 

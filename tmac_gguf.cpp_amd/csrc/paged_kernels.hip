@@ -336,8 +336,7 @@ __device__ __forceinline__ void select_body(const SelectArgs& a) {
 // Decode attention by (columns, kv head, run of pages) on fp32 MFMA
 // (v_mfma_f32_16x16x4_f32, products and sums of fp32: the cache rows are
 // widened exactly, so every cache type gets the fp32 result).  A tile is one
-// page, 16 keys x up to NC blocks of 16 columns; a column is a query head of
-// one sequence.
+// page, 16 keys x 16 columns; a column is a query head of one sequence.
 //   S^T (16 keys x 16 columns) = K (keys x dims) . Q^T.   Lane (i = l % 16,
 //     g = l / 16) holds key i's dims 32 m + 8 g + e of K and column i's of Q:
 //     step (m, e) contracts the four dims 32 m + 8 g + e, g = 0..3.
@@ -433,82 +432,67 @@ __device__ __forceinline__ float tile_v(const Tile<T>& t, int r, int b, int i) {
 
 constexpr float kNoMax = -__FLT_MAX__;  // running maximum of a column that has met no key
 
-// One wave's state for NC blocks of 16 columns.
-template <int NC>
+// One wave's state of a block of 16 columns.
 struct Cols {
-    float q[NC][16];
-    f32x4 o[NC][4];  // block b, row r: dim 16 g + 4 r + b
-    float m[NC], l[NC];  // m: the column's (equal in the four lane groups); l: this lane's keys
+    float q[16];
+    f32x4 o[4];   // block b, row r: dim 16 g + 4 r + b
+    float m, l;   // m: the column's (equal in the four lane groups); l: this lane's keys
 };
 
 // One tile: keys lo .. hi - 1 of the page take part.
-template <typename T, int NC>
-__device__ __forceinline__ void attend_tile(Cols<NC>& st, const Tile<T>& t, int lo, int hi, int lane) {
+template <typename T>
+__device__ __forceinline__ void attend_tile(Cols& st, const Tile<T>& t, int lo, int hi, int lane) {
     const int i = lane & 15, g = lane >> 4;
     const bool full = lo <= 0 && hi >= kPageRows;
-    f32x4 s[NC];
+    f32x4 s = {0.f, 0.f, 0.f, 0.f}, s1 = s;  // two sums: a chain of 16 dependent products would wait on itself
 #pragma unroll
-    for (int n = 0; n < NC; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float kx = tile_k<T>(t, m, e);
-#pragma unroll
-            for (int n = 0; n < NC; ++n)
-                s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx, st.q[n][8 * m + e], s[n], 0, 0, 0);
-        }
+    for (int e = 0; e < 8; ++e) {
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_k<T>(t, 0, e), st.q[e], s, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_k<T>(t, 1, e), st.q[8 + e], s1, 0, 0, 0);
+    }
+    s += s1;
     if (!full) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const bool in = 4 * g + r >= lo && 4 * g + r < hi;
+        for (int r = 0; r < 4; ++r) s[r] = 4 * g + r >= lo && 4 * g + r < hi ? s[r] : kNegInf;
+    }
+    const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    if (__any(top > st.m + kTau || st.m == kNoMax)) {
+        const float m1 = fmaxf(st.m, max4_rows(top));
+        const float w = fast_exp2(st.m - m1);
+        st.m = m1;
+        st.l *= w;
 #pragma unroll
-            for (int n = 0; n < NC; ++n) s[n][r] = in ? s[n][r] : kNegInf;
-        }
+        for (int b = 0; b < 4; ++b) st.o[b] *= w;
     }
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const float top = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3]));
-        if (__any(top > st.m[n] + kTau || st.m[n] == kNoMax)) {
-            const float m1 = fmaxf(st.m[n], max4_rows(top));
-            const float w = fast_exp2(st.m[n] - m1);
-            st.m[n] = m1;
-            st.l[n] *= w;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) st.o[n][b] *= w;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[n][r] = fast_exp2(s[n][r] - st.m[n]);
-        st.l[n] += (s[n][0] + s[n][1]) + (s[n][2] + s[n][3]);
-    }
+    for (int r = 0; r < 4; ++r) s[r] = fast_exp2(s[r] - st.m);
+    st.l += (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const bool in = full || (4 * g + r >= lo && 4 * g + r < hi);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const float vx = in ? tile_v<T>(t, r, b, i) : 0.f;  // a row outside may hold anything
-#pragma unroll
-            for (int n = 0; n < NC; ++n)
-                st.o[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx, s[n][r], st.o[n][b], 0, 0, 0);
+            st.o[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx, s[r], st.o[b], 0, 0, 0);
         }
     }
 }
 
-// A run of tiles.  Entry e (0 <= e < n) is page pages(e) of the pool (checked,
-// in range) with logical page index logical(e); rows row_lo .. row_hi - 1 of
-// the sequence take part.  The workgroup's waves take the entries in turn; a
-// wave looks up 64 of its entries at a time, one a lane.
-template <typename T, int NC, typename Look>
-__device__ __forceinline__ void attend_run(Cols<NC>& st, const PagedAttnArgs& a, int h, int n, int64_t row_lo,
+// A run of tiles.  look(e, logical, page) gives entry e (0 <= e < n) its page of
+// the pool (checked, in range) and its logical page index (-1: skipped); rows
+// row_lo .. row_hi - 1 of the sequence take part.  The NW waves take the
+// entries in turn; a wave looks up 64 of its entries at a time, one a lane.
+template <typename T, int NW, typename Look>
+__device__ __forceinline__ void attend_run(Cols& st, const PagedAttnArgs& a, int h, int n, int64_t row_lo,
                                            int64_t row_hi, int wave, int lane, Look look) {
     constexpr int HB = CacheFmt<T>::kHeadBytes;
     const int stride = a.n_kv_head * HB;
     const size_t page_bytes = (size_t)kPageRows * stride;
-    const int mine = (n - wave + kPagedWaves - 1) / kPagedWaves;  // this wave's entries
+    const int mine = (n - wave + NW - 1) / NW;  // this wave's entries
     for (int c0 = 0; c0 < mine; c0 += 64) {
         const int cnt = min(64, mine - c0);
         int logical = -1, page = 0;
-        if (lane < cnt) look((c0 + lane) * kPagedWaves + wave, logical, page);
+        if (lane < cnt) look((c0 + lane) * NW + wave, logical, page);
         Tile<T> t[2];
         auto fetch = [&](Tile<T>& x, int e) {
             const size_t at = (size_t)__builtin_amdgcn_readlane(page, e) * page_bytes + (size_t)h * HB;
@@ -524,26 +508,15 @@ __device__ __forceinline__ void attend_run(Cols<NC>& st, const PagedAttnArgs& a,
                     const int64_t r0 = (int64_t)j * kPageRows;
                     const int lo = (int)max((int64_t)0, min(row_lo - r0, (int64_t)kPageRows));
                     const int hi = j < 0 ? 0 : (int)max((int64_t)0, min(row_hi - r0, (int64_t)kPageRows));
-                    if (hi > lo) attend_tile<T, NC>(st, t[u], lo, hi, lane);
+                    if (hi > lo) attend_tile<T>(st, t[u], lo, hi, lane);
                 }
             }
         }
     }
 }
 
-template <int NC>
-__device__ __forceinline__ void cols_init(Cols<NC>& st) {
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        st.m[n] = kNoMax;
-        st.l[n] = 0.f;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) st.o[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-}
-
-// Column q row pointer (null: an unused column) -> pre-scaled operand.
-__device__ __forceinline__ void load_q(float (&q)[16], const float* p, float scale, int lane) {
+// Empty columns with the query rows p (null: an unused column), scaled.
+__device__ __forceinline__ void cols_init(Cols& st, const float* p, float scale, int lane) {
     const int g = lane >> 4;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -552,79 +525,84 @@ __device__ __forceinline__ void load_q(float (&q)[16], const float* p, float sca
             x = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g);
             y = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g + 4);
         }
-        float* o = q + 8 * m;
+        float* o = st.q + 8 * m;
         o[0] = x.x * scale; o[1] = x.y * scale; o[2] = x.z * scale; o[3] = x.w * scale;
         o[4] = y.x * scale; o[5] = y.y * scale; o[6] = y.z * scale; o[7] = y.w * scale;
     }
+    st.m = kNoMax;
+    st.l = 0.f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) st.o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// Merges the waves of the workgroup through LDS and hands every column's (m, l,
-// acc[dim]) to `put`, which runs once per (column, dim).
-template <int NC>
+// Merges the NW waves through LDS and hands every column's maximum, sum and
+// four dims to put(column, first dim, m, l, acc): one call a thread of the first
+// 256 (16 columns x 16 dim quads).
+template <int NW>
 struct MergeLds {
-    float o[kPagedWaves][NC * 16][kHeadDim + 1];
-    float m[kPagedWaves][NC * 16], l[kPagedWaves][NC * 16];
+    alignas(16) float o[NW][16][kHeadDim + 4];
+    float m[NW][16], l[NW][16];
 };
-template <int NC, typename Put>
-__device__ __forceinline__ void merge_waves(Cols<NC>& st, MergeLds<NC>& lds, int wave, int lane, Put put) {
+template <int NW, typename Put>
+__device__ __forceinline__ void merge_waves(Cols& st, MergeLds<NW>& lds, int wave, int lane, Put put) {
     const int i = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const float l = sum4_rows(st.l[n]);
-        if (g == 0) {
-            lds.m[wave][16 * n + i] = st.m[n];
-            lds.l[wave][16 * n + i] = l;
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) lds.o[wave][16 * n + i][16 * g + 4 * r + b] = st.o[n][b][r];
+    const float l = sum4_rows(st.l);
+    if (g == 0) {
+        lds.m[wave][i] = st.m;
+        lds.l[wave][i] = l;
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(&lds.o[wave][i][16 * g + 4 * r]) =
+            f32x4{st.o[0][r], st.o[1][r], st.o[2][r], st.o[3][r]};
     __syncthreads();
-    for (int c = wave; c < NC * 16; c += kPagedWaves) {
-        float M = lds.m[0][c];
+    const int c = threadIdx.x >> 4, d = 4 * (threadIdx.x & 15);
+    if (c >= 16) return;
+    float M = lds.m[0][c];
 #pragma unroll
-        for (int w = 1; w < kPagedWaves; ++w) M = fmaxf(M, lds.m[w][c]);
-        float L = 0.f, A = 0.f;
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, lds.m[w][c]);
+    float L = 0.f;
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kPagedWaves; ++w) {
-            const float x = fast_exp2(lds.m[w][c] - M);
-            L += x * lds.l[w][c];
-            A += x * lds.o[w][c][lane];
-        }
-        put(c, lane, M, L, A);
+    for (int w = 0; w < NW; ++w) {
+        const float x = fast_exp2(lds.m[w][c] - M);
+        L += x * lds.l[w][c];
+        A += x * *reinterpret_cast<const f32x4*>(&lds.o[w][c][d]);
     }
+    put(c, d, M, L, A);
 }
 
-__device__ __forceinline__ float finish_row(float acc, float l) { return l == 0.f ? 0.f : acc / l; }
+__device__ __forceinline__ f32x4 finish_row(f32x4 acc, float l) {
+    return l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : acc / l;
+}
 
-// Stores one (column, dim) of a partial.
-__device__ __forceinline__ void put_partial(const PagedAttnArgs& a, int s, int head, int slot, int d, float M, float L,
-                                            float A) {
-    float* w = a.ws + (((size_t)s * a.n_head + head) * a.n_slots + slot) * kPartialStride;
-    w[d] = A;
-    if (d == 0) {
-        w[kHeadDim] = M;
-        w[kHeadDim + 1] = L;
-    }
+// Partials: every row's slots of 64 sums, then every row's slots of (m, l).
+__device__ __forceinline__ void put_partial(const PagedAttnArgs& a, int64_t row, int slot, int d, float M, float L,
+                                            f32x4 A) {
+    const size_t at = (size_t)row * a.n_slots + slot;
+    *reinterpret_cast<f32x4*>(a.ws + at * kHeadDim + d) = A;
+    if (d == 0)
+        *reinterpret_cast<float2*>(a.ws + (size_t)a.n_seq * a.n_head * a.n_slots * kHeadDim + 2 * at) =
+            make_float2(M, L);
 }
 
 // Over a list: workgroup (split, kv head, sequence).
 template <typename T>
 __device__ __forceinline__ void selected_body(const PagedAttnArgs& a) {
-    __shared__ MergeLds<1> lds;
+    constexpr int NW = kPagedWaves;
+    __shared__ MergeLds<NW> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv = a.n_kv_head, G = a.n_head / kv;
+    const int kv = a.n_kv_head, G = a.group;
     const int split = blockIdx.x % a.n_slots, sk = blockIdx.x / a.n_slots, s = sk / kv, h = sk - s * kv;
     const int len = a.lengths[s];
     const int e0 = split * a.per_split, n = min(a.per_split, a.top - e0);
     const int32_t* list = a.selected + (size_t)sk * a.top + e0;
     const int32_t* table = a.block_table + (size_t)s * a.max_pages;
-    Cols<1> st;
-    cols_init(st);
+    const int64_t row0 = (int64_t)s * a.n_head + h * G;
     const int col = lane & 15;
-    load_q(st.q[0], col < G ? a.q + ((size_t)s * a.n_head + h * G + col) * kHeadDim : nullptr, a.qscale, lane);
-    attend_run<T, 1>(st, a, h, n, 0, len, wave, lane, [&](int e, int& logical, int& page) {
+    Cols st;
+    cols_init(st, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, a.qscale, lane);
+    attend_run<T, NW>(st, a, h, n, 0, len, wave, lane, [&](int e, int& logical, int& page) {
         const int j = list[e];
         if (j == -1) return;
         if (j < 0 || j >= a.max_pages) {
@@ -639,86 +617,106 @@ __device__ __forceinline__ void selected_body(const PagedAttnArgs& a) {
         }
         logical = j;
     });
-    merge_waves<1>(st, lds, wave, lane, [&](int c, int d, float M, float L, float A) {
+    merge_waves<NW>(st, lds, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         if (a.n_slots == 1)
-            a.out[((size_t)s * a.n_head + h * G + c) * kHeadDim + d] = finish_row(A, L);
+            *reinterpret_cast<f32x4*>(a.out + (row0 + c) * kHeadDim + d) = finish_row(A, L);
         else
-            put_partial(a, s, h * G + c, split, d, M, L, A);
+            put_partial(a, row0 + c, split, d, M, L, A);
     });
 }
 
-// Merge of `n` partials of one (sequence, query head): one wave, a dim a lane.
-__device__ __forceinline__ void merge_slots(const float* w, int n0, int skip_to, int n1, int lane, float& M, float& L,
-                                            float& A) {
-    // slots 0 .. n0 - 1 and skip_to .. skip_to + n1 - 1
-    const int n = n0 + n1;
-    M = kNoMax, L = 0.f, A = 0.f;
-    for (int c0 = 0; c0 < n; c0 += 64) {
-        const int e = c0 + lane, cnt = min(64, n - c0);
-        float m = kNoMax, l = 0.f;
-        if (e < n) {
-            const float* p = w + (size_t)(e < n0 ? e : skip_to + e - n0) * kPartialStride;
-            m = p[kHeadDim];
-            l = p[kHeadDim + 1];
+// Merge of one row's partials, slots 0 .. n0 - 1 and skip_to .. skip_to + n1 - 1,
+// by WPR waves: a wave reads four slots at once, 16 lanes of four dims each, 64
+// slots (WPR = 4) or 16 (WPR = 1) in one round of independent loads.  The
+// result is in the lanes 0 .. 15 of the row's first wave.  Every thread calls it.
+template <int WPR>
+__device__ __forceinline__ f32x4 merge_slots(const PagedAttnArgs& a, int64_t row, int n0, int skip_to, int n1, int w,
+                                             int lane, float& L) {
+    constexpr int kRound = 16 * WPR;
+    const int n = n0 + n1, sub = lane >> 4;
+    const float* acc = a.ws + (size_t)row * a.n_slots * kHeadDim + 4 * (lane & 15);
+    const float2* ml = reinterpret_cast<const float2*>(a.ws + (size_t)a.n_seq * a.n_head * a.n_slots * kHeadDim) +
+                       (size_t)row * a.n_slots;
+    auto slot = [&](int e) { return e < n0 ? e : skip_to + e - n0; };
+    float M = kNoMax;
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+    L = 0.f;
+    for (int c0 = 0; c0 < n; c0 += kRound) {
+        f32x4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = c0 + 4 * (WPR * i + w) + sub;
+            v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (e < n) v[i] = *reinterpret_cast<const f32x4*>(acc + (size_t)slot(e) * kHeadDim);
         }
-        const float m1 = fmaxf(M, xor_max<1>(m));
-        const float f = fast_exp2(M - m1);
-        const float x = fast_exp2(m - m1);
-        L = L * f + xor_sum<1>(l * x);
+        float2 x = make_float2(kNoMax, 0.f);
+        if (lane < kRound && c0 + lane < n) x = ml[slot(c0 + lane)];
+        const float m1 = fmaxf(M, xor_max<1>(x.x));
+        const float f = fast_exp2(M - m1), y = fast_exp2(x.x - m1);
+        L = L * f + xor_sum<1>(x.y * y);
         A *= f;
-        for (int i = 0; i < cnt; ++i) {
-            const int ei = c0 + i;
-            const float* p = w + (size_t)(ei < n0 ? ei : skip_to + ei - n0) * kPartialStride;
-            A += __shfl(x, i) * p[lane];
-        }
         M = m1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A += __shfl(y, (4 * (WPR * i + w) + sub) & 63) * v[i];
     }
-}
-
-__device__ __forceinline__ void selected_merge_body(const PagedAttnArgs& a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * kPagedWaves + (threadIdx.x >> 6);
-    if (row >= (int64_t)a.n_seq * a.n_head) return;
-    float M, L, A;
-    merge_slots(a.ws + (size_t)row * a.n_slots * kPartialStride, a.n_slots, a.n_slots, 0, lane, M, L, A);
-    a.out[(size_t)row * kHeadDim + lane] = finish_row(A, L);
-}
-
-// Group g's sequences [first, end), clamped into the batch.
-__device__ __forceinline__ void group_range(const PagedAttnArgs& a, int g, int& first, int& end) {
-    first = min(max(a.group_starts[g], 0), a.n_seq);
-    end = min(max(a.group_starts[g + 1], first), a.n_seq);
-}
-
-// The group of a sequence: the last one that starts at or before it and ends
-// behind it; -1: none.  Wave-wide.
-__device__ __forceinline__ int group_of(const PagedAttnArgs& a, int s, int lane) {
-    int found = -1;
-    for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
-        const int g = g0 + lane;
-        bool in = false;
-        if (g < a.n_groups) {
-            int first, end;
-            group_range(a, g, first, end);
-            in = s >= first && s < end;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) A[i] = xor_sum<16>(A[i]);
+    if constexpr (WPR > 1) {
+        __shared__ f32x4 s_a[WPR][16];
+        if (lane < 16) s_a[w][lane] = A;
+        __syncthreads();
+        if (lane < 16) {
+            A = s_a[0][lane];
+#pragma unroll
+            for (int i = 1; i < WPR; ++i) A += s_a[i][lane];
         }
-        const uint64_t b = __ballot(in);
-        if (b) found = g0 + 63 - __clzll(b);
     }
-    return found;
+    return A;
+}
+
+template <int WPR>
+__device__ __forceinline__ void selected_merge_body(const PagedAttnArgs& a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * (kPagedWaves / WPR) + wave / WPR;
+    if (row >= (int64_t)a.n_seq * a.n_head) return;
+    float L;
+    const f32x4 A = merge_slots<WPR>(a, row, a.n_slots, a.n_slots, 0, wave % WPR, lane, L);
+    if (wave % WPR == 0 && lane < 16) *reinterpret_cast<f32x4*>(a.out + row * kHeadDim + 4 * lane) = finish_row(A, L);
+}
+
+// A lane's group: its sequences [first, end), clamped into the batch, and its
+// prefix.  All of a group's numbers are loaded together: in these short kernels
+// every dependent load is a good part of a microsecond.
+struct Group {
+    int first, end, prefix;
+};
+__device__ __forceinline__ Group group_at(const PagedAttnArgs& a, int g) {
+    Group r = {0, 0, 0};
+    if (g < a.n_groups) {
+        const int s0 = a.group_starts[g], s1 = a.group_starts[g + 1];
+        r.prefix = max(a.prefix_lens[g], 0);
+        r.first = min(max(s0, 0), a.n_seq);
+        r.end = min(max(s1, r.first), a.n_seq);
+    }
+    return r;
 }
 
 // A sequence's rows: [0, prefix) through its group's first sequence, [prefix,
-// len) through its own pages.
+// len) through its own pages.  Its group is the last one that holds it.
 struct SharedSeq {
     int64_t prefix, len;
     bool bad;  // a length or prefix outside what the launch covers
 };
-__device__ __forceinline__ SharedSeq shared_seq(const PagedAttnArgs& a, int s, int g) {
+__device__ __forceinline__ SharedSeq shared_seq(const PagedAttnArgs& a, int s, int lane) {
     SharedSeq r;
     r.len = max(a.lengths[s], 0);
-    r.prefix = g >= 0 ? max(a.prefix_lens[g], 0) : 0;
+    r.prefix = 0;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
+        const Group g = group_at(a, g0 + lane);
+        const uint64_t b = __ballot(s >= g.first && s < g.end);
+        if (b) r.prefix = __builtin_amdgcn_readlane(g.prefix, 63 - __clzll(b));
+    }
     r.bad = r.len > 0 && (r.prefix > a.max_prefix || r.len < r.prefix || r.len - r.prefix > a.max_tail ||
                           r.len > (int64_t)a.max_pages * kPageRows);
     return r;
@@ -726,15 +724,15 @@ __device__ __forceinline__ SharedSeq shared_seq(const PagedAttnArgs& a, int s, i
 
 // Pages of one run of a prefix of `prefix` rows cut into prefix_splits runs.
 __device__ __forceinline__ int prefix_run_pages(const PagedAttnArgs& a, int64_t prefix) {
-    const int n = (int)((prefix + kPageRows - 1) >> kPageShift);
-    return max(1, (n + a.prefix_splits - 1) / a.prefix_splits);
+    const int n = (int)((prefix + kPageRows - 1) >> kPageShift), runs = max(1, a.prefix_splits);
+    return max(1, (n + runs - 1) / runs);
 }
 
 // ---------------------------------------------------------------------------
-// Shared prefix on 16-bit MFMA (v_mfma_f32_16x16x32).  A workgroup takes 64
-// columns, (sequence, query head) pairs of one group and kv head, over a run of
-// the prefix: wave (kg, cw) the columns 32 cw .. 32 cw + 31 and, of every
-// stage, the keys of half kg.  What bounds it is the products: every fp32
+// Shared prefix on 16-bit MFMA (v_mfma_f32_16x16x32).  A workgroup of 8 waves
+// takes 64 columns, (sequence, query head) pairs of one group and kv head, over
+// a run of the prefix: wave (kg, cw) the columns 32 cw .. 32 cw + 31 and, of
+// every stage, the keys of quarter kg.  What bounds it is the products: every fp32
 // operand is carried by 16-bit parts that together hold its 24 bits, so fp32
 // accuracy costs a multiple of the plain product,
 //   cache   K, V        q            P            products, Q.K and P.V
@@ -776,14 +774,16 @@ struct Px<float> {
     static constexpr int kParts = 3, kQ = 3, kP = 3, kSets = 1, kKeys = 32;
 };
 
-// One stage in LDS: rows of both key halves, `kParts` 16-bit images of K and V.
+constexpr int kPxGroups = kSharedWaves / 2;  // key groups: quarters of a stage
+
+// One stage in LDS: rows of all key groups, `kParts` 16-bit images of K and V.
 template <typename T>
 struct PxStage {
-    static constexpr int kRows = 2 * Px<T>::kKeys;
-    char k[Px<T>::kParts][kRows][128];
-    char v[Px<T>::kParts][kRows][128];
-    float kd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];  // Q8_0 scales by dim half
-    float vd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];
+    static constexpr int kRows = kPxGroups * Px<T>::kKeys;
+    alignas(16) char k[Px<T>::kParts][kRows][128];
+    alignas(16) char v[Px<T>::kParts][kRows][128];
+    alignas(16) float kd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];  // Q8_0 scales by dim half
+    alignas(16) float vd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];
 };
 
 __device__ __forceinline__ int px_k_at(int row, int chunk) { return (chunk ^ (row & 7)) << 4; }
@@ -794,32 +794,50 @@ template <typename T>
 struct PxRaw {
     static constexpr int N = __is_same(T, q8_0_t) ? 2 : 4;  // 16-byte chunks per tensor
     u32x4 k[N], v[N];
-    unsigned kd, vd;  // Q8_0: threads 0 .. 127 the scale words of their row
+    unsigned kd, vd;  // Q8_0: threads 0 .. 255 the scale words of their row
 };
 template <typename T>
 struct PxGeom {
     static constexpr int kPerRow = __is_same(T, float) ? 16 : __is_same(T, q8_0_t) ? 4 : 8;  // chunks per row
-    static constexpr int kStep = 256 / kPerRow;                                              // rows per fetch
+    static constexpr int kStep = 64 * kSharedWaves / kPerRow;                                              // rows per fetch
     static constexpr int kPages = PxStage<T>::kRows / kPageRows;                             // pages per stage
 };
 
 typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// Pool pages of a stage whose first page is logical page j0, as this wave
+// fetches them (scalar loads, issued a stage before the rows).
 template <typename T>
-__device__ __forceinline__ void px_fetch(PxRaw<T>& r, const PagedAttnArgs& a, int h, const const_i32_ptr table, int j0,
-                                         int j_last, int tid, unsigned& bad) {
+struct PxPages {
+    static constexpr int N = __is_same(T, q8_0_t) ? 6 : 4;
+    int page[N];
+};
+template <typename T>
+__device__ __forceinline__ void px_pages(PxPages<T>& p, const const_i32_ptr table, int j0, int j_last, int wave) {
+    using G = PxGeom<T>;
+#pragma unroll
+    for (int i = 0; i < PxPages<T>::N; ++i) {
+        // rows of fetch i, then (Q8_0) of the scale words
+        const int row0 = i < PxRaw<T>::N ? i * G::kStep + wave * 64 / G::kPerRow
+                                         : 64 * (wave & 3) + kPageRows * (i - PxRaw<T>::N);
+        p.page[i] = table[min(j0 + row0 / kPageRows, j_last)];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void px_fetch(PxRaw<T>& r, const PagedAttnArgs& a, int h, const PxPages<T>& pages, int tid,
+                                         unsigned& bad) {
     using G = PxGeom<T>;
     constexpr int HB = CacheFmt<T>::kHeadBytes;
     const int stride = a.n_kv_head * HB;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    auto base_of = [&](int row0) {  // of the page that holds stage row row0 (wave-uniform)
-        const int pg = table[min(j0 + row0 / kPageRows, j_last)];
+    auto base_of = [&](int i) {
+        const int pg = pages.page[i];
         bad |= (unsigned)pg >= (unsigned)a.n_pages;
         return (size_t)min(max(pg, 0), a.n_pages - 1) * ((size_t)kPageRows * stride) + (size_t)h * HB;
     };
 #pragma unroll
     for (int i = 0; i < PxRaw<T>::N; ++i) {
-        const size_t base = base_of(i * G::kStep + wave * 64 / G::kPerRow);
+        const size_t base = base_of(i);
         const int row = (tid / G::kPerRow) % kPageRows;  // kStep is a multiple of a page's rows
         const size_t at = base + (size_t)row * stride + (tid % G::kPerRow) * 16;
         if constexpr (__is_same(T, q8_0_t)) {  // head rows are 4-byte aligned
@@ -831,12 +849,12 @@ __device__ __forceinline__ void px_fetch(PxRaw<T>& r, const PagedAttnArgs& a, in
         }
     }
     if constexpr (__is_same(T, q8_0_t)) {
-        // lanes of waves 0 and 1: rows 64 wave + lane, four pages a wave
-        const int row = tid & 127;
+        // lanes of waves 0 .. 3: rows 64 wave + lane, four pages a wave (waves 4 .. 7 repeat them)
+        const int row = tid & 255;
         size_t base = 0;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            const size_t b = base_of(64 * (wave & 1) + 16 * p);
+            const size_t b = base_of(PxRaw<T>::N + p);
             base = (row & 63) / kPageRows == p ? b : base;
         }
         const size_t at = base + (size_t)(row % kPageRows) * stride + 64;
@@ -1011,6 +1029,7 @@ __device__ __forceinline__ void px_attend(PxCols<T>& c, PxStage<T>& s, int row0,
         }
     }
     if (valid < X::kKeys) {
+        asm volatile("");  // a branch: as selects the masks would cost every stage 48 instructions
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -1089,10 +1108,10 @@ __device__ __forceinline__ void px_attend(PxCols<T>& c, PxStage<T>& s, int row0,
     }
 }
 
-// Both key halves' columns through LDS; put(column, dim, m, l, acc).
+// The key groups' columns through LDS.
 struct PxMerge {
-    float o[2][kSharedCols][kHeadDim + 4];
-    float m[2][kSharedCols], l[2][kSharedCols];
+    alignas(16) float o[kPxGroups][kSharedCols][kHeadDim + 4];
+    float m[kPxGroups][kSharedCols], l[kPxGroups][kSharedCols];
 };
 template <typename T>
 union PxLds {
@@ -1114,7 +1133,10 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
     const bool busy = 32 * cw < n_cols;
     unsigned bad = 0;
     PxRaw<T> raw;
-    px_fetch<T>(raw, a, h, table, j0, j_last, tid, bad);
+    PxPages<T> pages;
+    px_pages<T>(pages, table, j0, j_last, wave);
+    px_fetch<T>(raw, a, h, pages, tid, bad);
+    px_pages<T>(pages, table, j0 + G::kPages, j_last, wave);
     PxCols<T> c;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -1129,7 +1151,10 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
     for (int st = 0; st < n_stage; ++st) {
         PxStage<T>& cur = lds.stage[NB == 2 ? st & 1 : 0];
         const bool more = st + 1 < n_stage;
-        if (more) px_fetch<T>(raw, a, h, table, j0 + (st + 1) * G::kPages, j_last, tid, bad);
+        if (more) {
+            px_fetch<T>(raw, a, h, pages, tid, bad);
+            px_pages<T>(pages, table, j0 + (st + 2) * G::kPages, j_last, wave);
+        }
         const int valid = min(n_rows - st * PxStage<T>::kRows - kg * X::kKeys, X::kKeys);
         if (busy && valid > 0) px_attend<T>(c, cur, kg * X::kKeys, valid, lane);
         if (more) {
@@ -1155,12 +1180,22 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
         }
     }
     __syncthreads();
-    for (int col = wave; col < min(n_cols, kSharedCols); col += kPagedWaves) {
-        const float m0 = lds.merge.m[0][col], m1 = lds.merge.m[1][col], M = fmaxf(m0, m1);
-        const float x0 = fast_exp2(m0 - M), x1 = fast_exp2(m1 - M);
-        put(col, lane, M, x0 * lds.merge.l[0][col] + x1 * lds.merge.l[1][col],
-            x0 * lds.merge.o[0][col][lane] + x1 * lds.merge.o[1][col][lane]);
+    // 8 threads a column, dims 4 d .. and 32 + 4 d ..
+    const int col = tid >> 3, d = 4 * (tid & 7);
+    if (col >= n_cols) return;
+    float M = lds.merge.m[0][col], L = 0.f;
+#pragma unroll
+    for (int k = 1; k < kPxGroups; ++k) M = fmaxf(M, lds.merge.m[k][col]);
+    f32x4 A = {0.f, 0.f, 0.f, 0.f}, B = A;
+#pragma unroll
+    for (int k = 0; k < kPxGroups; ++k) {
+        const float x = fast_exp2(lds.merge.m[k][col] - M);
+        L += x * lds.merge.l[k][col];
+        A += x * *reinterpret_cast<const f32x4*>(&lds.merge.o[k][col][d]);
+        B += x * *reinterpret_cast<const f32x4*>(&lds.merge.o[k][col][32 + d]);
     }
+    put(col, d, M, L, A);
+    put(col, 32 + d, M, L, B);
 }
 
 // Shared prefixes and own rows: the first prefix_blocks * n_kv_head *
@@ -1170,70 +1205,65 @@ template <typename T>
 __device__ __forceinline__ void shared_body(const PagedAttnArgs& a) {
     __shared__ union {
         PxLds<T> p;
-        MergeLds<1> t;
+        MergeLds<kSharedWaves> t;
     } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv = a.n_kv_head, G = a.n_head / kv;
+    const int kv = a.n_kv_head, G = a.group;
     const int n_prefix = a.prefix_blocks * kv * a.prefix_splits;
-    const int col = lane & 15;
     if ((int)blockIdx.x < n_prefix) {
-        const int split = blockIdx.x % a.prefix_splits, bh = blockIdx.x / a.prefix_splits, h = bh % kv, block = bh / kv;
+        const int split = blockIdx.x % a.prefix_splits, bh = blockIdx.x / a.prefix_splits, block = bh / kv,
+                  h = bh - block * kv;
         // the group whose column blocks hold this one
-        int g = -1, first = 0, end = 0, left = block;
-        for (int g0 = 0; g0 < a.n_groups && g < 0; g0 += 64) {
-            int f = 0, e = 0;
-            if (g0 + lane < a.n_groups) group_range(a, g0 + lane, f, e);
-            const int nb = (int)(((int64_t)(e - f) * G + kSharedCols - 1) / kSharedCols);
+        Group grp = {0, 0, 0};
+        int left = block;
+        bool found = false;
+        for (int g0 = 0; g0 < a.n_groups && !found; g0 += 64) {
+            const Group g = group_at(a, g0 + lane);
+            const int nb = (int)(((int64_t)(g.end - g.first) * G + kSharedCols - 1) / kSharedCols);
             int incl = nb;
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) {
+            for (int m = 1; m < min(64, a.n_groups - g0); m *= 2) {
                 const int o = __shfl_up(incl, m);
                 if (lane >= m) incl += o;
             }
             const uint64_t b = __ballot(incl > left);
+            const int at = b ? __builtin_ctzll(b) : 63;
             if (b) {
-                const int at = __ffsll((unsigned long long)b) - 1;
-                g = g0 + at;
-                first = __shfl(f, at);
-                end = __shfl(e, at);
-                left -= __shfl(incl - nb, at);
-            } else {
-                left -= __shfl(incl, 63);
+                grp.first = __builtin_amdgcn_readlane(g.first, at);
+                grp.end = __builtin_amdgcn_readlane(g.end, at);
+                grp.prefix = __builtin_amdgcn_readlane(g.prefix, at);
+                found = true;
             }
+            left -= __builtin_amdgcn_readlane(found ? incl - nb : incl, at);
         }
-        g = __builtin_amdgcn_readfirstlane(g);
-        first = __builtin_amdgcn_readfirstlane(first);
-        end = __builtin_amdgcn_readfirstlane(end);
-        left = __builtin_amdgcn_readfirstlane(left);
-        if (g < 0) return;
-        const int64_t prefix = max(a.prefix_lens[g], 0);
-        if (prefix == 0 || prefix > a.max_prefix || prefix > (int64_t)a.max_pages * kPageRows) return;
+        const int64_t prefix = grp.prefix;
+        if (!found || prefix == 0 || prefix > a.max_prefix) return;
         const int per = prefix_run_pages(a, prefix), j0 = split * per;
-        const int n_all = (int)((prefix + kPageRows - 1) >> kPageShift);
-        const int n = min(per, n_all - j0);
+        const int n = min(per, (int)((prefix + kPageRows - 1) >> kPageShift) - j0);
         if (n <= 0) return;
-        const int cols = (end - first) * G - left * kSharedCols;  // of the group, from this block's first on
-        auto seq_of = [&](int c) { return first + (left * kSharedCols + c) / G; };
-        auto head_of = [&](int c) { return h * G + (left * kSharedCols + c) % G; };
+        const int c0 = left * kSharedCols;                 // this block's first column of the group
+        const int cols = (grp.end - grp.first) * G - c0;   // columns from there on
+        auto row_of = [&](int c) {
+            const int s = (c0 + c) / G;
+            return (int64_t)(grp.first + s) * a.n_head + h * G + (c0 + c - s * G);
+        };
         px_run<T>(
-            a, lds.p, a.block_table + (size_t)first * a.max_pages, h, j0, n, prefix, cols, threadIdx.x,
-            [&](int c) -> const float* {
-                return c < cols ? a.q + ((size_t)seq_of(c) * a.n_head + head_of(c)) * kHeadDim : nullptr;
-            },
-            [&](int c, int d, float M, float L, float A) { put_partial(a, seq_of(c), head_of(c), split, d, M, L, A); });
+            a, lds.p, a.block_table + (size_t)grp.first * a.max_pages, h, j0, n, prefix, cols, threadIdx.x,
+            [&](int c) -> const float* { return c < cols ? a.q + row_of(c) * kHeadDim : nullptr; },
+            [&](int c, int d, float M, float L, f32x4 A) { put_partial(a, row_of(c), split, d, M, L, A); });
     } else {
         const int id = blockIdx.x - n_prefix;
         const int split = id % a.tail_splits, sk = id / a.tail_splits, s = sk / kv, h = sk - s * kv;
-        const SharedSeq q = shared_seq(a, s, group_of(a, s, lane));
+        const int64_t row0 = (int64_t)s * a.n_head + h * G;
+        const int col = lane & 15;
+        Cols st;
+        cols_init(st, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, a.qscale, lane);
+        const SharedSeq q = shared_seq(a, s, lane);
         if (q.bad) return;
         const int64_t lo = q.prefix + (int64_t)split * a.tail_rows, hi = min(q.len, lo + a.tail_rows);
         if (lo >= hi) return;
         const int j0 = (int)(lo >> kPageShift), n = (int)((hi - 1) >> kPageShift) - j0 + 1;
-        Cols<1> st;
-        cols_init(st);
-        load_q(st.q[0], col < G ? a.q + ((size_t)s * a.n_head + h * G + col) * kHeadDim : nullptr, a.qscale, lane);
         const int32_t* table = a.block_table + (size_t)s * a.max_pages;
-        attend_run<T, 1>(st, a, h, n, lo, hi, wave, lane, [&](int e, int& logical, int& page) {
+        attend_run<T, kSharedWaves>(st, a, h, n, lo, hi, wave, lane, [&](int e, int& logical, int& page) {
             logical = j0 + e;
             page = table[logical];
             if (page < 0 || page >= a.n_pages) {
@@ -1241,31 +1271,35 @@ __device__ __forceinline__ void shared_body(const PagedAttnArgs& a) {
                 page = min(max(page, 0), a.n_pages - 1);
             }
         });
-        merge_waves<1>(st, lds.t, wave, lane, [&](int c, int d, float M, float L, float A) {
-            if (c < G) put_partial(a, s, h * G + c, a.prefix_splits + split, d, M, L, A);
+        merge_waves<kSharedWaves>(st, lds.t, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
+            if (c < G) put_partial(a, row0 + c, a.prefix_splits + split, d, M, L, A);
         });
     }
 }
 
+template <int WPR>
 __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * kPagedWaves + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * (kPagedWaves / WPR) + wave / WPR;
     if (row >= (int64_t)a.n_seq * a.n_head) return;
-    const int s = (int)(row / a.n_head);
-    const SharedSeq q = shared_seq(a, s, group_of(a, s, lane));
-    float y = 0.f;
+    const int s = __builtin_amdgcn_readfirstlane((int)(row / a.n_head));
+    const SharedSeq q = shared_seq(a, s, lane);
+    int n0 = 0, n1 = 0;
+    if (!q.bad && q.len > 0) {
+        const int64_t per = (int64_t)prefix_run_pages(a, q.prefix) * kPageRows;
+        n0 = (int)((q.prefix + per - 1) / per);
+        n1 = (int)((q.len - q.prefix + a.tail_rows - 1) / a.tail_rows);
+    }
+    float L;
+    f32x4 y = merge_slots<WPR>(a, row, n0, a.prefix_splits, n1, wave % WPR, lane, L);
+    if (wave % WPR || lane >= 16) return;
+    y = finish_row(y, L);
     if (q.bad) {
         if (lane == 0) atomicOr(a.err, 2);
-        y = __builtin_nanf("");
-    } else if (q.len > 0) {
-        const int64_t per = q.prefix ? (int64_t)prefix_run_pages(a, q.prefix) * kPageRows : 1;
-        const int n0 = (int)((q.prefix + per - 1) / per);
-        const int n1 = (int)((q.len - q.prefix + a.tail_rows - 1) / a.tail_rows);
-        float M, L, A;
-        merge_slots(a.ws + (size_t)row * a.n_slots * kPartialStride, n0, a.prefix_splits, n1, lane, M, L, A);
-        y = finish_row(A, L);
+        const float nan = __builtin_nanf("");
+        y = f32x4{nan, nan, nan, nan};
     }
-    a.out[(size_t)row * kHeadDim + lane] = y;
+    *reinterpret_cast<f32x4*>(a.out + row * kHeadDim + 4 * lane) = y;
 }
 
 }  // namespace
@@ -1274,7 +1308,7 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     extern "C" __global__ __launch_bounds__(256) void tmac_append_##NAME(AppendArgs a) { append_body<T>(a); }          \
     extern "C" __global__ __launch_bounds__(256) void tmac_page_bounds_##NAME(BoundsArgs a) { bounds_body<T>(a); }     \
     extern "C" __global__ __launch_bounds__(256) void tmac_selected_##NAME(PagedAttnArgs a) { selected_body<T>(a); }   \
-    extern "C" __global__ __launch_bounds__(256, 2) void tmac_shared_##NAME(PagedAttnArgs a) { shared_body<T>(a); }
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_shared_##NAME(PagedAttnArgs a) { shared_body<T>(a); }
 TMAC_PAGED_KERNELS(f32, float)
 TMAC_PAGED_KERNELS(bf16, __bf16)
 TMAC_PAGED_KERNELS(f16, _Float16)
@@ -1291,5 +1325,12 @@ TMAC_SCORE_KERNEL(6)
 TMAC_SCORE_KERNEL(7)
 TMAC_SCORE_KERNEL(8)
 extern "C" __global__ __launch_bounds__(kSelectThreads) void tmac_select_pages(SelectArgs a) { select_body(a); }
-extern "C" __global__ __launch_bounds__(256) void tmac_selected_merge(PagedAttnArgs a) { selected_merge_body(a); }
-extern "C" __global__ __launch_bounds__(256) void tmac_shared_merge(PagedAttnArgs a) { shared_merge_body(a); }
+#define TMAC_MERGE_KERNELS(WPR)                                                                          \
+    extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_selected_merge_w##WPR(PagedAttnArgs a) { \
+        selected_merge_body<WPR>(a);                                                                     \
+    }                                                                                                    \
+    extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_shared_merge_w##WPR(PagedAttnArgs a) { \
+        shared_merge_body<WPR>(a);                                                                       \
+    }
+TMAC_MERGE_KERNELS(1)
+TMAC_MERGE_KERNELS(4)

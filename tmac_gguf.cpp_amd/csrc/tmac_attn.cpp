@@ -139,7 +139,7 @@ struct tmac_context {
                   k_cvt_q8 = nullptr;
     // serving operators on paged caches, by kv_dtype; page scores by query heads per pass - 1
     hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_shared[4] = {}, k_scores[8] = {};
-    hipFunction_t k_select = nullptr, k_selected_merge = nullptr, k_shared_merge = nullptr;
+    hipFunction_t k_select = nullptr, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
     float* ws = nullptr;
@@ -1067,8 +1067,10 @@ int tmac_init(tmac_context** out, int device) {
                 return bail(hip_fail(ctx, e, name));
         }
         if ((e = get_function(ctx, &ctx->k_select, "tmac_select_pages")) != hipSuccess ||
-            (e = get_function(ctx, &ctx->k_selected_merge, "tmac_selected_merge")) != hipSuccess ||
-            (e = get_function(ctx, &ctx->k_shared_merge, "tmac_shared_merge")) != hipSuccess)
+            (e = get_function(ctx, &ctx->k_selected_merge[0], "tmac_selected_merge_w1")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_selected_merge[1], "tmac_selected_merge_w4")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_shared_merge[0], "tmac_shared_merge_w1")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_shared_merge[1], "tmac_shared_merge_w4")) != hipSuccess)
             return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
     }
     if ((e = hipStreamCreateWithFlags(&ctx->aux, hipStreamNonBlocking)) != hipSuccess)
@@ -1611,7 +1613,7 @@ static int paged_attn_args(tmac_context* ctx, const char* what, int kv_dtype, co
         return rc;
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || (uintptr_t)lengths % 4)
         return fail(ctx, TMAC_ERR_MISALIGNED, std::string(what) + ": q, out and pools must be 16-byte aligned");
-    if ((rc = check_units(ctx, what, cdiv((int64_t)n_seq * n_head, tmac::kPagedWaves)))) return rc;
+    if ((rc = check_units(ctx, what, (int64_t)n_seq * n_head))) return rc;
     a->q = q;
     a->k_pages = static_cast<const char*>(k_pages);
     a->v_pages = static_cast<const char*>(v_pages);
@@ -1624,15 +1626,25 @@ static int paged_attn_args(tmac_context* ctx, const char* what, int kv_dtype, co
     a->n_seq = n_seq;
     a->n_head = n_head;
     a->n_kv_head = n_kv_head;
+    a->group = n_head / n_kv_head;
     a->qscale = kQScale;
     return TMAC_OK;
 }
 
 static int paged_partials(tmac_context* ctx, tmac_stream stream, PagedAttnArgs* a) {
-    const size_t floats = (size_t)a->n_seq * a->n_head * a->n_slots * kPartialStride;
+    const size_t floats = (size_t)a->n_seq * a->n_head * a->n_slots * (kHeadDim + 2);
     int rc = ensure_workspace(ctx, (hipStream_t)stream, floats);
     if (rc == TMAC_OK) a->ws = workspace(ctx);
     return rc;
+}
+
+// The merge of every row's partials: one wave a row up to kMergeWideSlots of them, four beyond.
+constexpr int kMergeWideSlots = 8;
+static int launch_paged_merge(tmac_context* ctx, tmac_stream stream, const hipFunction_t (&kernel)[2],
+                              PagedAttnArgs* a) {
+    const bool wide = a->n_slots > kMergeWideSlots;
+    return launch(ctx, kernel[wide], (unsigned)cdiv((int64_t)a->n_seq * a->n_head, wide ? 1 : tmac::kPagedWaves), 1,
+                  64 * tmac::kPagedWaves, (hipStream_t)stream, a);
 }
 
 int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
@@ -1661,8 +1673,7 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
                      (hipStream_t)stream, &a)) ||
         a.n_slots == 1)
         return rc;
-    return launch(ctx, ctx->k_selected_merge, (unsigned)cdiv((int64_t)n_seq * n_head, tmac::kPagedWaves), 1,
-                  64 * tmac::kPagedWaves, (hipStream_t)stream, &a);
+    return launch_paged_merge(ctx, stream, ctx->k_selected_merge, &a);
 }
 
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
@@ -1697,25 +1708,24 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     a.prefix_splits = 0;
     if (blocks) {
         const int64_t pages = cdiv(max_prefix, kPageRows);
-        const int64_t splits = std::min<int64_t>(cdiv(ctx->n_cu, blocks * n_kv_head), cdiv(pages, 2 * tmac::kPagedWaves));
+        const int64_t splits = std::min<int64_t>(ctx->n_cu / (blocks * n_kv_head), cdiv(pages, tmac::kSharedWaves));
         a.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
     }
     a.tail_rows = kPageRows;
     if (max_tail) {
         const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(2 * ctx->n_cu, n_sk), kMaxSplits));
         a.tail_rows = (int)std::max<int64_t>(cdiv(cdiv(max_tail, splits), kPageRows) * kPageRows,
-                                             kPageRows * tmac::kPagedWaves);
+                                             kPageRows * tmac::kSharedWaves);
         a.tail_splits = (int)cdiv(max_tail, a.tail_rows);
     }
     a.n_slots = a.prefix_splits + a.tail_splits;
     const int64_t units = blocks * n_kv_head * a.prefix_splits + n_sk * a.tail_splits;
     if ((rc = check_units(ctx, what, units)) || (rc = set_device(ctx))) return rc;
     if (a.n_slots && (rc = paged_partials(ctx, stream, &a))) return rc;
-    if (units && (rc = launch(ctx, ctx->k_shared[kv_dtype], (unsigned)units, 1, 64 * tmac::kPagedWaves,
+    if (units && (rc = launch(ctx, ctx->k_shared[kv_dtype], (unsigned)units, 1, 64 * tmac::kSharedWaves,
                               (hipStream_t)stream, &a)))
         return rc;
-    return launch(ctx, ctx->k_shared_merge, (unsigned)cdiv((int64_t)n_seq * n_head, tmac::kPagedWaves), 1,
-                  64 * tmac::kPagedWaves, (hipStream_t)stream, &a);
+    return launch_paged_merge(ctx, stream, ctx->k_shared_merge, &a);
 }
 
 int tmac_kv_convert(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* src, void* dst, int64_t n) {
