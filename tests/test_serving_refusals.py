@@ -155,9 +155,9 @@ def test_legal_edges(fake):
     assert fake.call("tmac_kv_append_paged", n_rows=0) == (TMAC_OK, [])
     assert fake.call("tmac_kv_page_bounds", max_new=0) == (TMAC_OK, [])
     assert ok("tmac_attention_decode_shared", n_groups=0, group_starts=None, prefix_lens=None)
-    # no rows possible: the merge alone writes the zero outputs
+    # no rows possible: the last launch alone writes the zero outputs
     rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=0, max_tail=0)
-    assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_shared_merge_w1"]
+    assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_tail_finish_f32"]
     # every list holds all pages: no scores
     rc, launches = fake.call("tmac_select_pages", top=40)
     assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_select_pages"]
@@ -193,5 +193,5 @@ def test_shared_grid_covers_every_grouping(fake):
         need = max(sum(-(-(b - a) * 7 // 64) for a, b in zip(c, c[1:])) for c in cuts)
         rc, launches = fake.call("tmac_attention_decode_shared", n_seq=n_seq, n_groups=n_groups, max_tail=0,
                                  max_prefix=16)
-        assert rc == TMAC_OK and launches[0][0] == "tmac_shared_f32"
-        assert launches[0][1] >= 2 * need  # 2 kv heads, one run
+        assert rc == TMAC_OK and launches[0] == ("tmac_prefix_f32", 1)  # one run
+        assert fake.lib.fake_launch_grid(0, 1) == 2 and fake.lib.fake_launch_grid(0, 2) >= need

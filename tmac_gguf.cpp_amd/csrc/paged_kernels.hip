@@ -1198,69 +1198,67 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
     put(col, 32 + d, M, L, B);
 }
 
-// Shared prefixes and own rows: the first prefix_blocks * n_kv_head *
-// prefix_splits workgroups take (64 columns of a group, kv head, run of its
-// prefix), the rest (own rows of a sequence, kv head, run).
+// Shared prefixes: workgroup (run of the prefix, kv head, block of 64 columns).
 template <typename T>
-__device__ __forceinline__ void shared_body(const PagedAttnArgs& a) {
-    __shared__ union {
-        PxLds<T> p;
-        MergeLds<kSharedWaves> t;
-    } lds;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv = a.n_kv_head, G = a.group;
-    const int n_prefix = a.prefix_blocks * kv * a.prefix_splits;
-    if ((int)blockIdx.x < n_prefix) {
-        const int split = blockIdx.x % a.prefix_splits, bh = blockIdx.x / a.prefix_splits, block = bh / kv,
-                  h = bh - block * kv;
-        // the group whose column blocks hold this one
-        Group grp = {0, 0, 0};
-        int left = block;
-        bool found = false;
-        for (int g0 = 0; g0 < a.n_groups && !found; g0 += 64) {
-            const Group g = group_at(a, g0 + lane);
-            const int nb = (int)(((int64_t)(g.end - g.first) * G + kSharedCols - 1) / kSharedCols);
-            int incl = nb;
-            for (int m = 1; m < min(64, a.n_groups - g0); m *= 2) {
-                const int o = __shfl_up(incl, m);
-                if (lane >= m) incl += o;
-            }
-            const uint64_t b = __ballot(incl > left);
-            const int at = b ? __builtin_ctzll(b) : 63;
-            if (b) {
-                grp.first = __builtin_amdgcn_readlane(g.first, at);
-                grp.end = __builtin_amdgcn_readlane(g.end, at);
-                grp.prefix = __builtin_amdgcn_readlane(g.prefix, at);
-                found = true;
-            }
-            left -= __builtin_amdgcn_readlane(found ? incl - nb : incl, at);
+__device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
+    __shared__ PxLds<T> lds;
+    const int lane = threadIdx.x & 63, G = a.group;
+    const int split = blockIdx.x, h = blockIdx.y;
+    // the group whose column blocks hold this one
+    Group grp = {0, 0, 0};
+    int left = blockIdx.z;
+    bool found = false;
+    for (int g0 = 0; g0 < a.n_groups && !found; g0 += 64) {
+        const Group g = group_at(a, g0 + lane);
+        const int nb = (int)(((int64_t)(g.end - g.first) * G + kSharedCols - 1) / kSharedCols);
+        int incl = nb;
+        for (int m = 1; m < min(64, a.n_groups - g0); m *= 2) {
+            const int o = __shfl_up(incl, m);
+            if (lane >= m) incl += o;
         }
-        const int64_t prefix = grp.prefix;
-        if (!found || prefix == 0 || prefix > a.max_prefix) return;
-        const int per = prefix_run_pages(a, prefix), j0 = split * per;
-        const int n = min(per, (int)((prefix + kPageRows - 1) >> kPageShift) - j0);
-        if (n <= 0) return;
-        const int c0 = left * kSharedCols;                 // this block's first column of the group
-        const int cols = (grp.end - grp.first) * G - c0;   // columns from there on
-        auto row_of = [&](int c) {
-            const int s = (c0 + c) / G;
-            return (int64_t)(grp.first + s) * a.n_head + h * G + (c0 + c - s * G);
-        };
-        px_run<T>(
-            a, lds.p, a.block_table + (size_t)grp.first * a.max_pages, h, j0, n, prefix, cols, threadIdx.x,
-            [&](int c) -> const float* { return c < cols ? a.q + row_of(c) * kHeadDim : nullptr; },
-            [&](int c, int d, float M, float L, f32x4 A) { put_partial(a, row_of(c), split, d, M, L, A); });
-    } else {
-        const int id = blockIdx.x - n_prefix;
-        const int split = id % a.tail_splits, sk = id / a.tail_splits, s = sk / kv, h = sk - s * kv;
-        const int64_t row0 = (int64_t)s * a.n_head + h * G;
-        const int col = lane & 15;
-        Cols st;
-        cols_init(st, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, a.qscale, lane);
-        const SharedSeq q = shared_seq(a, s, lane);
-        if (q.bad) return;
-        const int64_t lo = q.prefix + (int64_t)split * a.tail_rows, hi = min(q.len, lo + a.tail_rows);
-        if (lo >= hi) return;
+        const uint64_t b = __ballot(incl > left);
+        const int at = b ? __builtin_ctzll(b) : 63;
+        if (b) {
+            grp.first = __builtin_amdgcn_readlane(g.first, at);
+            grp.end = __builtin_amdgcn_readlane(g.end, at);
+            grp.prefix = __builtin_amdgcn_readlane(g.prefix, at);
+            found = true;
+        }
+        left -= __builtin_amdgcn_readlane(found ? incl - nb : incl, at);
+    }
+    const int64_t prefix = grp.prefix;
+    if (!found || prefix == 0 || prefix > a.max_prefix) return;
+    const int per = prefix_run_pages(a, prefix), j0 = split * per;
+    const int n = min(per, (int)((prefix + kPageRows - 1) >> kPageShift) - j0);
+    if (n <= 0) return;
+    const int c0 = left * kSharedCols;                // this block's first column of the group
+    const int cols = (grp.end - grp.first) * G - c0;  // columns from there on
+    auto row_of = [&](int c) {
+        const int s = (c0 + c) / G;
+        return (int64_t)(grp.first + s) * a.n_head + h * G + (c0 + c - s * G);
+    };
+    px_run<T>(
+        a, lds, a.block_table + (size_t)grp.first * a.max_pages, h, j0, n, prefix, cols, threadIdx.x,
+        [&](int c) -> const float* { return c < cols ? a.q + row_of(c) * kHeadDim : nullptr; },
+        [&](int c, int d, float M, float L, f32x4 A) { put_partial(a, row_of(c), split, d, M, L, A); });
+}
+
+// A sequence's own rows: workgroup (run of them, kv head, sequence).  FINISH:
+// one run holds them all, and the workgroup merges the prefix's partials and
+// writes the output; otherwise the run leaves one more partial.
+template <typename T, bool FINISH>
+__device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
+    __shared__ MergeLds<kSharedWaves> lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int G = a.group, split = FINISH ? 0 : blockIdx.x, h = blockIdx.y, s = blockIdx.z;
+    const int64_t row0 = (int64_t)s * a.n_head + h * G;
+    const int col = lane & 15;
+    Cols st;
+    cols_init(st, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, a.qscale, lane);
+    const SharedSeq q = shared_seq(a, s, lane);
+    const int64_t lo = q.prefix + (int64_t)split * a.tail_rows, hi = min(q.len, lo + a.tail_rows);
+    if (!FINISH && (q.bad || lo >= hi)) return;
+    if (!q.bad && lo < hi) {
         const int j0 = (int)(lo >> kPageShift), n = (int)((hi - 1) >> kPageShift) - j0 + 1;
         const int32_t* table = a.block_table + (size_t)s * a.max_pages;
         attend_run<T, kSharedWaves>(st, a, h, n, lo, hi, wave, lane, [&](int e, int& logical, int& page) {
@@ -1271,10 +1269,50 @@ __device__ __forceinline__ void shared_body(const PagedAttnArgs& a) {
                 page = min(max(page, 0), a.n_pages - 1);
             }
         });
-        merge_waves<kSharedWaves>(st, lds.t, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
-            if (c < G) put_partial(a, row0 + c, a.prefix_splits + split, d, M, L, A);
-        });
     }
+    merge_waves<kSharedWaves>(st, lds, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
+        if (c >= G) return;
+        if constexpr (FINISH) {
+            const int64_t per = (int64_t)prefix_run_pages(a, q.prefix) * kPageRows;
+            const int n = q.bad || q.len == 0 ? 0 : (int)((q.prefix + per - 1) / per);
+            const size_t at = (size_t)(row0 + c) * a.n_slots;
+            const float* acc = a.ws + at * kHeadDim + d;
+            const float2* ml =
+                reinterpret_cast<const float2*>(a.ws + (size_t)a.n_seq * a.n_head * a.n_slots * kHeadDim) + at;
+            for (int e0 = 0; e0 < n; e0 += 8) {  // eight partials at a time, their loads independent
+                float2 x[8];
+                f32x4 v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int e = min(e0 + u, n - 1);
+                    x[u] = ml[e];
+                    v[u] = *reinterpret_cast<const f32x4*>(acc + (size_t)e * kHeadDim);
+                }
+                float m1 = M;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) m1 = fmaxf(m1, x[u].x);
+                const float f = fast_exp2(M - m1);
+                L *= f;
+                A *= f;
+                M = m1;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float w = e0 + u < n ? fast_exp2(x[u].x - m1) : 0.f;
+                    L += w * x[u].y;
+                    A += w * v[u];
+                }
+            }
+            A = finish_row(A, L);
+            if (q.bad) {
+                if (c == 0 && d == 0) atomicOr(a.err, 2);
+                const float nan = __builtin_nanf("");
+                A = f32x4{nan, nan, nan, nan};
+            }
+            *reinterpret_cast<f32x4*>(a.out + (row0 + c) * kHeadDim + d) = A;
+        } else {
+            put_partial(a, row0 + c, a.prefix_splits + split, d, M, L, A);
+        }
+    });
 }
 
 template <int WPR>
@@ -1308,7 +1346,15 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     extern "C" __global__ __launch_bounds__(256) void tmac_append_##NAME(AppendArgs a) { append_body<T>(a); }          \
     extern "C" __global__ __launch_bounds__(256) void tmac_page_bounds_##NAME(BoundsArgs a) { bounds_body<T>(a); }     \
     extern "C" __global__ __launch_bounds__(256) void tmac_selected_##NAME(PagedAttnArgs a) { selected_body<T>(a); }   \
-    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_shared_##NAME(PagedAttnArgs a) { shared_body<T>(a); }
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_prefix_##NAME(PagedAttnArgs a) {               \
+        prefix_body<T>(a);                                                                                             \
+    }                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_tail_##NAME(PagedAttnArgs a) {                 \
+        tail_body<T, false>(a);                                                                                        \
+    }                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_tail_finish_##NAME(PagedAttnArgs a) {          \
+        tail_body<T, true>(a);                                                                                         \
+    }
 TMAC_PAGED_KERNELS(f32, float)
 TMAC_PAGED_KERNELS(bf16, __bf16)
 TMAC_PAGED_KERNELS(f16, _Float16)

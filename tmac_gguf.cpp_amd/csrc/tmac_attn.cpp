@@ -138,7 +138,8 @@ struct tmac_context {
     hipFunction_t k_rope = nullptr, k_copy = nullptr, k_pos = nullptr, k_qkv = nullptr, k_cvt16 = nullptr,
                   k_cvt_q8 = nullptr;
     // serving operators on paged caches, by kv_dtype; page scores by query heads per pass - 1
-    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_shared[4] = {}, k_scores[8] = {};
+    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_scores[8] = {};
+    hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[4] = {};  // shared prefixes, own rows
     hipFunction_t k_select = nullptr, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
@@ -1055,7 +1056,9 @@ int tmac_init(tmac_context** out, int device) {
             const std::pair<const char*, hipFunction_t*> by_type[] = {{"tmac_append", &ctx->k_append[dt]},
                                                                       {"tmac_page_bounds", &ctx->k_bounds[dt]},
                                                                       {"tmac_selected", &ctx->k_selected[dt]},
-                                                                      {"tmac_shared", &ctx->k_shared[dt]}};
+                                                                      {"tmac_prefix", &ctx->k_prefix[dt]},
+                                                                      {"tmac_tail", &ctx->k_tail[dt]},
+                                                                      {"tmac_tail_finish", &ctx->k_tail_finish[dt]}};
             for (auto& k : by_type) {
                 std::snprintf(name, sizeof(name), "%s_%s", k.first, kTypeName[dt]);
                 if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
@@ -1676,6 +1679,9 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
     return launch_paged_merge(ctx, stream, ctx->k_selected_merge, &a);
 }
 
+constexpr int kTailWholeRows = 256;  // own rows that one workgroup takes without help
+constexpr int kFinishSlots = 16;     // prefix partials that the own rows' workgroup merges itself
+constexpr int kMaxGridYZ = 65535;
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                  const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                  int max_pages, const int32_t* lengths, const int32_t* group_starts,
@@ -1711,19 +1717,33 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
         const int64_t splits = std::min<int64_t>(ctx->n_cu / (blocks * n_kv_head), cdiv(pages, tmac::kSharedWaves));
         a.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
     }
-    a.tail_rows = kPageRows;
-    if (max_tail) {
-        const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(2 * ctx->n_cu, n_sk), kMaxSplits));
+    // Own rows: one run a sequence where that fills half of the CUs or the rows are few, and then, with few prefix
+    // partials, its workgroup merges them and writes the output.
+    a.tail_rows = (int)std::max<int64_t>(kPageRows, cdiv(max_tail, kPageRows) * kPageRows);
+    if (2 * n_sk < ctx->n_cu && max_tail > kTailWholeRows) {
+        const int64_t splits = std::min<int64_t>(cdiv(ctx->n_cu, n_sk), kMaxSplits);
         a.tail_rows = (int)std::max<int64_t>(cdiv(cdiv(max_tail, splits), kPageRows) * kPageRows,
                                              kPageRows * tmac::kSharedWaves);
-        a.tail_splits = (int)cdiv(max_tail, a.tail_rows);
     }
-    a.n_slots = a.prefix_splits + a.tail_splits;
-    const int64_t units = blocks * n_kv_head * a.prefix_splits + n_sk * a.tail_splits;
-    if ((rc = check_units(ctx, what, units)) || (rc = set_device(ctx))) return rc;
+    a.tail_splits = (int)cdiv(max_tail, a.tail_rows);
+    const bool finish = a.tail_splits <= 1 && a.prefix_splits <= kFinishSlots;
+    a.n_slots = a.prefix_splits + (finish ? 0 : a.tail_splits);
+    if ((rc = check_units(ctx, what, blocks * n_kv_head * a.prefix_splits)) ||
+        (rc = check_units(ctx, what, n_sk * std::max(1, a.tail_splits))))
+        return rc;
+    if (n_kv_head > kMaxGridYZ || n_seq > kMaxGridYZ || blocks > kMaxGridYZ)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_shared: more than 65535 sequences or kv heads");
+    if ((rc = set_device(ctx))) return rc;
     if (a.n_slots && (rc = paged_partials(ctx, stream, &a))) return rc;
-    if (units && (rc = launch(ctx, ctx->k_shared[kv_dtype], (unsigned)units, 1, 64 * tmac::kSharedWaves,
-                              (hipStream_t)stream, &a)))
+    const unsigned threads = 64 * tmac::kSharedWaves;
+    if (blocks && (rc = launch(ctx, ctx->k_prefix[kv_dtype], (unsigned)a.prefix_splits, (unsigned)n_kv_head, threads,
+                               (hipStream_t)stream, &a, (unsigned)blocks)))
+        return rc;
+    if (finish)
+        return launch(ctx, ctx->k_tail_finish[kv_dtype], 1, (unsigned)n_kv_head, threads, (hipStream_t)stream, &a,
+                      (unsigned)n_seq);
+    if (a.tail_splits && (rc = launch(ctx, ctx->k_tail[kv_dtype], (unsigned)a.tail_splits, (unsigned)n_kv_head, threads,
+                                      (hipStream_t)stream, &a, (unsigned)n_seq)))
         return rc;
     return launch_paged_merge(ctx, stream, ctx->k_shared_merge, &a);
 }
