@@ -193,5 +193,5 @@ def test_shared_grid_covers_every_grouping(fake):
         need = max(sum(-(-(b - a) * 7 // 64) for a, b in zip(c, c[1:])) for c in cuts)
         rc, launches = fake.call("tmac_attention_decode_shared", n_seq=n_seq, n_groups=n_groups, max_tail=0,
                                  max_prefix=16)
-        assert rc == TMAC_OK and launches[0] == ("tmac_prefix_f32", 1)  # one run
-        assert fake.lib.fake_launch_grid(0, 1) == 2 and fake.lib.fake_launch_grid(0, 2) >= need
+        assert rc == TMAC_OK and launches[0][0] == "tmac_prefix_f32"
+        assert launches[0][1] >= 2 * need  # 2 kv heads, one run

@@ -333,228 +333,618 @@ __device__ __forceinline__ void select_body(const SelectArgs& a) {
 }
 
 // ---------------------------------------------------------------------------
-// Decode attention by (columns, kv head, run of pages) on fp32 MFMA
-// (v_mfma_f32_16x16x4_f32, products and sums of fp32: the cache rows are
-// widened exactly, so every cache type gets the fp32 result).  A tile is one
-// page, 16 keys x 16 columns; a column is a query head of one sequence.
-//   S^T (16 keys x 16 columns) = K (keys x dims) . Q^T.   Lane (i = l % 16,
-//     g = l / 16) holds key i's dims 32 m + 8 g + e of K and column i's of Q:
-//     step (m, e) contracts the four dims 32 m + 8 g + e, g = 0..3.
-//   P^T = exp2(S^T - m), online per column with a lazy maximum.
-//   O^T (64 dims x 16 columns) += V^T . P^T.  The accumulator S^T leaves keys
-//     4 g + r, r = 0..3, in lane group g, so step r contracts the keys 4 g + r
-//     straight from the same registers; row i of block b is dim 4 i + b, so
-//     lane (i, g) reads V of key 4 g + r as the four dims 4 i + 0..3.
-// No operand passes through LDS or another lane.
+// Decode attention, common parts.  A column is one query head of one sequence;
+// scores and sums are kept transposed, S^T (keys x columns) and O^T (dims x
+// columns), so that a lane owns columns and the softmax is lane-local but for a
+// rare exchange.
+//
+// bf16, fp16 and Q8_0 rows run on 16-bit MFMA, every fp32 operand carried by
+// 16-bit parts that together hold its 24 bits, so the result keeps fp32
+// accuracy:
+//   cache   K, V        q            P            products, Q.K and P.V
+//   bf16    exact       3 bf16       3 bf16       3, 3
+//   fp16    exact       2 fp16       2 fp16       2, 2
+//   Q8_0    int8 exact  2 fp16       3 bf16 x 2   2, 3 (scales on S and on P)
+//   fp32    3 bf16      3 bf16       3 bf16       6, 6 (parts i + j <= 2; the rest is below 2^-24)
+// (Two bf16 parts of P, 2^-18, left 2e-6 of the output's norm.)  fp32 rows are
+// split where many columns share them (prefixes) and go to fp32 MFMA where only
+// one group of query heads reads them.
 template <typename T>
-struct Tile {};
+struct Parts;
 template <>
-struct Tile<float> {
-    f32x4 k[4], v[4];
+struct Parts<__bf16> {
+    using KOps = MMath<__bf16>;
+    using VOps = MMath<__bf16>;
+    static constexpr int kCache = 1, kQ = 3, kP = 3, kSets = 1;
 };
 template <>
-struct Tile<__bf16> {
-    u32x4 k[2];
-    u32x2 v[4];
+struct Parts<_Float16> {
+    using KOps = MMath<_Float16>;
+    using VOps = MMath<_Float16>;
+    static constexpr int kCache = 1, kQ = 2, kP = 2, kSets = 1;
 };
 template <>
-struct Tile<_Float16> {
-    u32x4 k[2];
-    u32x2 v[4];
+struct Parts<q8_0_t> {
+    using KOps = MMath<_Float16>;
+    using VOps = MMath<__bf16>;
+    static constexpr int kCache = 1, kQ = 2, kP = 3, kSets = 2;
 };
 template <>
-struct Tile<q8_0_t> {
-    unsigned k[4], kd, v[4], vd[4];
+struct Parts<float> {
+    using KOps = MMath<__bf16>;
+    using VOps = MMath<__bf16>;
+    static constexpr int kCache = 3, kQ = 3, kP = 3, kSets = 1;
 };
 
-// kp / vp: row 0 of the page's head; stride: bytes between rows.
-template <typename T>
-__device__ __forceinline__ void tile_load(Tile<T>& t, const char* kp, const char* vp, int stride, int lane) {
-    const int i = lane & 15, g = lane >> 4;
-    const char* kr = kp + i * stride;
-    constexpr int DB = CacheFmt<T>::kDimBytes;
-    if constexpr (__is_same(T, float)) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            t.k[2 * m] = *reinterpret_cast<const f32x4*>(kr + (32 * m + 8 * g) * DB);
-            t.k[2 * m + 1] = *reinterpret_cast<const f32x4*>(kr + (32 * m + 8 * g + 4) * DB);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) t.v[r] = *reinterpret_cast<const f32x4*>(vp + (4 * g + r) * stride + 4 * i * DB);
-    } else if constexpr (__is_same(T, q8_0_t)) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            t.k[2 * m] = *reinterpret_cast<const unsigned*>(kr + 32 * m + 8 * g);
-            t.k[2 * m + 1] = *reinterpret_cast<const unsigned*>(kr + 32 * m + 8 * g + 4);
-        }
-        t.kd = *reinterpret_cast<const unsigned*>(kr + 64);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            t.v[r] = *reinterpret_cast<const unsigned*>(vp + (4 * g + r) * stride + 4 * i);
-            t.vd[r] = *reinterpret_cast<const unsigned*>(vp + (4 * g + r) * stride + 64);
-        }
+// Whether part i of one operand meets part j of the other.
+template <int NA, int NB>
+constexpr bool parts_meet(int i, int j) {
+    return NA == 1 || NB == 1 || i + j <= 2;
+}
+
+// (-1, 0) and (0, -1) as pairs of 16-bit values: a dot product with one of
+// them takes a half of a packed word from an fp32 value in one instruction,
+// exactly.  They are kept in registers: as immediates the compiler encodes them
+// for another operand width.  The other half is multiplied by 0, so a pair must
+// hold values whose NaN or infinity may spread to each other: q and P, whose
+// pairs end in the same score and the same sum, not V.
+struct NegPair {
+    unsigned lo, hi;
+    __device__ NegPair(unsigned minus_one) : lo(minus_one), hi(minus_one << 16) {
+        asm("" : "+s"(lo));
+        asm("" : "+s"(hi));
+    }
+};
+template <typename M>
+constexpr unsigned minus_one() {
+    return M::kScaleQ ? 0xBC00u : 0xBF80u;
+}
+
+// Three bf16 parts of two fp32 values (element 0 in the low half), cut bits: exact.
+__device__ __forceinline__ unsigned top_pair(float x, float y) {
+    return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+__device__ __forceinline__ void split3(float x, float y, unsigned (&w)[3]) {
+    auto top = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); };
+    w[0] = top_pair(x, y);
+    const float x1 = x - top(x), y1 = y - top(y);
+    w[1] = top_pair(x1, y1);
+    w[2] = top_pair(x1 - top(x1), y1 - top(y1));
+}
+// The same for a pair that may share its non-finite values; KP parts.  fp16: two parts, each the nearest.
+template <typename M, int KP>
+__device__ __forceinline__ void split(float x, float y, const NegPair& neg, unsigned (&w)[3]) {
+    if constexpr (M::kScaleQ) {
+        static_assert(KP == 2, "fp16: 22 bits in two parts");
+        w[0] = M::pack2(x, y);
+        const f16x2 v = __builtin_bit_cast(f16x2, w[0]);
+        w[1] = M::pack2(__builtin_amdgcn_fdot2(v, __builtin_bit_cast(f16x2, neg.lo), x, false),
+                        __builtin_amdgcn_fdot2(v, __builtin_bit_cast(f16x2, neg.hi), y, false));
     } else {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) t.k[m] = *reinterpret_cast<const u32x4*>(kr + (32 * m + 8 * g) * DB);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) t.v[r] = *reinterpret_cast<const u32x2*>(vp + (4 * g + r) * stride + 4 * i * DB);
+        for (int p = 0; p < KP; ++p) {
+            w[p] = top_pair(x, y);
+            const bf16x2 v = __builtin_bit_cast(bf16x2, w[p]);
+            if (p + 1 < KP) {
+                x = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, neg.lo), x, false);
+                y = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, neg.hi), y, false);
+            }
+        }
     }
-}
-
-template <typename T>
-__device__ __forceinline__ float half16(unsigned w, int e) {  // element e (0, 1) of a word of 16-bit values
-    if constexpr (__is_same(T, __bf16))
-        return __uint_as_float(e ? w & 0xFFFF0000u : w << 16);
-    else
-        return half_bits_to_float(e ? w >> 16 : w & 0xFFFFu);
-}
-
-// Element (m, e) of the K operand; element b of the V operand of step r.
-template <typename T>
-__device__ __forceinline__ float tile_k(const Tile<T>& t, int m, int e) {
-    if constexpr (__is_same(T, float))
-        return t.k[2 * m + e / 4][e % 4];
-    else if constexpr (__is_same(T, q8_0_t))
-        return (float)(signed char)(t.k[2 * m + e / 4] >> (8 * (e % 4))) *
-               half_bits_to_float(m ? t.kd >> 16 : t.kd & 0xFFFFu);
-    else
-        return half16<T>(t.k[m][e / 2], e % 2);
-}
-template <typename T>
-__device__ __forceinline__ float tile_v(const Tile<T>& t, int r, int b, int i) {
-    if constexpr (__is_same(T, float))
-        return t.v[r][b];
-    else if constexpr (__is_same(T, q8_0_t))
-        return (float)(signed char)(t.v[r] >> (8 * b)) * half_bits_to_float(i < 8 ? t.vd[r] & 0xFFFFu : t.vd[r] >> 16);
-    else
-        return half16<T>(t.v[r][b / 2], b % 2);
 }
 
 constexpr float kNoMax = -__FLT_MAX__;  // running maximum of a column that has met no key
 
-// One wave's state of a block of 16 columns.
-struct Cols {
-    float q[16];
-    f32x4 o[4];   // block b, row r: dim 16 g + 4 r + b
-    float m, l;   // m: the column's (equal in the four lane groups); l: this lane's keys
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// MFMA shapes.  Cols columns, lane groups g of Cols lanes; a product contracts
+// Depth values, 8 a lane group.  In an accumulator lane (column, g) holds rows
+// row(r) + 4 g, four in a run.
+struct Mfma16 {
+    static constexpr int kCols = 16, kDepth = 32, kAcc = 4;
+    using Acc = f32x4;
+    template <typename M>
+    __device__ static Acc mul(typename M::v8 a, typename M::v8 b, Acc c) { return M::mfma32(a, b, c); }
+    __device__ static float top(float x) { return max4_rows(x); }
+    __device__ static float sum(float x) { return sum4_rows(x); }
+};
+struct Mfma32 {
+    static constexpr int kCols = 32, kDepth = 16, kAcc = 16;
+    using Acc = f32x16;
+    template <typename M>
+    __device__ static Acc mul(typename M::v8 a, typename M::v8 b, Acc c) {
+        if constexpr (M::kScaleQ)
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    __device__ static float top(float x) { return xor_max<32>(x); }
+    __device__ static float sum(float x) { return xor_sum<32>(x); }
 };
 
-// One tile: keys lo .. hi - 1 of the page take part.
-template <typename T>
-__device__ __forceinline__ void attend_tile(Cols& st, const Tile<T>& t, int lo, int hi, int lane) {
-    const int i = lane & 15, g = lane >> 4;
-    const bool full = lo <= 0 && hi >= kPageRows;
-    f32x4 s = {0.f, 0.f, 0.f, 0.f}, s1 = s;  // two sums: a chain of 16 dependent products would wait on itself
+// One wave's columns on shape S.  Operand of q: depth block m, part p: lane
+// (column, g) the dims kDepth m + 8 g + 0..7.  Sums: dim block b of 64 / kCols.
+template <typename T, typename S>
+struct Cols {
+    static constexpr int kDepthBlocks = kHeadDim / S::kDepth, kDimBlocks = kHeadDim / S::kCols;
+    typename Parts<T>::KOps::v8 q[kDepthBlocks][Parts<T>::kQ];
+    typename S::Acc o[kDimBlocks];
+    float unscale;  // fp16 operands: undoes the column's power of two
+    float m, l;     // m: kNoMax until a key was met; l: this lane's keys
+    float base;     // what is subtracted from the scores: m, 0 before the first key
+};
+
+template <typename Acc>
+__device__ __forceinline__ Acc acc_of(float x) {
+    Acc a;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        s = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_k<T>(t, 0, e), st.q[e], s, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_k<T>(t, 1, e), st.q[8 + e], s1, 0, 0, 0);
-    }
-    s += s1;
-    if (!full) {
+    for (int r = 0; r < (int)(sizeof(Acc) / 4); ++r) a[r] = x;
+    return a;
+}
+
+// The raw query values of a lane (p null: an unused column), and empty columns made of them.
+template <typename T, typename S>
+struct RawQ {
+    f32x4 x[Cols<T, S>::kDepthBlocks][2];
+};
+template <typename T, typename S>
+__device__ __forceinline__ void load_q(RawQ<T, S>& r, const float* p, int lane) {
+    const int g = lane / S::kCols;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = 4 * g + r >= lo && 4 * g + r < hi ? s[r] : kNegInf;
-    }
-    const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    if (__any(top > st.m + kTau || st.m == kNoMax)) {
-        const float m1 = fmaxf(st.m, max4_rows(top));
-        const float w = fast_exp2(st.m - m1);
-        st.m = m1;
-        st.l *= w;
+    for (int m = 0; m < Cols<T, S>::kDepthBlocks; ++m)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) st.o[b] *= w;
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = fast_exp2(s[r] - st.m);
-    st.l += (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const bool in = full || (4 * g + r >= lo && 4 * g + r < hi);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const float vx = in ? tile_v<T>(t, r, b, i) : 0.f;  // a row outside may hold anything
-            st.o[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx, s[r], st.o[b], 0, 0, 0);
+        for (int i = 0; i < 2; ++i) {
+            r.x[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p) r.x[m][i] = *reinterpret_cast<const f32x4*>(p + S::kDepth * m + 8 * g + 4 * i);
         }
+}
+template <typename T, typename S>
+__device__ __forceinline__ void cols_init(Cols<T, S>& c, const RawQ<T, S>& raw, float scale) {
+    using KO = typename Parts<T>::KOps;
+    constexpr int MB = Cols<T, S>::kDepthBlocks;
+    const NegPair neg(minus_one<KO>());
+    float x[MB][8];
+    float top = 0.f;
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[m][e] = raw.x[m][e / 4][e % 4] * scale;
+            top = fmaxf(top, fabsf(x[m][e]));
+        }
+    c.unscale = 1.f;
+    if constexpr (KO::kScaleQ) {  // the column's largest value to [2^14, 2^15)
+        top = S::top(top);
+        const int e = min(max(14 - ((int)(__float_as_uint(top) >> 23) - 127), -126), 126);
+        const float up = __uint_as_float((unsigned)(127 + e) << 23);
+        c.unscale = __uint_as_float((unsigned)(127 - e) << 23);
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[m][i] *= up;
+    }
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+        u32x4 w[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unsigned y[3] = {0, 0, 0};
+            split<KO, Parts<T>::kQ>(x[m][2 * i], x[m][2 * i + 1], neg, y);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) w[k][i] = y[k];
+        }
+#pragma unroll
+        for (int k = 0; k < Parts<T>::kQ; ++k) c.q[m][k] = __builtin_bit_cast(typename KO::v8, w[k]);
+    }
+    c.m = kNoMax;
+    c.l = c.base = 0.f;
+#pragma unroll
+    for (int b = 0; b < Cols<T, S>::kDimBlocks; ++b) c.o[b] = acc_of<typename S::Acc>(0.f);
+}
+
+// Scores minus base of one tile of S::kCols keys.  key(m, p): the K operand,
+// depth block m, part p.  kd0 / kd1 (Q8_0): the keys' scales by dim half.
+// bf16 operands are summed onto -base.
+template <typename T, typename S, typename Key>
+__device__ __forceinline__ typename S::Acc score_tile(const Cols<T, S>& c, const float* kd0, const float* kd1, int g,
+                                                      Key key) {
+    using P = Parts<T>;
+    using KO = typename P::KOps;
+    constexpr bool Q8 = __is_same(T, q8_0_t), FROM_BASE = !Q8 && !KO::kScaleQ;
+    constexpr int MB = Cols<T, S>::kDepthBlocks;
+    typename S::Acc acc[2] = {acc_of<typename S::Acc>(FROM_BASE ? -c.base : 0.f), acc_of<typename S::Acc>(0.f)};
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int kp = 0; kp < P::kCache; ++kp) {
+            const auto kx = key(m, kp);
+#pragma unroll
+            for (int qp = 0; qp < P::kQ; ++qp)
+                if (parts_meet<P::kCache, P::kQ>(kp, qp)) {
+                    const int half = Q8 && 2 * m >= MB;
+                    acc[half] = S::template mul<KO>(kx, c.q[m][qp], acc[half]);
+                }
+        }
+    if constexpr (Q8) {
+#pragma unroll
+        for (int r4 = 0; r4 < S::kAcc / 4; ++r4) {
+            const f32x4 d0 = *reinterpret_cast<const f32x4*>(kd0 + 8 * r4 + 4 * g);
+            const f32x4 d1 = *reinterpret_cast<const f32x4*>(kd1 + 8 * r4 + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                acc[0][4 * r4 + r] = __builtin_fmaf(
+                    __builtin_fmaf(acc[1][4 * r4 + r], d1[r], acc[0][4 * r4 + r] * d0[r]), c.unscale, -c.base);
+        }
+    } else if constexpr (!FROM_BASE) {
+#pragma unroll
+        for (int r = 0; r < S::kAcc; ++r) acc[0][r] = __builtin_fmaf(acc[0][r], c.unscale, -c.base);
+    }
+    return acc[0];
+}
+
+// Scores minus base of NT tiles -> weights, online: the base is raised only
+// when a score exceeds it by more than kTau.
+template <typename S, int NB, int NT>
+__device__ __forceinline__ void softmax_step(float& m, float& l, float& base, typename S::Acc (&o)[NB],
+                                             typename S::Acc (&st)[NT]) {
+    // Whether any score is over the base by more than kTau, as integers: their order is that of the floats where it
+    // matters (above a positive bound), and a maximum of them needs no quieting of NaN.
+    int over = INT32_MIN;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < S::kAcc; ++r) over = max(over, (int)__float_as_uint(st[t][r]));
+    if (__any(over > (int)__float_as_uint(kTau) || m == kNoMax)) {
+        float top = kNegInf;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < S::kAcc; ++r) top = fmaxf(top, st[t][r]);
+        const float m1 = fmaxf(m, base + S::top(top));
+        const float b1 = m1 == kNoMax ? 0.f : m1, shift = b1 - base;
+        const float w = fast_exp2(m - m1);
+        m = m1;
+        base = b1;
+        l *= w;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] *= w;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) st[t] -= shift;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < S::kAcc; ++r) {
+            st[t][r] = fast_exp2(st[t][r]);
+            sum += st[t][r];
+        }
+        l += sum;
     }
 }
 
-// A run of tiles.  look(e, logical, page) gives entry e (0 <= e < n) its page of
+// 16-byte chunks of a 128-byte LDS row are XORed with the row, K by row & 7, V
+// by 2 row & 7, so that operand reads touch all banks.
+__device__ __forceinline__ int k_chunk(int row, int chunk) { return (chunk ^ (row & 7)) << 4; }
+__device__ __forceinline__ int v_chunk(int row, int chunk) { return (chunk ^ ((2 * row) & 7)) << 4; }
+
+// O^T += V^T . P^T over one product depth of keys.  w0, w1: four weights each of
+// the lane's keys r + 4 g and of those kDepth / 2 rows behind; v: the V image's
+// first row of the block (a multiple of 4 rows), part images part_bytes apart;
+// vd0 / vd1 (Q8_0): the keys' scales by dim half.  V is read back transposed:
+// with ds_read_b64_tr_b16 the 16 lanes of a group point at 4 rows x 32 bytes,
+// and each receives 4 consecutive keys of one dim.
+template <typename T, typename S>
+__device__ __forceinline__ void values_step(Cols<T, S>& c, f32x4 w0, f32x4 w1, char* v, int part_bytes,
+                                            const float* vd0, const float* vd1, const NegPair& neg, int lane) {
+    using P = Parts<T>;
+    using VO = typename P::VOps;
+    constexpr bool Q8 = __is_same(T, q8_0_t);
+    constexpr int kBack = S::kDepth / 2;
+    const int i = lane & 15, g = lane / S::kCols;
+    typename VO::v8 px[P::kSets][P::kP];
+#pragma unroll
+    for (int set = 0; set < P::kSets; ++set) {
+        u32x4 w[3];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            f32x4 x = half ? w1 : w0;
+            if constexpr (Q8)
+                x *= *reinterpret_cast<const f32x4*>((set ? vd1 : vd0) + kBack * half + 4 * g);
+            else if constexpr (VO::kPScale != 1.0f)
+                x *= VO::kPScale;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                unsigned z[3] = {0, 0, 0};
+                split<VO, P::kP>(x[2 * r], x[2 * r + 1], neg, z);
+#pragma unroll
+                for (int p = 0; p < P::kP; ++p) w[p][2 * half + r] = z[p];
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P::kP; ++p) px[set][p] = __builtin_bit_cast(typename VO::v8, w[p]);
+    }
+    const int sub = (lane / 16) % (S::kCols / 16);  // which 16 dims of a 32-dim block this lane's group reads
+#pragma unroll
+    for (int b = 0; b < Cols<T, S>::kDimBlocks; ++b)
+#pragma unroll
+        for (int vp = 0; vp < P::kCache; ++vp) {
+            const int r0 = 4 * g + (i >> 2), r1 = r0 + kBack;
+            const int chunk = S::kCols / 8 * b + 2 * sub + ((i & 3) >> 1);
+            char* p = v + vp * part_bytes + 8 * (i & 1);
+            const auto vx = VO::cat(VO::read_tr(p + r0 * 128 + v_chunk(r0, chunk)),
+                                    VO::read_tr(p + r1 * 128 + v_chunk(r1, chunk)));
+#pragma unroll
+            for (int pp = 0; pp < P::kP; ++pp)
+                if (parts_meet<P::kCache, P::kP>(vp, pp))
+                    c.o[b] = S::template mul<VO>(vx, px[P::kSets == 2 ? b * S::kCols / 32 : 0][pp], c.o[b]);
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Own rows: one group of query heads (up to 16 columns) over a run of pages,
+// which its wave alone reads.  What bounds it is the rows' bytes; a wave holds
+// one step of pages while the next is in flight.
+typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
+
+// 16-bit and Q8_0 rows: two pages a step, 32 keys.  K is read as the MFMA operand
+// it is, V through LDS (a buffer of the wave's own, no barrier), where it comes
+// back transposed.  fp32 MFMA on widened rows, 16 times the cycles for a
+// product, took 20.2 us for 64 x 128 bf16 pages of 2 kv heads, and a wave 1,000
+// cycles a page where it waits on its own products.
+template <typename T>
+struct Own {
+    using S = Mfma16;
+    using State = Cols<T, S>;
+    using RawQuery = RawQ<T, S>;
+    static constexpr int kTiles = 2;
+    static constexpr bool Q8 = __is_same(T, q8_0_t);
+    struct Tile {
+        u32x4 k[Q8 ? 1 : 2], v[Q8 ? 1 : 2];
+        unsigned kd, vd;  // Q8_0: the scale words of row lane % 16
+    };
+    struct Lds {
+        alignas(16) char v[32][128];
+        alignas(16) float kd[Q8 ? 2 : 1][Q8 ? 32 : 1], vd[Q8 ? 2 : 1][Q8 ? 32 : 1];
+    };
+    __device__ static void query(RawQuery& q, const float* p, int lane) { load_q<T, S>(q, p, lane); }
+    __device__ static void init(State& st, const RawQuery& q, float scale) { cols_init<T, S>(st, q, scale); }
+
+    // kp / vp: row 0 of the page's head; stride: bytes between rows.
+    __device__ static void fetch(Tile& t, const char* kp, const char* vp, int stride, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        if constexpr (Q8) {  // dims 8 g .. and 32 + 8 g .. of key i; 16 values of row lane / 4
+            const u32x2 a = *reinterpret_cast<const u32x2_a4*>(kp + i * stride + 8 * g);
+            const u32x2 b = *reinterpret_cast<const u32x2_a4*>(kp + i * stride + 32 + 8 * g);
+            t.k[0] = u32x4{a[0], a[1], b[0], b[1]};
+            t.kd = *reinterpret_cast<const unsigned*>(kp + i * stride + 64);
+            t.v[0] = *reinterpret_cast<const u32x4_a4*>(vp + (lane >> 2) * stride + 16 * (lane & 3));
+            t.vd = *reinterpret_cast<const unsigned*>(vp + i * stride + 64);
+        } else {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                t.k[m] = *reinterpret_cast<const u32x4*>(kp + i * stride + 64 * m + 16 * g);
+                t.v[m] = *reinterpret_cast<const u32x4*>(vp + (8 * m + (lane >> 3)) * stride + 16 * (lane & 7));
+            }
+        }
+    }
+    // Keys lo[u] .. hi[u] - 1 of page u take part.
+    __device__ static void attend(State& st, const Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles],
+                                  Lds& lds, const NegPair& neg, int lane) {
+        using KO = typename Parts<T>::KOps;
+        const int i = lane & 15, g = lane >> 4;
+        const u32x4 zero = {0, 0, 0, 0};
+        const bool full = lo[0] <= 0 && lo[1] <= 0 && hi[0] >= kPageRows && hi[1] >= kPageRows;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // a row outside may hold anything: zeros
+            auto in = [&](int r) { return full || (r >= lo[u] && r < hi[u]); };
+            if constexpr (Q8) {
+                const int r = lane >> 2, q = lane & 3, row = 16 * u + r;
+                const u32x4 v = in(r) ? t[u].v[0] : zero;
+                const u32x2 a = i8x4_to_bf16(v[0]), b = i8x4_to_bf16(v[1]), c = i8x4_to_bf16(v[2]),
+                            d = i8x4_to_bf16(v[3]);
+                *reinterpret_cast<u32x4*>(&lds.v[row][v_chunk(row, 2 * q)]) = u32x4{a[0], a[1], b[0], b[1]};
+                *reinterpret_cast<u32x4*>(&lds.v[row][v_chunk(row, 2 * q + 1)]) = u32x4{c[0], c[1], d[0], d[1]};
+                if (lane < 16) {
+                    const unsigned vd = in(i) ? t[u].vd : 0u;
+                    lds.kd[0][16 * u + i] = half_bits_to_float(t[u].kd & 0xFFFFu);
+                    lds.kd[1][16 * u + i] = half_bits_to_float(t[u].kd >> 16);
+                    lds.vd[0][16 * u + i] = half_bits_to_float(vd & 0xFFFFu);
+                    lds.vd[1][16 * u + i] = half_bits_to_float(vd >> 16);
+                }
+            } else {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const int r = 8 * m + (lane >> 3), row = 16 * u + r;
+                    *reinterpret_cast<u32x4*>(&lds.v[row][v_chunk(row, lane & 7)]) = in(r) ? t[u].v[m] : zero;
+                }
+            }
+        }
+        f32x4 w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            w[u] = score_tile<T, S>(st, &lds.kd[0][Q8 ? 16 * u : 0], &lds.kd[Q8 ? 1 : 0][Q8 ? 16 * u : 0], g,
+                                    [&](int m, int) {
+                                        if constexpr (Q8) {
+                                            const u32x2 a = i8x4_to_f16(t[u].k[0][2 * m]),
+                                                        b = i8x4_to_f16(t[u].k[0][2 * m + 1]);
+                                            return __builtin_bit_cast(typename KO::v8, u32x4{a[0], a[1], b[0], b[1]});
+                                        } else {
+                                            return __builtin_bit_cast(typename KO::v8, t[u].k[m]);
+                                        }
+                                    });
+        if (!full) {
+            asm volatile("");  // a branch, not selects
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[u][r] = 4 * g + r >= lo[u] && 4 * g + r < hi[u] ? w[u][r] : kNegInf;
+        }
+        softmax_step<S>(st.m, st.l, st.base, st.o, w);
+        values_step<T, S>(st, w[0], w[1], &lds.v[0][0], 0, lds.vd[0], lds.vd[Q8 ? 1 : 0], neg, lane);
+    }
+    // This lane's sums of column lane % 16, ready to merge: dims 16 b + 4 g + 0..3.
+    static constexpr int dim(int b, int g) { return 16 * b + 4 * g; }
+    __device__ static f32x4 sums(const State& st, int b) {
+        constexpr float k = Parts<T>::VOps::kPScale;
+        return k != 1.0f ? st.o[b] * (1.0f / k) : st.o[b];
+    }
+};
+
+// fp32 rows: one page a step on v_mfma_f32_16x16x4_f32, straight from registers.
+// Step (m, e) of K contracts the four dims 32 m + 8 g + e, g = 0..3.  The
+// accumulator S^T leaves keys 4 g + r in lane group g, so step r of V contracts
+// the keys 4 g + r from the same registers; row i of block b is dim 4 i + b, so
+// lane (i, g) reads V of key 4 g + r as the four dims 4 i + 0..3.
+template <>
+struct Own<float> {
+    using S = Mfma16;
+    static constexpr int kTiles = 1;
+    struct State {
+        float q[16];
+        f32x4 o[4];  // block b, row r: dim 16 g + 4 r + b
+        float m, l, base;
+    };
+    struct RawQuery {
+        f32x4 x[4];
+    };
+    struct Tile {
+        f32x4 k[4], v[4];
+    };
+    struct Lds {};
+    __device__ static void query(RawQuery& q, const float* p, int lane) {
+        const int g = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            q.x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p) q.x[j] = *reinterpret_cast<const f32x4*>(p + 32 * (j / 2) + 8 * g + 4 * (j % 2));
+        }
+    }
+    __device__ static void init(State& st, const RawQuery& q, float scale) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) st.q[j] = q.x[j / 4][j % 4] * scale;
+        st.m = kNoMax;
+        st.l = st.base = 0.f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) st.o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ static void fetch(Tile& t, const char* kp, const char* vp, int stride, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            t.k[j] = *reinterpret_cast<const f32x4*>(kp + i * stride + 128 * (j / 2) + 32 * g + 16 * (j % 2));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t.v[r] = *reinterpret_cast<const f32x4*>(vp + (4 * g + r) * stride + 16 * i);
+    }
+    __device__ static void attend(State& st, const Tile (&tiles)[1], const int (&lo)[1], const int (&hi)[1], Lds&,
+                                  const NegPair&, int lane) {
+        const Tile& t = tiles[0];
+        const int g = lane >> 4;
+        const bool full = lo[0] <= 0 && hi[0] >= kPageRows;
+        // two sums: a chain of 16 dependent products would wait on itself
+        f32x4 w[1] = {f32x4{-st.base, -st.base, -st.base, -st.base}}, w1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            w[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[e / 4][e % 4], st.q[e], w[0], 0, 0, 0);
+            w1 = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[2 + e / 4][e % 4], st.q[8 + e], w1, 0, 0, 0);
+        }
+        w[0] += w1;
+        auto in = [&](int r) { return full || (4 * g + r >= lo[0] && 4 * g + r < hi[0]); };
+        if (!full) {
+            asm volatile("");
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[0][r] = in(r) ? w[0][r] : kNegInf;
+        }
+        softmax_step<S>(st.m, st.l, st.base, st.o, w);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)  // a row outside may hold anything
+                st.o[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(in(r) ? t.v[r][b] : 0.f, w[0][r], st.o[b], 0, 0, 0);
+    }
+    static constexpr int dim(int b, int g) { return 16 * g + 4 * b; }
+    __device__ static f32x4 sums(const State& st, int b) { return f32x4{st.o[0][b], st.o[1][b], st.o[2][b], st.o[3][b]}; }
+};
+
+// LDS of a workgroup of NW waves on own rows: the waves' buffers, then the merge.
+template <int NW>
+struct MergeLds {
+    alignas(16) float o[NW][16][kHeadDim + 4];
+    float m[NW][16], l[NW][16];
+};
+template <typename T, int NW>
+union OwnLds {
+    typename Own<T>::Lds own[NW];
+    MergeLds<NW> merge;
+    __device__ OwnLds() {}
+};
+
+// A run of pages.  look(e, logical, page) gives entry e (0 <= e < n) its page of
 // the pool (checked, in range) and its logical page index (-1: skipped); rows
 // row_lo .. row_hi - 1 of the sequence take part.  The NW waves take the
-// entries in turn; a wave looks up 64 of its entries at a time, one a lane.
+// entries in turn, kTiles at once; a wave looks up 64 of its entries at a time,
+// one a lane.
 template <typename T, int NW, typename Look>
-__device__ __forceinline__ void attend_run(Cols& st, const PagedAttnArgs& a, int h, int n, int64_t row_lo,
-                                           int64_t row_hi, int wave, int lane, Look look) {
-    constexpr int HB = CacheFmt<T>::kHeadBytes;
+__device__ __forceinline__ void attend_run(typename Own<T>::State& st, const PagedAttnArgs& a, int h, int n,
+                                           int64_t row_lo, int64_t row_hi, typename Own<T>::Lds& lds, int wave,
+                                           int lane, Look look) {
+    using O = Own<T>;
+    constexpr int HB = CacheFmt<T>::kHeadBytes, KT = O::kTiles;
     const int stride = a.n_kv_head * HB;
     const size_t page_bytes = (size_t)kPageRows * stride;
-    const int mine = (n - wave + NW - 1) / NW;  // this wave's entries
-    for (int c0 = 0; c0 < mine; c0 += 64) {
-        const int cnt = min(64, mine - c0);
+    const NegPair neg(minus_one<typename Parts<T>::VOps>());
+    const int steps = ((n + KT - 1) / KT - wave + NW - 1) / NW;  // this wave's
+    for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
+        const int cnt = min(64 / KT, steps - s0);
         int logical = -1, page = 0;
-        if (lane < cnt) look((c0 + lane) * NW + wave, logical, page);
-        Tile<T> t[2];
-        auto fetch = [&](Tile<T>& x, int e) {
-            const size_t at = (size_t)__builtin_amdgcn_readlane(page, e) * page_bytes + (size_t)h * HB;
-            tile_load<T>(x, a.k_pages + at, a.v_pages + at, stride, lane);
+        const int e = ((s0 + lane / KT) * NW + wave) * KT + lane % KT;
+        if (lane < cnt * KT && e < n) look(e, logical, page);
+        typename O::Tile t[2][KT];
+        auto fetch = [&](typename O::Tile (&x)[KT], int step) {
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
+                const size_t at = (size_t)__builtin_amdgcn_readlane(page, KT * step + u) * page_bytes + (size_t)h * HB;
+                O::fetch(x[u], a.k_pages + at, a.v_pages + at, stride, lane);
+            }
         };
         fetch(t[0], 0);
-        for (int e = 0; e < cnt; e += 2) {
+        for (int step = 0; step < cnt; step += 2) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (e + u < cnt) {
-                    fetch(t[1 - u], min(e + u + 1, cnt - 1));
-                    const int j = __builtin_amdgcn_readlane(logical, e + u);
-                    const int64_t r0 = (int64_t)j * kPageRows;
-                    const int lo = (int)max((int64_t)0, min(row_lo - r0, (int64_t)kPageRows));
-                    const int hi = j < 0 ? 0 : (int)max((int64_t)0, min(row_hi - r0, (int64_t)kPageRows));
-                    if (hi > lo) attend_tile<T>(st, t[u], lo, hi, lane);
+            for (int d = 0; d < 2; ++d) {
+                if (step + d < cnt) {
+                    if (step + d + 1 < cnt) fetch(t[1 - d], step + d + 1);
+                    int lo[KT], hi[KT], any = 0;
+#pragma unroll
+                    for (int u = 0; u < KT; ++u) {
+                        const int j = __builtin_amdgcn_readlane(logical, KT * (step + d) + u);
+                        const int64_t r0 = (int64_t)j * kPageRows;
+                        lo[u] = (int)max((int64_t)0, min(row_lo - r0, (int64_t)kPageRows));
+                        hi[u] = j < 0 ? 0 : (int)max((int64_t)0, min(row_hi - r0, (int64_t)kPageRows));
+                        any |= hi[u] > lo[u];
+                    }
+                    if (any) O::attend(st, t[d], lo, hi, lds, neg, lane);
                 }
             }
         }
     }
 }
 
-// Empty columns with the query rows p (null: an unused column), scaled.
-__device__ __forceinline__ void cols_init(Cols& st, const float* p, float scale, int lane) {
-    const int g = lane >> 4;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (p) {
-            x = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g);
-            y = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g + 4);
-        }
-        float* o = st.q + 8 * m;
-        o[0] = x.x * scale; o[1] = x.y * scale; o[2] = x.z * scale; o[3] = x.w * scale;
-        o[4] = y.x * scale; o[5] = y.y * scale; o[6] = y.z * scale; o[7] = y.w * scale;
-    }
-    st.m = kNoMax;
-    st.l = 0.f;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) st.o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-}
-
 // Merges the NW waves through LDS and hands every column's maximum, sum and
 // four dims to put(column, first dim, m, l, acc): one call a thread of the first
 // 256 (16 columns x 16 dim quads).
-template <int NW>
-struct MergeLds {
-    alignas(16) float o[NW][16][kHeadDim + 4];
-    float m[NW][16], l[NW][16];
-};
-template <int NW, typename Put>
-__device__ __forceinline__ void merge_waves(Cols& st, MergeLds<NW>& lds, int wave, int lane, Put put) {
+template <typename T, int NW, typename Put>
+__device__ __forceinline__ void merge_waves(const typename Own<T>::State& st, MergeLds<NW>& lds, int wave, int lane,
+                                            Put put) {
     const int i = lane & 15, g = lane >> 4;
     const float l = sum4_rows(st.l);
+    __syncthreads();  // the buffers of all waves are done with
     if (g == 0) {
         lds.m[wave][i] = st.m;
         lds.l[wave][i] = l;
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<f32x4*>(&lds.o[wave][i][16 * g + 4 * r]) =
-            f32x4{st.o[0][r], st.o[1][r], st.o[2][r], st.o[3][r]};
+    for (int b = 0; b < 4; ++b) *reinterpret_cast<f32x4*>(&lds.o[wave][i][Own<T>::dim(b, g)]) = Own<T>::sums(st, b);
     __syncthreads();
     const int c = threadIdx.x >> 4, d = 4 * (threadIdx.x & 15);
     if (c >= 16) return;
@@ -590,7 +980,7 @@ __device__ __forceinline__ void put_partial(const PagedAttnArgs& a, int64_t row,
 template <typename T>
 __device__ __forceinline__ void selected_body(const PagedAttnArgs& a) {
     constexpr int NW = kPagedWaves;
-    __shared__ MergeLds<NW> lds;
+    __shared__ OwnLds<T, NW> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv = a.n_kv_head, G = a.group;
     const int split = blockIdx.x % a.n_slots, sk = blockIdx.x / a.n_slots, s = sk / kv, h = sk - s * kv;
@@ -600,9 +990,11 @@ __device__ __forceinline__ void selected_body(const PagedAttnArgs& a) {
     const int32_t* table = a.block_table + (size_t)s * a.max_pages;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
     const int col = lane & 15;
-    Cols st;
-    cols_init(st, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, a.qscale, lane);
-    attend_run<T, NW>(st, a, h, n, 0, len, wave, lane, [&](int e, int& logical, int& page) {
+    typename Own<T>::RawQuery raw;
+    typename Own<T>::State st;
+    Own<T>::query(raw, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, lane);
+    Own<T>::init(st, raw, a.qscale);
+    attend_run<T, NW>(st, a, h, n, 0, len, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
         const int j = list[e];
         if (j == -1) return;
         if (j < 0 || j >= a.max_pages) {
@@ -617,7 +1009,7 @@ __device__ __forceinline__ void selected_body(const PagedAttnArgs& a) {
         }
         logical = j;
     });
-    merge_waves<NW>(st, lds, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
+    merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         if (a.n_slots == 1)
             *reinterpret_cast<f32x4*>(a.out + (row0 + c) * kHeadDim + d) = finish_row(A, L);
@@ -729,65 +1121,27 @@ __device__ __forceinline__ int prefix_run_pages(const PagedAttnArgs& a, int64_t 
 }
 
 // ---------------------------------------------------------------------------
-// Shared prefix on 16-bit MFMA (v_mfma_f32_16x16x32).  A workgroup of 8 waves
-// takes 64 columns, (sequence, query head) pairs of one group and kv head, over
-// a run of the prefix: wave (kg, cw) the columns 32 cw .. 32 cw + 31 and, of
-// every stage, the keys of quarter kg.  What bounds it is the products: every fp32
-// operand is carried by 16-bit parts that together hold its 24 bits, so fp32
-// accuracy costs a multiple of the plain product,
-//   cache   K, V        q            P            products, Q.K and P.V
-//   bf16    exact       3 bf16       3 bf16       3, 3
-//   fp16    exact       2 fp16       2 fp16       2, 2
-//   Q8_0    int8 exact  2 fp16       3 bf16 x 2   2, 3 (scales on S and on P)
-//   fp32    3 bf16      3 bf16       3 bf16       6, 6 (parts i + j <= 2; the rest is below 2^-24)
-// against fp32 MFMA at 1/16 of the 16-bit rate.  (Two bf16 parts of P, 2^-18,
-// left 2e-6 of the output's norm.)
-//
+// Shared prefix.  A workgroup of 8 waves takes 64 columns, (sequence, query
+// head) pairs of one group and kv head, over a run of the prefix: wave (kg, cw)
+// the columns 32 cw .. 32 cw + 31 and, of every stage, the keys of quarter kg,
+// on v_mfma_f32_32x32x16.  What bounds it is the issue of products and of the
+// softmax beside them, about 3,000 cycles for a wave's 64 keys x 32 columns.
 // A stage's K and V rows go through registers (fetched one stage ahead) to LDS
-// once, converted there, and feed both column waves; V is read back transposed
-// (ds_read_b64_tr_b16).  16-byte chunks of a 128-byte LDS row are XORed with
-// the row, K by row & 7, V by 2 row & 7, so that both reads touch all banks.
+// once, converted there, and feed both column waves.
 template <typename T>
-struct Px;
-template <>
-struct Px<__bf16> {
-    using KOps = MMath<__bf16>;
-    using VOps = MMath<__bf16>;
-    static constexpr int kParts = 1, kQ = 3, kP = 3, kSets = 1, kKeys = 64;
-};
-template <>
-struct Px<_Float16> {
-    using KOps = MMath<_Float16>;
-    using VOps = MMath<_Float16>;
-    static constexpr int kParts = 1, kQ = 2, kP = 2, kSets = 1, kKeys = 64;
-};
-template <>
-struct Px<q8_0_t> {
-    using KOps = MMath<_Float16>;
-    using VOps = MMath<__bf16>;
-    static constexpr int kParts = 1, kQ = 2, kP = 3, kSets = 2, kKeys = 64;
-};
-template <>
-struct Px<float> {
-    using KOps = MMath<__bf16>;
-    using VOps = MMath<__bf16>;
-    static constexpr int kParts = 3, kQ = 3, kP = 3, kSets = 1, kKeys = 32;
-};
+constexpr int kPxKeys = __is_same(T, float) ? 32 : 64;  // keys a wave takes of a stage
+constexpr int kPxGroups = kSharedWaves / 2;             // key groups: quarters of a stage
 
-constexpr int kPxGroups = kSharedWaves / 2;  // key groups: quarters of a stage
-
-// One stage in LDS: rows of all key groups, `kParts` 16-bit images of K and V.
+// One stage in LDS: rows of all key groups, Parts::kCache 16-bit images of K and V.
 template <typename T>
 struct PxStage {
-    static constexpr int kRows = kPxGroups * Px<T>::kKeys;
-    alignas(16) char k[Px<T>::kParts][kRows][128];
-    alignas(16) char v[Px<T>::kParts][kRows][128];
-    alignas(16) float kd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];  // Q8_0 scales by dim half
-    alignas(16) float vd[__is_same(T, q8_0_t) ? 2 : 1][__is_same(T, q8_0_t) ? kRows : 1];
+    static constexpr int kRows = kPxGroups * kPxKeys<T>;
+    static constexpr bool Q8 = __is_same(T, q8_0_t);
+    alignas(16) char k[Parts<T>::kCache][kRows][128];
+    alignas(16) char v[Parts<T>::kCache][kRows][128];
+    alignas(16) float kd[Q8 ? 2 : 1][Q8 ? kRows : 1];  // Q8_0 scales by dim half
+    alignas(16) float vd[Q8 ? 2 : 1][Q8 ? kRows : 1];
 };
-
-__device__ __forceinline__ int px_k_at(int row, int chunk) { return (chunk ^ (row & 7)) << 4; }
-__device__ __forceinline__ int px_v_at(int row, int chunk) { return (chunk ^ ((2 * row) & 7)) << 4; }
 
 // This thread's share of a stage as fetched.
 template <typename T>
@@ -802,8 +1156,6 @@ struct PxGeom {
     static constexpr int kStep = 64 * kSharedWaves / kPerRow;                                              // rows per fetch
     static constexpr int kPages = PxStage<T>::kRows / kPageRows;                             // pages per stage
 };
-
-typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // Pool pages of a stage whose first page is logical page j0, as this wave
 // fetches them (scalar loads, issued a stage before the rows).
@@ -863,21 +1215,6 @@ __device__ __forceinline__ void px_fetch(PxRaw<T>& r, const PagedAttnArgs& a, in
     }
 }
 
-// Three bf16 parts of two fp32 values (element 0 in the low half), cut bits: exact.
-__device__ __forceinline__ void split3(float x, float y, unsigned (&w)[3]) {
-    auto top = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); };
-    auto pair = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); };
-    w[0] = pair(x, y);
-    const float x1 = x - top(x), y1 = y - top(y);
-    w[1] = pair(x1, y1);
-    w[2] = pair(x1 - top(x1), y1 - top(y1));
-}
-// Two fp16 parts (nearest, then the nearest to what is left).
-__device__ __forceinline__ void split2(float x, float y, unsigned (&w)[3]) {
-    w[0] = MMath<_Float16>::pack2(x, y);
-    w[1] = MMath<_Float16>::pack2(x - MMath<_Float16>::lo(w[0]), y - MMath<_Float16>::hi(w[0]));
-}
-
 // Rows at or past `valid` of the stage: V is written as zeros (P is 0 there, and the row may hold anything).
 template <typename T>
 __device__ __forceinline__ void px_store(PxStage<T>& s, const PxRaw<T>& r, int valid, int tid) {
@@ -896,20 +1233,20 @@ __device__ __forceinline__ void px_store(PxStage<T>& s, const PxRaw<T>& r, int v
             split3(__uint_as_float(v[2]), __uint_as_float(v[3]), v1);
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
-                *reinterpret_cast<u32x2*>(&s.k[p][row][px_k_at(row, q / 2) + half]) = u32x2{k0[p], k1[p]};
-                *reinterpret_cast<u32x2*>(&s.v[p][row][px_v_at(row, q / 2) + half]) = u32x2{v0[p], v1[p]};
+                *reinterpret_cast<u32x2*>(&s.k[p][row][k_chunk(row, q / 2) + half]) = u32x2{k0[p], k1[p]};
+                *reinterpret_cast<u32x2*>(&s.v[p][row][v_chunk(row, q / 2) + half]) = u32x2{v0[p], v1[p]};
             }
         } else if constexpr (__is_same(T, q8_0_t)) {  // 16 values: chunks 2 q, 2 q + 1
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const u32x2 ka = i8x4_to_f16(r.k[i][2 * c]), kb = i8x4_to_f16(r.k[i][2 * c + 1]);
                 const u32x2 va = i8x4_to_bf16(v[2 * c]), vb = i8x4_to_bf16(v[2 * c + 1]);
-                *reinterpret_cast<u32x4*>(&s.k[0][row][px_k_at(row, 2 * q + c)]) = u32x4{ka[0], ka[1], kb[0], kb[1]};
-                *reinterpret_cast<u32x4*>(&s.v[0][row][px_v_at(row, 2 * q + c)]) = u32x4{va[0], va[1], vb[0], vb[1]};
+                *reinterpret_cast<u32x4*>(&s.k[0][row][k_chunk(row, 2 * q + c)]) = u32x4{ka[0], ka[1], kb[0], kb[1]};
+                *reinterpret_cast<u32x4*>(&s.v[0][row][v_chunk(row, 2 * q + c)]) = u32x4{va[0], va[1], vb[0], vb[1]};
             }
         } else {
-            *reinterpret_cast<u32x4*>(&s.k[0][row][px_k_at(row, q)]) = r.k[i];
-            *reinterpret_cast<u32x4*>(&s.v[0][row][px_v_at(row, q)]) = v;
+            *reinterpret_cast<u32x4*>(&s.k[0][row][k_chunk(row, q)]) = r.k[i];
+            *reinterpret_cast<u32x4*>(&s.v[0][row][v_chunk(row, q)]) = v;
         }
     }
     if constexpr (__is_same(T, q8_0_t)) {
@@ -923,189 +1260,44 @@ __device__ __forceinline__ void px_store(PxStage<T>& s, const PxRaw<T>& r, int v
     }
 }
 
-// Whether part i of one operand meets part j of the other.
-template <int NA, int NB>
-constexpr bool px_pair(int i, int j) {
-    return NA == 1 || NB == 1 || i + j <= 2;
-}
-
-// One wave's columns.
+// The wave's keys of one stage (rows row0 .. row0 + kPxKeys - 1, of which `valid` take part).
 template <typename T>
-struct PxCols {
-    typename Px<T>::KOps::v8 q[2][2][Px<T>::kQ];  // [column block][dim half][part]
-    float unscale[2];                             // fp16 operands: undoes the column's power of two
-    f32x4 o[2][4];                                // block b, row r: dim 16 b + 4 g + r
-    float m[2], l[2];
-};
-
-template <typename T>
-__device__ __forceinline__ void px_load_q(PxCols<T>& c, int t, const float* p, float scale, int lane) {
-    using X = Px<T>;
-    const int g = lane >> 4;
-    float x[2][8];
-    float top = 0.f;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
-        if (p) {
-            u = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g);
-            w = *reinterpret_cast<const float4*>(p + 32 * m + 8 * g + 4);
-        }
-        const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            x[m][e] = y[e] * scale;
-            top = fmaxf(top, fabsf(x[m][e]));
-        }
-    }
-    c.unscale[t] = 1.f;
-    if constexpr (X::KOps::kScaleQ) {  // the column's largest value to [2^14, 2^15)
-        top = max4_rows(top);
-        const int e = min(max(14 - ((int)(__float_as_uint(top) >> 23) - 127), -126), 126);
-        const float up = __uint_as_float((unsigned)(127 + e) << 23);
-        c.unscale[t] = __uint_as_float((unsigned)(127 - e) << 23);
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[m][i] *= up;
-    }
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        u32x4 w[3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            unsigned y[3] = {0, 0, 0};
-            if constexpr (X::KOps::kScaleQ)
-                split2(x[m][2 * i], x[m][2 * i + 1], y);
-            else
-                split3(x[m][2 * i], x[m][2 * i + 1], y);
-#pragma unroll
-            for (int k = 0; k < 3; ++k) w[k][i] = y[k];
-        }
-#pragma unroll
-        for (int k = 0; k < X::kQ; ++k) c.q[t][m][k] = __builtin_bit_cast(typename X::KOps::v8, w[k]);
-    }
-}
-
-// The wave's keys of one stage (rows row0 .. row0 + kKeys - 1, of which `valid` take part).
-template <typename T>
-__device__ __forceinline__ void px_attend(PxCols<T>& c, PxStage<T>& s, int row0, int valid, int lane) {
-    using X = Px<T>;
-    using KO = typename X::KOps;
-    using VO = typename X::VOps;
-    constexpr int KT = X::kKeys / 16;  // 16-key tiles
-    constexpr bool Q8 = __is_same(T, q8_0_t);
-    const int i = lane & 15, g = lane >> 4;
-    f32x4 st[2][KT];
+__device__ __forceinline__ void px_attend(Cols<T, Mfma32>& c, PxStage<T>& s, int row0, int valid, const NegPair& neg,
+                                          int lane) {
+    using S = Mfma32;
+    using KO = typename Parts<T>::KOps;
+    constexpr bool Q8 = PxStage<T>::Q8;
+    constexpr int KT = kPxKeys<T> / 32;  // 32-key tiles
+    const int i = lane & 31, g = lane >> 5;
+    f32x16 st[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-        const int row = row0 + 16 * kt + i;
-        f32x4 acc[2][2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int kp = 0; kp < X::kParts; ++kp) {
-                const auto kx = *reinterpret_cast<const typename KO::v8*>(&s.k[kp][row][px_k_at(row, 4 * m + g)]);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int qp = 0; qp < X::kQ; ++qp)
-                        if (px_pair<X::kParts, X::kQ>(kp, qp))
-                            acc[t][Q8 ? m : 0] = KO::mfma32(kx, c.q[t][m][qp], acc[t][Q8 ? m : 0]);
-            }
-        if constexpr (Q8) {
-            const f32x4 d0 = *reinterpret_cast<const f32x4*>(&s.kd[0][row0 + 16 * kt + 4 * g]);
-            const f32x4 d1 = *reinterpret_cast<const f32x4*>(&s.kd[1][row0 + 16 * kt + 4 * g]);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) st[t][kt] = (acc[t][0] * d0 + acc[t][1] * d1) * c.unscale[t];
-        } else {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                st[t][kt] = acc[t][0];
-                if constexpr (KO::kScaleQ) st[t][kt] *= c.unscale[t];
-            }
-        }
+        const int first = row0 + 32 * kt, row = first + i;
+        st[kt] = score_tile<T, S>(c, &s.kd[0][Q8 ? first : 0], &s.kd[Q8 ? 1 : 0][Q8 ? first : 0], g,
+                                  [&](int m, int p) {
+                                      return *reinterpret_cast<const typename KO::v8*>(
+                                          &s.k[p][row][k_chunk(row, 2 * m + g)]);
+                                  });
     }
-    if (valid < X::kKeys) {
+    if (valid < kPxKeys<T>) {
         asm volatile("");  // a branch: as selects the masks would cost every stage 48 instructions
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) st[t][kt][r] = 16 * kt + 4 * g + r < valid ? st[t][kt][r] : kNegInf;
+            for (int r = 0; r < 16; ++r)
+                st[kt][r] = 32 * kt + 8 * (r / 4) + 4 * g + r % 4 < valid ? st[kt][r] : kNegInf;
     }
+    softmax_step<S>(c.m, c.l, c.base, c.o, st);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        float top = kNegInf;
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-            top = fmaxf(top, fmaxf(fmaxf(st[t][kt][0], st[t][kt][1]), fmaxf(st[t][kt][2], st[t][kt][3])));
-        if (__any(top > c.m[t] + kTau || c.m[t] == kNoMax)) {
-            const float m1 = fmaxf(c.m[t], max4_rows(top));
-            const float w = fast_exp2(c.m[t] - m1);
-            c.m[t] = m1;
-            c.l[t] *= w;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) c.o[t][b] *= w;
+        for (int h = 0; h < 2; ++h) {  // 16 keys at a time: the lane's weights 8 h + 0..3 and 8 h + 4..7
+            const int first = row0 + 32 * kt + 16 * h;
+            const f32x4 w0 = {st[kt][8 * h], st[kt][8 * h + 1], st[kt][8 * h + 2], st[kt][8 * h + 3]};
+            const f32x4 w1 = {st[kt][8 * h + 4], st[kt][8 * h + 5], st[kt][8 * h + 6], st[kt][8 * h + 7]};
+            values_step<T, S>(c, w0, w1, &s.v[0][first][0], sizeof(s.v[0]), &s.vd[0][Q8 ? first : 0],
+                              &s.vd[Q8 ? 1 : 0][Q8 ? first : 0], neg, lane);
         }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) st[t][kt][r] = fast_exp2(st[t][kt][r] - c.m[t]);
-            c.l[t] += (st[t][kt][0] + st[t][kt][1]) + (st[t][kt][2] + st[t][kt][3]);
-        }
-    }
-    // 32 keys at a time: slots 8 g + e hold key 4 g + e of the first tile (e < 4) and of the second
-#pragma unroll
-    for (int ks = 0; ks < KT / 2; ++ks) {
-        typename VO::v8 px[2][X::kSets][X::kP];
-#pragma unroll
-        for (int set = 0; set < X::kSets; ++set) {
-            u32x4 w[2][3];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                f32x4 d = {VO::kPScale, VO::kPScale, VO::kPScale, VO::kPScale};
-                if constexpr (Q8)
-                    d = *reinterpret_cast<const f32x4*>(&s.vd[set][row0 + 32 * ks + 16 * half + 4 * g]);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float x = st[t][2 * ks + half][2 * r], y = st[t][2 * ks + half][2 * r + 1];
-                        if constexpr (Q8 || VO::kPScale != 1.0f) x *= d[2 * r], y *= d[2 * r + 1];
-                        unsigned z[3] = {0, 0, 0};
-                        if constexpr (X::kP == 2)
-                            split2(x, y, z);
-                        else
-                            split3(x, y, z);
-#pragma unroll
-                        for (int p = 0; p < X::kP; ++p) w[t][p][2 * half + r] = z[p];
-                    }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int p = 0; p < X::kP; ++p) px[t][set][p] = __builtin_bit_cast(typename VO::v8, w[t][p]);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int vp = 0; vp < X::kParts; ++vp) {
-                const int r0 = row0 + 32 * ks + 4 * g + (i >> 2), r1 = r0 + 16, chunk = 2 * b + ((i & 3) >> 1);
-                const auto v0 = VO::read_tr(&s.v[vp][r0][px_v_at(r0, chunk) + 8 * (i & 1)]);
-                const auto v1 = VO::read_tr(&s.v[vp][r1][px_v_at(r1, chunk) + 8 * (i & 1)]);
-                const auto vx = VO::cat(v0, v1);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int p = 0; p < X::kP; ++p)
-                        if (px_pair<X::kParts, X::kP>(vp, p))
-                            c.o[t][b] = VO::mfma32(vx, px[t][X::kSets == 2 ? b / 2 : 0][p], c.o[t][b]);
-            }
-    }
 }
 
 // The key groups' columns through LDS.
@@ -1122,29 +1314,26 @@ union PxLds {
 template <typename T, typename ColPtr, typename Put>
 __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, const int32_t* table_, int h, int j0,
                                        int n_pages, int64_t rows, int n_cols, int tid, ColPtr col_ptr, Put put) {
-    using X = Px<T>;
     using G = PxGeom<T>;
     constexpr int NB = __is_same(T, float) ? 1 : 2;
     const const_i32_ptr table = (const_i32_ptr)table_;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave >> 1, cw = wave & 1;
-    const int i = lane & 15, g = lane >> 4;
+    const int i = lane & 31, g = lane >> 5;
     const int n_stage = (n_pages + G::kPages - 1) / G::kPages, j_last = j0 + n_pages - 1;
     const int n_rows = (int)min((int64_t)n_pages * kPageRows, rows - (int64_t)j0 * kPageRows);  // of this run
     const bool busy = 32 * cw < n_cols;
+    const NegPair neg(minus_one<typename Parts<T>::VOps>());
     unsigned bad = 0;
     PxRaw<T> raw;
     PxPages<T> pages;
+    Cols<T, Mfma32> c;
     px_pages<T>(pages, table, j0, j_last, wave);
-    px_fetch<T>(raw, a, h, pages, tid, bad);
-    px_pages<T>(pages, table, j0 + G::kPages, j_last, wave);
-    PxCols<T> c;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        px_load_q<T>(c, t, col_ptr(32 * cw + 16 * t + i), a.qscale, lane);
-        c.m[t] = kNoMax;
-        c.l[t] = 0.f;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) c.o[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    {
+        RawQ<T, Mfma32> q;
+        load_q<T, Mfma32>(q, col_ptr(32 * cw + i), lane);
+        px_fetch<T>(raw, a, h, pages, tid, bad);
+        px_pages<T>(pages, table, j0 + G::kPages, j_last, wave);
+        cols_init<T, Mfma32>(c, q, a.qscale);
     }
     px_store<T>(lds.stage[0], raw, n_rows, tid);
     __syncthreads();
@@ -1155,8 +1344,8 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
             px_fetch<T>(raw, a, h, pages, tid, bad);
             px_pages<T>(pages, table, j0 + (st + 2) * G::kPages, j_last, wave);
         }
-        const int valid = min(n_rows - st * PxStage<T>::kRows - kg * X::kKeys, X::kKeys);
-        if (busy && valid > 0) px_attend<T>(c, cur, kg * X::kKeys, valid, lane);
+        const int valid = min(n_rows - st * PxStage<T>::kRows - kg * kPxKeys<T>, kPxKeys<T>);
+        if (busy && valid > 0) px_attend<T>(c, cur, kg * kPxKeys<T>, valid, neg, lane);
         if (more) {
             if constexpr (NB == 1) __syncthreads();
             px_store<T>(lds.stage[NB == 2 ? (st + 1) & 1 : 0], raw, n_rows - (st + 1) * PxStage<T>::kRows, tid);
@@ -1164,20 +1353,20 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
         __syncthreads();
     }
     if (bad && lane == 0) atomicOr(a.err, 4);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int col = 32 * cw + 16 * t + i;
-        const float l = sum4_rows(c.l[t]);
+    {
+        const int col = 32 * cw + i;
+        const float l = Mfma32::sum(c.l);
         if (g == 0) {
-            lds.merge.m[kg][col] = c.m[t];
+            lds.merge.m[kg][col] = c.m;
             lds.merge.l[kg][col] = l;
         }
+        constexpr float k = 1.0f / Parts<T>::VOps::kPScale;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            f32x4 o = c.o[t][b];
-            if constexpr (X::VOps::kPScale != 1.0f) o *= 1.0f / X::VOps::kPScale;
-            *reinterpret_cast<f32x4*>(&lds.merge.o[kg][col][16 * b + 4 * g]) = o;
-        }
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                *reinterpret_cast<f32x4*>(&lds.merge.o[kg][col][32 * b + 8 * r4 + 4 * g]) =
+                    f32x4{c.o[b][4 * r4], c.o[b][4 * r4 + 1], c.o[b][4 * r4 + 2], c.o[b][4 * r4 + 3]} * k;
     }
     __syncthreads();
     // 8 threads a column, dims 4 d .. and 32 + 4 d ..
@@ -1199,14 +1388,20 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
 }
 
 // Shared prefixes: workgroup (run of the prefix, kv head, block of 64 columns).
+// Consecutive workgroups go to the eight XCDs in turn, and the blocks of a run
+// read the same rows: every XCD takes a contiguous eighth of the (run, kv head,
+// block) order, so that a row is read into one L2, or two, and not all eight.
 template <typename T>
 __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
     __shared__ PxLds<T> lds;
     const int lane = threadIdx.x & 63, G = a.group;
-    const int split = blockIdx.x, h = blockIdx.y;
+    const int n_units = a.prefix_splits * a.n_kv_head * a.prefix_blocks, per_xcd = gridDim.x / kXcds;
+    const int unit = (int)(blockIdx.x % kXcds) * per_xcd + (int)(blockIdx.x / kXcds);
+    if (unit >= n_units) return;
+    const int run = unit / a.prefix_blocks, h = run % a.n_kv_head, split = run / a.n_kv_head;
     // the group whose column blocks hold this one
     Group grp = {0, 0, 0};
-    int left = blockIdx.z;
+    int left = unit - run * a.prefix_blocks;
     bool found = false;
     for (int g0 = 0; g0 < a.n_groups && !found; g0 += 64) {
         const Group g = group_at(a, g0 + lane);
@@ -1248,20 +1443,22 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
 // writes the output; otherwise the run leaves one more partial.
 template <typename T, bool FINISH>
 __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
-    __shared__ MergeLds<kSharedWaves> lds;
+    __shared__ OwnLds<T, kSharedWaves> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.group, split = FINISH ? 0 : blockIdx.x, h = blockIdx.y, s = blockIdx.z;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
     const int col = lane & 15;
-    Cols st;
-    cols_init(st, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, a.qscale, lane);
+    typename Own<T>::RawQuery raw;
+    typename Own<T>::State st;
+    Own<T>::query(raw, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, lane);
     const SharedSeq q = shared_seq(a, s, lane);
+    Own<T>::init(st, raw, a.qscale);
     const int64_t lo = q.prefix + (int64_t)split * a.tail_rows, hi = min(q.len, lo + a.tail_rows);
     if (!FINISH && (q.bad || lo >= hi)) return;
     if (!q.bad && lo < hi) {
         const int j0 = (int)(lo >> kPageShift), n = (int)((hi - 1) >> kPageShift) - j0 + 1;
         const int32_t* table = a.block_table + (size_t)s * a.max_pages;
-        attend_run<T, kSharedWaves>(st, a, h, n, lo, hi, wave, lane, [&](int e, int& logical, int& page) {
+        attend_run<T, kSharedWaves>(st, a, h, n, lo, hi, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
             logical = j0 + e;
             page = table[logical];
             if (page < 0 || page >= a.n_pages) {
@@ -1270,7 +1467,7 @@ __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
             }
         });
     }
-    merge_waves<kSharedWaves>(st, lds, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
+    merge_waves<T, kSharedWaves>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         if constexpr (FINISH) {
             const int64_t per = (int64_t)prefix_run_pages(a, q.prefix) * kPageRows;

@@ -1728,16 +1728,17 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     a.tail_splits = (int)cdiv(max_tail, a.tail_rows);
     const bool finish = a.tail_splits <= 1 && a.prefix_splits <= kFinishSlots;
     a.n_slots = a.prefix_splits + (finish ? 0 : a.tail_splits);
-    if ((rc = check_units(ctx, what, blocks * n_kv_head * a.prefix_splits)) ||
+    if ((rc = check_units(ctx, what, blocks * n_kv_head * a.prefix_splits + tmac::kXcds)) ||
         (rc = check_units(ctx, what, n_sk * std::max(1, a.tail_splits))))
         return rc;
-    if (n_kv_head > kMaxGridYZ || n_seq > kMaxGridYZ || blocks > kMaxGridYZ)
+    if (n_kv_head > kMaxGridYZ || n_seq > kMaxGridYZ)
         return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_shared: more than 65535 sequences or kv heads");
     if ((rc = set_device(ctx))) return rc;
     if (a.n_slots && (rc = paged_partials(ctx, stream, &a))) return rc;
     const unsigned threads = 64 * tmac::kSharedWaves;
-    if (blocks && (rc = launch(ctx, ctx->k_prefix[kv_dtype], (unsigned)a.prefix_splits, (unsigned)n_kv_head, threads,
-                               (hipStream_t)stream, &a, (unsigned)blocks)))
+    const int64_t units = blocks * n_kv_head * a.prefix_splits;
+    if (blocks && (rc = launch(ctx, ctx->k_prefix[kv_dtype], (unsigned)(cdiv(units, tmac::kXcds) * tmac::kXcds), 1,
+                               threads, (hipStream_t)stream, &a)))
         return rc;
     if (finish)
         return launch(ctx, ctx->k_tail_finish[kv_dtype], 1, (unsigned)n_kv_head, threads, (hipStream_t)stream, &a,
