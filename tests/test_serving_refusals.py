@@ -160,7 +160,7 @@ def test_legal_edges(fake):
     assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_tail_finish_f32"]
     # every list holds all pages: no scores
     rc, launches = fake.call("tmac_select_pages", top=40)
-    assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_select_pages"]
+    assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_select_pages_256"]
 
 
 def test_growth_is_refused_while_capturing(fake):

@@ -229,11 +229,11 @@ struct SelectArgs {
     uint32_t* keys;          // workspace [n_seq][n_kv_head][key_stride]: order-preserving score bits
     int* err;
     int n_pages, max_pages, n_seq, n_head, n_kv_head;
+    int group;               // n_head / n_kv_head
     int max_len, key_stride;
     int top, first, last;
-    int chunks;              // score kernel: workgroups per (sequence, kv head)
 };
-constexpr int kScorePages = 128;  // score kernel: pages per workgroup
+constexpr int kScorePages = 64;  // score kernel: pages a workgroup scores at once
 
 // Decode attention by (sequence or group, kv head, run of pages): over the
 // pages of a list, or over shared prefixes and each sequence's own rows.

@@ -172,18 +172,16 @@ __device__ __forceinline__ void bounds_body(const BoundsArgs& a) {
 // group's query heads, of sum_d max(q_d hi_d, q_d lo_d): no key of the page
 // has a larger q . k.  The sum runs in 64 bits and is rounded once, so scores,
 // and with them the selection, do not depend on the order of the sum (up to
-// 2^-53).  max(q hi, q lo) is q times hi where q >= 0 and times lo elsewhere; a
-// bf16 value as a double has a low word of zero, so one bit select of the high
-// words picks the factor.
+// 2^-53).  max(q hi, q lo) = max(q, 0) hi + min(q, 0) lo, one of the products
+// zero, so a score is a product of length 128 and runs on v_mfma_f64_4x4x4:
+// four blocks of 4 pages x 4 heads x 4 dims in 16 cycles, where fp64 FMAs with
+// a select and a sum over lanes took 2.5 times as long (27 us for 64 sequences
+// of 2,048 pages at most, 2 kv heads, 7 heads each).
 //
-// Slot of 8 lanes = one page, 8 dims a lane; the queries' 8 dims of every head
-// stay in registers over the workgroup's kScorePages pages.
-__device__ __forceinline__ double slot_sum64(double x) {
-#pragma unroll
-    for (int m = 1; m < 8; m *= 2) x += __shfl_xor(x, m);
-    return x;
-}
-
+// Lane l holds for a step of 16 pages: of the bounds, page 4 p + l % 4 (p =
+// l / 4 % 4), dims 16 k .. 16 k + 15 (k = l / 16), product step t taking dim
+// 16 k + t of every k; of the queries, head 4 hg + l % 4; of the sums, page
+// 4 p + l / 16 and head 4 hg + l % 4.
 // fp32 -> unsigned of the same order; NaN as +infinity.
 __device__ __forceinline__ unsigned order_key(float x) {
     const unsigned u = x == x ? __float_as_uint(x) : 0x7F800000u;
@@ -195,140 +193,254 @@ __device__ __forceinline__ int select_pages_of(const SelectArgs& a, int s) {  //
     return len > a.max_len ? -1 : (len + kPageRows - 1) >> kPageShift;
 }
 
-template <int GT>
+__device__ __forceinline__ double bf16_to_f64(unsigned w, int e) {
+    return (double)__uint_as_float(e ? w & 0xFFFF0000u : w << 16);
+}
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_u(unsigned x) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);
+}
+
+// HG: groups of 4 query heads a pass takes.
+template <int HG>
 __device__ __forceinline__ void score_body(const SelectArgs& a) {
-    const int lane = threadIdx.x & 63, c = lane & 7, slot = threadIdx.x >> 3;
-    const int kv = a.n_kv_head, G = a.n_head / kv;
-    const int chunk = blockIdx.x % a.chunks, sk = blockIdx.x / a.chunks, s = sk / kv, h = sk - s * kv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kv = a.n_kv_head, G = a.group;
+    const int h = blockIdx.y, s = blockIdx.z, sk = s * kv + h;
     const int n = select_pages_of(a, s);
-    const int j0 = chunk * kScorePages, j1 = min(n, j0 + kScorePages);
-    if (n <= a.top || j0 >= j1) return;  // every page is taken, or none left
-    for (int g0 = 0; g0 < G; g0 += GT) {
-        double q[GT][8];
-        unsigned up[GT][8];  // all ones where the query value is not negative
+    const int first = (blockIdx.x * kPagedWaves + wave) * 16;  // this wave's pages: 16 from here on, then every `stride`
+    const int stride = gridDim.x * kPagedWaves * 16;
+    if (n <= a.top || first >= n) return;  // every page is taken, or none left
+    const int k = lane >> 4, p = (lane >> 2) & 3, i = lane & 3;
+    const int32_t* table = a.block_table + (size_t)s * a.max_pages;
+    unsigned* keys = a.keys + (size_t)sk * a.key_stride;
+    auto page_at = [&](int j0) {
+        const int j = min(j0 + 4 * p + i, n - 1), page = table[j];
+        // the first and last pages are taken whatever their bounds
+        if ((page < 0 || page >= a.n_pages) && k == 0 && j >= a.first && j < n - a.last) atomicOr(a.err, 4);
+        return min(max(page, 0), a.n_pages - 1);
+    };
+    u32x4 hi[2], lo[2];
+    auto fetch = [&](int page) {
+        const uint16_t* b = a.bounds + ((size_t)page * kv + h) * (kBoundsBytes / 2) + 16 * k;
 #pragma unroll
-        for (int g = 0; g < GT; ++g) {
-            float x[8];
-            const float* p = a.q + ((size_t)s * a.n_head + h * G + min(g0 + g, G - 1)) * kHeadDim + 8 * c;
-            const float4 u = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
-            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-            x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+        for (int u = 0; u < 2; ++u) {
+            hi[u] = *reinterpret_cast<const u32x4*>(b + 8 * u);
+            lo[u] = *reinterpret_cast<const u32x4*>(b + kHeadDim + 8 * u);
+        }
+    };
+    for (int g0 = 0; g0 < G; g0 += 4 * HG) {
+        int page = page_at(first);
+        fetch(page);
+        page = page_at(first + stride);
+        double up[HG][16], down[HG][16];
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                q[g][t] = (double)x[t];
-                up[g][t] = x[t] < 0.f ? 0u : ~0u;
+        for (int hg = 0; hg < HG; ++hg) {
+            const int head = g0 + 4 * hg + i;
+            const float* q = a.q + ((size_t)s * a.n_head + h * G + min(head, G - 1)) * kHeadDim + 16 * k;
+#pragma unroll
+            for (int t = 0; t < 16; t += 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(q + t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    up[hg][t + e] = x[e] > 0.f ? (double)x[e] : 0.0;
+                    down[hg][t + e] = x[e] < 0.f ? (double)x[e] : 0.0;
+                }
             }
         }
-        for (int j = j0 + slot; j < j1; j += 32) {
-            int page = a.block_table[(size_t)s * a.max_pages + j];
-            if (page < 0 || page >= a.n_pages) {
-                if (c == 0) atomicOr(a.err, 4);
-                page = min(max(page, 0), a.n_pages - 1);
+        for (int j0 = first; j0 < n; j0 += stride) {
+            const u32x4 vh[2] = {hi[0], hi[1]}, vl[2] = {lo[0], lo[1]};
+            if (j0 + stride < n) {
+                fetch(page);
+                page = page_at(j0 + 2 * stride);
             }
-            const uint16_t* b = a.bounds + ((size_t)page * kv + h) * (kBoundsBytes / 2) + 8 * c;
-            const u32x4 uh = *reinterpret_cast<const u32x4*>(b), ul = *reinterpret_cast<const u32x4*>(b + kHeadDim);
-            double sum[GT];
+            double sum[HG][2];  // two chains a head group
 #pragma unroll
-            for (int g = 0; g < GT; ++g) sum[g] = 0.0;
+            for (int hg = 0; hg < HG; ++hg) sum[hg][0] = sum[hg][1] = 0.0;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const unsigned hi = __double2hiint(__uint_as_float(t & 1 ? uh[t / 2] & 0xFFFF0000u : uh[t / 2] << 16));
-                const unsigned lo = __double2hiint(__uint_as_float(t & 1 ? ul[t / 2] & 0xFFFF0000u : ul[t / 2] << 16));
+            for (int t = 0; t < 16; ++t) {
+                const double x = bf16_to_f64(vh[t / 8][t % 8 / 2], t % 2), y = bf16_to_f64(vl[t / 8][t % 8 / 2], t % 2);
 #pragma unroll
-                for (int g = 0; g < GT; ++g) {
-                    const unsigned x = (hi & up[g][t]) | (lo & ~up[g][t]);
-                    sum[g] = __builtin_fma(q[g][t], __hiloint2double((int)x, 0), sum[g]);
+                for (int hg = 0; hg < HG; ++hg) {
+                    sum[hg][0] = __builtin_amdgcn_mfma_f64_4x4x4f64(x, up[hg][t], sum[hg][0], 0, 0, 0);
+                    sum[hg][1] = __builtin_amdgcn_mfma_f64_4x4x4f64(y, down[hg][t], sum[hg][1], 0, 0, 0);
                 }
             }
             unsigned best = 0;
 #pragma unroll
-            for (int g = 0; g < GT; ++g) best = max(best, order_key((float)slot_sum64(sum[g])));
-            if (c == 0) {
-                unsigned* key = a.keys + (size_t)sk * a.key_stride + j;
-                *key = g0 ? max(*key, best) : best;
-            }
+            for (int hg = 0; hg < HG; ++hg)
+                if (g0 + 4 * hg + i < G) best = max(best, order_key((float)(sum[hg][0] + sum[hg][1])));
+            best = max(best, dpp_u<0xB1>(best));
+            best = max(best, dpp_u<0x4E>(best));
+            const int j = j0 + 4 * p + k;
+            if (i == 0 && j < n) keys[j] = g0 ? max(keys[j], best) : best;
         }
     }
 }
 
-// The top pages of one (sequence, kv head), ascending.  Digit by digit from the
-// top, a histogram of the keys that agree with the digits found so far gives
-// the digit of the top-th largest key; then one pass in page order takes the
-// keys above it and the first of those equal to it.
-constexpr int kSelectThreads = 256;
-__device__ __forceinline__ unsigned key_of(const SelectArgs& a, const unsigned* keys, int j, int n) {
-    return j < a.first || j >= n - a.last ? 0xFFFFFFFFu : keys[j];
+// The top pages of one (sequence, kv head), ascending.  The top-th largest key
+// is found two bits at a time from the highest bit in which the keys differ:
+// three candidates are counted at once by ballots, and a count of exactly top
+// ends the search.  Then the keys above it and the first of those equal to it
+// are written in page order.  The keys stay in registers (the first kSelectRegs
+// a thread; longer sequences read the rest again).  What bounds it is the
+// latency of a count, a ballot a key, a barrier and a read of the waves' counts.
+constexpr int kSelectRegs = 8;
+
+// Maximum over a wave, and sum over each row of 16 lanes, without the LDS crossbar.
+__device__ __forceinline__ unsigned wave_max_u(unsigned x) {
+    x = max(x, dpp_u<0xB1>(x));
+    x = max(x, dpp_u<0x4E>(x));
+    x = max(x, dpp_u<0x141>(x));
+    x = max(x, dpp_u<0x128>(x));
+    const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((unsigned)p[0], (unsigned)p[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max((unsigned)q[0], (unsigned)q[1]);
+}
+__device__ __forceinline__ unsigned row_sum_u(unsigned x) {
+    x += dpp_u<0xB1>(x);
+    x += dpp_u<0x4E>(x);
+    x += dpp_u<0x141>(x);
+    return x + dpp_u<0x128>(x);
 }
 
+template <int NT>
 __device__ __forceinline__ void select_body(const SelectArgs& a) {
-    __shared__ unsigned s_hist[256];
-    __shared__ unsigned s_prefix, s_left;
-    __shared__ int s_gt[kSelectThreads / 64], s_eq[kSelectThreads / 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int NW = NT / 64;
+    static_assert(NW <= 16, "a row of lanes sums the waves' counts");
+    __shared__ unsigned s_count[2][3][16];  // by turn, candidate, wave
+    __shared__ unsigned s_range[2][16];
+    __shared__ unsigned s_scan[kSelectRegs * NW];  // by round, wave: pages above the threshold << 16 | pages equal to it
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sk = blockIdx.x, s = sk / a.n_kv_head;
     const int n = select_pages_of(a, s);
     int32_t* out = a.selected + (size_t)sk * a.top;
     if (n < 0 && tid == 0) atomicOr(a.err, 2);
     if (n <= a.top) {
-        for (int i = tid; i < a.top; i += kSelectThreads) out[i] = i < n ? i : -1;
+        for (int i = tid; i < a.top; i += NT) out[i] = i < n ? i : -1;
         return;
     }
     const unsigned* keys = a.keys + (size_t)sk * a.key_stride;
-    unsigned prefix = 0, left = (unsigned)a.top;  // keys still to take among those that agree with prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        s_hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < n; j += kSelectThreads) {
-            const unsigned k = key_of(a, keys, j, n);
-            if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[k >> shift & 255], 1u);
-        }
-        __syncthreads();
-        if (tid < 64) {  // lane l: digits 255 - 4 l .. 252 - 4 l, from the top
-            unsigned cnt[4], sum = 0;
+    const int rounds = (n + NT - 1) / NT, held = min(rounds, kSelectRegs);
+    // Key of page j: forced pages above every score (a score's key is at most that of +infinity), none below.
+    auto key_at = [&](int j) {
+        const unsigned k = j < n ? keys[j] : 0u;
+        return j >= n ? 0u : j < a.first || j >= n - a.last ? 0xFFFFFFFFu : k;
+    };
+    unsigned k[kSelectRegs];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum += cnt[i] = s_hist[255 - 4 * lane - i];
-            unsigned incl = sum;
+    for (int r = 0; r < kSelectRegs; ++r) k[r] = r < held ? key_at(r * NT + tid) : 0u;
+    if (tid < 96) s_count[tid / 48][tid / 16 % 3][tid % 16] = 0;
+    // The highest bit in which the scored keys differ (as the largest key and the largest complement of one).
+    unsigned hi = 0u, nlo = 0u;
+    auto range = [&](unsigned x) {
+        if (x && x != 0xFFFFFFFFu) hi = max(hi, x), nlo = max(nlo, ~x);
+    };
 #pragma unroll
-            for (int m = 1; m < 64; m *= 2) {
-                const unsigned o = __shfl_up(incl, m);
-                if (lane >= m) incl += o;
+    for (int r = 0; r < kSelectRegs; ++r) range(k[r]);
+    for (int r = kSelectRegs; r < rounds; ++r) range(key_at(r * NT + tid));
+    hi = wave_max_u(hi);
+    nlo = wave_max_u(nlo);
+    if (lane == 0) s_range[0][wave] = hi, s_range[1][wave] = nlo;
+    __syncthreads();
+    hi = wave_max_u(s_range[0][lane % NW]);
+    const unsigned lo = ~wave_max_u(s_range[1][lane % NW]);
+    // n > top >= first + last, so there are scored keys; the top-th largest key is one of them or, with top = first +
+    // last, the threshold stays above them all.
+    const unsigned top = (unsigned)a.top;
+    unsigned prefix;  // no fewer than top keys are >= prefix; in the end the top-th largest key, or all >= are taken
+    if (a.first + a.last == a.top) {
+        prefix = 0xFFFFFFFFu;
+    } else {
+        int bits = lo == hi ? 0 : 32 - __builtin_clz(lo ^ hi);
+        bits = (bits + 1) & ~1;
+        prefix = bits >= 32 ? 0u : lo >> bits << bits;
+        prefix = __builtin_amdgcn_readfirstlane(prefix);
+        bits = __builtin_amdgcn_readfirstlane(bits);
+        for (int turn = 0; bits > 0; turn ^= 1) {
+            bits -= 2;
+            unsigned c[3] = {0, 0, 0};
+            auto count = [&](unsigned x) {
+#pragma unroll
+                for (int d = 0; d < 3; ++d) c[d] += __popcll(__ballot(x >= (prefix | (unsigned)(d + 1) << bits)));
+            };
+#pragma unroll
+            for (int r = 0; r < kSelectRegs; ++r)
+                if (r < held) count(k[r]);
+            for (int r = kSelectRegs; r < rounds; ++r) count(key_at(r * NT + tid));
+            if (lane == 0) {
+#pragma unroll
+                for (int d = 0; d < 3; ++d) s_count[turn][d][wave] = c[d];
             }
-            unsigned above = incl - sum;
-            if (above < left && incl >= left) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (above < left && above + cnt[i] >= left) {
-                        s_prefix = prefix | (unsigned)(255 - 4 * lane - i) << shift;
-                        s_left = left - above;
-                    }
-                    above += cnt[i];
-                }
-            }
+            __syncthreads();
+            const unsigned t = row_sum_u(s_count[turn][min(lane / 16, 2)][lane % 16]);
+            const unsigned t0 = __builtin_amdgcn_readlane(t, 0), t1 = __builtin_amdgcn_readlane(t, 16),
+                           t2 = __builtin_amdgcn_readlane(t, 32);
+            const int d = t2 >= top ? 3 : t1 >= top ? 2 : t0 >= top ? 1 : 0;
+            prefix |= (unsigned)d << bits;
+            if ((d == 3 ? t2 : d == 2 ? t1 : d == 1 ? t0 : 0) == top) break;  // exactly the keys >= prefix
         }
-        __syncthreads();
-        prefix = s_prefix;
-        left = s_left;
     }
-    int n_gt = 0, n_eq = 0;  // taken so far, equal keys seen so far
-    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
-        const int j = j0 + tid;
-        const unsigned k = j < n ? key_of(a, keys, j, n) : 0;
-        const bool gt = j < n && k > prefix, eq = j < n && k == prefix;
-        const uint64_t bg = __ballot(gt), be = __ballot(eq), below = (1ull << lane) - 1;
+    // Taken: keys > prefix, then the first of those equal to it, as many as are left.  (After an exact end the equal
+    // ones are just those.)  Of the held rounds every wave leaves its counts; a scan over (round, wave) places them.
+    int places[kSelectRegs];  // this thread's pages before it in its wave and round: above << 16 | equal
+#pragma unroll
+    for (int r = 0; r < kSelectRegs; ++r) {
+        if (r >= held) break;
+        const uint64_t bg = __ballot(k[r] > prefix), be = __ballot(k[r] == prefix), below = (1ull << lane) - 1;
+        places[r] = __popcll(bg & below) << 16 | __popcll(be & below);
+        if (lane == 0) s_scan[r * NW + wave] = (unsigned)__popcll(bg) << 16 | (unsigned)__popcll(be);
+    }
+    __syncthreads();
+    // entries 2 lane, 2 lane + 1 of the scan (NW * kSelectRegs <= 128)
+    const unsigned e0 = 2 * lane < held * NW ? s_scan[2 * lane] : 0u;
+    const unsigned e1 = 2 * lane + 1 < held * NW ? s_scan[2 * lane + 1] : 0u;
+    unsigned incl = e0 + e1;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        const unsigned o = __shfl_up(incl, m);
+        if (lane >= m) incl += o;
+    }
+    const unsigned all = __builtin_amdgcn_readlane(incl, 63), before = incl - e0 - e1;
+    // keys above the threshold: those of the rounds that are not held count too
+    unsigned above = all >> 16;
+    if (rounds > kSelectRegs) {
+        unsigned more = 0;
+        for (int r = kSelectRegs; r < rounds; ++r) more += __popcll(__ballot(key_at(r * NT + tid) > prefix));
+        if (lane == 0) s_count[0][0][wave] = more;
         __syncthreads();
-        if (lane == 0) {
-            s_gt[wave] = __popcll(bg);
-            s_eq[wave] = __popcll(be);
-        }
+        above += __builtin_amdgcn_readlane(row_sum_u(s_count[0][0][lane % 16]), 0);
+    }
+    const int left = (int)(top - above);
+    auto place = [&](unsigned x, int j, int g, int e) {
+        if (j < n && (x > prefix || (x == prefix && e < left))) out[g + min(e, left)] = j;
+    };
+#pragma unroll
+    for (int r = 0; r < kSelectRegs; ++r) {
+        if (r >= held) break;
+        const int at = r * NW + wave;
+        const unsigned b = __builtin_amdgcn_readlane(before, at / 2) + (at % 2 ? __builtin_amdgcn_readlane(e0, at / 2) : 0u);
+        const unsigned p = b + (unsigned)places[r];
+        place(k[r], r * NT + tid, (int)(p >> 16), (int)(p & 0xFFFFu));
+    }
+    int b_gt = (int)(all >> 16), b_eq = (int)(all & 0xFFFFu);  // pages before a round that is not held
+    for (int r = kSelectRegs; r < rounds; ++r) {
+        const unsigned x = key_at(r * NT + tid);
+        const uint64_t bg = __ballot(x > prefix), be = __ballot(x == prefix), below = (1ull << lane) - 1;
         __syncthreads();
-        int g = n_gt, e = n_eq;  // before this thread's page
-        for (int w = 0; w < kSelectThreads / 64; ++w) {
-            if (w < wave) g += s_gt[w], e += s_eq[w];
-            n_gt += s_gt[w], n_eq += s_eq[w];
+        if (lane == 0) s_scan[wave] = (unsigned)__popcll(bg) << 16 | (unsigned)__popcll(be);
+        __syncthreads();
+        unsigned b = 0, sum = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            if (w < wave) b += s_scan[w];
+            sum += s_scan[w];
         }
-        g += __popcll(bg & below);
-        e += __popcll(be & below);
-        if (gt || (eq && e < (int)left)) out[g + min(e, (int)left)] = j;
+        place(x, r * NT + tid, b_gt + (int)(b >> 16) + __popcll(bg & below), b_eq + (int)(b & 0xFFFFu) + __popcll(be & below));
+        b_gt += (int)(sum >> 16);
+        b_eq += (int)(sum & 0xFFFFu);
     }
 }
 
@@ -1557,17 +1669,10 @@ TMAC_PAGED_KERNELS(bf16, __bf16)
 TMAC_PAGED_KERNELS(f16, _Float16)
 TMAC_PAGED_KERNELS(q8, q8_0_t)
 
-#define TMAC_SCORE_KERNEL(GT) \
-    extern "C" __global__ __launch_bounds__(256) void tmac_page_scores_g##GT(SelectArgs a) { score_body<GT>(a); }
-TMAC_SCORE_KERNEL(1)
-TMAC_SCORE_KERNEL(2)
-TMAC_SCORE_KERNEL(3)
-TMAC_SCORE_KERNEL(4)
-TMAC_SCORE_KERNEL(5)
-TMAC_SCORE_KERNEL(6)
-TMAC_SCORE_KERNEL(7)
-TMAC_SCORE_KERNEL(8)
-extern "C" __global__ __launch_bounds__(kSelectThreads) void tmac_select_pages(SelectArgs a) { select_body(a); }
+extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_page_scores_h4(SelectArgs a) { score_body<1>(a); }
+extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_page_scores_h8(SelectArgs a) { score_body<2>(a); }
+extern "C" __global__ __launch_bounds__(256) void tmac_select_pages_256(SelectArgs a) { select_body<256>(a); }
+extern "C" __global__ __launch_bounds__(1024) void tmac_select_pages_1024(SelectArgs a) { select_body<1024>(a); }
 #define TMAC_MERGE_KERNELS(WPR)                                                                          \
     extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_selected_merge_w##WPR(PagedAttnArgs a) { \
         selected_merge_body<WPR>(a);                                                                     \

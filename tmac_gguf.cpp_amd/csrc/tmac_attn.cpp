@@ -137,10 +137,10 @@ struct tmac_context {
     hipFunction_t any_combine[3] = {};
     hipFunction_t k_rope = nullptr, k_copy = nullptr, k_pos = nullptr, k_qkv = nullptr, k_cvt16 = nullptr,
                   k_cvt_q8 = nullptr;
-    // serving operators on paged caches, by kv_dtype; page scores by query heads per pass - 1
-    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_scores[8] = {};
+    // serving operators on paged caches, by kv_dtype; page scores: up to 4 query heads per kv head, more
+    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_scores[2] = {};
     hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[4] = {};  // shared prefixes, own rows
-    hipFunction_t k_select = nullptr, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
+    hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
     float* ws = nullptr;
@@ -1064,12 +1064,11 @@ int tmac_init(tmac_context** out, int device) {
                 if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
             }
         }
-        for (int g = 1; g <= 8; g++) {
-            std::snprintf(name, sizeof(name), "tmac_page_scores_g%d", g);
-            if ((e = get_function(ctx, &ctx->k_scores[g - 1], name)) != hipSuccess)
-                return bail(hip_fail(ctx, e, name));
-        }
-        if ((e = get_function(ctx, &ctx->k_select, "tmac_select_pages")) != hipSuccess ||
+        if ((e = get_function(ctx, &ctx->k_scores[0], "tmac_page_scores_h4")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_scores[1], "tmac_page_scores_h8")) != hipSuccess)
+            return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
+        if ((e = get_function(ctx, &ctx->k_select[0], "tmac_select_pages_256")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_select[1], "tmac_select_pages_1024")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_selected_merge[0], "tmac_selected_merge_w1")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_selected_merge[1], "tmac_selected_merge_w4")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_shared_merge[0], "tmac_shared_merge_w1")) != hipSuccess ||
@@ -1553,6 +1552,8 @@ int tmac_kv_page_bounds(tmac_context* ctx, tmac_stream stream, int kv_dtype, con
     return launch(ctx, ctx->k_bounds[kv_dtype], (unsigned)blocks, 1, 64 * tmac::kPagedWaves, (hipStream_t)stream, &a);
 }
 
+constexpr int kMaxGridYZ = 65535;
+constexpr int kSelectWidePages = 512;  // pages per list from which 1024 threads select
 int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, const void* bounds, int n_pages,
                       const int32_t* block_table, int max_pages, const int32_t* lengths, int32_t* selected, int n_seq,
                       int n_head, int n_kv_head, int head_dim, int max_len, int top, int first, int last) {
@@ -1572,8 +1573,10 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
         return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: need top >= 1, first, last >= 0, first + last <= top");
     if (n_seq == 0) return TMAC_OK;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head, pages = cdiv(max_len, kPageRows);
-    const int64_t chunks = cdiv(pages, tmac::kScorePages);
-    if ((rc = check_units(ctx, what, n_sk * chunks)) || (rc = set_device(ctx))) return rc;
+    if ((rc = check_units(ctx, what, n_sk * cdiv(pages, tmac::kScorePages)))) return rc;
+    if (n_kv_head > kMaxGridYZ || n_seq > kMaxGridYZ)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: more than 65535 sequences or kv heads");
+    if ((rc = set_device(ctx))) return rc;
     SelectArgs a{};
     a.q = q;
     a.bounds = static_cast<const uint16_t*>(bounds);
@@ -1586,21 +1589,25 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
     a.n_seq = n_seq;
     a.n_head = n_head;
     a.n_kv_head = n_kv_head;
+    a.group = n_head / n_kv_head;
     a.max_len = max_len;
     a.key_stride = (int)pages;
     a.top = top;
     a.first = first;
     a.last = last;
-    a.chunks = (int)chunks;
     if (pages > top) {  // otherwise every list holds all of its sequence's pages
         if ((rc = ensure_workspace(ctx, (hipStream_t)stream, (size_t)(n_sk * pages)))) return rc;
         a.keys = reinterpret_cast<uint32_t*>(workspace(ctx));
-        const int group = n_head / n_kv_head, passes = group > 8 ? 2 : 1;
-        if ((rc = launch(ctx, ctx->k_scores[cdiv(group, passes) - 1], (unsigned)(n_sk * chunks), 1, 256,
-                         (hipStream_t)stream, &a)))
+        // Workgroups per (sequence, kv head), which take its pages in turn: two per CU in all, so that few sequences
+        // fill the card and many do not load their queries more often than they must.
+        const int64_t groups =
+            std::min<int64_t>(cdiv(pages, tmac::kScorePages), std::max<int64_t>(1, cdiv(2 * ctx->n_cu, n_sk)));
+        if ((rc = launch(ctx, ctx->k_scores[a.group > 4], (unsigned)groups, (unsigned)n_kv_head, 64 * tmac::kPagedWaves,
+                         (hipStream_t)stream, &a, (unsigned)n_seq)))
             return rc;
     }
-    return launch(ctx, ctx->k_select, (unsigned)n_sk, 1, 256, (hipStream_t)stream, &a);
+    const bool wide = pages > kSelectWidePages;
+    return launch(ctx, ctx->k_select[wide], (unsigned)n_sk, 1, wide ? 1024 : 256, (hipStream_t)stream, &a);
 }
 
 // Checks and arguments that both attentions over paged caches share.
@@ -1681,7 +1688,6 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
 
 constexpr int kTailWholeRows = 256;  // own rows that one workgroup takes without help
 constexpr int kFinishSlots = 16;     // prefix partials that the own rows' workgroup merges itself
-constexpr int kMaxGridYZ = 65535;
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                  const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                  int max_pages, const int32_t* lengths, const int32_t* group_starts,
