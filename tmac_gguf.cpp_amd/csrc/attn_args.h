@@ -232,8 +232,9 @@ struct SelectArgs {
     int group;               // n_head / n_kv_head
     int max_len, key_stride;
     int top, first, last;
+    int dealt;               // score kernel: 1: all sequences' steps are dealt out evenly (at most kScoreSeqs)
 };
-constexpr int kScorePages = 64;  // score kernel: pages a workgroup scores at once
+constexpr int kScoreSeqs = 256;
 
 // Decode attention by (sequence or group, kv head, run of pages): over the
 // pages of a list, or over shared prefixes and each sequence's own rows.

@@ -1553,7 +1553,7 @@ int tmac_kv_page_bounds(tmac_context* ctx, tmac_stream stream, int kv_dtype, con
 }
 
 constexpr int kMaxGridYZ = 65535;
-constexpr int kSelectWidePages = 512;  // pages per list from which 1024 threads select
+constexpr int kSelectWidePages = 2048;  // pages that 256 threads hold in registers; beyond, 1024 threads select
 int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, const void* bounds, int n_pages,
                       const int32_t* block_table, int max_pages, const int32_t* lengths, int32_t* selected, int n_seq,
                       int n_head, int n_kv_head, int head_dim, int max_len, int top, int first, int last) {
@@ -1573,9 +1573,8 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
         return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: need top >= 1, first, last >= 0, first + last <= top");
     if (n_seq == 0) return TMAC_OK;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head, pages = cdiv(max_len, kPageRows);
-    if ((rc = check_units(ctx, what, n_sk * cdiv(pages, tmac::kScorePages)))) return rc;
-    if (n_kv_head > kMaxGridYZ || n_seq > kMaxGridYZ)
-        return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: more than 65535 sequences or kv heads");
+    if ((rc = check_units(ctx, what, n_sk * cdiv(pages, 16)))) return rc;
+    if (n_seq > kMaxGridYZ) return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: more than 65535 sequences");
     if ((rc = set_device(ctx))) return rc;
     SelectArgs a{};
     a.q = q;
@@ -1598,12 +1597,13 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
     if (pages > top) {  // otherwise every list holds all of its sequence's pages
         if ((rc = ensure_workspace(ctx, (hipStream_t)stream, (size_t)(n_sk * pages)))) return rc;
         a.keys = reinterpret_cast<uint32_t*>(workspace(ctx));
-        // Workgroups per (sequence, kv head), which take its pages in turn: two per CU in all, so that few sequences
-        // fill the card and many do not load their queries more often than they must.
-        const int64_t groups =
-            std::min<int64_t>(cdiv(pages, tmac::kScorePages), std::max<int64_t>(1, cdiv(2 * ctx->n_cu, n_sk)));
-        if ((rc = launch(ctx, ctx->k_scores[a.group > 4], (unsigned)groups, (unsigned)n_kv_head, 64 * tmac::kPagedWaves,
-                         (hipStream_t)stream, &a, (unsigned)n_seq)))
+        // Steps of 16 pages.  Where there are more than waves that fit the card, they are dealt out evenly (with more
+        // than kScoreSeqs sequences, whose lengths a wave does not read at once, every sequence has waves of its own).
+        const int64_t steps = cdiv(pages, 16), room = 2 * ctx->n_cu * tmac::kPagedWaves;
+        a.dealt = n_seq <= tmac::kScoreSeqs && n_sk * steps > room;
+        const int64_t waves = a.dealt ? room : n_kv_head * std::min<int64_t>(steps, cdiv(room, n_sk));
+        if ((rc = launch(ctx, ctx->k_scores[a.group > 4], (unsigned)cdiv(waves, tmac::kPagedWaves),
+                         a.dealt ? 1u : (unsigned)n_seq, 64 * tmac::kPagedWaves, (hipStream_t)stream, &a)))
             return rc;
     }
     const bool wide = pages > kSelectWidePages;
