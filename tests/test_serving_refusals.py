@@ -185,13 +185,14 @@ def test_bounds_grid_covers_every_start_in_a_page(fake):
         assert grid == -(-new // 16)
 
 
-def test_shared_grid_covers_every_grouping(fake):
-    """The column blocks of any grouping fit the launch's prefix workgroups."""
-    for n_seq, n_groups in ((1, 1), (9, 1), (10, 1), (30, 2), (30, 30), (200, 7)):
+def test_shared_grid(fake):
+    """The prefix kernel's workgroups share the units of any grouping: a multiple of the eight dies, no more than one
+    per CU (256) and, where every grouping has fewer units, no more than those."""
+    for n_seq, n_groups in ((1, 1), (9, 1), (10, 1), (30, 2), (30, 30), (200, 7), (2000, 1)):
         cuts = [[i * n_seq // n_groups for i in range(n_groups + 1)], [0] * n_groups + [n_seq],
                 list(range(n_groups)) + [n_seq], [0] + [n_seq - n_groups + i for i in range(1, n_groups + 1)]]
         need = max(sum(-(-(b - a) * 7 // 64) for a, b in zip(c, c[1:])) for c in cuts)
         rc, launches = fake.call("tmac_attention_decode_shared", n_seq=n_seq, n_groups=n_groups, max_tail=0,
                                  max_prefix=16)
         assert rc == TMAC_OK and launches[0][0] == "tmac_prefix_f32"
-        assert launches[0][1] >= 2 * need  # 2 kv heads, one run
+        assert launches[0][1] % 8 == 0 and min(2 * need, 256) <= launches[0][1] <= 256  # 2 kv heads, one run

@@ -262,8 +262,8 @@ struct PagedAttnArgs {
     int prefix_blocks;       // blocks of kSharedCols (sequence, query head) columns, at most
     int tail_splits, tail_rows;  // slots behind them: runs of tail_rows own rows
 };
-constexpr int kPagedWaves = 4;    // waves per workgroup: bounds, list, merges
-constexpr int kSharedWaves = 8;   // shared prefixes and own rows
+constexpr int kPagedWaves = 4;    // waves per workgroup
+constexpr int kSharedWaves = 8;   // the same, shared prefixes
 constexpr int kMaxGroupHeads = 16;  // query heads per kv head, at most (MFMA columns)
 constexpr int kXcds = 8;          // dies that workgroups are dealt to in turn, each with an L2 of its own
 constexpr int kSharedCols = 64;   // prefix workgroup: (sequence, query head) columns

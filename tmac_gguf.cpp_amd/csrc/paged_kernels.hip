@@ -1571,55 +1571,69 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
     put(col, 32 + d, M, L, B);
 }
 
-// Shared prefixes: workgroup (run of the prefix, kv head, block of 64 columns).
+// Shared prefixes: a unit is (run of the prefix, kv head, block of 64 columns).
 // Consecutive workgroups go to the eight XCDs in turn, and the blocks of a run
 // read the same rows: every XCD takes a contiguous eighth of the (run, kv head,
 // block) order, so that a row is read into one L2, or two, and not all eight.
+// How many blocks there are follows from the groups; a workgroup takes further
+// units where there are more than the grid.  None starts for nothing: one that
+// finds no work still waits for a CU with 100 KB of LDS to be free, and 160 of
+// them behind 240 others took 10 us.
 template <typename T>
 __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
     __shared__ PxLds<T> lds;
     const int lane = threadIdx.x & 63, G = a.group;
-    const int n_units = a.prefix_splits * a.n_kv_head * a.prefix_blocks, per_xcd = gridDim.x / kXcds;
-    const int unit = (int)(blockIdx.x % kXcds) * per_xcd + (int)(blockIdx.x / kXcds);
-    if (unit >= n_units) return;
-    const int run = unit / a.prefix_blocks, h = run % a.n_kv_head, split = run / a.n_kv_head;
-    // the group whose column blocks hold this one
-    Group grp = {0, 0, 0};
-    int left = unit - run * a.prefix_blocks;
-    bool found = false;
-    for (int g0 = 0; g0 < a.n_groups && !found; g0 += 64) {
-        const Group g = group_at(a, g0 + lane);
-        const int nb = (int)(((int64_t)(g.end - g.first) * G + kSharedCols - 1) / kSharedCols);
-        int incl = nb;
-        for (int m = 1; m < min(64, a.n_groups - g0); m *= 2) {
-            const int o = __shfl_up(incl, m);
-            if (lane >= m) incl += o;
+    // The blocks there are: 64 groups at a time, one a lane, their blocks summed.
+    auto blocks_of = [&](const Group& g) { return (int)(((int64_t)(g.end - g.first) * G + kSharedCols - 1) / kSharedCols); };
+    const Group first64 = group_at(a, lane);
+    const int incl64 = wave_scan(blocks_of(first64), lane);
+    int n_blocks = __builtin_amdgcn_readlane(incl64, 63);
+    for (int g0 = 64; g0 < a.n_groups; g0 += 64)
+        n_blocks += __builtin_amdgcn_readlane(wave_scan(blocks_of(group_at(a, g0 + lane)), lane), 63);
+    n_blocks = min(n_blocks, a.prefix_blocks);
+    const int n_units = a.prefix_splits * a.n_kv_head * n_blocks, per_xcd = (n_units + kXcds - 1) / kXcds;
+    for (int at_xcd = (int)(blockIdx.x / kXcds); at_xcd < per_xcd; at_xcd += (int)(gridDim.x / kXcds)) {
+        const int unit = (int)(blockIdx.x % kXcds) * per_xcd + at_xcd;
+        if (unit >= n_units) break;
+        const int run = unit / n_blocks, h = run % a.n_kv_head, split = run / a.n_kv_head;
+        // the group that holds this block
+        int left = unit - run * n_blocks;
+        Group grp = first64;
+        int incl = incl64;
+        for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
+            if (g0) {
+                grp = group_at(a, g0 + lane);
+                incl = wave_scan(blocks_of(grp), lane);
+            }
+            const uint64_t b = __ballot(incl > left);
+            if (b) {
+                const int at = __builtin_ctzll(b);
+                left -= __builtin_amdgcn_readlane(incl - blocks_of(grp), at);
+                grp.first = __builtin_amdgcn_readlane(grp.first, at);
+                grp.end = __builtin_amdgcn_readlane(grp.end, at);
+                grp.prefix = __builtin_amdgcn_readlane(grp.prefix, at);
+                break;
+            }
+            left -= __builtin_amdgcn_readlane(incl, 63);
         }
-        const uint64_t b = __ballot(incl > left);
-        const int at = b ? __builtin_ctzll(b) : 63;
-        if (b) {
-            grp.first = __builtin_amdgcn_readlane(g.first, at);
-            grp.end = __builtin_amdgcn_readlane(g.end, at);
-            grp.prefix = __builtin_amdgcn_readlane(g.prefix, at);
-            found = true;
-        }
-        left -= __builtin_amdgcn_readlane(found ? incl - nb : incl, at);
+        const int64_t prefix = __builtin_amdgcn_readfirstlane(grp.prefix);
+        if (prefix == 0 || prefix > a.max_prefix) continue;
+        const int per = prefix_run_pages(a, prefix), j0 = split * per;
+        const int n = min(per, (int)((prefix + kPageRows - 1) >> kPageShift) - j0);
+        if (n <= 0) continue;
+        const int first = __builtin_amdgcn_readfirstlane(grp.first), end = __builtin_amdgcn_readfirstlane(grp.end);
+        const int c0 = left * kSharedCols;        // this block's first column of the group
+        const int cols = (end - first) * G - c0;  // columns from there on
+        auto row_of = [&](int c) {
+            const int s = (c0 + c) / G;
+            return (int64_t)(first + s) * a.n_head + h * G + (c0 + c - s * G);
+        };
+        px_run<T>(
+            a, lds, a.block_table + (size_t)first * a.max_pages, h, j0, n, prefix, cols, threadIdx.x,
+            [&](int c) -> const float* { return c < cols ? a.q + row_of(c) * kHeadDim : nullptr; },
+            [&](int c, int d, float M, float L, f32x4 A) { put_partial(a, row_of(c), split, d, M, L, A); });
+        __syncthreads();  // the stage buffers of the next unit are those of this one's merge
     }
-    const int64_t prefix = grp.prefix;
-    if (!found || prefix == 0 || prefix > a.max_prefix) return;
-    const int per = prefix_run_pages(a, prefix), j0 = split * per;
-    const int n = min(per, (int)((prefix + kPageRows - 1) >> kPageShift) - j0);
-    if (n <= 0) return;
-    const int c0 = left * kSharedCols;                // this block's first column of the group
-    const int cols = (grp.end - grp.first) * G - c0;  // columns from there on
-    auto row_of = [&](int c) {
-        const int s = (c0 + c) / G;
-        return (int64_t)(grp.first + s) * a.n_head + h * G + (c0 + c - s * G);
-    };
-    px_run<T>(
-        a, lds, a.block_table + (size_t)grp.first * a.max_pages, h, j0, n, prefix, cols, threadIdx.x,
-        [&](int c) -> const float* { return c < cols ? a.q + row_of(c) * kHeadDim : nullptr; },
-        [&](int c, int d, float M, float L, f32x4 A) { put_partial(a, row_of(c), split, d, M, L, A); });
 }
 
 // A sequence's own rows: workgroup (run of them, kv head, sequence).  FINISH:
@@ -1627,7 +1641,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
 // writes the output; otherwise the run leaves one more partial.
 template <typename T, bool FINISH>
 __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
-    __shared__ OwnLds<T, kSharedWaves> lds;
+    __shared__ OwnLds<T, kPagedWaves> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.group, split = FINISH ? 0 : blockIdx.x, h = blockIdx.y, s = blockIdx.z;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
@@ -1642,7 +1656,7 @@ __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
     if (!q.bad && lo < hi) {
         const int j0 = (int)(lo >> kPageShift), n = (int)((hi - 1) >> kPageShift) - j0 + 1;
         const int32_t* table = a.block_table + (size_t)s * a.max_pages;
-        attend_run<T, kSharedWaves>(st, a, h, n, lo, hi, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
+        attend_run<T, kPagedWaves>(st, a, h, n, lo, hi, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
             logical = j0 + e;
             page = table[logical];
             if (page < 0 || page >= a.n_pages) {
@@ -1651,7 +1665,7 @@ __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
             }
         });
     }
-    merge_waves<T, kSharedWaves>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
+    merge_waves<T, kPagedWaves>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         if constexpr (FINISH) {
             const int64_t per = (int64_t)prefix_run_pages(a, q.prefix) * kPageRows;
@@ -1730,10 +1744,10 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_prefix_##NAME(PagedAttnArgs a) {               \
         prefix_body<T>(a);                                                                                             \
     }                                                                                                                  \
-    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_tail_##NAME(PagedAttnArgs a) {                 \
+    extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_tail_##NAME(PagedAttnArgs a) {                 \
         tail_body<T, false>(a);                                                                                        \
     }                                                                                                                  \
-    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_tail_finish_##NAME(PagedAttnArgs a) {          \
+    extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_tail_finish_##NAME(PagedAttnArgs a) {          \
         tail_body<T, true>(a);                                                                                         \
     }
 TMAC_PAGED_KERNELS(f32, float)

@@ -1686,7 +1686,7 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
     return launch_paged_merge(ctx, stream, ctx->k_selected_merge, &a);
 }
 
-constexpr int kTailWholeRows = 256;  // own rows that one workgroup takes without help
+constexpr int kTailWholeRows = 1024;  // own rows that one workgroup takes without help
 constexpr int kFinishSlots = 16;     // prefix partials that the own rows' workgroup merges itself
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                  const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
@@ -1713,23 +1713,25 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     a.max_prefix = max_prefix;
     a.max_tail = max_tail;
     const int64_t group = n_head / n_kv_head, n_sk = (int64_t)n_seq * n_kv_head;
-    // blocks of columns: every group's last one may be partly filled
+    // Blocks of columns: every group's last one may be partly filled.  The runs of a prefix aim for one workgroup per
+    // CU over the blocks there are if the groups fill theirs; the launch has room for any grouping.
+    const int64_t least = std::max<int64_t>(n_groups, cdiv(n_seq * group, tmac::kSharedCols));
     const int64_t blocks =
         n_groups && max_prefix ? std::min<int64_t>(n_seq, n_seq * group / tmac::kSharedCols + n_groups) : 0;
     a.prefix_blocks = (int)blocks;
     a.prefix_splits = 0;
     if (blocks) {
-        const int64_t pages = cdiv(max_prefix, kPageRows);
-        const int64_t splits = std::min<int64_t>(ctx->n_cu / (blocks * n_kv_head), cdiv(pages, tmac::kSharedWaves));
+        const int64_t splits = std::min<int64_t>(ctx->n_cu / (std::min(least, blocks) * n_kv_head),
+                                                 cdiv(cdiv(max_prefix, kPageRows), tmac::kSharedWaves));
         a.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
     }
-    // Own rows: one run a sequence where that fills half of the CUs or the rows are few, and then, with few prefix
-    // partials, its workgroup merges them and writes the output.
+    // Own rows: one run a sequence unless they are many and the sequences few, and then, with few prefix partials, its
+    // workgroup merges them and writes the output.
     a.tail_rows = (int)std::max<int64_t>(kPageRows, cdiv(max_tail, kPageRows) * kPageRows);
-    if (2 * n_sk < ctx->n_cu && max_tail > kTailWholeRows) {
-        const int64_t splits = std::min<int64_t>(cdiv(ctx->n_cu, n_sk), kMaxSplits);
-        a.tail_rows = (int)std::max<int64_t>(cdiv(cdiv(max_tail, splits), kPageRows) * kPageRows,
-                                             kPageRows * tmac::kSharedWaves);
+    if (n_sk < 2 * ctx->n_cu && max_tail > kTailWholeRows) {
+        const int64_t splits = std::min<int64_t>({cdiv(2 * ctx->n_cu, n_sk), cdiv(2 * max_tail, kTailWholeRows),
+                                                  (int64_t)kMaxSplits});
+        a.tail_rows = (int)(cdiv(cdiv(max_tail, splits), kPageRows) * kPageRows);
     }
     a.tail_splits = (int)cdiv(max_tail, a.tail_rows);
     const bool finish = a.tail_splits <= 1 && a.prefix_splits <= kFinishSlots;
@@ -1742,15 +1744,17 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     if ((rc = set_device(ctx))) return rc;
     if (a.n_slots && (rc = paged_partials(ctx, stream, &a))) return rc;
     const unsigned threads = 64 * tmac::kSharedWaves;
-    const int64_t units = blocks * n_kv_head * a.prefix_splits;
+    // one workgroup per CU, or fewer; they share the units there are
+    const int64_t units = std::min<int64_t>(blocks * n_kv_head * a.prefix_splits, ctx->n_cu);
     if (blocks && (rc = launch(ctx, ctx->k_prefix[kv_dtype], (unsigned)(cdiv(units, tmac::kXcds) * tmac::kXcds), 1,
                                threads, (hipStream_t)stream, &a)))
         return rc;
+    const unsigned tail_threads = 64 * tmac::kPagedWaves;
     if (finish)
-        return launch(ctx, ctx->k_tail_finish[kv_dtype], 1, (unsigned)n_kv_head, threads, (hipStream_t)stream, &a,
+        return launch(ctx, ctx->k_tail_finish[kv_dtype], 1, (unsigned)n_kv_head, tail_threads, (hipStream_t)stream, &a,
                       (unsigned)n_seq);
-    if (a.tail_splits && (rc = launch(ctx, ctx->k_tail[kv_dtype], (unsigned)a.tail_splits, (unsigned)n_kv_head, threads,
-                                      (hipStream_t)stream, &a, (unsigned)n_seq)))
+    if (a.tail_splits && (rc = launch(ctx, ctx->k_tail[kv_dtype], (unsigned)a.tail_splits, (unsigned)n_kv_head,
+                                      tail_threads, (hipStream_t)stream, &a, (unsigned)n_seq)))
         return rc;
     return launch_paged_merge(ctx, stream, ctx->k_shared_merge, &a);
 }
