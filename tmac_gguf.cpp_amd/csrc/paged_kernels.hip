@@ -1278,30 +1278,45 @@ __device__ __forceinline__ Group group_at(const PagedAttnArgs& a, int g) {
     return r;
 }
 
+// Blocks of 64 columns a group has.
+__device__ __forceinline__ int blocks_of(const PagedAttnArgs& a, const Group& g) {
+    return (int)(((int64_t)(g.end - g.first) * a.group + kSharedCols - 1) / kSharedCols);
+}
+
+// Runs that every prefix is cut into: as many as give each workgroup of the
+// prefix kernel's grid one unit, with n_blocks blocks in all, and at most those
+// there are slots for.  Pages of one run of a prefix of `prefix` rows.
+__device__ __forceinline__ int prefix_runs(const PagedAttnArgs& a, int n_blocks) {
+    return max(1, min(a.prefix_splits, a.prefix_groups / max(1, n_blocks * a.n_kv_head)));
+}
+__device__ __forceinline__ int run_pages(int64_t prefix, int runs) {
+    const int n = (int)((prefix + kPageRows - 1) >> kPageShift);
+    return max(1, (n + runs - 1) / runs);
+}
+
 // A sequence's rows: [0, prefix) through its group's first sequence, [prefix,
 // len) through its own pages.  Its group is the last one that holds it.
 struct SharedSeq {
     int64_t prefix, len;
-    bool bad;  // a length or prefix outside what the launch covers
+    int slots;  // partials that the prefix left
+    bool bad;   // a length or prefix outside what the launch covers
 };
 __device__ __forceinline__ SharedSeq shared_seq(const PagedAttnArgs& a, int s, int lane) {
     SharedSeq r;
     r.len = max(a.lengths[s], 0);
     r.prefix = 0;
+    int n_blocks = 0;
     for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
         const Group g = group_at(a, g0 + lane);
         const uint64_t b = __ballot(s >= g.first && s < g.end);
         if (b) r.prefix = __builtin_amdgcn_readlane(g.prefix, 63 - __clzll(b));
+        n_blocks += (int)__builtin_amdgcn_readfirstlane(wave_sum_u((unsigned)blocks_of(a, g)));
     }
     r.bad = r.len > 0 && (r.prefix > a.max_prefix || r.len < r.prefix || r.len - r.prefix > a.max_tail ||
                           r.len > (int64_t)a.max_pages * kPageRows);
+    const int64_t per = (int64_t)run_pages(r.prefix, prefix_runs(a, min(n_blocks, a.prefix_blocks))) * kPageRows;
+    r.slots = r.bad || r.len == 0 ? 0 : (int)((r.prefix + per - 1) / per);
     return r;
-}
-
-// Pages of one run of a prefix of `prefix` rows cut into prefix_splits runs.
-__device__ __forceinline__ int prefix_run_pages(const PagedAttnArgs& a, int64_t prefix) {
-    const int n = (int)((prefix + kPageRows - 1) >> kPageShift), runs = max(1, a.prefix_splits);
-    return max(1, (n + runs - 1) / runs);
 }
 
 // ---------------------------------------------------------------------------
@@ -1584,14 +1599,13 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
     __shared__ PxLds<T> lds;
     const int lane = threadIdx.x & 63, G = a.group;
     // The blocks there are: 64 groups at a time, one a lane, their blocks summed.
-    auto blocks_of = [&](const Group& g) { return (int)(((int64_t)(g.end - g.first) * G + kSharedCols - 1) / kSharedCols); };
     const Group first64 = group_at(a, lane);
-    const int incl64 = wave_scan(blocks_of(first64), lane);
+    const int incl64 = wave_scan(blocks_of(a, first64), lane);
     int n_blocks = __builtin_amdgcn_readlane(incl64, 63);
     for (int g0 = 64; g0 < a.n_groups; g0 += 64)
-        n_blocks += __builtin_amdgcn_readlane(wave_scan(blocks_of(group_at(a, g0 + lane)), lane), 63);
+        n_blocks += __builtin_amdgcn_readlane(wave_scan(blocks_of(a, group_at(a, g0 + lane)), lane), 63);
     n_blocks = min(n_blocks, a.prefix_blocks);
-    const int n_units = a.prefix_splits * a.n_kv_head * n_blocks, per_xcd = (n_units + kXcds - 1) / kXcds;
+    const int runs = prefix_runs(a, n_blocks), n_units = runs * a.n_kv_head * n_blocks, per_xcd = (n_units + kXcds - 1) / kXcds;
     for (int at_xcd = (int)(blockIdx.x / kXcds); at_xcd < per_xcd; at_xcd += (int)(gridDim.x / kXcds)) {
         const int unit = (int)(blockIdx.x % kXcds) * per_xcd + at_xcd;
         if (unit >= n_units) break;
@@ -1603,12 +1617,12 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
         for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
             if (g0) {
                 grp = group_at(a, g0 + lane);
-                incl = wave_scan(blocks_of(grp), lane);
+                incl = wave_scan(blocks_of(a, grp), lane);
             }
             const uint64_t b = __ballot(incl > left);
             if (b) {
                 const int at = __builtin_ctzll(b);
-                left -= __builtin_amdgcn_readlane(incl - blocks_of(grp), at);
+                left -= __builtin_amdgcn_readlane(incl - blocks_of(a, grp), at);
                 grp.first = __builtin_amdgcn_readlane(grp.first, at);
                 grp.end = __builtin_amdgcn_readlane(grp.end, at);
                 grp.prefix = __builtin_amdgcn_readlane(grp.prefix, at);
@@ -1618,7 +1632,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
         }
         const int64_t prefix = __builtin_amdgcn_readfirstlane(grp.prefix);
         if (prefix == 0 || prefix > a.max_prefix) continue;
-        const int per = prefix_run_pages(a, prefix), j0 = split * per;
+        const int per = run_pages(prefix, runs), j0 = split * per;
         const int n = min(per, (int)((prefix + kPageRows - 1) >> kPageShift) - j0);
         if (n <= 0) continue;
         const int first = __builtin_amdgcn_readfirstlane(grp.first), end = __builtin_amdgcn_readfirstlane(grp.end);
@@ -1668,8 +1682,7 @@ __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
     merge_waves<T, kPagedWaves>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         if constexpr (FINISH) {
-            const int64_t per = (int64_t)prefix_run_pages(a, q.prefix) * kPageRows;
-            const int n = q.bad || q.len == 0 ? 0 : (int)((q.prefix + per - 1) / per);
+            const int n = q.slots;
             const size_t at = (size_t)(row0 + c) * a.n_slots;
             const float* acc = a.ws + at * kHeadDim + d;
             const float2* ml =
@@ -1717,12 +1730,8 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     if (row >= (int64_t)a.n_seq * a.n_head) return;
     const int s = __builtin_amdgcn_readfirstlane((int)(row / a.n_head));
     const SharedSeq q = shared_seq(a, s, lane);
-    int n0 = 0, n1 = 0;
-    if (!q.bad && q.len > 0) {
-        const int64_t per = (int64_t)prefix_run_pages(a, q.prefix) * kPageRows;
-        n0 = (int)((q.prefix + per - 1) / per);
-        n1 = (int)((q.len - q.prefix + a.tail_rows - 1) / a.tail_rows);
-    }
+    const int n0 = q.slots;
+    const int n1 = q.bad || q.len == 0 ? 0 : (int)((q.len - q.prefix + a.tail_rows - 1) / a.tail_rows);
     float L;
     f32x4 y = merge_slots<WPR>(a, row, n0, a.prefix_splits, n1, wave % WPR, lane, L);
     if (wave % WPR || lane >= 16) return;
