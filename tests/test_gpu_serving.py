@@ -270,6 +270,32 @@ def test_select_long(ctx):
     no_fault(ctx)
 
 
+@pytest.mark.parametrize("n,longest", [(70, 4000), (256, 1100), (300, 1100), (1030, 300)])
+def test_select_many_lists(ctx, n, longest):
+    """More steps of pages than waves that fit the card, dealt out over a wave's sequences; more sequences than are
+    dealt out.  The lengths are ragged and the first, the last and a run of others are empty."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(1, longest + 1, n).astype(np.int32)
+    lens[[0, 40, 41, 42, n - 1]] = 0
+    lens[50] = longest
+    table, n_pages = tables(rng, lens)
+    q, b = oracle.normal(312 + n, (n, 6, 64)), random_bounds(313 + n, n_pages, 2)
+    np.testing.assert_array_equal(run_select(ctx, q, b, table, lens, 2, 9, 1, 1),
+                                  select_ref(q, b, table, lens, 2, 9, 1, 1))
+    no_fault(ctx)
+
+
+def test_select_more_pages_than_registers_hold(ctx):
+    rng = np.random.default_rng(4)
+    lens = np.array([140001, 131073], np.int32)
+    table, n_pages = tables(rng, lens)
+    q, b = oracle.normal(316, (2, 7, 64)), random_bounds(317, n_pages, 1)
+    for top, first, last in ((1000, 1, 1), (1, 0, 0), (8700, 0, 3)):
+        np.testing.assert_array_equal(run_select(ctx, q, b, table, lens, 1, top, first, last),
+                                      select_ref(q, b, table, lens, 1, top, first, last))
+    no_fault(ctx)
+
+
 def test_select_ties_go_to_the_lower_page(ctx):
     """A zero query (all scores 0), equal bounds on many pages, and scores that differ only beyond fp32."""
     rng = np.random.default_rng(4)
@@ -564,6 +590,24 @@ def test_shared_many_sequences(ctx, dt):
     starts = [0] + list(cuts) + [200]
     shared_case(ctx, dt, 4, 1, [int(x) for x in starts], [int(x) for x in rng.integers(1, 120, 70)],
                 list(rng.integers(0, 40, 200)), 541, zero=(3, 50, 199))
+
+
+@pytest.mark.parametrize("dt", ALL_DT)
+@pytest.mark.parametrize("nh,nkv", [(4, 1), (14, 2)])
+def test_shared_few_sequences_long_rows(ctx, dt, nh, nkv):
+    """A prefix in more runs than one workgroup merges, own rows that are split, and one of them without the other."""
+    shared_case(ctx, dt, nh, nkv, [0, 2], [6011], [30, 5], 560, max_tail=64)
+    shared_case(ctx, dt, nh, nkv, [1, 3], [6011], [40, 2999, 1], 561, max_tail=3000)
+    shared_case(ctx, dt, nh, nkv, [0, 2], [33], [2100, 1030], 562)
+    shared_case(ctx, dt, nh, nkv, [], [], [2100, 0, 1030], 563)
+
+
+@pytest.mark.parametrize("dt", ALL_DT)
+def test_shared_more_blocks_than_workgroups(ctx, dt):
+    """Groups of one sequence each on 8 kv heads: a workgroup takes several (block, kv head, run) units."""
+    rng = np.random.default_rng(7)
+    shared_case(ctx, dt, 32, 8, list(range(91)), [int(x) for x in rng.integers(0, 150, 90)],
+                list(rng.integers(0, 20, 90)), 570, zero=(0, 44))
 
 
 def test_shared_without_groups_or_tails(ctx):

@@ -124,6 +124,8 @@ def test_shapes_outside_the_domain(fake, name):
     # q_out one row behind q, q_out = q with rows further apart than q_out's
     ("tmac_kv_append_paged", dict(q_out=P + 896 * 4), TMAC_ERR_INVALID_ARG),
     ("tmac_kv_append_paged", dict(q_out=P, q_stride=1152), TMAC_ERR_INVALID_ARG),
+    ("tmac_kv_append_paged", dict(q_out=3 * P + 4 * 127 * 4), TMAC_ERR_INVALID_ARG),  # over k, over v
+    ("tmac_kv_append_paged", dict(q_out=4 * P - 5 * 896 * 4 + 16), TMAC_ERR_INVALID_ARG),
     ("tmac_kv_page_bounds", dict(max_new=-1), TMAC_ERR_INVALID_ARG),
     ("tmac_select_pages", dict(max_len=0), TMAC_ERR_INVALID_ARG),
     ("tmac_select_pages", dict(max_len=641), TMAC_ERR_INVALID_ARG),

@@ -1491,11 +1491,15 @@ int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, co
     if (!(base > 0.f) || !std::isfinite(base)) return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: bad base");
     if (n_seq == 0 || n_rows == 0) return TMAC_OK;
     // q_out may be q itself (same rows); any other overlap would let a row be overwritten before it is read
-    if (q && !(q == q_out && (q_stride == q_row || n_rows == 1))) {
-        const uintptr_t q0 = (uintptr_t)q, q1 = (uintptr_t)(q + (n_rows - 1) * q_stride + q_row);
+    if (q) {
         const uintptr_t o0 = (uintptr_t)q_out, o1 = (uintptr_t)(q_out + n_rows * q_row);
-        if (q0 < o1 && o0 < q1)
+        auto overlaps = [&](const float* p, int64_t stride, int64_t row) {
+            return (uintptr_t)p < o1 && o0 < (uintptr_t)(p + (n_rows - 1) * stride + row);
+        };
+        if (!(q == q_out && (q_stride == q_row || n_rows == 1)) && overlaps(q, q_stride, q_row))
             return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: q_out overlaps q without being it");
+        if (overlaps(k, k_stride, kv_row) || overlaps(v, v_stride, kv_row))
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_paged: q_out overlaps k or v");
     }
     if ((rc = set_device(ctx))) return rc;
     const RopeTable* rt = nullptr;
