@@ -295,6 +295,8 @@ class DeviceArray:
 
 
 def _p(x) -> Optional[int]:
+    if type(x) is int:  # most calls: an address, taken as it is
+        return x
     if x is None:
         return None
     if isinstance(x, DeviceArray):
