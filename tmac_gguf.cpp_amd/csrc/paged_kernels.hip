@@ -1414,6 +1414,40 @@ __device__ __forceinline__ void px_fetch(PxRaw<T>& r, const PagedAttnArgs& a, in
     }
 }
 
+// 16-bit rows need no conversion and go from memory to LDS without registers
+// between (64 lanes x 16 bytes, 8 rows, to consecutive LDS): the XOR of a row's
+// chunks is in the address that a lane reads.  Rows at or past `valid` of the
+// stage are past the end of the descriptor and come as zeros.  The loads are
+// counted with vmcnt; px_landed() before the barrier that opens the stage.
+__device__ __forceinline__ void load_lds16(u32x4 descriptor, unsigned offset, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 ::"s"(lds), "v"(offset), "s"(descriptor) : "memory");  // nothing else here uses m0
+}
+__device__ __forceinline__ void px_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <typename T>
+__device__ __forceinline__ void px_direct(PxStage<T>& s, const PagedAttnArgs& a, int h, const PxPages<T>& pages,
+                                          int valid, int wave, int lane, unsigned& bad) {
+    using G = PxGeom<T>;
+    const unsigned stride = a.n_kv_head * 128u;
+    const int row = 8 * wave + lane / 8, slot = lane & 7;  // + 64 i: the same place in its page, the same XOR
+    const unsigned at = row % kPageRows * stride, ko = at + k_chunk(row, slot), vo = at + v_chunk(row, slot);
+#pragma unroll
+    for (int i = 0; i < PxRaw<T>::N; ++i) {
+        const int pg = pages.page[i], r0 = i * G::kStep + 8 * wave, rows = valid - r0 / kPageRows * kPageRows;
+        bad |= (unsigned)pg >= (unsigned)a.n_pages;
+        const size_t base =
+            (size_t)min(max(pg, 0), a.n_pages - 1) * ((size_t)kPageRows * stride) + (size_t)h * 128;
+        const unsigned bytes = rows > 0 ? (min(rows, kPageRows) - 1) * stride + 128 : 0;
+        auto load = [&](const char* pool, unsigned offset, char* to) {
+            const uint64_t p = reinterpret_cast<uint64_t>(pool + base);
+            load_lds16(u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xFFFFu, bytes, 0x00020000u}, offset,
+                       (unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)to));
+        };
+        load(a.k_pages, ko, &s.k[0][r0][0]);
+        load(a.v_pages, vo, &s.v[0][r0][0]);
+    }
+}
+
 // Rows at or past `valid` of the stage: V is written as zeros (P is 0 there, and the row may hold anything).
 template <typename T>
 __device__ __forceinline__ void px_store(PxStage<T>& s, const PxRaw<T>& r, int valid, int tid) {
@@ -1515,6 +1549,7 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
                                        int n_pages, int64_t rows, int n_cols, int tid, ColPtr col_ptr, Put put) {
     using G = PxGeom<T>;
     constexpr int NB = __is_same(T, float) ? 1 : 2;
+    constexpr bool Direct = CacheFmt<T>::kHeadBytes == 128;
     const const_i32_ptr table = (const_i32_ptr)table_;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave >> 1, cw = wave & 1;
     const int i = lane & 31, g = lane >> 5;
@@ -1530,25 +1565,31 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
     {
         RawQ<T, Mfma32> q;
         load_q<T, Mfma32>(q, col_ptr(32 * cw + i), lane);
-        px_fetch<T>(raw, a, h, pages, tid, bad);
+        if constexpr (Direct) px_direct<T>(lds.stage[0], a, h, pages, n_rows, wave, lane, bad);
+        else px_fetch<T>(raw, a, h, pages, tid, bad);
         px_pages<T>(pages, table, j0 + G::kPages, j_last, wave);
         cols_init<T, Mfma32>(c, q, a.qscale);
     }
-    px_store<T>(lds.stage[0], raw, n_rows, tid);
+    if constexpr (Direct) px_landed();
+    else px_store<T>(lds.stage[0], raw, n_rows, tid);
     __syncthreads();
     for (int st = 0; st < n_stage; ++st) {
         PxStage<T>& cur = lds.stage[NB == 2 ? st & 1 : 0];
+        PxStage<T>& next = lds.stage[NB == 2 ? (st + 1) & 1 : 0];
         const bool more = st + 1 < n_stage;
+        const int after = n_rows - (st + 1) * PxStage<T>::kRows;
         if (more) {
-            px_fetch<T>(raw, a, h, pages, tid, bad);
+            if constexpr (Direct) px_direct<T>(next, a, h, pages, after, wave, lane, bad);
+            else px_fetch<T>(raw, a, h, pages, tid, bad);
             px_pages<T>(pages, table, j0 + (st + 2) * G::kPages, j_last, wave);
         }
         const int valid = min(n_rows - st * PxStage<T>::kRows - kg * kPxKeys<T>, kPxKeys<T>);
         if (busy && valid > 0) px_attend<T>(c, cur, kg * kPxKeys<T>, valid, neg, lane);
         if (more) {
             if constexpr (NB == 1) __syncthreads();
-            px_store<T>(lds.stage[NB == 2 ? (st + 1) & 1 : 0], raw, n_rows - (st + 1) * PxStage<T>::kRows, tid);
+            if constexpr (!Direct) px_store<T>(next, raw, after, tid);
         }
+        if constexpr (Direct) px_landed();
         __syncthreads();
     }
     if (bad && lane == 0) atomicOr(a.err, 4);
