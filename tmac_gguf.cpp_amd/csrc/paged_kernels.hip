@@ -566,24 +566,6 @@ constexpr bool parts_meet(int i, int j) {
     return NA == 1 || NB == 1 || i + j <= 2;
 }
 
-// (-1, 0) and (0, -1) as pairs of 16-bit values: a dot product with one of
-// them takes a half of a packed word from an fp32 value in one instruction,
-// exactly.  They are kept in registers: as immediates the compiler encodes them
-// for another operand width.  The other half is multiplied by 0, so a pair must
-// hold values whose NaN or infinity may spread to each other: q and P, whose
-// pairs end in the same score and the same sum, not V.
-struct NegPair {
-    unsigned lo, hi;
-    __device__ NegPair(unsigned minus_one) : lo(minus_one), hi(minus_one << 16) {
-        asm("" : "+s"(lo));
-        asm("" : "+s"(hi));
-    }
-};
-template <typename M>
-constexpr unsigned minus_one() {
-    return M::kScaleQ ? 0xBC00u : 0xBF80u;
-}
-
 // Three bf16 parts of two fp32 values (element 0 in the low half), cut bits: exact.
 __device__ __forceinline__ unsigned top_pair(float x, float y) {
     return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
@@ -595,25 +577,20 @@ __device__ __forceinline__ void split3(float x, float y, unsigned (&w)[3]) {
     w[1] = top_pair(x1, y1);
     w[2] = top_pair(x1 - top(x1), y1 - top(y1));
 }
-// The same for a pair that may share its non-finite values; KP parts.  fp16: two parts, each the nearest.
+// Q and P: KP parts; fp16: two, each the nearest.  What remains of a value is
+// taken with a mask and a subtraction, which issue beside a product (4 in the 32
+// cycles of one cost 1 more): a dot product with (-1, 0) does it in one
+// instruction, but runs on the matrix unit's time, 8 cycles and a product's wait.
 template <typename M, int KP>
-__device__ __forceinline__ void split(float x, float y, const NegPair& neg, unsigned (&w)[3]) {
+__device__ __forceinline__ void split(float x, float y, unsigned (&w)[3]) {
     if constexpr (M::kScaleQ) {
         static_assert(KP == 2, "fp16: 22 bits in two parts");
         w[0] = M::pack2(x, y);
         const f16x2 v = __builtin_bit_cast(f16x2, w[0]);
-        w[1] = M::pack2(__builtin_amdgcn_fdot2(v, __builtin_bit_cast(f16x2, neg.lo), x, false),
-                        __builtin_amdgcn_fdot2(v, __builtin_bit_cast(f16x2, neg.hi), y, false));
+        w[1] = M::pack2(x - (float)v[0], y - (float)v[1]);
     } else {
-#pragma unroll
-        for (int p = 0; p < KP; ++p) {
-            w[p] = top_pair(x, y);
-            const bf16x2 v = __builtin_bit_cast(bf16x2, w[p]);
-            if (p + 1 < KP) {
-                x = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, neg.lo), x, false);
-                y = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, neg.hi), y, false);
-            }
-        }
+        static_assert(KP == 3, "bf16: 24 bits in three parts");
+        split3(x, y, w);
     }
 }
 
@@ -686,7 +663,6 @@ template <typename T, typename S>
 __device__ __forceinline__ void cols_init(Cols<T, S>& c, const RawQ<T, S>& raw, float scale) {
     using KO = typename Parts<T>::KOps;
     constexpr int MB = Cols<T, S>::kDepthBlocks;
-    const NegPair neg(minus_one<KO>());
     float x[MB][8];
     float top = 0.f;
 #pragma unroll
@@ -713,7 +689,7 @@ __device__ __forceinline__ void cols_init(Cols<T, S>& c, const RawQ<T, S>& raw, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             unsigned y[3] = {0, 0, 0};
-            split<KO, Parts<T>::kQ>(x[m][2 * i], x[m][2 * i + 1], neg, y);
+            split<KO, Parts<T>::kQ>(x[m][2 * i], x[m][2 * i + 1], y);
 #pragma unroll
             for (int k = 0; k < 3; ++k) w[k][i] = y[k];
         }
@@ -820,7 +796,7 @@ __device__ __forceinline__ int v_chunk(int row, int chunk) { return (chunk ^ ((2
 // and each receives 4 consecutive keys of one dim.
 template <typename T, typename S>
 __device__ __forceinline__ void values_step(Cols<T, S>& c, f32x4 w0, f32x4 w1, char* v, int part_bytes,
-                                            const float* vd0, const float* vd1, const NegPair& neg, int lane) {
+                                            const float* vd0, const float* vd1, int lane) {
     using P = Parts<T>;
     using VO = typename P::VOps;
     constexpr bool Q8 = __is_same(T, q8_0_t);
@@ -840,7 +816,7 @@ __device__ __forceinline__ void values_step(Cols<T, S>& c, f32x4 w0, f32x4 w1, c
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 unsigned z[3] = {0, 0, 0};
-                split<VO, P::kP>(x[2 * r], x[2 * r + 1], neg, z);
+                split<VO, P::kP>(x[2 * r], x[2 * r + 1], z);
 #pragma unroll
                 for (int p = 0; p < P::kP; ++p) w[p][2 * half + r] = z[p];
             }
@@ -915,7 +891,7 @@ struct Own {
     }
     // Keys lo[u] .. hi[u] - 1 of page u take part.
     __device__ static void attend(State& st, const Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles],
-                                  Lds& lds, const NegPair& neg, int lane) {
+                                  Lds& lds, int lane) {
         using KO = typename Parts<T>::KOps;
         const int i = lane & 15, g = lane >> 4;
         const u32x4 zero = {0, 0, 0, 0};
@@ -966,7 +942,7 @@ struct Own {
                 for (int r = 0; r < 4; ++r) w[u][r] = 4 * g + r >= lo[u] && 4 * g + r < hi[u] ? w[u][r] : kNegInf;
         }
         softmax_step<S>(st.m, st.l, st.base, st.o, w);
-        values_step<T, S>(st, w[0], w[1], &lds.v[0][0], 0, lds.vd[0], lds.vd[Q8 ? 1 : 0], neg, lane);
+        values_step<T, S>(st, w[0], w[1], &lds.v[0][0], 0, lds.vd[0], lds.vd[Q8 ? 1 : 0], lane);
     }
     // This lane's sums of column lane % 16, ready to merge: dims 16 b + 4 g + 0..3.
     static constexpr int dim(int b, int g) { return 16 * b + 4 * g; }
@@ -1022,7 +998,7 @@ struct Own<float> {
         for (int r = 0; r < 4; ++r) t.v[r] = *reinterpret_cast<const f32x4*>(vp + (4 * g + r) * stride + 16 * i);
     }
     __device__ static void attend(State& st, const Tile (&tiles)[1], const int (&lo)[1], const int (&hi)[1], Lds&,
-                                  const NegPair&, int lane) {
+                                  int lane) {
         const Tile& t = tiles[0];
         const int g = lane >> 4;
         const bool full = lo[0] <= 0 && hi[0] >= kPageRows;
@@ -1077,7 +1053,6 @@ __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const Pag
     constexpr int HB = CacheFmt<T>::kHeadBytes, KT = O::kTiles;
     const int stride = a.n_kv_head * HB;
     const size_t page_bytes = (size_t)kPageRows * stride;
-    const NegPair neg(minus_one<typename Parts<T>::VOps>());
     const int steps = ((n + KT - 1) / KT - wave + NW - 1) / NW;  // this wave's
     for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
         const int cnt = min(64 / KT, steps - s0);
@@ -1107,7 +1082,7 @@ __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const Pag
                         hi[u] = j < 0 ? 0 : (int)max((int64_t)0, min(row_hi - r0, (int64_t)kPageRows));
                         any |= hi[u] > lo[u];
                     }
-                    if (any) O::attend(st, t[d], lo, hi, lds, neg, lane);
+                    if (any) O::attend(st, t[d], lo, hi, lds, lane);
                 }
             }
         }
@@ -1495,7 +1470,7 @@ __device__ __forceinline__ void px_store(PxStage<T>& s, const PxRaw<T>& r, int v
 
 // The wave's keys of one stage (rows row0 .. row0 + kPxKeys - 1, of which `valid` take part).
 template <typename T>
-__device__ __forceinline__ void px_attend(Cols<T, Mfma32>& c, PxStage<T>& s, int row0, int valid, const NegPair& neg,
+__device__ __forceinline__ void px_attend(Cols<T, Mfma32>& c, PxStage<T>& s, int row0, int valid,
                                           int lane) {
     using S = Mfma32;
     using KO = typename Parts<T>::KOps;
@@ -1529,7 +1504,7 @@ __device__ __forceinline__ void px_attend(Cols<T, Mfma32>& c, PxStage<T>& s, int
             const f32x4 w0 = {st[kt][8 * h], st[kt][8 * h + 1], st[kt][8 * h + 2], st[kt][8 * h + 3]};
             const f32x4 w1 = {st[kt][8 * h + 4], st[kt][8 * h + 5], st[kt][8 * h + 6], st[kt][8 * h + 7]};
             values_step<T, S>(c, w0, w1, &s.v[0][first][0], sizeof(s.v[0]), &s.vd[0][Q8 ? first : 0],
-                              &s.vd[Q8 ? 1 : 0][Q8 ? first : 0], neg, lane);
+                              &s.vd[Q8 ? 1 : 0][Q8 ? first : 0], lane);
         }
 }
 
@@ -1556,7 +1531,6 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
     const int n_stage = (n_pages + G::kPages - 1) / G::kPages, j_last = j0 + n_pages - 1;
     const int n_rows = (int)min((int64_t)n_pages * kPageRows, rows - (int64_t)j0 * kPageRows);  // of this run
     const bool busy = 32 * cw < n_cols;
-    const NegPair neg(minus_one<typename Parts<T>::VOps>());
     unsigned bad = 0;
     PxRaw<T> raw;
     PxPages<T> pages;
@@ -1584,7 +1558,7 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
             px_pages<T>(pages, table, j0 + (st + 2) * G::kPages, j_last, wave);
         }
         const int valid = min(n_rows - st * PxStage<T>::kRows - kg * kPxKeys<T>, kPxKeys<T>);
-        if (busy && valid > 0) px_attend<T>(c, cur, kg * kPxKeys<T>, valid, neg, lane);
+        if (busy && valid > 0) px_attend<T>(c, cur, kg * kPxKeys<T>, valid, lane);
         if (more) {
             if constexpr (NB == 1) __syncthreads();
             if constexpr (!Direct) px_store<T>(next, raw, after, tid);
