@@ -144,6 +144,11 @@ def test_shapes_outside_the_domain(fake, name):
     ("tmac_select_pages", dict(n_seq=2 ** 31 - 1, max_pages=2 ** 27, max_len=2 ** 31 - 1), TMAC_ERR_INVALID_ARG),
     ("tmac_attention_decode_selected", dict(n_seq=2 ** 31 - 1), TMAC_ERR_INVALID_ARG),
     ("tmac_attention_decode_shared", dict(n_seq=2 ** 31 - 1), TMAC_ERR_INVALID_ARG),
+    # more threads than 32 bits
+    ("tmac_kv_append_paged", dict(q=None, q_out=None, n_rows=2 ** 30), TMAC_ERR_INVALID_ARG),
+    ("tmac_kv_page_bounds", dict(n_seq=2 ** 25), TMAC_ERR_INVALID_ARG),
+    ("tmac_select_pages", dict(n_seq=2 ** 24, top=40), TMAC_ERR_INVALID_ARG),
+    ("tmac_attention_decode_selected", dict(n_seq=2 ** 24), TMAC_ERR_INVALID_ARG),
 ])
 def test_refused(fake, name, kw, status):
     assert fake.call(name, **kw) == (status, [])

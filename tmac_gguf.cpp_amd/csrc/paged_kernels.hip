@@ -118,7 +118,7 @@ __device__ __forceinline__ void bounds_body(const BoundsArgs& a) {
         return;
     }
     const int j = (first >> kPageShift) + i;
-    const int n = min(kPageRows, len - j * kPageRows);
+    const int n = (int)min((int64_t)kPageRows, len - (int64_t)j * kPageRows);
     if (n <= 0) return;
     const int page = a.block_table[(size_t)s * a.max_pages + j];
     if (page < 0 || page >= a.n_pages) {
@@ -190,7 +190,7 @@ __device__ __forceinline__ unsigned order_key(float x) {
 
 __device__ __forceinline__ int select_pages_of(const SelectArgs& a, int s) {  // -1: a bad length
     const int len = max(a.lengths[s], 0);
-    return len > a.max_len ? -1 : (len + kPageRows - 1) >> kPageShift;
+    return len > a.max_len ? -1 : (len >> kPageShift) + ((len & (kPageRows - 1)) != 0);
 }
 
 __device__ __forceinline__ double bf16_to_f64(unsigned w, int e) {

@@ -1456,8 +1456,9 @@ static int check_serving(tmac_context* ctx, const char* what, int kv_dtype, int 
 }
 
 // A grid of `units` workgroups, refused where its index would not fit.
-static int check_units(tmac_context* ctx, const char* what, int64_t units) {
-    if (units > INT_MAX) return fail(ctx, TMAC_ERR_INVALID_ARG, std::string(what) + ": too many units of work");
+// Units of work that the kernels number in 32 bits, a launch of `threads` each if not 0.
+static int check_units(tmac_context* ctx, const char* what, int64_t units, int64_t threads = 0) {
+    if (units > INT_MAX || units * threads > UINT32_MAX) return fail(ctx, TMAC_ERR_INVALID_ARG, std::string(what) + ": too many units of work");
     return TMAC_OK;
 }
 
@@ -1527,8 +1528,9 @@ int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, co
     a.n_kv_head = n_kv_head;
     a.capacity = max_len;
     a.rows_per_group = (int)std::min<int64_t>(tmac::kAppendRows, std::max<int64_t>(1, n_rows / (8 * ctx->n_cu)));
-    return launch(ctx, ctx->k_append[kv_dtype], (unsigned)cdiv(n_rows, a.rows_per_group), 1, 256, (hipStream_t)stream,
-                  &a);
+    const int64_t blocks = cdiv(n_rows, a.rows_per_group);
+    if ((rc = check_units(ctx, what, blocks, 256))) return rc;
+    return launch(ctx, ctx->k_append[kv_dtype], (unsigned)blocks, 1, 256, (hipStream_t)stream, &a);
 }
 
 int tmac_kv_page_bounds(tmac_context* ctx, tmac_stream stream, int kv_dtype, const void* k_pages, int n_pages,
@@ -1552,7 +1554,7 @@ int tmac_kv_page_bounds(tmac_context* ctx, tmac_stream stream, int kv_dtype, con
                  ctx->err, n_pages, max_pages, n_seq, n_kv_head, max_new, (int)n_grid};
     if (n_grid * n_kv_head > INT_MAX) return check_units(ctx, what, n_grid * n_kv_head);
     const int64_t blocks = cdiv(n_grid * n_kv_head * n_seq, tmac::kPagedWaves);
-    if ((rc = check_units(ctx, what, blocks)) || (rc = set_device(ctx))) return rc;
+    if ((rc = check_units(ctx, what, blocks, 64 * tmac::kPagedWaves)) || (rc = set_device(ctx))) return rc;
     return launch(ctx, ctx->k_bounds[kv_dtype], (unsigned)blocks, 1, 64 * tmac::kPagedWaves, (hipStream_t)stream, &a);
 }
 
@@ -1577,7 +1579,9 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
         return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: need top >= 1, first, last >= 0, first + last <= top");
     if (n_seq == 0) return TMAC_OK;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head, pages = cdiv(max_len, kPageRows);
-    if ((rc = check_units(ctx, what, n_sk * cdiv(pages, 16)))) return rc;
+    const bool wide = pages > kSelectWidePages;
+    const unsigned threads = wide ? 1024 : 256;
+    if ((rc = check_units(ctx, what, n_sk * cdiv(pages, 16))) || (rc = check_units(ctx, what, n_sk, threads))) return rc;
     if (n_seq > kMaxGridYZ) return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: more than 65535 sequences");
     if ((rc = set_device(ctx))) return rc;
     SelectArgs a{};
@@ -1610,8 +1614,7 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
                          a.dealt ? 1u : (unsigned)n_seq, 64 * tmac::kPagedWaves, (hipStream_t)stream, &a)))
             return rc;
     }
-    const bool wide = pages > kSelectWidePages;
-    return launch(ctx, ctx->k_select[wide], (unsigned)n_sk, 1, wide ? 1024 : 256, (hipStream_t)stream, &a);
+    return launch(ctx, ctx->k_select[wide], (unsigned)n_sk, 1, threads, (hipStream_t)stream, &a);
 }
 
 // Checks and arguments that both attentions over paged caches share.
@@ -1627,7 +1630,7 @@ static int paged_attn_args(tmac_context* ctx, const char* what, int kv_dtype, co
         return rc;
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || (uintptr_t)lengths % 4)
         return fail(ctx, TMAC_ERR_MISALIGNED, std::string(what) + ": q, out and pools must be 16-byte aligned");
-    if ((rc = check_units(ctx, what, (int64_t)n_seq * n_head))) return rc;
+    if ((rc = check_units(ctx, what, (int64_t)n_seq * n_head, 64 * tmac::kPagedWaves))) return rc;
     a->q = q;
     a->k_pages = static_cast<const char*>(k_pages);
     a->v_pages = static_cast<const char*>(v_pages);
@@ -1681,7 +1684,7 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
     splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
     a.per_split = (int)cdiv(top, splits);
     a.n_slots = (int)cdiv(top, a.per_split);
-    if ((rc = check_units(ctx, what, n_sk * a.n_slots)) || (rc = set_device(ctx))) return rc;
+    if ((rc = check_units(ctx, what, n_sk * a.n_slots, 64 * tmac::kPagedWaves)) || (rc = set_device(ctx))) return rc;
     if (a.n_slots > 1 && (rc = paged_partials(ctx, stream, &a))) return rc;
     if ((rc = launch(ctx, ctx->k_selected[kv_dtype], (unsigned)(n_sk * a.n_slots), 1, 64 * tmac::kPagedWaves,
                      (hipStream_t)stream, &a)) ||
