@@ -550,7 +550,17 @@ def run_shared(ctx, q, kp, vp, table, lens, starts, prefix, nkv, dt, max_prefix=
     return dout.numpy()
 
 
+def once_for_all(table, nkv, longest):
+    """(table, max_prefix) with room for a prefix so long that it is read once for all sequences."""
+    room = max(longest, (1 << 17) // (len(table) * nkv) + 1)
+    wide = np.full((len(table), max(table.shape[1], -(-room // PR))), 2 ** 30, np.int32)
+    wide[:, :table.shape[1]] = table
+    return wide, room
+
+
 def shared_case(ctx, dt, nh, nkv, starts, prefix, tails, seed, zero=(), scale=1.0, **kw):
+    """The call as it is, and with room for a prefix so long that it is read once for all (short ones every sequence
+    reads itself)."""
     rng = np.random.default_rng(seed)
     of = np.full(len(tails), -1)
     for g in range(len(prefix)):
@@ -561,8 +571,13 @@ def shared_case(ctx, dt, nh, nkv, starts, prefix, tails, seed, zero=(), scale=1.
     kp, kwd = make_pool(seed + 1, total, nkv, dt)
     vp, vwd = make_pool(seed + 2, total, nkv, dt)
     q = oracle.normal(seed + 3, (len(tails), nh, 64)) * np.float32(scale)
-    got = run_shared(ctx, q, kp, vp, table, lens, starts, prefix, nkv, dt, **kw)
-    close(got, decode64(q, kwd, vwd, rows_shared(table, starts, prefix, of, lens), nkv), f"{nh}/{nkv} {prefix}")
+    ref = decode64(q, kwd, vwd, rows_shared(table, starts, prefix, of, lens), nkv)
+    close(run_shared(ctx, q, kp, vp, table, lens, starts, prefix, nkv, dt, **kw), ref, f"{nh}/{nkv} {prefix}")
+    if prefix:
+        wide, room = once_for_all(table, nkv, max(prefix))
+        kw.setdefault("max_tail", table.shape[1] * PR)
+        close(run_shared(ctx, q, kp, vp, wide, lens, starts, prefix, nkv, dt, max_prefix=room, **kw), ref,
+              f"{nh}/{nkv} {prefix}, once for all")
     no_fault(ctx)
 
 
@@ -637,14 +652,20 @@ def test_shared_ignores_what_lies_outside(ctx, dt):
         a[~used] = bad
         b[~used] = bad
         close(run_shared(ctx, q, store(a, dt), store(b, dt), table, lens, starts, prefix, 2, dt), ref, f"{bad}")
+        wide, room = once_for_all(table, 2, 37)
+        close(run_shared(ctx, q, store(a, dt), store(b, dt), wide, lens, starts, prefix, 2, dt, max_prefix=room), ref,
+              f"{bad}, once for all")
     no_fault(ctx)
 
 
-def test_shared_errors(ctx):
-    """Lengths and prefixes outside the call's bounds: NaN for those sequences and bit 1, the others unharmed."""
+@pytest.mark.parametrize("more", [0, 400])
+def test_shared_errors(ctx, more):
+    """Lengths and prefixes outside the call's bounds: NaN for those sequences and bit 1, the others unharmed;
+    prefixes that every sequence reads itself, and longer ones that are read once."""
     rng = np.random.default_rng(37)
-    starts, prefix = [0, 3, 5], [50, 80]
-    lens = np.array([60, 49, 0, 85, 400], np.int32)  # 49 is shorter than its prefix, 400 - 80 longer than max_tail
+    starts, prefix = [0, 3, 5], [50 + more, 80 + more]
+    # the second is shorter than its prefix, the last's own rows are more than max_tail
+    lens = np.array([60 + more, 49 + more, 0, 85 + more, 400 + more], np.int32)
     table, total, of = shared_tables(rng, starts, prefix, lens)
     kp, kw = make_pool(570, total, 2, F32)
     vp, vw = make_pool(571, total, 2, F32)
@@ -652,11 +673,12 @@ def test_shared_errors(ctx):
     ok = lens.copy()
     ok[[1, 4]] = 0
     ref = decode64(q, kw, vw, rows_shared(table, starts, prefix, of, ok), 2)
-    got = run_shared(ctx, q, kp, vp, table, lens, starts, prefix, 2, F32, max_prefix=80, max_tail=300)
+    got = run_shared(ctx, q, kp, vp, table, lens, starts, prefix, 2, F32, max_prefix=80 + more, max_tail=300)
     assert np.isnan(got[[1, 4]]).all()
     close(got[[0, 2, 3]], ref[[0, 2, 3]], "others")
     assert ctx.check_device_error() == FAULT
-    got = run_shared(ctx, q, kp, vp, table, ok, starts, prefix, 2, F32, max_prefix=79)  # group 1's prefix is too long
+    # the second group's prefix is too long
+    got = run_shared(ctx, q, kp, vp, table, ok, starts, prefix, 2, F32, max_prefix=79 + more)
     assert np.isnan(got[3]).all()
     close(got[[0, 1, 2, 4]], ref[[0, 1, 2, 4]], "others")
     assert ctx.check_device_error() == FAULT
@@ -745,7 +767,7 @@ def test_captured_step_replays(ctx):
     nh, nkv, n, top, dt = 14, 2, 4, 6, BF16
     rng = np.random.default_rng(42)
     base = np.array([300, 200, 250, 490], np.int32)
-    table, n_pages = tables(rng, base + 8)
+    table, n_pages = tables(rng, base + 8, width=1030)
     kp, _ = make_pool(630, n_pages, nkv, dt)
     vp, _ = make_pool(631, n_pages, nkv, dt)
     W = table.shape[1]
@@ -755,7 +777,7 @@ def test_captured_step_replays(ctx):
     db = ctx.upload((b0.view(np.uint32) >> 16).astype(np.uint16))
     dx, dq = ctx.empty((n, nh + 2 * nkv, 64)), ctx.empty((n, nh, 64))
     dpos, dlen, dstart = ctx.empty(n, np.int32), ctx.empty(n, np.int32), ctx.upload(np.arange(n + 1, dtype=np.int32))
-    dsel, o1, o2 = ctx.empty((n, nkv, top), np.int32), ctx.empty((n, nh, 64)), ctx.empty((n, nh, 64))
+    dsel, o1, o2, o3 = ctx.empty((n, nkv, top), np.int32), *(ctx.empty((n, nh, 64)) for _ in range(3))
     dg, dpre = ctx.upload(np.array([0, 2, 4], np.int32)), ctx.upload(np.array([150, 64], np.int32))
     stride = (nh + 2 * nkv) * 64
 
@@ -765,12 +787,13 @@ def test_captured_step_replays(ctx):
         ctx.kv_page_bounds(dkp, n_pages, dtab, W, dpos, dlen, db, n, nkv, 64, 1, stream=s, kv_dtype=dt)
         ctx.select_pages(dq, db, n_pages, dtab, W, dlen, dsel, n, nh, nkv, 64, 500, top, 1, 1, stream=s)
         ctx.decode_selected(dq, dkp, dvp, n_pages, dtab, W, dlen, dsel, top, o1, n, nh, nkv, 64, stream=s, kv_dtype=dt)
-        ctx.decode_shared(dq, dkp, dvp, n_pages, dtab, W, dlen, dg, dpre, 2, o2, n, nh, nkv, 64, 160, 500, stream=s,
-                          kv_dtype=dt)
+        for o, room in ((o2, 160), (o3, 16400)):  # the prefix read by every sequence, and once for all
+            ctx.decode_shared(dq, dkp, dvp, n_pages, dtab, W, dlen, dg, dpre, 2, o, n, nh, nkv, 64, room, 500, stream=s,
+                              kv_dtype=dt)
 
     def results():
         ctx.synchronize(s)
-        return [d.numpy() for d in (dq, dkp, dvp, db, dsel, o1, o2)]
+        return [d.numpy() for d in (dq, dkp, dvp, db, dsel, o1, o2, o3)]
 
     def load(i):
         dx.copy_from(oracle.normal(640 + i, (n, nh + 2 * nkv, 64)), s)
@@ -832,10 +855,12 @@ def test_same_call_same_bits_and_two_streams_of_two_contexts(ctx):
     no_fault(ctx)
 
 
-def test_offsets_beyond_32_bits(ctx):
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_offsets_beyond_32_bits(ctx, dt):
     """A pool of more than 2^32 bytes whose last pages are used: page offsets need 64 bits."""
-    n_pages = (1 << 32) // (PR * 256) + 40  # one kv head, fp32: 4 KiB a page
-    dk, dv = ctx.empty((n_pages, PR, 1, 64)), ctx.empty((n_pages, PR, 1, 64))
+    kind = np.float32 if dt == F32 else np.uint16
+    n_pages = (1 << 32) // (PR * 64 * np.dtype(kind).itemsize) + 40  # one kv head
+    dk, dv = ctx.empty((n_pages, PR, 1, 64), kind), ctx.empty((n_pages, PR, 1, 64), kind)
     lens = np.array([40], np.int32)
     table = np.array([[n_pages - 1, 5, n_pages - 20]], np.int32)
     x = oracle.normal(670, (40, 6, 64))
@@ -843,17 +868,21 @@ def test_offsets_beyond_32_bits(ctx):
     dq = ctx.empty((40, 4, 64))
     dtab = ctx.upload(table)
     ctx.kv_append_paged(dx.ptr, 384, dq, dx.at(256), 384, dx.at(320), 384, dk, dv, n_pages, dtab, 3,
-                        ctx.upload(np.array([0, 40], np.int32)), ctx.upload(np.zeros(1, np.int32)), 1, 40, 4, 1, 64, 48)
+                        ctx.upload(np.array([0, 40], np.int32)), ctx.upload(np.zeros(1, np.int32)), 1, 40, 4, 1, 64, 48,
+                        kv_dtype=dt)
     k = np.stack([oracle.rope_heads(x[p, 4], 1, 64, p) for p in range(40)]).reshape(40, 64)
     q = dq.numpy()[39:]
-    ref = attend64(q[0], k, x[:, 5])[None]
+    ref = attend64(q[0], widen(store(k, dt), dt), widen(store(x[:, 5], dt), dt))[None]
     dlen, dout = ctx.upload(lens), ctx.empty((1, 4, 64))
     dsel = ctx.upload(np.array([[[0, 1, 2]]], np.int32))
-    ctx.decode_selected(dq.at(39 * 256), dk, dv, n_pages, dtab, 3, dlen, dsel, 3, dout, 1, 4, 1, 64)
+    ctx.decode_selected(dq.at(39 * 256), dk, dv, n_pages, dtab, 3, dlen, dsel, 3, dout, 1, 4, 1, 64, kv_dtype=dt)
     close(dout.numpy(), ref, "selected")
-    ctx.decode_shared(dq.at(39 * 256), dk, dv, n_pages, dtab, 3, dlen, ctx.upload(np.array([0, 1], np.int32)),
-                      ctx.upload(np.array([20], np.int32)), 1, dout, 1, 4, 1, 64, 20, 20)
-    close(dout.numpy(), ref, "shared")
+    wide, room = once_for_all(table, 1, 20)
+    for t, most in ((table, 20), (wide, room)):
+        ctx.decode_shared(dq.at(39 * 256), dk, dv, n_pages, ctx.upload(t), t.shape[1], dlen,
+                          ctx.upload(np.array([0, 1], np.int32)), ctx.upload(np.array([20], np.int32)), 1, dout, 1, 4, 1,
+                          64, most, 20, kv_dtype=dt)
+        close(dout.numpy(), ref, "shared")
     for d in (dk, dv):
         d.free()
     no_fault(ctx)

@@ -258,10 +258,10 @@ struct PagedAttnArgs {
     const int32_t* group_starts;  // [n_groups + 1]
     const int32_t* prefix_lens;   // [n_groups]
     int n_groups, max_prefix, max_tail;
-    int prefix_splits;       // slots 0 .. prefix_splits - 1: runs of the prefix, at most
+    int prefix_splits;       // slots 0 .. prefix_splits - 1: runs of the prefix, at most; 0: a sequence reads it itself
     int prefix_groups;       // workgroups of the prefix kernel that share its units
     int prefix_blocks;       // blocks of kSharedCols (sequence, query head) columns, at most
-    int tail_splits, tail_rows;  // slots behind them: runs of tail_rows own rows
+    int tail_splits, tail_rows;  // slots behind them: runs of tail_rows own rows (of all, if it reads the prefix itself)
 };
 constexpr int kPagedWaves = 4;    // waves per workgroup
 constexpr int kSharedWaves = 8;   // the same, shared prefixes

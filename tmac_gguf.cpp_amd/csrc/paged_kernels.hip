@@ -1273,24 +1273,31 @@ __device__ __forceinline__ int run_pages(int64_t prefix, int runs) {
 // len) through its own pages.  Its group is the last one that holds it.
 struct SharedSeq {
     int64_t prefix, len;
-    int slots;  // partials that the prefix left
+    int64_t own;  // first row that the sequence reads itself
+    int leader;   // the group's first sequence
+    int slots;    // partials that the prefix left
     bool bad;   // a length or prefix outside what the launch covers
 };
 __device__ __forceinline__ SharedSeq shared_seq(const PagedAttnArgs& a, int s, int lane) {
     SharedSeq r;
     r.len = max(a.lengths[s], 0);
     r.prefix = 0;
+    r.leader = s;
     int n_blocks = 0;
     for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
         const Group g = group_at(a, g0 + lane);
         const uint64_t b = __ballot(s >= g.first && s < g.end);
-        if (b) r.prefix = __builtin_amdgcn_readlane(g.prefix, 63 - __clzll(b));
+        if (b) {
+            r.prefix = __builtin_amdgcn_readlane(g.prefix, 63 - __clzll(b));
+            r.leader = __builtin_amdgcn_readlane(g.first, 63 - __clzll(b));
+        }
         n_blocks += (int)__builtin_amdgcn_readfirstlane(wave_sum_u((unsigned)blocks_of(a, g)));
     }
     r.bad = r.len > 0 && (r.prefix > a.max_prefix || r.len < r.prefix || r.len - r.prefix > a.max_tail ||
                           r.len > (int64_t)a.max_pages * kPageRows);
     const int64_t per = (int64_t)run_pages(r.prefix, prefix_runs(a, min(n_blocks, a.prefix_blocks))) * kPageRows;
-    r.slots = r.bad || r.len == 0 ? 0 : (int)((r.prefix + per - 1) / per);
+    r.own = a.prefix_splits ? r.prefix : 0;
+    r.slots = r.bad || r.len == 0 ? 0 : (int)((r.own + per - 1) / per);
     return r;
 }
 
@@ -1680,12 +1687,16 @@ __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
     Own<T>::query(raw, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, lane);
     const SharedSeq q = shared_seq(a, s, lane);
     Own<T>::init(st, raw, a.qscale);
-    const int64_t lo = q.prefix + (int64_t)split * a.tail_rows, hi = min(q.len, lo + a.tail_rows);
+    const int64_t lo = q.own + (int64_t)split * a.tail_rows, hi = min(q.len, lo + a.tail_rows);
     if (!FINISH && (q.bad || lo >= hi)) return;
-    if (!q.bad && lo < hi) {
-        const int j0 = (int)(lo >> kPageShift), n = (int)((hi - 1) >> kPageShift) - j0 + 1;
-        const int32_t* table = a.block_table + (size_t)s * a.max_pages;
-        attend_run<T, kPagedWaves>(st, a, h, n, lo, hi, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
+    // rows of the prefix through the first sequence's table, then its own
+#pragma unroll 1
+    for (int part = lo < q.prefix ? 0 : 1; part < 2; ++part) {
+        const int64_t r0 = part ? max(lo, q.prefix) : lo, r1 = part ? hi : min(hi, q.prefix);
+        if (q.bad || r0 >= r1) continue;
+        const int j0 = (int)(r0 >> kPageShift), n = (int)((r1 - 1) >> kPageShift) - j0 + 1;
+        const int32_t* table = a.block_table + (size_t)(part ? s : q.leader) * a.max_pages;
+        attend_run<T, kPagedWaves>(st, a, h, n, r0, r1, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
             logical = j0 + e;
             page = table[logical];
             if (page < 0 || page >= a.n_pages) {
@@ -1746,7 +1757,7 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     const int s = __builtin_amdgcn_readfirstlane((int)(row / a.n_head));
     const SharedSeq q = shared_seq(a, s, lane);
     const int n0 = q.slots;
-    const int n1 = q.bad || q.len == 0 ? 0 : (int)((q.len - q.prefix + a.tail_rows - 1) / a.tail_rows);
+    const int n1 = q.bad || q.len == 0 ? 0 : (int)((q.len - q.own + a.tail_rows - 1) / a.tail_rows);
     float L;
     f32x4 y = merge_slots<WPR>(a, row, n0, a.prefix_splits, n1, wave % WPR, lane, L);
     if (wave % WPR || lane >= 16) return;

@@ -1695,6 +1695,13 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
 
 constexpr int kTailWholeRows = 1024;  // own rows that one workgroup takes without help
 constexpr int kFinishSlots = 16;     // prefix partials that the own rows' workgroup merges itself
+// Prefix rows, times sequences and kv heads, up to which every sequence reads the prefix itself, and of fp32 caches the
+// rows of one prefix: a launch less (one less again without partials) against rows that all read.  Kernels of a call,
+// shared / alone, us: bf16, 14 heads on 2: 1 x 256 rows 12.3 / 7.9, 96 x 256 14.9 / 8.5, 256 x 256 17.2 / 10.8,
+// 16 x 2,048 15.8 / 12.6, 45 x 2,048 16.4 / 16.6, 96 x 1,400 17.7 / 23.0, 16 x 16,384 22.0 / 23.0, 45 x 16,384 27.4 / 62.3;
+// Q8_0: 16 x 256 16.6 / 9.4, 45 x 2,048 17.2 / 18.8; fp32, whose own rows take the fp32 products: 5 x 256 15.0 / 11.0,
+// 5 x 384 14.7 / 13.2, 5 x 512 15.2 / 15.3.
+constexpr int kAloneRows = 1 << 17, kAloneRowsF32 = 384;
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                  const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                  int max_pages, const int32_t* lengths, const int32_t* group_starts,
@@ -1725,8 +1732,10 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     // can be.  (45 sequences of 32 heads on 8 kv heads in 3 uneven groups, fp32, 2,500 rows: 19.2 us, 23.4 with the
     // runs of the fewest blocks whatever there are, since some CUs then take two.)
     const int64_t least = std::max<int64_t>(n_groups, cdiv(n_seq * group, tmac::kSharedCols));
+    const bool alone =
+        n_sk * max_prefix <= kAloneRows && (kv_dtype != TMAC_KV_F32 || max_prefix <= kAloneRowsF32);
     const int64_t blocks =
-        n_groups && max_prefix ? std::min<int64_t>(n_seq, n_seq * group / tmac::kSharedCols + n_groups) : 0;
+        n_groups && !alone ? std::min<int64_t>(n_seq, n_seq * group / tmac::kSharedCols + n_groups) : 0;
     a.prefix_blocks = (int)blocks;
     a.prefix_splits = 0;
     if (blocks) {
@@ -1735,15 +1744,17 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
         a.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
         a.prefix_groups = ctx->n_cu;
     }
-    // Own rows: one run a sequence unless they are many and the sequences few, and then, with few prefix partials, its
-    // workgroup merges them and writes the output.
-    a.tail_rows = (int)std::max<int64_t>(kPageRows, cdiv(max_tail, kPageRows) * kPageRows);
-    if (n_sk < 2 * ctx->n_cu && max_tail > kTailWholeRows) {
-        const int64_t splits = std::min<int64_t>({cdiv(2 * ctx->n_cu, n_sk), cdiv(2 * max_tail, kTailWholeRows),
+    // Own rows (all of them where a sequence reads the prefix itself): one run a sequence unless they are many and the
+    // sequences few, and then, with few prefix partials, its workgroup merges them and writes the output.
+    const int64_t own = n_groups && alone ? std::min<int64_t>((int64_t)max_prefix + max_tail, (int64_t)max_pages * kPageRows)
+                                         : max_tail;
+    a.tail_rows = (int)std::max<int64_t>(kPageRows, cdiv(own, kPageRows) * kPageRows);
+    if (n_sk < 2 * ctx->n_cu && own > kTailWholeRows) {
+        const int64_t splits = std::min<int64_t>({cdiv(2 * ctx->n_cu, n_sk), cdiv(2 * own, kTailWholeRows),
                                                   (int64_t)kMaxSplits});
-        a.tail_rows = (int)(cdiv(cdiv(max_tail, splits), kPageRows) * kPageRows);
+        a.tail_rows = (int)(cdiv(cdiv(own, splits), kPageRows) * kPageRows);
     }
-    a.tail_splits = (int)cdiv(max_tail, a.tail_rows);
+    a.tail_splits = (int)cdiv(own, a.tail_rows);
     const bool finish = a.tail_splits <= 1 && a.prefix_splits <= kFinishSlots;
     a.n_slots = a.prefix_splits + (finish ? 0 : a.tail_splits);
     if ((rc = check_units(ctx, what, blocks * n_kv_head * a.prefix_splits + tmac::kXcds)) ||
