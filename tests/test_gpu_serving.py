@@ -552,7 +552,7 @@ def run_shared(ctx, q, kp, vp, table, lens, starts, prefix, nkv, dt, max_prefix=
 
 def once_for_all(table, nkv, longest):
     """(table, max_prefix) with room for a prefix so long that it is read once for all sequences."""
-    room = max(longest, (1 << 17) // (len(table) * nkv) + 1)
+    room = max(longest, (3 << 16) // (len(table) * nkv) + 1)
     wide = np.full((len(table), max(table.shape[1], -(-room // PR))), 2 ** 30, np.int32)
     wide[:, :table.shape[1]] = table
     return wide, room
@@ -767,7 +767,7 @@ def test_captured_step_replays(ctx):
     nh, nkv, n, top, dt = 14, 2, 4, 6, BF16
     rng = np.random.default_rng(42)
     base = np.array([300, 200, 250, 490], np.int32)
-    table, n_pages = tables(rng, base + 8, width=1030)
+    table, n_pages = tables(rng, base + 8, width=1540)
     kp, _ = make_pool(630, n_pages, nkv, dt)
     vp, _ = make_pool(631, n_pages, nkv, dt)
     W = table.shape[1]
@@ -787,7 +787,7 @@ def test_captured_step_replays(ctx):
         ctx.kv_page_bounds(dkp, n_pages, dtab, W, dpos, dlen, db, n, nkv, 64, 1, stream=s, kv_dtype=dt)
         ctx.select_pages(dq, db, n_pages, dtab, W, dlen, dsel, n, nh, nkv, 64, 500, top, 1, 1, stream=s)
         ctx.decode_selected(dq, dkp, dvp, n_pages, dtab, W, dlen, dsel, top, o1, n, nh, nkv, 64, stream=s, kv_dtype=dt)
-        for o, room in ((o2, 160), (o3, 16400)):  # the prefix read by every sequence, and once for all
+        for o, room in ((o2, 160), (o3, 24600)):  # the prefix read by every sequence, and once for all
             ctx.decode_shared(dq, dkp, dvp, n_pages, dtab, W, dlen, dg, dpre, 2, o, n, nh, nkv, 64, room, 500, stream=s,
                               kv_dtype=dt)
 

@@ -199,10 +199,10 @@ def test_shared_grid(fake):
         cuts = [[i * n_seq // n_groups for i in range(n_groups + 1)], [0] * n_groups + [n_seq],
                 list(range(n_groups)) + [n_seq], [0] + [n_seq - n_groups + i for i in range(1, n_groups + 1)]]
         need = max(sum(-(-(b - a) * 7 // 64) for a, b in zip(c, c[1:])) for c in cuts)
-        args = dict(n_seq=n_seq, n_groups=n_groups, max_tail=0, max_pages=8192)
-        room = 2 ** 17 // (2 * n_seq)  # 2 kv heads: rows that every sequence reads itself
+        args = dict(n_seq=n_seq, n_groups=n_groups, max_tail=0, max_pages=16384)
+        room = 3 * 2 ** 16 // (2 * n_seq)  # 2 kv heads: rows that every sequence reads itself
         rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=min(room, 384), **args)
-        assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_tail_finish_f32"]
+        assert rc == TMAC_OK and launches[0][0].startswith("tmac_tail_")
         rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=max(room, 384) + 1, **args)
         assert rc == TMAC_OK and launches[0][0] == "tmac_prefix_f32"
         assert launches[0][1] % 8 == 0 and min(2 * need, 256) <= launches[0][1] <= 256

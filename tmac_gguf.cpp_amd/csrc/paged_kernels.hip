@@ -1675,9 +1675,9 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
 // A sequence's own rows: workgroup (run of them, kv head, sequence).  FINISH:
 // one run holds them all, and the workgroup merges the prefix's partials and
 // writes the output; otherwise the run leaves one more partial.
-template <typename T, bool FINISH>
+template <typename T, int NW, bool FINISH>
 __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
-    __shared__ OwnLds<T, kPagedWaves> lds;
+    __shared__ OwnLds<T, NW> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.group, split = FINISH ? 0 : blockIdx.x, h = blockIdx.y, s = blockIdx.z;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
@@ -1696,7 +1696,7 @@ __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
         if (q.bad || r0 >= r1) continue;
         const int j0 = (int)(r0 >> kPageShift), n = (int)((r1 - 1) >> kPageShift) - j0 + 1;
         const int32_t* table = a.block_table + (size_t)(part ? s : q.leader) * a.max_pages;
-        attend_run<T, kPagedWaves>(st, a, h, n, r0, r1, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
+        attend_run<T, NW>(st, a, h, n, r0, r1, lds.own[wave], wave, lane, [&](int e, int& logical, int& page) {
             logical = j0 + e;
             page = table[logical];
             if (page < 0 || page >= a.n_pages) {
@@ -1705,7 +1705,7 @@ __device__ __forceinline__ void tail_body(const PagedAttnArgs& a) {
             }
         });
     }
-    merge_waves<T, kPagedWaves>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
+    merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         if constexpr (FINISH) {
             const int n = q.slots;
@@ -1780,10 +1780,13 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
         prefix_body<T>(a);                                                                                             \
     }                                                                                                                  \
     extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_tail_##NAME(PagedAttnArgs a) {                 \
-        tail_body<T, false>(a);                                                                                        \
+        tail_body<T, kPagedWaves, false>(a);                                                                           \
     }                                                                                                                  \
     extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_tail_finish_##NAME(PagedAttnArgs a) {          \
-        tail_body<T, true>(a);                                                                                         \
+        tail_body<T, kPagedWaves, true>(a);                                                                            \
+    }                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_tail_finish_wide_##NAME(PagedAttnArgs a) {    \
+        tail_body<T, kSharedWaves, true>(a);                                                                           \
     }
 TMAC_PAGED_KERNELS(f32, float)
 TMAC_PAGED_KERNELS(bf16, __bf16)

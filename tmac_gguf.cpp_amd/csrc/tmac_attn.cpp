@@ -139,7 +139,7 @@ struct tmac_context {
                   k_cvt_q8 = nullptr;
     // serving operators on paged caches, by kv_dtype; page scores: up to 4 query heads per kv head, more
     hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_scores[2] = {};
-    hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[4] = {};  // shared prefixes, own rows
+    hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[2][4] = {};  // shared prefixes, own rows
     hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
@@ -1058,7 +1058,8 @@ int tmac_init(tmac_context** out, int device) {
                                                                       {"tmac_selected", &ctx->k_selected[dt]},
                                                                       {"tmac_prefix", &ctx->k_prefix[dt]},
                                                                       {"tmac_tail", &ctx->k_tail[dt]},
-                                                                      {"tmac_tail_finish", &ctx->k_tail_finish[dt]}};
+                                                                      {"tmac_tail_finish", &ctx->k_tail_finish[0][dt]},
+                                                                      {"tmac_tail_finish_wide", &ctx->k_tail_finish[1][dt]}};
             for (auto& k : by_type) {
                 std::snprintf(name, sizeof(name), "%s_%s", k.first, kTypeName[dt]);
                 if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
@@ -1694,14 +1695,15 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
 }
 
 constexpr int kTailWholeRows = 1024;  // own rows that one workgroup takes without help
+constexpr int kTailNarrowRows = 192;  // own rows up to which four waves do
 constexpr int kFinishSlots = 16;     // prefix partials that the own rows' workgroup merges itself
 // Prefix rows, times sequences and kv heads, up to which every sequence reads the prefix itself, and of fp32 caches the
-// rows of one prefix: a launch less (one less again without partials) against rows that all read.  Kernels of a call,
-// shared / alone, us: bf16, 14 heads on 2: 1 x 256 rows 12.3 / 7.9, 96 x 256 14.9 / 8.5, 256 x 256 17.2 / 10.8,
-// 16 x 2,048 15.8 / 12.6, 45 x 2,048 16.4 / 16.6, 96 x 1,400 17.7 / 23.0, 16 x 16,384 22.0 / 23.0, 45 x 16,384 27.4 / 62.3;
-// Q8_0: 16 x 256 16.6 / 9.4, 45 x 2,048 17.2 / 18.8; fp32, whose own rows take the fp32 products: 5 x 256 15.0 / 11.0,
-// 5 x 384 14.7 / 13.2, 5 x 512 15.2 / 15.3.
-constexpr int kAloneRows = 1 << 17, kAloneRowsF32 = 384;
+// rows of one prefix: a launch less (one less again without partials) against rows that all read.  Kernels of a call
+// with 64 own rows, 14 heads on 2, shared / alone, us: bf16: 1 x 256 rows 12.3 / 7.0, 96 x 256 14.9 / 7.6, 96 x 900
+// 15.8 / 12.2, 16 x 2,048 15.8 / 12.6, 45 x 2,048 16.0 / 15.8, 8 x 10,000 19.0 / 16.4, 96 x 1,400 17.7 / 23.0, 16 x 16,384
+// 22.0 / 23.0, 45 x 16,384 27.4 / 62.3; Q8_0: 96 x 900 17.7 / 14.9, 45 x 2,048 18.0 / 18.6; fp32, whose own rows take the
+// fp32 products: 5 x 256 15.0 / 9.6, 200 x 384 18.3 / 18.6, 5 x 2,048 16.0 / 17.1.
+constexpr int kAloneRows = 3 << 16, kAloneRowsF32 = 384;
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                  const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                  int max_pages, const int32_t* lengths, const int32_t* group_starts,
@@ -1770,10 +1772,15 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     if (blocks && (rc = launch(ctx, ctx->k_prefix[kv_dtype], (unsigned)(cdiv(units, tmac::kXcds) * tmac::kXcds), 1,
                                threads, (hipStream_t)stream, &a)))
         return rc;
+    if (finish) {
+        // 8 waves where a CU has no more than one workgroup and they have rows enough (14 heads on 2, 16 sequences, bf16 and
+        // Q8_0: 320 rows 8.3 -> 7.4 and 9.3 -> 7.9 us, 764 rows 12.1 -> 10.3 and 15.2 -> 11.8; 128 rows 6.7 -> 7.0; 256
+        // sequences, 128 rows 8.0 -> 12.2)
+        const bool wide = n_sk <= ctx->n_cu && own > kTailNarrowRows;
+        return launch(ctx, ctx->k_tail_finish[wide][kv_dtype], 1, (unsigned)n_kv_head,
+                      64 * (wide ? tmac::kSharedWaves : tmac::kPagedWaves), (hipStream_t)stream, &a, (unsigned)n_seq);
+    }
     const unsigned tail_threads = 64 * tmac::kPagedWaves;
-    if (finish)
-        return launch(ctx, ctx->k_tail_finish[kv_dtype], 1, (unsigned)n_kv_head, tail_threads, (hipStream_t)stream, &a,
-                      (unsigned)n_seq);
     if (a.tail_splits && (rc = launch(ctx, ctx->k_tail[kv_dtype], (unsigned)a.tail_splits, (unsigned)n_kv_head,
                                       tail_threads, (hipStream_t)stream, &a, (unsigned)n_seq)))
         return rc;
