@@ -405,7 +405,7 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
  * the other sequences' tables for pages wholly inside the prefix are not read.)  A sequence in no
  * group has no prefix.  The result is tmac_attention_decode_paged's, up to rounding, where the tables
  * agree on the prefix.  Length 0 gives a zero output.  prefix_lens[g] <= max_prefix and lengths[s] -
- * prefix <= max_tail (both size the grid; each <= 16 * max_pages), and a length above 0 is at least
+ * prefix <= max_tail (both size the grid; more than 16 * max_pages is as much), and a length above 0 is at least
  * its prefix and at most 16 * max_pages: otherwise the sequence's output is NaN and bit 1 is set.  A
  * block-table entry outside the pool is clamped and sets bit 2.  n_groups = 0: group_starts and
  * prefix_lens may be null. */

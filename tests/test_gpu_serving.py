@@ -405,9 +405,9 @@ def test_selected_shapes(ctx, dt, nh, nkv):
 
 @pytest.mark.parametrize("dt", ALL_DT)
 def test_selected_long_lists(ctx, dt):
-    """Lists that fill several lookups of a wave (over 256 pages a workgroup) and many splits."""
+    """Lists that fill several lookups of a wave (over 64 pages each), in many splits, in eight waves and in four."""
     rng = np.random.default_rng(31)
-    for n, top in ((1, 700), (130, 300)):
+    for n, top in ((1, 700), (130, 600), (300, 300)):
         lens = np.full(n, 16 * 710 - 3, np.int32)
         table = rng.integers(0, 900, (n, 710)).astype(np.int32)
         kp, kw = make_pool(410, 900, 1, dt)
@@ -552,7 +552,7 @@ def run_shared(ctx, q, kp, vp, table, lens, starts, prefix, nkv, dt, max_prefix=
 
 def once_for_all(table, nkv, longest):
     """(table, max_prefix) with room for a prefix so long that it is read once for all sequences."""
-    room = max(longest, (3 << 16) // (len(table) * nkv) + 1)
+    room = max(longest, (9 << 15) // (len(table) * nkv) + 1)
     wide = np.full((len(table), max(table.shape[1], -(-room // PR))), 2 ** 30, np.int32)
     wide[:, :table.shape[1]] = table
     return wide, room
@@ -631,6 +631,8 @@ def test_shared_without_groups_or_tails(ctx):
     # a padded batch: lengths of zero, the group's first sequence among them (its table still holds the prefix)
     shared_case(ctx, Q8, 14, 2, [0, 5], [100], [5, 6, 7, 8, 9], 552, zero=(0, 3))
     shared_case(ctx, F32, 14, 2, [0, 3], [100], [5, 6, 7], 553, zero=(0, 1, 2))
+    # bounds that are more than the table holds
+    shared_case(ctx, BF16, 14, 2, [0, 3], [100], [5, 6, 7], 554, max_tail=10 ** 6)
 
 
 @pytest.mark.parametrize("dt", [F32, BF16, F16])

@@ -137,8 +137,7 @@ def test_shapes_outside_the_domain(fake, name):
     ("tmac_attention_decode_selected", dict(top=0), TMAC_ERR_INVALID_ARG),
     ("tmac_attention_decode_shared", dict(n_groups=-1), TMAC_ERR_INVALID_ARG),
     ("tmac_attention_decode_shared", dict(max_prefix=-1), TMAC_ERR_INVALID_ARG),
-    ("tmac_attention_decode_shared", dict(max_prefix=641), TMAC_ERR_INVALID_ARG),
-    ("tmac_attention_decode_shared", dict(max_tail=641), TMAC_ERR_INVALID_ARG),
+    ("tmac_attention_decode_shared", dict(max_tail=-1), TMAC_ERR_INVALID_ARG),
     # more units of work than a grid can number
     ("tmac_kv_page_bounds", dict(n_seq=2 ** 31 - 1, max_pages=2 ** 27, max_new=2 ** 31 - 1), TMAC_ERR_INVALID_ARG),
     ("tmac_select_pages", dict(n_seq=2 ** 31 - 1, max_pages=2 ** 27, max_len=2 ** 31 - 1), TMAC_ERR_INVALID_ARG),
@@ -162,6 +161,9 @@ def test_legal_edges(fake):
     assert fake.call("tmac_kv_append_paged", n_rows=0) == (TMAC_OK, [])
     assert fake.call("tmac_kv_page_bounds", max_new=0) == (TMAC_OK, [])
     assert ok("tmac_attention_decode_shared", n_groups=0, group_starts=None, prefix_lens=None)
+    # bounds beyond the table are the table's
+    assert fake.call("tmac_attention_decode_shared", max_prefix=2 ** 31 - 1, max_tail=2 ** 31 - 1) == fake.call(
+        "tmac_attention_decode_shared", max_prefix=640, max_tail=640)
     # no rows possible: the last launch alone writes the zero outputs
     rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=0, max_tail=0)
     assert rc == TMAC_OK and [k for k, _ in launches] == ["tmac_tail_finish_f32"]
@@ -200,7 +202,7 @@ def test_shared_grid(fake):
                 list(range(n_groups)) + [n_seq], [0] + [n_seq - n_groups + i for i in range(1, n_groups + 1)]]
         need = max(sum(-(-(b - a) * 7 // 64) for a, b in zip(c, c[1:])) for c in cuts)
         args = dict(n_seq=n_seq, n_groups=n_groups, max_tail=0, max_pages=16384)
-        room = 3 * 2 ** 16 // (2 * n_seq)  # 2 kv heads: rows that every sequence reads itself
+        room = (9 * 2 ** 15 if n_seq >= 64 else 3 * 2 ** 16) // (2 * n_seq)  # 2 kv heads: rows that every sequence reads itself
         rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=min(room, 384), **args)
         assert rc == TMAC_OK and launches[0][0].startswith("tmac_tail_")
         rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=max(room, 384) + 1, **args)

@@ -1136,9 +1136,8 @@ __device__ __forceinline__ void put_partial(const PagedAttnArgs& a, int64_t row,
 }
 
 // Over a list: workgroup (split, kv head, sequence).
-template <typename T>
+template <typename T, int NW>
 __device__ __forceinline__ void selected_body(const PagedAttnArgs& a) {
-    constexpr int NW = kPagedWaves;
     __shared__ OwnLds<T, NW> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv = a.n_kv_head, G = a.group;
@@ -1775,7 +1774,12 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
 #define TMAC_PAGED_KERNELS(NAME, T)                                                                                    \
     extern "C" __global__ __launch_bounds__(256) void tmac_append_##NAME(AppendArgs a) { append_body<T>(a); }          \
     extern "C" __global__ __launch_bounds__(256) void tmac_page_bounds_##NAME(BoundsArgs a) { bounds_body<T>(a); }     \
-    extern "C" __global__ __launch_bounds__(256) void tmac_selected_##NAME(PagedAttnArgs a) { selected_body<T>(a); }   \
+    extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_selected_##NAME(PagedAttnArgs a) {             \
+        selected_body<T, kPagedWaves>(a);                                                                              \
+    }                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_selected_wide_##NAME(PagedAttnArgs a) {       \
+        selected_body<T, kSharedWaves>(a);                                                                             \
+    }                                                                                                                  \
     extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_prefix_##NAME(PagedAttnArgs a) {               \
         prefix_body<T>(a);                                                                                             \
     }                                                                                                                  \

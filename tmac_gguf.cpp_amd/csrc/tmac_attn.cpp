@@ -138,7 +138,7 @@ struct tmac_context {
     hipFunction_t k_rope = nullptr, k_copy = nullptr, k_pos = nullptr, k_qkv = nullptr, k_cvt16 = nullptr,
                   k_cvt_q8 = nullptr;
     // serving operators on paged caches, by kv_dtype; page scores: up to 4 query heads per kv head, more
-    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[4] = {}, k_scores[2] = {};
+    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[2][4] = {}, k_scores[2] = {};
     hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[2][4] = {};  // shared prefixes, own rows
     hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
@@ -1055,7 +1055,8 @@ int tmac_init(tmac_context** out, int device) {
         for (int dt = 0; dt < 4; dt++) {
             const std::pair<const char*, hipFunction_t*> by_type[] = {{"tmac_append", &ctx->k_append[dt]},
                                                                       {"tmac_page_bounds", &ctx->k_bounds[dt]},
-                                                                      {"tmac_selected", &ctx->k_selected[dt]},
+                                                                      {"tmac_selected", &ctx->k_selected[0][dt]},
+                                                                      {"tmac_selected_wide", &ctx->k_selected[1][dt]},
                                                                       {"tmac_prefix", &ctx->k_prefix[dt]},
                                                                       {"tmac_tail", &ctx->k_tail[dt]},
                                                                       {"tmac_tail_finish", &ctx->k_tail_finish[0][dt]},
@@ -1665,6 +1666,21 @@ static int launch_paged_merge(tmac_context* ctx, tmac_stream stream, const hipFu
                   64 * tmac::kPagedWaves, (hipStream_t)stream, a);
 }
 
+// Pages that one workgroup attends for a (sequence, kv head) without help, n_sk of them in all: a launch and its partials
+// less, against waves that would share them.  Kernels, us, split / whole (14 heads on 2): 32 lists of 32 pages bf16 7.8 /
+// 8.1, of 64 8.7 / 10.6; fp32, whose products take four times as long, of 16 8.0 / 8.3, of 32 8.4 / 11.5.  128 lists
+// (half the CUs have one): bf16 64 pages 15.5 / 12.2, 128 21.0 / 17.4, 256 30.5 / 31.0, 500 46.6 / 56.2; fp32 32 16.1 /
+// 13.0, 64 20.4 / 20.1, 128 29.8 / 36.6.  200 lists: bf16 128 32.6 / 22.5, 500 82 / 68, fp32 500 135 / 132.  360 lists: bf16
+// 128 43.7 / 35.2, 500 121 / 113; fp32 128 72.6 / 71.8, 256 128 / 136, 500 195 / 243.
+static int64_t whole_pages(const tmac_context* ctx, int kv_dtype, int64_t n_sk) {
+    const bool f32 = kv_dtype == TMAC_KV_F32;
+    if (n_sk > ctx->n_cu) return f32 ? 128 : INT_MAX;
+    if (2 * n_sk > ctx->n_cu) return INT_MAX;
+    return 8 * n_sk >= 3 * ctx->n_cu ? (f32 ? 64 : 192) : (f32 ? 16 : 32);
+}
+// A whole list is taken by eight waves where a CU has no more than one, and by four if it is short (bf16, 16 lists: 8
+// pages 5.1 against 5.4, 16 pages 6.5 against 6.1) or there are more (512 of 8 pages 8.0 against 12.2).
+constexpr int kListNarrow = 8;
 int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                    const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                    int max_pages, const int32_t* lengths, const int32_t* selected, int top, float* out,
@@ -1681,14 +1697,15 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
     a.selected = selected;
     a.top = top;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head;
-    int64_t splits = std::min<int64_t>(cdiv(2 * ctx->n_cu, n_sk), cdiv(top, tmac::kPagedWaves));
+    const bool whole = top <= whole_pages(ctx, kv_dtype, n_sk), wide = whole && n_sk <= ctx->n_cu && top > kListNarrow;
+    int64_t splits = whole ? 1 : std::min<int64_t>(cdiv(2 * ctx->n_cu, n_sk), cdiv(top, tmac::kPagedWaves));
     splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
     a.per_split = (int)cdiv(top, splits);
     a.n_slots = (int)cdiv(top, a.per_split);
-    if ((rc = check_units(ctx, what, n_sk * a.n_slots, 64 * tmac::kPagedWaves)) || (rc = set_device(ctx))) return rc;
+    if ((rc = check_units(ctx, what, n_sk * a.n_slots, 64 * tmac::kSharedWaves)) || (rc = set_device(ctx))) return rc;
     if (a.n_slots > 1 && (rc = paged_partials(ctx, stream, &a))) return rc;
-    if ((rc = launch(ctx, ctx->k_selected[kv_dtype], (unsigned)(n_sk * a.n_slots), 1, 64 * tmac::kPagedWaves,
-                     (hipStream_t)stream, &a)) ||
+    if ((rc = launch(ctx, ctx->k_selected[wide][kv_dtype], (unsigned)(n_sk * a.n_slots), 1,
+                     64 * (wide ? tmac::kSharedWaves : tmac::kPagedWaves), (hipStream_t)stream, &a)) ||
         a.n_slots == 1)
         return rc;
     return launch_paged_merge(ctx, stream, ctx->k_selected_merge, &a);
@@ -1697,13 +1714,14 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
 constexpr int kTailWholeRows = 1024;  // own rows that one workgroup takes without help
 constexpr int kTailNarrowRows = 192;  // own rows up to which four waves do
 constexpr int kFinishSlots = 16;     // prefix partials that the own rows' workgroup merges itself
-// Prefix rows, times sequences and kv heads, up to which every sequence reads the prefix itself, and of fp32 caches the
-// rows of one prefix: a launch less (one less again without partials) against rows that all read.  Kernels of a call
-// with 64 own rows, 14 heads on 2, shared / alone, us: bf16: 1 x 256 rows 12.3 / 7.0, 96 x 256 14.9 / 7.6, 96 x 900
-// 15.8 / 12.2, 16 x 2,048 15.8 / 12.6, 45 x 2,048 16.0 / 15.8, 8 x 10,000 19.0 / 16.4, 96 x 1,400 17.7 / 23.0, 16 x 16,384
-// 22.0 / 23.0, 45 x 16,384 27.4 / 62.3; Q8_0: 96 x 900 17.7 / 14.9, 45 x 2,048 18.0 / 18.6; fp32, whose own rows take the
-// fp32 products: 5 x 256 15.0 / 9.6, 200 x 384 18.3 / 18.6, 5 x 2,048 16.0 / 17.1.
-constexpr int kAloneRows = 3 << 16, kAloneRowsF32 = 384;
+// Prefix rows, times sequences and kv heads, up to which every sequence reads the prefix itself (kAloneRowsMany: where
+// these are at least half as many as CUs), and of fp32 caches the rows of one prefix: a launch less (one less again
+// without partials) against rows that all read.  Kernels of a call with 64 own rows, 14 heads on 2, shared / alone, us:
+// bf16: 1 x 256 rows 12.3 / 7.0, 96 x 256 14.9 / 7.6, 16 x 2,048 15.8 / 12.6, 45 x 2,048 16.0 / 15.8, 45 x 3,000 20.4 /
+// 22.4, 16 x 16,384 22.0 / 23.0, 45 x 16,384 27.4 / 62.3; 96 x 1,400 17.0 / 14.4, 200 x 700 18.6 / 15.6, 200 x 1,200
+// 18.1 / 20.8; Q8_0: 45 x 2,048 18.6 / 18.6, 96 x 1,400 18.4 / 17.3, 200 x 700 20.0 / 20.4, 64 x 2,500 22.8 / 25.8; fp32,
+// whose own rows take the fp32 products: 5 x 256 15.0 / 9.6, 200 x 384 18.3 / 18.6, 5 x 2,048 16.0 / 17.1.
+constexpr int kAloneRows = 3 << 16, kAloneRowsMany = 9 << 15, kAloneRowsF32 = 384;
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                  const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                  int max_pages, const int32_t* lengths, const int32_t* group_starts,
@@ -1720,9 +1738,10 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
         return fail(ctx, TMAC_ERR_NULL_POINTER, "decode_shared: null group_starts or prefix_lens");
     if ((uintptr_t)group_starts % 4 || (uintptr_t)prefix_lens % 4)
         return fail(ctx, TMAC_ERR_MISALIGNED, "decode_shared: group_starts, prefix_lens");
-    if (max_prefix > (int64_t)max_pages * kPageRows || max_tail > (int64_t)max_pages * kPageRows)
-        return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_shared: max_prefix, max_tail <= 16 * max_pages");
     if (n_seq == 0) return TMAC_OK;
+    // no prefix and no length is beyond the table
+    max_prefix = (int)std::min<int64_t>(max_prefix, (int64_t)max_pages * kPageRows);
+    max_tail = (int)std::min<int64_t>(max_tail, (int64_t)max_pages * kPageRows);
     a.group_starts = group_starts;
     a.prefix_lens = prefix_lens;
     a.n_groups = n_groups;
@@ -1734,8 +1753,8 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     // can be.  (45 sequences of 32 heads on 8 kv heads in 3 uneven groups, fp32, 2,500 rows: 19.2 us, 23.4 with the
     // runs of the fewest blocks whatever there are, since some CUs then take two.)
     const int64_t least = std::max<int64_t>(n_groups, cdiv(n_seq * group, tmac::kSharedCols));
-    const bool alone =
-        n_sk * max_prefix <= kAloneRows && (kv_dtype != TMAC_KV_F32 || max_prefix <= kAloneRowsF32);
+    const bool alone = n_sk * max_prefix <= (2 * n_sk >= ctx->n_cu ? kAloneRowsMany : kAloneRows) &&
+                       (kv_dtype != TMAC_KV_F32 || max_prefix <= kAloneRowsF32);
     const int64_t blocks =
         n_groups && !alone ? std::min<int64_t>(n_seq, n_seq * group / tmac::kSharedCols + n_groups) : 0;
     a.prefix_blocks = (int)blocks;
@@ -1751,7 +1770,7 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     const int64_t own = n_groups && alone ? std::min<int64_t>((int64_t)max_prefix + max_tail, (int64_t)max_pages * kPageRows)
                                          : max_tail;
     a.tail_rows = (int)std::max<int64_t>(kPageRows, cdiv(own, kPageRows) * kPageRows);
-    if (n_sk < 2 * ctx->n_cu && own > kTailWholeRows) {
+    if (n_sk < 2 * ctx->n_cu && own > std::max<int64_t>(kTailWholeRows, whole_pages(ctx, kv_dtype, n_sk) * kPageRows)) {
         const int64_t splits = std::min<int64_t>({cdiv(2 * ctx->n_cu, n_sk), cdiv(2 * own, kTailWholeRows),
                                                   (int64_t)kMaxSplits});
         a.tail_rows = (int)(cdiv(cdiv(own, splits), kPageRows) * kPageRows);
