@@ -516,6 +516,16 @@ __device__ __forceinline__ void select_body(const SelectArgs& a) {
     }
 }
 
+// Short lists: scores and selection of one list in one workgroup.
+template <int HG>
+__device__ __forceinline__ void select_short_body(const SelectArgs& a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sk = blockIdx.x, s = sk / a.n_kv_head, n = select_pages_of(a, s), steps = (n + 15) / 16;
+    if (n > a.top && wave < steps) score_steps<HG>(a, s, sk - s * a.n_kv_head, n, wave, steps, kPagedWaves, lane);
+    __syncthreads();
+    select_body<64 * kPagedWaves>(a);
+}
+
 // ---------------------------------------------------------------------------
 // Decode attention, common parts.  A column is one query head of one sequence;
 // scores and sums are kept transposed, S^T (keys x columns) and O^T (dims x
@@ -1799,6 +1809,8 @@ TMAC_PAGED_KERNELS(q8, q8_0_t)
 
 extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_page_scores_h4(SelectArgs a) { score_body<1>(a); }
 extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_page_scores_h8(SelectArgs a) { score_body<2>(a); }
+extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_select_short_h4(SelectArgs a) { select_short_body<1>(a); }
+extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_select_short_h8(SelectArgs a) { select_short_body<2>(a); }
 extern "C" __global__ __launch_bounds__(256) void tmac_select_pages_256(SelectArgs a) { select_body<256>(a); }
 extern "C" __global__ __launch_bounds__(1024) void tmac_select_pages_1024(SelectArgs a) { select_body<1024>(a); }
 #define TMAC_MERGE_KERNELS(WPR)                                                                          \

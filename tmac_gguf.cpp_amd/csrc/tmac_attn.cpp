@@ -138,7 +138,7 @@ struct tmac_context {
     hipFunction_t k_rope = nullptr, k_copy = nullptr, k_pos = nullptr, k_qkv = nullptr, k_cvt16 = nullptr,
                   k_cvt_q8 = nullptr;
     // serving operators on paged caches, by kv_dtype; page scores: up to 4 query heads per kv head, more
-    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[2][4] = {}, k_scores[2] = {};
+    hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[2][4] = {}, k_scores[2] = {}, k_select_short[2] = {};
     hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[2][4] = {};  // shared prefixes, own rows
     hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
@@ -1067,7 +1067,9 @@ int tmac_init(tmac_context** out, int device) {
             }
         }
         if ((e = get_function(ctx, &ctx->k_scores[0], "tmac_page_scores_h4")) != hipSuccess ||
-            (e = get_function(ctx, &ctx->k_scores[1], "tmac_page_scores_h8")) != hipSuccess)
+            (e = get_function(ctx, &ctx->k_scores[1], "tmac_page_scores_h8")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_select_short[0], "tmac_select_short_h4")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_select_short[1], "tmac_select_short_h8")) != hipSuccess)
             return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
         if ((e = get_function(ctx, &ctx->k_select[0], "tmac_select_pages_256")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_select[1], "tmac_select_pages_1024")) != hipSuccess ||
@@ -1561,6 +1563,10 @@ int tmac_kv_page_bounds(tmac_context* ctx, tmac_stream stream, int kv_dtype, con
 }
 
 constexpr int kMaxGridYZ = 65535;
+// Pages up to which a list is scored and selected by one workgroup, and where there are at least half as many lists as
+// CUs.  Kernels, us, two / one (14 heads on 2): 1 sequence of 64 pages 11.2 / 10.0, 128 10.7 / 10.0, 256 10.6 / 12.1, 512
+// 11.6 / 14.8; 64 of 128 12.3 / 11.3, 256 13.6 / 12.9, 512 18.5 / 18.2; 256 of 128 19.8 / 14.6.
+constexpr int kSelectShort = 128, kSelectShortMany = 512;
 constexpr int kSelectWidePages = 2048;  // pages that 256 threads hold in registers; beyond, 1024 threads select
 int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, const void* bounds, int n_pages,
                       const int32_t* block_table, int max_pages, const int32_t* lengths, int32_t* selected, int n_seq,
@@ -1607,6 +1613,9 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
     if (pages > top) {  // otherwise every list holds all of its sequence's pages
         if ((rc = ensure_workspace(ctx, (hipStream_t)stream, (size_t)(n_sk * pages)))) return rc;
         a.keys = reinterpret_cast<uint32_t*>(workspace(ctx));
+        if (pages <= (2 * n_sk >= ctx->n_cu ? kSelectShortMany : kSelectShort))
+            return launch(ctx, ctx->k_select_short[a.group > 4], (unsigned)n_sk, 1, 64 * tmac::kPagedWaves,
+                          (hipStream_t)stream, &a);
         // Steps of 16 pages.  Where there are more than waves that fit the card, they are dealt out evenly (with more
         // than kScoreSeqs sequences, whose lengths a wave does not read at once, every sequence has waves of its own).
         const int64_t steps = cdiv(pages, 16), room = 2 * ctx->n_cu * tmac::kPagedWaves;
