@@ -400,7 +400,8 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
                                    int n_seq, int n_head, int n_kv_head, int head_dim);
 /* Decode of a batch whose sequences share long prefixes: group g = sequences group_starts[g] ..
  * group_starts[g + 1] - 1 (group_starts [n_groups + 1], ascending) shares its first prefix_lens[g]
- * rows, which are read, once for all of them, through the block table of the group's first sequence;
+ * rows, which are read, once for all of them (once each where they are short or the sequences few),
+ * through the block table of the group's first sequence;
  * a sequence's rows from there to lengths[s] - 1 are its own, through its own table.  (The entries of
  * the other sequences' tables for pages wholly inside the prefix are not read.)  A sequence in no
  * group has no prefix.  The result is tmac_attention_decode_paged's, up to rounding, where the tables
