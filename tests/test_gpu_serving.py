@@ -893,3 +893,47 @@ def test_offsets_beyond_32_bits(ctx, dt):
     for d in (dk, dv):
         d.free()
     no_fault(ctx)
+
+
+def put(ctx, ptr, host):
+    host = np.ascontiguousarray(host)
+    ctx._check(ctx.lib.tmac_memcpy_h2d(ctx.handle, None, ptr, host.ctypes.data, host.nbytes), "memcpy_h2d")
+    ctx.synchronize()
+
+
+def get(ctx, ptr, shape, kind=np.float32):
+    host = np.empty(shape, kind)
+    ctx.synchronize()
+    ctx._check(ctx.lib.tmac_memcpy_d2h(ctx.handle, None, host.ctypes.data, ptr, host.nbytes), "memcpy_d2h")
+    ctx.synchronize()
+    return host
+
+
+@pytest.mark.parametrize("dt", ALL_DT)
+def test_selected_rows_of_a_page_beyond_31_bits(ctx, dt):
+    """So many kv heads that the last rows of one page lie 2^31 bytes and more behind its first: row offsets inside a
+    page need 64 bits.  Of the pools, the queries and the outputs only the first and last three heads are looked at."""
+    width, kind = (68, np.uint8) if dt == Q8 else (64, np.float32 if dt == F32 else np.uint16)
+    size = width * np.dtype(kind).itemsize
+    nkv, some = (1 << 31) // (15 * size) + 60, 3
+    heads = (0, nkv - some)
+    x, y, q = oracle.normal(680, (PR, 2 * some, 64)), oracle.normal(681, (PR, 2 * some, 64)), oracle.normal(682, (2 * some, 64))
+    k, v = store(x, dt), store(y, dt)
+    dk, dv = ctx.empty((PR, nkv, width), kind), ctx.empty((PR, nkv, width), kind)
+    dq, dout = ctx.empty((nkv, 64)), ctx.empty((nkv, 64))
+    dtab, dsel = ctx.upload(np.zeros((1, 1), np.int32)), ctx.upload(np.zeros((1, nkv, 1), np.int32))
+    for i, h in enumerate(heads):
+        part = slice(some * i, some * (i + 1))
+        put(ctx, dq.at(h * 64), q[part])
+        for r in range(PR):
+            put(ctx, dk.at((r * nkv + h) * width), k[r, part])
+            put(ctx, dv.at((r * nkv + h) * width), v[r, part])
+    for n in (PR, 13):
+        ctx.decode_selected(dq, dk, dv, 1, dtab, 1, ctx.upload(np.array([n], np.int32)), dsel, 1, dout, 1, nkv, nkv, 64,
+                            kv_dtype=dt)
+        got = np.concatenate([get(ctx, dout.at(h * 64), (some, 64)) for h in heads])
+        ref = np.stack([attend64(q[i:i + 1], widen(k[:n, i], dt), widen(v[:n, i], dt))[0] for i in range(2 * some)])
+        close(got, ref, f"{n} rows")
+    for d in (dk, dv, dq, dout, dsel):
+        d.free()
+    no_fault(ctx)

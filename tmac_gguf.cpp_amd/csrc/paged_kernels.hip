@@ -886,8 +886,8 @@ struct Own {
     __device__ static void query(RawQuery& q, const float* p, int lane) { load_q<T, S>(q, p, lane); }
     __device__ static void init(State& st, const RawQuery& q, float scale) { cols_init<T, S>(st, q, scale); }
 
-    // kp / vp: row 0 of the page's head; stride: bytes between rows.
-    __device__ static void fetch(Tile& t, const char* kp, const char* vp, int stride, int lane) {
+    // kp / vp: row 0 of the page's head; stride: bytes between rows (64 bits: 15 rows of 559,241 fp32 kv heads pass 2^31).
+    __device__ static void fetch(Tile& t, const char* kp, const char* vp, size_t stride, int lane) {
         const int i = lane & 15, g = lane >> 4;
         if constexpr (Q8) {  // dims 8 g .. and 32 + 8 g .. of key i; 16 values of row lane / 4
             const u32x2 a = *reinterpret_cast<const u32x2_a4*>(kp + i * stride + 8 * g);
@@ -1004,7 +1004,7 @@ struct Own<float> {
 #pragma unroll
         for (int b = 0; b < 4; ++b) st.o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    __device__ static void fetch(Tile& t, const char* kp, const char* vp, int stride, int lane) {
+    __device__ static void fetch(Tile& t, const char* kp, const char* vp, size_t stride, int lane) {
         const int i = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1066,8 +1066,7 @@ __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const Pag
                                            int lane, Look look) {
     using O = Own<T>;
     constexpr int HB = CacheFmt<T>::kHeadBytes, KT = O::kTiles;
-    const int stride = a.n_kv_head * HB;
-    const size_t page_bytes = (size_t)kPageRows * stride;
+    const size_t stride = (size_t)a.n_kv_head * HB, page_bytes = kPageRows * stride;
     const int steps = ((n + KT - 1) / KT - wave + NW - 1) / NW;  // this wave's
     for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
         const int cnt = min(64 / KT, steps - s0);
