@@ -937,3 +937,23 @@ def test_selected_rows_of_a_page_beyond_31_bits(ctx, dt):
     for d in (dk, dv, dq, dout, dsel):
         d.free()
     no_fault(ctx)
+
+
+def test_append_heads_of_a_row_beyond_31_bits(ctx):
+    """One row of 2^25 query heads and a few, 8.6 GB, rotated in place: the last heads' offsets pass 2^31 floats."""
+    nh, some, pos = (1 << 25) + 64, 3, 77
+    q, kv = oracle.normal(690, (2 * some, 64)), oracle.normal(691, (2, 1, 64))
+    dq, dkv = ctx.empty((nh, 64)), ctx.upload(kv)
+    heads = (0, nh - some)
+    for i, h in enumerate(heads):
+        put(ctx, dq.at(h * 64), q[some * i:some * (i + 1)])
+    dk, dv = ctx.upload(np.zeros((5, PR, 1, 64), np.float32)), ctx.upload(np.zeros((5, PR, 1, 64), np.float32))
+    i32 = lambda x: ctx.upload(np.asarray(x, np.int32))  # noqa: E731
+    ctx.kv_append_paged(dq, 0, dq, dkv, 0, dkv.at(64), 0, dk, dv, 5, i32([[4, 3, 2, 1, 0]]), 5, i32([0, 1]), i32([pos]), 1, 1,
+                        nh, 1, 64, 80)
+    got = np.concatenate([get(ctx, dq.at(h * 64), (some, 64)) for h in heads])
+    np.testing.assert_array_equal(got, oracle.rope_heads(q, 2 * some, 64, pos).reshape(got.shape))
+    np.testing.assert_array_equal(dk.numpy()[0, pos % PR, 0], oracle.rope_heads(kv[0], 1, 64, pos).reshape(64))
+    np.testing.assert_array_equal(dv.numpy()[0, pos % PR], kv[1])
+    dq.free()
+    no_fault(ctx)

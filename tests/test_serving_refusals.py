@@ -208,3 +208,11 @@ def test_shared_grid(fake):
         rc, launches = fake.call("tmac_attention_decode_shared", max_prefix=max(room, 384) + 1, **args)
         assert rc == TMAC_OK and launches[0][0] == "tmac_prefix_f32"
         assert launches[0][1] % 8 == 0 and min(2 * need, 256) <= launches[0][1] <= 256
+
+
+def test_append_heads_of_a_workgroup(fake):
+    """A workgroup numbers the heads of its rows in 32 bits: more are refused."""
+    big = dict(q=None, q_out=None, n_rows=1, k_stride=0, v_stride=0, n_seq=1)
+    assert fake.call("tmac_kv_append_paged", n_head=2 ** 30, n_kv_head=2 ** 30, **big) == (TMAC_ERR_INVALID_ARG, [])
+    assert fake.call("tmac_kv_append_paged", n_head=2 ** 30 - 16, n_kv_head=2 ** 30 - 16, **big) == (TMAC_ERR_INVALID_ARG, [])
+    assert fake.call("tmac_kv_append_paged", n_head=2 ** 30 - 17, n_kv_head=2 ** 30 - 17, **big)[0] == TMAC_OK

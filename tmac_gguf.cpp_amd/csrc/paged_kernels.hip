@@ -74,13 +74,13 @@ __device__ __forceinline__ void append_body(const AppendArgs& a) {
         const int64_t t = t0 + r, row = s_row[r];
         float x[8];
         if (h < nh) {
-            load8(x, a.q + t * a.q_stride + h * kHeadDim + 4 * c);
+            load8(x, a.q + t * a.q_stride + (int64_t)h * kHeadDim + 4 * c);
             rope8(x, a.rope_cs + (size_t)pos * (kHeadDim / 2), c);
             store8(a.q_out + (t * nh + h) * kHeadDim + 4 * c, x);
         } else if (row >= 0) {
             const bool key = h < nh + kv;
             const int hk = key ? h - nh : h - nh - kv;
-            load8(x, (key ? a.k + t * a.k_stride : a.v + t * a.v_stride) + hk * kHeadDim + 4 * c);
+            load8(x, (key ? a.k + t * a.k_stride : a.v + t * a.v_stride) + (int64_t)hk * kHeadDim + 4 * c);
             if (key) rope8(x, a.rope_cs + (size_t)pos * (kHeadDim / 2), c);
             char* p = (key ? a.k_pages : a.v_pages) + (row * kv + hk) * HB + 4 * c * DB;
             put_row<T>(x, p, c, true);

@@ -1533,7 +1533,9 @@ int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, co
     a.capacity = max_len;
     a.rows_per_group = (int)std::min<int64_t>(tmac::kAppendRows, std::max<int64_t>(1, n_rows / (8 * ctx->n_cu)));
     const int64_t blocks = cdiv(n_rows, a.rows_per_group);
-    if ((rc = check_units(ctx, what, blocks, 256))) return rc;
+    // a workgroup numbers the heads of its rows in 32 bits, and counts past the last by its 32 slots
+    const int64_t heads = a.rows_per_group * (2 * (int64_t)n_kv_head + (q ? n_head : 0));
+    if ((rc = check_units(ctx, what, blocks, 256)) || (rc = check_units(ctx, what, heads + 32))) return rc;
     return launch(ctx, ctx->k_append[kv_dtype], (unsigned)blocks, 1, 256, (hipStream_t)stream, &a);
 }
 
