@@ -1459,10 +1459,10 @@ static int check_serving(tmac_context* ctx, const char* what, int kv_dtype, int 
     return TMAC_OK;
 }
 
-// A grid of `units` workgroups, refused where its index would not fit.
 // Units of work that the kernels number in 32 bits, a launch of `threads` each if not 0.
 static int check_units(tmac_context* ctx, const char* what, int64_t units, int64_t threads = 0) {
-    if (units > INT_MAX || units * threads > UINT32_MAX) return fail(ctx, TMAC_ERR_INVALID_ARG, std::string(what) + ": too many units of work");
+    if (units > INT_MAX || units * threads > UINT32_MAX)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, std::string(what) + ": too many units of work");
     return TMAC_OK;
 }
 
@@ -1591,7 +1591,8 @@ int tmac_select_pages(tmac_context* ctx, tmac_stream stream, const float* q, con
     const int64_t n_sk = (int64_t)n_seq * n_kv_head, pages = cdiv(max_len, kPageRows);
     const bool wide = pages > kSelectWidePages;
     const unsigned threads = wide ? 1024 : 256;
-    if ((rc = check_units(ctx, what, n_sk * cdiv(pages, 16))) || (rc = check_units(ctx, what, n_sk, threads))) return rc;
+    // lists first: with no more of them than a grid takes, their steps fit 64 bits
+    if ((rc = check_units(ctx, what, n_sk, threads)) || (rc = check_units(ctx, what, n_sk * cdiv(pages, 16)))) return rc;
     if (n_seq > kMaxGridYZ) return fail(ctx, TMAC_ERR_INVALID_ARG, "select_pages: more than 65535 sequences");
     if ((rc = set_device(ctx))) return rc;
     SelectArgs a{};
