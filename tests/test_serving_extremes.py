@@ -42,3 +42,15 @@ for name, good in t.GOOD.items():
             fake.call(name, **{i: big, j: big})
             fake.call(name, **{**{k: big for k in ("n_head", "n_kv_head") if k in good}, i: big, j: big})
 """)
+
+
+def test_a_rotation_table_too_large_for_memory_is_an_error(sanitized):
+    """An append whose max_len asks for more host memory than there is returns a status; no exception leaves the C entry,
+    and the next call finds the context as it was."""
+    status = child(sanitized, """
+import resource
+resource.setrlimit(resource.RLIMIT_AS, (8 << 30, 8 << 30))  # the table of 2^26 positions is 16 GiB
+print(fake.call("tmac_kv_append_paged", max_pages=2 ** 23, max_len=2 ** 26, base=1e4))
+print(fake.call("tmac_kv_append_paged", base=1e4))
+""")
+    assert "".join(status) == "(1002,[])(0,[('tmac_append_f32',5)])"

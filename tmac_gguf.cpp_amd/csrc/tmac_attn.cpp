@@ -19,6 +19,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <map>
 #include <memory>
 #include <numeric>
@@ -567,7 +568,13 @@ int rope_table(tmac_context* ctx, hipStream_t stream, int head_dim, float base, 
         new_rows *= 2;
     }
     const int pairs = head_dim / 2;
-    std::vector<float2> host((size_t)new_rows * pairs);
+    std::vector<float2> host;
+    try {
+        host.resize((size_t)new_rows * pairs);
+    } catch (const std::exception&) {
+        return fail(ctx, TMAC_ERR_HIP_BASE + hipErrorOutOfMemory,
+                    "RoPE table of " + std::to_string(new_rows) + " positions: out of host memory");
+    }
     for (int pos = 0; pos < new_rows; pos++) {
         for (int d = 0; d < head_dim; d += 2) {
             float theta = 1.0f / powf(base, (float)d / head_dim);
