@@ -342,8 +342,11 @@ int tmac_layer_attention_paged(tmac_context* ctx, tmac_stream stream, int kv_dty
  * heads per kv head (more: TMAC_ERR_UNSUPPORTED).  Row, length and position arrays are DEVICE arrays,
  * so a captured call replays with new ones.  n_seq = 0 does nothing.  Which workgroup sums what
  * depends on the call's host arguments and, for shared prefixes, on the groups: the same call gives
- * the same bits.  A stored key or value that is not finite makes the attention outputs that read it
- * not finite; rows that no sequence reads may hold anything.
+ * the same bits.  Rows that no sequence reads may hold anything.  Of those that are read, a NaN key or
+ * a key whose score is +infinity makes the outputs that read it not finite, a value that is not
+ * finite its dim of them (a Q8_0 scale its 32 dims).  A row whose infinite keys give a score of
+ * -infinity takes weight 0 or makes the outputs that read it not finite: which of the two depends on
+ * the cache type, on the query's bits and on what reads the row (max_prefix decides that).
  *
  * Append: a ragged batch of new rows (prompt chunks and single tokens mixed).  Rows
  * row_starts[s] .. row_starts[s + 1] - 1 of q / k / v (row_starts [n_seq + 1], ascending) belong to

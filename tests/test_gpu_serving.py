@@ -957,3 +957,95 @@ def test_append_heads_of_a_row_beyond_31_bits(ctx):
     np.testing.assert_array_equal(dv.numpy()[0, pos % PR], kv[1])
     dq.free()
     no_fault(ctx)
+
+
+# ---- stored rows that are not finite and are read -----------------------------------------------
+
+def spoil(pool, dt, page, row, dim, bad):
+    """Copy of a stored pool with one value of kv head 0 set to `bad` (Q8_0: the scale of its 32 dims)."""
+    p = pool.copy()
+    if dt == Q8:
+        at = 64 + 2 * (dim // 32)
+        p[page, row, 0, at:at + 2] = np.array([bad], np.float16).view(np.uint8)
+    else:
+        p[page, row, 0, dim] = store(np.array([bad], np.float32), dt)[0]
+    return p
+
+
+def check_spoilt(got, ref, without, what, key=None, value=None):
+    """One (sequence, kv head)'s outputs [heads][64] over a row with a key or a value that is not finite; ref: with
+    the row as it was, without: without the row.  key: its score; value: the dims that it spoils."""
+    if value is not None:
+        rest = np.setdiff1d(np.arange(64), value)
+        assert not np.isfinite(got[:, value]).any(), what
+        close(got[:, rest], ref[:, rest], what)
+    elif key == -np.inf:  # weight 0, or nothing finite
+        for h in range(len(got)):
+            if np.isfinite(got[h]).any():
+                close(got[h], without[h], what)
+    else:
+        assert not np.isfinite(got).any(), what
+
+
+@pytest.mark.parametrize("route", ["whole list", "split list", "own", "prefix, read by each", "prefix, once for all"])
+@pytest.mark.parametrize("dt", ALL_DT)
+def test_rows_that_are_read_and_not_finite(ctx, dt, route):
+    """NaN and infinities in one stored row that is read: what they do to the outputs that read it, and that the other
+    kv head and a sequence that does not read it keep their values."""
+    rng = np.random.default_rng(38)
+    nh, nkv, row, dim = 14, 2, 333, 5
+    lens = np.array([700, 690], np.int32)
+    shared = route.startswith("prefix") or route == "own"
+    if shared:
+        starts, prefix = [0, 2], [600 if route != "own" else 40]
+        table, total, of = shared_tables(rng, starts, prefix, lens)
+        rows = rows_shared(table, starts, prefix, of, lens)
+    else:
+        table, total = tables(rng, lens)
+        n = 12 if route == "whole list" else 44
+        sel = np.full((2, nkv, n), -1, np.int32)
+        sel[:, :, 0], sel[:, :, 1:] = row // PR, [j for j in range(44) if j != row // PR][:n - 1]
+        rows = rows_of_list(table, lens, sel)
+    kp, kw = make_pool(700, total, nkv, dt)
+    vp, vw = make_pool(701, total, nkv, dt)
+    q = oracle.normal(702, (2, nh, 64))
+    q[:, :, dim] = np.abs(q[:, :, dim]) + np.float32(0.3)
+    if dt == Q8:  # a scale spoils 32 keys: their integers decide the sign of the score
+        kp[:, :, :, :32] = (rng.integers(1, 120, kp[..., :32].shape) * 1).astype(np.int8).view(np.uint8)
+        kw = widen(kp, dt)
+        q[:, :, :32] = np.abs(q[:, :, :32]) + np.float32(0.01)
+    pages, at = rows(0, 0)
+    logical = np.concatenate([PR * j + np.arange(PR) for j in sel[0, 0] if j >= 0]) if not shared else np.arange(lens[0])
+    logical = logical[logical < lens[0]]
+    i = int(np.flatnonzero(logical == row)[0])
+    page, r = int(pages[i]), int(at[i])
+    readers = [0, 1] if route.startswith("prefix") else [0]
+
+    def run(a, b):
+        if not shared:
+            return run_selected(ctx, q, a, b, table, lens, sel, nkv, dt)
+        if route != "prefix, once for all":
+            return run_shared(ctx, q, a, b, table, lens, starts, prefix, nkv, dt)
+        wide, room = once_for_all(table, nkv, prefix[0])
+        return run_shared(ctx, q, a, b, wide, lens, starts, prefix, nkv, dt, max_prefix=room)
+
+    ref = decode64(q, kw, vw, rows, nkv)
+
+    def others(s, h):
+        pg, x = rows(s, h)
+        keep = ~((pg == page) & (x == r))
+        return pg[keep], x[keep]
+    without = decode64(q, kw, vw, others, nkv)
+    close(run(kp, vp), ref, "finite")
+    for name, bad in (("NaN", np.nan), ("+inf", np.inf), ("-inf", -np.inf)):
+        for what, a, b in ((f"key {name}", spoil(kp, dt, page, r, dim, bad), vp),
+                           (f"value {name}", kp, spoil(vp, dt, page, r, dim, bad))):
+            got = run(a, b)
+            value = None if b is vp else (np.arange(32) if dt == Q8 else np.array([dim]))
+            for s in range(2):
+                if s in readers:
+                    check_spoilt(got[s, :7], ref[s, :7], without[s, :7], what, key=bad, value=value)
+                else:
+                    close(got[s, :7], ref[s, :7], f"{what}, another sequence")
+                close(got[s, 7:], ref[s, 7:], f"{what}, the other kv head")
+    no_fault(ctx)
