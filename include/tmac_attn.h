@@ -50,6 +50,7 @@
  *    result to compare against (parity there is unpinned).
  *    The bf16 / fp16 / Q8_0 caches, the paged caches and chunked prefill keep
  *    head_dim 64 and the compiled groups; other shapes return TMAC_ERR_UNSUPPORTED.
+ *    The calls under "serving on paged caches" take other groups too (see there).
  */
 #ifndef TMAC_ATTN_H
 #define TMAC_ATTN_H
@@ -339,7 +340,9 @@ int tmac_layer_attention_paged(tmac_context* ctx, tmac_stream stream, int kv_dty
 /* ---- serving on paged caches (extensions; no counterpart in the reference, whose engine holds one
  *      sequence) ----
  * Pools, pages, block tables and kv_dtype as above; head_dim 64, any n_kv_head, at most 16 query
- * heads per kv head (more: TMAC_ERR_UNSUPPORTED).  Row, length and position arrays are DEVICE arrays,
+ * heads per kv head (more: TMAC_ERR_UNSUPPORTED).  tmac_select_pages and tmac_attention_decode_shared
+ * take at most 65,535 sequences, the latter as many kv heads, and every call as much work as a grid of
+ * 2^32 threads holds (more: TMAC_ERR_INVALID_ARG).  Row, length and position arrays are DEVICE arrays,
  * so a captured call replays with new ones.  n_seq = 0 does nothing.  Which workgroup sums what
  * depends on the call's host arguments and, for shared prefixes, on the groups: the same call gives
  * the same bits.  Rows that no sequence reads may hold anything.  Of those that are read, a NaN key or
@@ -360,7 +363,9 @@ int tmac_layer_attention_paged(tmac_context* ctx, tmac_stream stream, int kv_dty
  * q_out rows keep what they held.  A row whose position is outside [0, max_len) is skipped and sets
  * bit 0 of the device error word; max_len <= 16 * max_pages.  A row whose block-table entry is outside
  * the pool is rotated but not stored (bit 2; unlike a read, a write is never clamped onto another
- * page).  No two rows of a call may fall on the same pool row. */
+ * page).  No two rows of a call may fall on the same pool row.  The rotation table has a row of 256
+ * bytes for every position below max_len; a call that finds a shorter one builds it (on the host:
+ * tmac_rope_prepare does so ahead, which a capture needs). */
 int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q, int64_t q_stride,
                          float* q_out, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                          void* k_pages, void* v_pages, int n_pages, const int32_t* block_table, int max_pages,
@@ -383,7 +388,7 @@ int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, co
  *     [n_seq][n_kv_head][top]: the logical pages of the sequence's first `first` and last `last` pages
  *     and, up to `top` in all, those with the highest scores (ties: the lower page), ascending, then
  *     -1; all pages where there are no more than top.  first + last <= top.  Bounds of the first and
- *     last pages are not read.  A length above max_len gives an empty list (all -1) and sets bit 1; an
+ *     last pages may hold anything.  A length above max_len gives an empty list (all -1) and sets bit 1; an
  *     entry outside the pool is clamped and sets bit 2.  With a query that is not finite the list holds
  *     valid, distinct pages, which ones is not defined.
  *   tmac_attention_decode_selected: one query token per sequence over the rows 16 j .. 16 j + 15 below

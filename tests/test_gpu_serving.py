@@ -1049,3 +1049,19 @@ def test_rows_that_are_read_and_not_finite(ctx, dt, route):
                     close(got[s, :7], ref[s, :7], f"{what}, another sequence")
                 close(got[s, 7:], ref[s, 7:], f"{what}, the other kv head")
     no_fault(ctx)
+
+
+@pytest.mark.parametrize("bits", [0x7FC0, 0xFFFF, 0x7F80, 0xFF80, 0x7F7F])
+def test_select_bounds_of_pages_that_are_taken_anyway(ctx, bits):
+    """Bounds of a sequence's first and last pages may hold anything: NaN, infinities, stale values."""
+    rng = np.random.default_rng(7)
+    for lens, top, first, last in (([1600, 333], 12, 2, 3), ([40000, 33000], 40, 1, 2)):
+        lens = np.array(lens, np.int32)
+        table, n_pages = tables(rng, lens)
+        q, b = oracle.normal(350, (2, 14, 64)), random_bounds(351, n_pages, 2)
+        ref = select_ref(q, b, table, lens, 2, top, first, last)
+        for s, n in enumerate(-(-lens // PR)):
+            forced = np.r_[table[s, :first], table[s, n - last:n]]
+            b.view(np.uint32)[forced] = np.uint32(bits) << 16
+        np.testing.assert_array_equal(run_select(ctx, q, b, table, lens, 2, top, first, last), ref)
+    no_fault(ctx)

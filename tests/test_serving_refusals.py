@@ -216,3 +216,16 @@ def test_append_heads_of_a_workgroup(fake):
     assert fake.call("tmac_kv_append_paged", n_head=2 ** 30, n_kv_head=2 ** 30, **big) == (TMAC_ERR_INVALID_ARG, [])
     assert fake.call("tmac_kv_append_paged", n_head=2 ** 30 - 16, n_kv_head=2 ** 30 - 16, **big) == (TMAC_ERR_INVALID_ARG, [])
     assert fake.call("tmac_kv_append_paged", n_head=2 ** 30 - 17, n_kv_head=2 ** 30 - 17, **big)[0] == TMAC_OK
+
+
+def test_most_sequences(fake):
+    """The limits the header names: 65,535 sequences, and kv heads where a grid numbers them."""
+    for name in ("tmac_select_pages", "tmac_attention_decode_shared"):
+        assert fake.call(name, n_seq=65535)[0] == TMAC_OK
+        assert fake.call(name, n_seq=65536) == (TMAC_ERR_INVALID_ARG, [])
+    assert fake.call("tmac_attention_decode_shared", n_head=65535, n_kv_head=65535)[0] == TMAC_OK
+    assert fake.call("tmac_attention_decode_shared", n_head=65536, n_kv_head=65536) == (TMAC_ERR_INVALID_ARG, [])
+    # the others have no such limit
+    assert fake.call("tmac_kv_append_paged", n_seq=65536)[0] == TMAC_OK
+    assert fake.call("tmac_kv_page_bounds", n_seq=65536)[0] == TMAC_OK
+    assert fake.call("tmac_attention_decode_selected", n_seq=65536)[0] == TMAC_OK
