@@ -2,7 +2,7 @@
 // layer: linked with tmac_attn.cpp instead of libamdhip64.  Device memory is host
 // memory, streams are always idle (or capturing, fake_set_capturing), and a launch
 // is only written down: fake_launch_name(i) and fake_launch_grid(i, d) give its
-// kernel and grid.
+// kernel and grid, fake_launch_prefix(i, field) how a prefix kernel's work is cut.
 #include <hip/hip_runtime_api.h>
 
 #include <cstdint>
@@ -11,10 +11,13 @@
 #include <string>
 #include <vector>
 
+#include "attn_args.h"
+
 namespace {
 struct Launch {
     std::string name;
     unsigned grid[3], block;
+    int prefix[3];  // tmac_prefix_*: most runs of a prefix, workgroups that share the units, most blocks of columns
 };
 std::vector<Launch> g_launches;
 std::vector<std::string*> g_names;  // hipFunction_t values
@@ -39,6 +42,7 @@ int fake_launches() { return (int)g_launches.size(); }
 void fake_clear() { g_launches.clear(); }
 const char* fake_launch_name(int i) { return g_launches[(size_t)i].name.c_str(); }
 unsigned fake_launch_grid(int i, int d) { return g_launches[(size_t)i].grid[d]; }
+int fake_launch_prefix(int i, int field) { return g_launches[(size_t)i].prefix[field]; }
 unsigned fake_launch_block(int i) { return g_launches[(size_t)i].block; }
 void fake_set_capturing(int on) { g_capturing = on != 0; }
 
@@ -77,13 +81,19 @@ hipError_t hipModuleGetFunction(hipFunction_t* f, hipModule_t, const char* name)
     return hipSuccess;
 }
 hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned gx, unsigned gy, unsigned gz, unsigned bx, unsigned, unsigned,
-                                 unsigned, hipStream_t, void**, void**) {
+                                 unsigned, hipStream_t, void** params, void**) {
     Launch l{};
     l.name = *reinterpret_cast<std::string*>(f);
     l.grid[0] = gx;
     l.grid[1] = gy;
     l.grid[2] = gz;
     l.block = bx;
+    if (l.name.rfind("tmac_prefix_", 0) == 0) {
+        const auto* a = static_cast<const tmac::PagedAttnArgs*>(params[0]);
+        l.prefix[0] = a->prefix_splits;
+        l.prefix[1] = a->prefix_groups;
+        l.prefix[2] = a->prefix_blocks;
+    }
     g_launches.push_back(l);
     return hipSuccess;
 }

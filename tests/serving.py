@@ -124,3 +124,28 @@ def select_ref(q, b, table, lens, n_kv, top, first, last):
             order = np.lexsort((j, -sc.astype(np.float64), ~force))
             out[s, h] = np.sort(order[:top])
     return out
+
+
+# Shared prefixes that a unit of the prefix kernel walks in several stages (256 rows, fp32 128): name, query heads, kv
+# heads, group starts, prefix lengths.
+def staged_cases():
+    rng = np.random.default_rng(44)
+    return [("one group of 96", 14, 2, [0, 96], [12300]),
+            ("90 groups of one", 16, 4, list(range(91)), [int(x) for x in rng.integers(500, 901, 90)])]
+
+
+def stage_rows(dt):
+    return 128 if dt == F32 else 256
+
+
+def runs_of_prefixes(splits, workgroups, most_blocks, starts, nh, nkv):
+    """Runs that every prefix is cut into (the kernel's rule), from the arguments of the launch."""
+    blocks = min(most_blocks, sum(-(-(b - a) * (nh // nkv) // 64) for a, b in zip(starts, starts[1:])))
+    return max(1, min(splits, workgroups // max(1, blocks * nkv)))
+
+
+def run_rows(prefix, runs):
+    """Rows of every run of a prefix, in order."""
+    pages = -(-prefix // PR)
+    per = max(1, -(-pages // runs)) * PR
+    return [(at, min(at + per, prefix)) for at in range(0, prefix, per)]
