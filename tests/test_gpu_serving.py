@@ -1065,3 +1065,21 @@ def test_select_bounds_of_pages_that_are_taken_anyway(ctx, bits):
             b.view(np.uint32)[forced] = np.uint32(bits) << 16
         np.testing.assert_array_equal(run_select(ctx, q, b, table, lens, 2, top, first, last), ref)
     no_fault(ctx)
+
+
+@pytest.mark.parametrize("dt", ALL_DT)
+def test_selected_long_lists_of_many_sequences(ctx, dt):
+    """Around 2/3 of the CUs, above and below one list a CU: lists split in three or two and whole ones of eight waves
+    and of four, long enough that a wave looks its pages up twice."""
+    rng = np.random.default_rng(39)
+    for n, top in ((168, 790), (180, 600), (260, 300)):
+        lens = np.full(n, 16 * 800 - 5, np.int32)
+        table = rng.integers(0, 500, (n, 800)).astype(np.int32)
+        kp, kw = make_pool(490, 500, 1, dt)
+        vp, vw = make_pool(491, 500, 1, dt)
+        q = oracle.normal(492, (n, 4, 64))
+        sel = random_lists(rng, lens, 1, top)
+        sel[1, 0, 5:] = -1
+        got = run_selected(ctx, q, kp, vp, table, lens, sel, 1, dt)
+        close(got, decode64(q, kw, vw, rows_of_list(table, lens, sel), 1), f"{n} x {top}")
+    no_fault(ctx)

@@ -229,3 +229,38 @@ def test_most_sequences(fake):
     assert fake.call("tmac_kv_append_paged", n_seq=65536)[0] == TMAC_OK
     assert fake.call("tmac_kv_page_bounds", n_seq=65536)[0] == TMAC_OK
     assert fake.call("tmac_attention_decode_selected", n_seq=65536)[0] == TMAC_OK
+
+
+def lists(fake, n_sk, top, dt):
+    """(kernel, workgroups a list) of an attention over n_sk lists."""
+    rc, launches = fake.call("tmac_attention_decode_selected", kv_dtype=dt, n_seq=n_sk, n_head=7, n_kv_head=1, top=top)
+    assert rc == TMAC_OK and launches[0][1] % n_sk == 0
+    return launches[0][0], launches[0][1] // n_sk
+
+
+@pytest.mark.parametrize("dt", range(4))
+def test_split_lists_fit_the_card_at_once(fake, dt):
+    """A split list has no more workgroups than all lists find room for at once (two a CU, 256 CUs): one more each would
+    be a second round.  From 341 lists on no list is split, and up to one a CU a split one has two at least."""
+    for n_sk in list(range(1, 260)) + [300, 340, 342, 400, 511, 512, 600]:
+        for top in (1, 16, 64, 100, 500, 2000, 100000):
+            kernel, each = lists(fake, n_sk, top, dt)
+            assert each == 1 or each * n_sk <= 512 or (n_sk > 256 and each == 2 and 3 * n_sk <= 1024)
+
+
+@pytest.mark.parametrize("dt", range(4))
+def test_long_lists_are_split_where_cus_would_be_idle(fake, dt):
+    """No step at half the CUs: a long list is split below and above it, a short one is not, and the length between
+    grows with the lists."""
+    for n_sk in (1, 60, 127, 128, 129, 130, 144, 160, 170):
+        assert lists(fake, n_sk, 2000, dt)[1] >= 3
+        assert lists(fake, n_sk, 8, dt)[1] == 1
+    most = []
+    for n_sk in (64, 96, 112, 128, 129, 150, 170):
+        most.append(max(top for top in range(8, 1200, 4) if lists(fake, n_sk, top, dt)[1] == 1))
+    assert most == sorted(most) and most[4] < 1.1 * most[3] + 4
+    # own rows by the same rule
+    for n_seq in (72, 85):
+        rc, launches = fake.call("tmac_attention_decode_shared", kv_dtype=dt, n_seq=n_seq, n_groups=0, max_pages=1024,
+                                 max_prefix=0, max_tail=16384)
+        assert rc == TMAC_OK and launches[0][0].startswith("tmac_tail_") and launches[0][1] == 3, launches

@@ -1685,17 +1685,33 @@ static int launch_paged_merge(tmac_context* ctx, tmac_stream stream, const hipFu
                   64 * tmac::kPagedWaves, (hipStream_t)stream, a);
 }
 
-// Pages that one workgroup attends for a (sequence, kv head) without help, n_sk of them in all: a launch and its partials
-// less, against waves that would share them.  Kernels, us, split / whole (14 heads on 2): 32 lists of 32 pages bf16 7.8 /
-// 8.1, of 64 8.7 / 10.6; fp32, whose products take four times as long, of 16 8.0 / 8.3, of 32 8.4 / 11.5.  128 lists
-// (half the CUs have one): bf16 64 pages 15.5 / 12.2, 128 21.0 / 17.4, 256 30.5 / 31.0, 500 46.6 / 56.2; fp32 32 16.1 /
-// 13.0, 64 20.4 / 20.1, 128 29.8 / 36.6.  200 lists: bf16 128 32.6 / 22.5, 500 82 / 68, fp32 500 135 / 132.  360 lists: bf16
-// 128 43.7 / 35.2, 500 121 / 113; fp32 128 72.6 / 71.8, 256 128 / 136, 500 195 / 243.
+// Lists (or own rows) of a (sequence, kv head), n_sk of them in all, go to one workgroup each or are split over several
+// of four waves, of which a CU holds two: as many as all lists have at once, since one more is a second round for all
+// (130 lists of 500 bf16 pages: 4 workgroups each 70.7 us, 3 50.7; 60 of 500: 9 35.0, 8 28.8; 100 fp32 of 500: 84.6, 73.2).
+static int64_t list_splits(const tmac_context* ctx, int64_t n_sk) {
+    return std::max<int64_t>(2, 2 * ctx->n_cu / n_sk);
+}
+// Pages up to which one workgroup takes a list: a launch and the partials less, and up to one list a CU its eight waves
+// read as one, against CUs that stay idle.  Where no three workgroups a list fit at once (from 2/3 of the CUs on), two
+// never made up for the merge, but for fp32 just above one list a CU, when few CUs would have two and all wait for them.
+// Below, the length from which splitting wins grows with the lists.  Captured calls of 14 heads on 2, us, one workgroup
+// / split:
+//   bf16   80 lists: 64 pages 12.6 / 13.0, 128 17.8 / 16.2;  96: 128 17.8 / 18.2, 192 22.8 / 21.7;  128: 256 28.2 / 30.2,
+//          384 43.7 / 40.7;  144: 256 29.5 / 33.6, 500 58.2 / 55.2, 1,000 118 / 108;  170: 500 63.1 / 63.7, 1,000 128 / 126;
+//          176: 128 21.0 / 24.4, 2,000 258 / 275;  256: 128 28.2 / 29.9, 2,000 354 / 365;  360: 128 35.6 / 42.7, 1,000 277 / 292
+//   fp16   80 lists: 128 16.3 / 16.2;  96: 256 25.2 / 25.3;  128: 256 26.0 / 29.9, 384 42.5 / 40.9
+//   Q8_0   80 lists: 32 10.2 / 10.4, 64 14.8 / 14.1;  128: 64 15.3 / 15.5, 128 23.2 / 21.2;  144: 128 23.6 / 24.4, 192 31.0 / 28.9;
+//          170: 192 31.7 / 32.0, 256 39.6 / 38.2;  176: 128 24.3 / 27.8, 2,000 276 / 288;  360: 128 41.3 / 44.1, 1,000 284 / 278
+//   fp32   60 lists: 32 13.6 / 10.4;  112: 32 13.7 / 14.4, 64 21.0 / 18.8;  144: 64 21.2 / 22.5, 128 34.8 / 32.6;  176: 128
+//          37.4 / 41.1, 2,000 514 / 534;  300: 64 36.6 / 36.1, 128 70.7 / 66.1, 1,000 515 / 488;  360: 128 73.2 / 75.8, 1,000
+//          536 / 537;  420: 128 78.6 / 97.9
 static int64_t whole_pages(const tmac_context* ctx, int kv_dtype, int64_t n_sk) {
     const bool f32 = kv_dtype == TMAC_KV_F32;
-    if (n_sk > ctx->n_cu) return f32 ? 128 : INT_MAX;
-    if (2 * n_sk > ctx->n_cu) return INT_MAX;
-    return 8 * n_sk >= 3 * ctx->n_cu ? (f32 ? 64 : 192) : (f32 ? 16 : 32);
+    if (3 * n_sk > 2 * ctx->n_cu) return f32 && n_sk > ctx->n_cu && 3 * n_sk <= 4 * ctx->n_cu ? 64 : INT_MAX;
+    const double r = 2.0 * (double)n_sk / ctx->n_cu;  // lists by half the CUs
+    if (f32) return std::max(16, (int)(60 * r * r));
+    if (kv_dtype == TMAC_KV_Q8_0) return std::max(32, (int)(115 * r * r));
+    return std::max(32, (int)(300 * r * r * r));
 }
 // A whole list is taken by eight waves where a CU has no more than one, and by four if it is short (bf16, 16 lists: 8
 // pages 5.1 against 5.4, 16 pages 6.5 against 6.1) or there are more (512 of 8 pages 8.0 against 12.2).
@@ -1717,7 +1733,7 @@ int tmac_attention_decode_selected(tmac_context* ctx, tmac_stream stream, int kv
     a.top = top;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head;
     const bool whole = top <= whole_pages(ctx, kv_dtype, n_sk), wide = whole && n_sk <= ctx->n_cu && top > kListNarrow;
-    int64_t splits = whole ? 1 : std::min<int64_t>(cdiv(2 * ctx->n_cu, n_sk), cdiv(top, tmac::kPagedWaves));
+    int64_t splits = whole ? 1 : std::min<int64_t>(list_splits(ctx, n_sk), cdiv(top, tmac::kPagedWaves));
     splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
     a.per_split = (int)cdiv(top, splits);
     a.n_slots = (int)cdiv(top, a.per_split);
@@ -1789,8 +1805,11 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     const int64_t own = n_groups && alone ? std::min<int64_t>((int64_t)max_prefix + max_tail, (int64_t)max_pages * kPageRows)
                                          : max_tail;
     a.tail_rows = (int)std::max<int64_t>(kPageRows, cdiv(own, kPageRows) * kPageRows);
-    if (n_sk < 2 * ctx->n_cu && own > std::max<int64_t>(kTailWholeRows, whole_pages(ctx, kv_dtype, n_sk) * kPageRows)) {
-        const int64_t splits = std::min<int64_t>({cdiv(2 * ctx->n_cu, n_sk), cdiv(2 * own, kTailWholeRows),
+    // (a quarter longer than lists: they are cut into no fewer than kTailWholeRows / 2; Q8_0, 96 sequences and kv heads, whole /
+    // split: 80 pages 16.1 / 18.3, 160 26.3 / 21.0; bf16, 128: 256 pages 27.8 / 30.1, 500 47.6 / 50.7, 1,000 113 / 93)
+    if (n_sk < 2 * ctx->n_cu &&
+        own > std::max<int64_t>(kTailWholeRows, whole_pages(ctx, kv_dtype, n_sk) * kPageRows * 5 / 4)) {
+        const int64_t splits = std::min<int64_t>({list_splits(ctx, n_sk), cdiv(2 * own, kTailWholeRows),
                                                   (int64_t)kMaxSplits});
         a.tail_rows = (int)(cdiv(cdiv(own, splits), kPageRows) * kPageRows);
     }
