@@ -264,3 +264,12 @@ def test_long_lists_are_split_where_cus_would_be_idle(fake, dt):
         rc, launches = fake.call("tmac_attention_decode_shared", kv_dtype=dt, n_seq=n_seq, n_groups=0, max_pages=1024,
                                  max_prefix=0, max_tail=16384)
         assert rc == TMAC_OK and launches[0][0].startswith("tmac_tail_") and launches[0][1] == 3, launches
+
+
+def test_q8_prefixes_of_many_sequences_are_read_once(fake):
+    """More Q8_0 readers than CUs convert a prefix of 700 rows slower than one launch more; other types do not."""
+    for dt, n_seq, n_kv, rows, first in ((3, 200, 2, 700, "prefix"), (3, 45, 8, 800, "prefix"), (3, 200, 2, 500, "tail"),
+                                         (3, 128, 2, 1100, "tail"), (1, 200, 2, 700, "tail"), (2, 45, 8, 800, "tail")):
+        rc, launches = fake.call("tmac_attention_decode_shared", kv_dtype=dt, n_seq=n_seq, n_head=n_kv, n_kv_head=n_kv,
+                                 n_groups=1, max_pages=1024, max_prefix=rows, max_tail=64)
+        assert rc == TMAC_OK and launches[0][0].startswith("tmac_" + first), (dt, n_seq, rows, launches)

@@ -1750,13 +1750,21 @@ constexpr int kTailWholeRows = 1024;  // own rows that one workgroup takes witho
 constexpr int kTailNarrowRows = 192;  // own rows up to which four waves do
 constexpr int kFinishSlots = 16;     // prefix partials that the own rows' workgroup merges itself
 // Prefix rows, times sequences and kv heads, up to which every sequence reads the prefix itself (kAloneRowsMany: where
-// these are at least half as many as CUs), and of fp32 caches the rows of one prefix: a launch less (one less again
-// without partials) against rows that all read.  Kernels of a call with 64 own rows, 14 heads on 2, shared / alone, us:
-// bf16: 1 x 256 rows 12.3 / 7.0, 96 x 256 14.9 / 7.6, 16 x 2,048 15.8 / 12.6, 45 x 2,048 16.0 / 15.8, 45 x 3,000 20.4 /
-// 22.4, 16 x 16,384 22.0 / 23.0, 45 x 16,384 27.4 / 62.3; 96 x 1,400 17.0 / 14.4, 200 x 700 18.6 / 15.6, 200 x 1,200
-// 18.1 / 20.8; Q8_0: 45 x 2,048 18.6 / 18.6, 96 x 1,400 18.4 / 17.3, 200 x 700 20.0 / 20.4, 64 x 2,500 22.8 / 25.8; fp32,
-// whose own rows take the fp32 products: 5 x 256 15.0 / 9.6, 200 x 384 18.3 / 18.6, 5 x 2,048 16.0 / 17.1.
-constexpr int kAloneRows = 3 << 16, kAloneRowsMany = 9 << 15, kAloneRowsF32 = 384;
+// these are at least half as many as CUs; of Q8_0, whose values every reader converts, kAloneRowsQ8 where they are more
+// than CUs), and of fp32 caches the rows of one prefix: a launch less (one less again without partials) against rows that
+// all read.  Captured calls with 64 own rows, us, shared / alone:
+//   bf16  14 heads on 2: 16 x 6,021 rows 18.4 / 16.3, 16 x 15,360 21.3 / 21.3, 45 x 2,140 18.9 / 15.4, 45 x 5,460 21.2 / 22.6, 96 x
+//         1,505 17.9 / 15.0, 96 x 2,304 18.1 / 18.8, 200 x 722 18.4 / 16.3, 200 x 1,105 18.7 / 19.8;  32 on 8: 16 x 2,257 18.4 /
+//         18.3, 45 x 802 16.5 / 17.3;  8 on 8: 5 x 7,372 18.1 / 17.9, 45 x 409 15.1 / 13.0, 45 x 802 15.0 / 17.1
+//   Q8_0  14 on 2: 16 x 6,021 20.3 / 20.0, 45 x 3,276 22.2 / 22.5, 96 x 1,505 19.7 / 19.2, 200 x 368 18.5 / 14.1, 200 x 722
+//         20.6 / 21.4;  16 on 1: 200 x 1,444 23.2 / 19.3;  32 on 8: 45 x 409 18.7 / 16.8, 45 x 802 19.1 / 23.6;  8 on 8: 45 x 802 17.8 / 23.2
+//   fp32, whose own rows take the fp32 products  14 on 2: 16 x 376 16.9 / 12.9, 16 x 960 15.4 / 19.4, 200 x 376 20.8 / 21.6;  32
+//         on 8: 45 x 192 17.3 / 13.9, 45 x 376 19.5 / 21.4
+constexpr int kAloneRows = 3 << 16, kAloneRowsMany = 9 << 15, kAloneRowsQ8 = 7 << 15, kAloneRowsF32 = 384;
+static int64_t alone_rows(const tmac_context* ctx, int kv_dtype, int64_t n_sk) {
+    if (2 * n_sk < ctx->n_cu) return kAloneRows;
+    return kv_dtype == TMAC_KV_Q8_0 && n_sk > ctx->n_cu ? kAloneRowsQ8 : kAloneRowsMany;
+}
 int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                  const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                  int max_pages, const int32_t* lengths, const int32_t* group_starts,
@@ -1788,7 +1796,7 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
     // can be.  (45 sequences of 32 heads on 8 kv heads in 3 uneven groups, fp32, 2,500 rows: 19.2 us, 23.4 with the
     // runs of the fewest blocks whatever there are, since some CUs then take two.)
     const int64_t least = std::max<int64_t>(n_groups, cdiv(n_seq * group, tmac::kSharedCols));
-    const bool alone = n_sk * max_prefix <= (2 * n_sk >= ctx->n_cu ? kAloneRowsMany : kAloneRows) &&
+    const bool alone = n_sk * max_prefix <= alone_rows(ctx, kv_dtype, n_sk) &&
                        (kv_dtype != TMAC_KV_F32 || max_prefix <= kAloneRowsF32);
     const int64_t blocks =
         n_groups && !alone ? std::min<int64_t>(n_seq, n_seq * group / tmac::kSharedCols + n_groups) : 0;
