@@ -1419,7 +1419,7 @@ __device__ __forceinline__ void px_fetch(PxRaw<T>& r, const PagedAttnArgs& a, in
 // counted with vmcnt; px_landed() before the barrier that opens the stage.
 __device__ __forceinline__ void load_lds16(u32x4 descriptor, unsigned offset, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 ::"s"(lds), "v"(offset), "s"(descriptor) : "memory");  // nothing else here uses m0
+                 ::"s"(lds), "v"(offset), "s"(descriptor) : "memory", "m0");
 }
 __device__ __forceinline__ void px_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 template <typename T>
