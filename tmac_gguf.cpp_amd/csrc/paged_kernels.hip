@@ -23,8 +23,8 @@ namespace {
 // n_head query heads (rotated to q_out), n_kv_head keys (rotated, to the
 // cache) and n_kv_head values.  Rotation and storage are the layer step's
 // (rope8, put_row), so a row's bytes do not depend on which call wrote it.
-// Bound by memory: 18,095 fp16 rows of 14 query and 2 kv heads 31 us, 4.5 TB/s; 64
-// rows 3.4 us, a launch and three dependent loads.
+// Bound by memory: 18,095 fp16 rows of 14 query and 2 kv heads 32 us, 4.5 TB/s; 64
+// rows 3.5 us, a launch and three dependent loads.
 template <typename T>
 __device__ __forceinline__ void append_body(const AppendArgs& a) {
     __shared__ int s_seq[kAppendRows];
@@ -178,8 +178,8 @@ __device__ __forceinline__ void bounds_body(const BoundsArgs& a) {
 // 2^-53).  max(q hi, q lo) = max(q, 0) hi + min(q, 0) lo, one of the products
 // zero, so a score is a product of length 128 and runs on v_mfma_f64_4x4x4:
 // four blocks of 4 pages x 4 heads x 4 dims in 16 cycles, where fp64 FMAs with
-// a select and a sum over lanes took 2.5 times as long (27 us for 64 sequences
-// of 2,048 pages at most, 2 kv heads, 7 heads each).
+// a select and a sum over lanes took 37 us and this 21 (64 sequences of 2,048
+// pages at most, 2 kv heads, 7 heads each; 20 with the steps dealt out, below).
 //
 // Lane l holds for a step of 16 pages: of the bounds, page 4 p + l % 4 (p =
 // l / 4 % 4), dims 16 k .. 16 k + 15 (k = l / 16), product step t taking dim
@@ -537,13 +537,16 @@ __device__ __forceinline__ void select_short_body(const SelectArgs& a) {
 // rare exchange.
 //
 // bf16, fp16 and Q8_0 rows run on 16-bit MFMA, every fp32 operand carried by
-// 16-bit parts that together hold its 24 bits, so the result keeps fp32
-// accuracy:
+// 16-bit parts that together hold it (three bf16 all 24 bits, two fp16 to
+// 2^-23), so the result keeps fp32 accuracy:
 //   cache   K, V        q            P            products, Q.K and P.V
 //   bf16    exact       3 bf16       3 bf16       3, 3
 //   fp16    exact       2 fp16       2 fp16       2, 2
 //   Q8_0    int8 exact  2 fp16       3 bf16 x 2   2, 3 (scales on S and on P)
-//   fp32    3 bf16      3 bf16       3 bf16       6, 6 (parts i + j <= 2; the rest is below 2^-24)
+//   fp32    3 bf16      3 bf16       3 bf16       6, 6 (parts i + j <= 2)
+// Of fp32 rows the products i + j > 2 are left out.  Parts are cut, not rounded,
+// so these have the sign of the whole product; they are at most 2^-21 of it, and
+// 0.7 x 2^-24 of it on average.
 // (Two bf16 parts of P, 2^-18, left 2e-6 of the output's norm.)  fp32 rows are
 // split where many columns share them (prefixes) and go to fp32 MFMA where only
 // one group of query heads reads them.
@@ -859,7 +862,7 @@ __device__ __forceinline__ void values_step(Cols<T, S>& c, f32x4 w0, f32x4 w1, c
 // Own rows: one group of query heads (up to 16 columns) over a run of pages,
 // which its wave alone reads.  What bounds it is the rows' bytes; a wave holds
 // one step of pages while the next is in flight (three or four ahead were slower).
-// 64 lists of 128 bf16 pages, 2 kv heads: 17.4 us, 3.9 TB/s.
+// 64 sequences of 128 listed bf16 pages on 2 kv heads: 18.4 us, 3.7 TB/s.
 typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
 
@@ -1323,7 +1326,7 @@ __device__ __forceinline__ SharedSeq shared_seq(const PagedAttnArgs& a, int s, i
 // A stage's K and V rows go to LDS once, fetched one stage ahead, and feed both
 // column waves: 16-bit rows directly, fp32 and Q8_0 ones through registers, where
 // they are converted.  96 sequences of 14 heads on 2 behind 16,384 rows: bf16 26.4
-// us, 217 TFLOP/s (651 of parts), of 6,000 cycles a stage 3,072 are products;
+// us, 214 TFLOP/s (641 of parts); of the 6,000 cycles of a stage half are products;
 // fp16 25.2, Q8_0 36.5, fp32, six products each, 50 us.
 template <typename T>
 constexpr int kPxKeys = __is_same(T, float) ? 32 : 64;  // keys a wave takes of a stage
@@ -1630,8 +1633,8 @@ __device__ __forceinline__ void px_run(const PagedAttnArgs& a, PxLds<T>& lds, co
 // block) order, so that a row is read into one L2, or two, and not all eight.
 // How many blocks there are follows from the groups; a workgroup takes further
 // units where there are more than the grid.  None starts for nothing: one that
-// finds no work still waits for a CU with 100 KB of LDS to be free, and 160 of
-// them behind 240 others took 10 us.
+// finds no work still waits for a CU with its LDS free (131 KB for 16-bit rows, 139
+// for Q8_0, 98 for fp32), and 160 of them behind 240 others took 10 us.
 template <typename T>
 __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a) {
     __shared__ PxLds<T> lds;
