@@ -1083,3 +1083,55 @@ def test_selected_long_lists_of_many_sequences(ctx, dt):
         got = run_selected(ctx, q, kp, vp, table, lens, sel, 1, dt)
         close(got, decode64(q, kw, vw, rows_of_list(table, lens, sel), 1), f"{n} x {top}")
     no_fault(ctx)
+
+
+@pytest.mark.parametrize("dt", ALL_DT)
+def test_selected_pages_listed_twice(ctx, dt):
+    """A page listed twice counts twice, the last, partly filled one too, in one workgroup and in several; a length beyond
+    the table leaves the listed pages whole."""
+    rng = np.random.default_rng(47)
+    lens = np.array([700, 693, 2 ** 31 - 1], np.int32)
+    table, n_pages = tables(rng, [700, 693, 704])
+    kp, kw = make_pool(493, n_pages, 2, dt)
+    vp, vw = make_pool(494, n_pages, 2, dt)
+    q = oracle.normal(495, (3, 14, 64))
+    for top in (7, 90):
+        sel = rng.integers(0, 44, (3, 2, top)).astype(np.int32)
+        sel[..., 0], sel[..., top // 2], sel[..., -1], sel[1, 0, 2:4] = 43, 43, 43, -1
+        got = run_selected(ctx, q, kp, vp, table, lens, sel, 2, dt)
+        close(got, decode64(q, kw, vw, rows_of_list(table, lens.astype(np.int64), sel), 2), f"top {top}")
+    no_fault(ctx)
+
+
+def test_two_captured_steps_share_the_workspace(ctx):
+    """Two captured calls of one context, whose partials lie in the same workspace, replayed in turn: each gives its eager
+    result every time."""
+    rng = np.random.default_rng(48)
+    s, steps = ctx.stream(), []
+    for i, (n, top, dt) in enumerate(((3, 60, BF16), (5, 90, F32))):
+        lens = np.full(n, 1600, np.int32)
+        table, n_pages = tables(rng, lens)
+        kp, _ = make_pool(496 + i, n_pages, 2, dt)
+        sel = random_lists(rng, lens, 2, top)
+        d = [ctx.upload(x) for x in (oracle.normal(498 + i, (n, 14, 64)), kp, kp, table, lens, sel)] + [ctx.empty((n, 14, 64))]
+
+        def call(d=d, n=n, n_pages=n_pages, width=table.shape[1], top=top, dt=dt):
+            ctx.decode_selected(d[0], d[1], d[2], n_pages, d[3], width, d[4], d[5], top, d[6], n, 14, 2, 64, stream=s,
+                                kv_dtype=dt)
+        call()
+        eager = d[6].numpy(s)
+        steps.append([call, d[6], eager, None])
+    for step in steps:
+        ctx.step_begin(s)
+        step[0]()
+        step[3] = ctx.step_end(s)
+    for _ in range(4):
+        for _, out, _, graph in steps:
+            out.fill_bytes(0xFF, s)
+            ctx.graph_launch(graph, s)
+        for _, out, eager, _ in steps:
+            np.testing.assert_array_equal(out.numpy(s).view(np.uint32), eager.view(np.uint32))
+    for step in steps:
+        ctx.graph_destroy(step[3])
+    ctx.destroy_stream(s)
+    no_fault(ctx)
