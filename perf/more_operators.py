@@ -354,8 +354,8 @@ def _run_own(s):
         return {"weights": s.after, **_pools_own(s, ctx, dt, stream)}
     w = k == "weigh"
     ctx.decode_weighted(p(s.q), p(s.kp), p(s.vp), s.total, p(s.table), s.width, p(s.lens), p(s.before) if w else None,
-                        p(s.after) if w else None, c["max_len"], p(s.out), n, nh, nkv, HD, c["max_len"], stream=stream,
-                        kv_dtype=dt)
+                        p(s.after) if w else None, c["max_len"], p(s.out), n, nh, nkv, HD,
+                        min(c["max_len"], s.width * PAGE), stream=stream, kv_dtype=dt)
     return {"out": s.out, "weights": s.after} if w else s.out
 
 
