@@ -50,7 +50,8 @@
  *    result to compare against (parity there is unpinned).
  *    The bf16 / fp16 / Q8_0 caches, the paged caches and chunked prefill keep
  *    head_dim 64 and the compiled groups; other shapes return TMAC_ERR_UNSUPPORTED.
- *    The calls under "serving on paged caches" take other groups too (see there).
+ *    The calls under "serving on paged caches" and "long contexts in a small cache" take other groups too
+ *    (see there).
  */
 #ifndef TMAC_ATTN_H
 #define TMAC_ATTN_H
@@ -284,7 +285,15 @@ int tmac_model_free(tmac_context* ctx, tmac_model* model);
  * d stored with float_to_fp16, :53-74, which truncates the mantissa and
  * flushes fp16-subnormal values to 0).  These calls use the default 8-wave
  * group and head kernels whatever TMAC_OPT_GROUP_WAVES / _HEAD_WAVES say. */
-enum tmac_kv_dtype { TMAC_KV_F32 = 0, TMAC_KV_BF16 = 1, TMAC_KV_F16 = 2, TMAC_KV_Q8_0 = 3 };
+enum tmac_kv_dtype {
+    TMAC_KV_F32 = 0,
+    TMAC_KV_BF16 = 1,
+    TMAC_KV_F16 = 2,
+    TMAC_KV_Q8_0 = 3,
+    /* From 16 on: types of whole pages, whose rows have no address of their own; for the calls under "long
+     * contexts in a small cache" alone. */
+    TMAC_KV_Q4_PAGES = 16
+};
 int tmac_attention_decode_batched_kv(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                      const void* k, const void* v, float* out, int n_seq, int n_head,
                                      int n_kv_head, int head_dim, int n_pos, int64_t seq_stride);
@@ -423,6 +432,79 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
                                  int max_pages, const int32_t* lengths, const int32_t* group_starts,
                                  const int32_t* prefix_lens, int n_groups, float* out, int n_seq, int n_head,
                                  int n_kv_head, int head_dim, int max_prefix, int max_tail);
+
+/* ---- long contexts in a small cache (extensions; no counterpart in the reference): a cache held in
+ *      4 bits, the eviction of rows by the attention that they got, and rows whose place in the cache
+ *      is not their position ----
+ * Limits, pools and arrays as under "serving on paged caches"; kv_dtype is any tmac_kv_dtype,
+ * TMAC_KV_Q4_PAGES among them.
+ *
+ * 4-bit pages: a page is [n_kv_head][576 bytes], K and V pools alike: the codes of 16 rows of 64 dims,
+ * then fp16 scales, one a row and block of 32 dims; value = (code - 8) * scale, 4.5 bits a value.  The
+ * scale of a block is the value of its largest magnitude over -8 (the negative one of two), rounded to 7
+ * significant bits, so that values are exact in fp16; below 2^-14 it is 0 and the block's values are 0,
+ * above 8,128 it is infinity, and a NaN makes it NaN.  Codes are the nearest (x / scale + 8, ties to even,
+ * 0 .. 15).  Codes lie in the order in which the products read them; tmac_kv_widen_pages gives the rows
+ * back.  In a (page, kv head) block (row r of the page, dim d, c = d % 8; the low half of a byte holds the
+ * lower of its two dims):
+ *   K code:  byte 8 (16 (d / 16) + r) + 4 (d / 8 % 2) + c / 4 + 2 (c % 2), its high half if c / 2 is odd
+ *   V code:  byte 8 (16 (r / 4) + d % 16) + 4 (d / 32) + {0, 2, 1, 3}[r % 4], its high half if d / 16 is odd
+ *   K scale of dims 32 b ..: half word 256 + 16 b + r;  V: half word 256 + 8 (r / 4) + 4 b + r % 4
+ *
+ * Append: tmac_kv_append_paged with places and positions apart.  Row i of sequence s goes to cache row
+ * first_rows[s] + i (below 16 * max_pages).  Row t of the batch has a position on each of n_axes (1 to 4)
+ * axes, positions [n_axes][n_rows] (DEVICE), below max_pos; pair p (dims 2 p, 2 p + 1) turns by the one on
+ * axis pair_axis[p] (HOST, 32 bytes, read during the call; null: all by axis 0), with the frequency that
+ * p has anyway: time, height and width of images and video as a model deals them to the pairs.  A row with
+ * a place or a position outside is skipped and sets bit 0 of the device error word, one whose block-table
+ * entry is outside the pool is rotated but not stored (bit 2).  With one axis, positions equal to the
+ * places and a row type, q_out and the pages get the bits that tmac_kv_append_paged gives them.  Everything
+ * else is as there.
+ *
+ * Attention with weights: one query token per sequence over its rows 0 .. lengths[s] - 1, as
+ * tmac_attention_decode_paged (max_len as there; a longer sequence gives NaN and bit 1, length 0 zeros).
+ * weights_out (null: not wanted) [n_seq][n_kv_head][weight_stride]: for r < lengths[s], weights_in of row r
+ * (null: 0) plus the softmax weights that the kv head's query heads gave row r, summed; other entries are
+ * left as they were, those of sequences that are too long among them.  weights_in may be weights_out;
+ * another overlap is refused.  weight_stride >= max_len.  At most 65,535 sequences times kv heads with
+ * weights.  The scores wait in the context's workspace, 4 bytes a row and query head of max_len.
+ *
+ * Rows to keep: kept [n_seq][n_kv_head][keep]: the sequence's first `first` and last `last` rows and, up to
+ * keep in all, those with the largest weights (ties: the lower row; a NaN as +infinity), ascending, then -1;
+ * all rows where there are no more than keep.  first + last <= keep.  A length above max_len gives an empty
+ * list (all -1) and sets bit 1.  The weights of the first and last rows may hold anything.
+ *
+ * Compaction: kv head h of row kept[s][h][j] becomes row j of the pages to_table[s] (to_pages of them a
+ * sequence), k and v, bit for bit; the row stays where it was too.  An entry of -1 leaves its row of the
+ * destination as it was; another entry outside [0, lengths[s]) does too, and sets bit 2.  A block-table
+ * entry outside the pool is clamped (bit 2), a to_table entry outside it leaves its page out (bit 2).  The
+ * destination pages are pages of the same pools that hold no row of the call's sequences, each named once;
+ * once the call has run, the pages of block_table that nobody else shares are free.  weights_out (both
+ * null: not wanted; strides alike; no overlap) gets the weight of every kept row at j, and 0 where there is
+ * none, up to weight_stride: the next rows start from nothing.  The sequence goes on with length
+ * min(lengths[s], keep), where appended rows keep counting their positions from the old length. */
+int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q, int64_t q_stride,
+                              float* q_out, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                              void* k_pages, void* v_pages, int n_pages, const int32_t* block_table, int max_pages,
+                              const int32_t* row_starts, const int32_t* first_rows, const int32_t* positions, int n_axes,
+                              const uint8_t* pair_axis, int n_seq, int n_rows, int n_head, int n_kv_head, int head_dim,
+                              int max_pos, float base);
+int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
+                                   const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
+                                   int max_pages, const int32_t* lengths, const float* weights_in, float* weights_out,
+                                   int64_t weight_stride, float* out, int n_seq, int n_head, int n_kv_head, int head_dim,
+                                   int max_len);
+int tmac_select_rows(tmac_context* ctx, tmac_stream stream, const float* weights, int64_t weight_stride,
+                     const int32_t* lengths, int32_t* kept, int n_seq, int n_kv_head, int max_len, int keep, int first,
+                     int last);
+int tmac_kv_compact_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, void* k_pages, void* v_pages, int n_pages,
+                          const int32_t* block_table, int max_pages, const int32_t* lengths, const int32_t* kept,
+                          int keep, const int32_t* to_table, int to_pages, const float* weights_in, float* weights_out,
+                          int64_t weight_stride, int n_seq, int n_kv_head, int head_dim);
+/* Pool pages 0 .. n_pages - 1 of any kv_dtype as fp32 rows [n_pages][16][n_kv_head][64], exactly.  Either
+ * pool, with its output, may be null. */
+int tmac_kv_widen_pages(tmac_context* ctx, tmac_stream stream, int kv_dtype, const void* k_pages, const void* v_pages,
+                        float* k_out, float* v_out, int n_pages, int n_kv_head, int head_dim);
 
 /* ---- chunked causal prefill (extension; the reference feeds prompts one token at a time,
  *      tmac_gguf.cpp:1621-1658, so its oracle is attention_op per query row) ----

@@ -262,12 +262,64 @@ struct PagedAttnArgs {
     int prefix_groups;       // workgroups of the prefix kernel that share its units
     int prefix_blocks;       // blocks of kSharedCols (sequence, query head) columns, at most
     int tail_splits, tail_rows;  // slots behind them: runs of tail_rows own rows (of all, if it reads the prefix itself)
+    // whole sequences (rows kernel): slot i holds rows i * slot_rows ..
+    int max_len, slot_rows;
+    float* scores;           // [n_seq][n_head][score_stride] in log2 units; null: no weights are wanted
+    int64_t score_stride;    // a multiple of kPageRows
+    const float* weights_in;  // [n_seq][n_kv_head][weight_stride]; null: zeros
+    float* weights_out;
+    int64_t weight_stride;
 };
 constexpr int kPagedWaves = 4;    // waves per workgroup
 constexpr int kSharedWaves = 8;   // the same, shared prefixes
 constexpr int kMaxGroupHeads = 16;  // query heads per kv head, at most (MFMA columns)
 constexpr int kXcds = 8;          // dies that workgroups are dealt to in turn, each with an L2 of its own
 constexpr int kSharedCols = 64;   // prefix workgroup: (sequence, query head) columns
+
+// Append of a ragged batch of rows to given cache rows: row t of q / k / v belongs
+// to the last sequence s with row_starts[s] <= t, goes to cache row first_rows[s] +
+// t - row_starts[s] and is turned, pair by pair, by the position on the pair's axis.
+struct AppendAxesArgs {
+    AppendArgs a;            // positions: first_rows; capacity: of cache rows
+    const int32_t* pos;      // [n_axes][n_rows]
+    int max_pos;             // positions lie below it
+    int n_axes;
+    uint64_t pair_axis;      // 2 bits a pair: its axis
+};
+
+// The rows to keep of every (sequence, kv head): all up to keep, else the first and
+// last ones and those of the largest weights.
+struct SelectRowsArgs {
+    const float* weights;    // [n_seq][n_kv_head][weight_stride]
+    const int32_t* lengths;
+    int32_t* kept;           // [n_seq][n_kv_head][keep]
+    int* err;
+    int64_t weight_stride;
+    int n_seq, n_kv_head, max_len, keep, first, last;
+};
+
+// Kept rows of k, v and the weights to the first rows of other pages.
+struct CompactArgs {
+    char* k_pages;
+    char* v_pages;
+    const int32_t* block_table;  // [n_seq][max_pages]
+    const int32_t* lengths;
+    const int32_t* kept;         // [n_seq][n_kv_head][keep]
+    const int32_t* to_table;     // [n_seq][to_pages]
+    const float* weights_in;     // [n_seq][n_kv_head][weight_stride]; null: no weights
+    float* weights_out;
+    int* err;
+    int64_t weight_stride;
+    int n_pages, max_pages, to_pages, n_seq, n_kv_head, keep;
+    int n_grid;                  // groups of kPageRows kept rows per (sequence, kv head)
+};
+
+// Pool pages -> fp32 rows [n_pages][16][n_kv_head][64].
+struct WidenArgs {
+    const char* pages[2];        // k, v; null: not wanted
+    float* out[2];
+    int n_pages, n_kv_head;
+};
 
 struct PosArgs {
     int* pos;

@@ -155,6 +155,36 @@ struct CacheFmt<q8_0_t> {
     static constexpr int kDimBytes = 1;
 };
 
+// 4-bit pages (TMAC_KV_Q4_PAGES).  A (page, kv head) is one block of kQ4Block
+// bytes, 512 of codes and 32 fp16 scales, laid out for the product that reads
+// it: lane l of a wave takes the eight code bytes from 8 l on, K as the operand
+// (row l % 16, dims 16 (l / 16) ..), V as the operand (dims l % 16 + 16 b, four
+// rows from 4 (l / 16) on), with no exchange between lanes.  A byte holds two
+// dims of one row, so that rows are written without reading what is there.
+//   K  byte 8 (16 g + row) + 4 m + c: dims d = 16 g + 8 m + 4 (c & 1) + (c >> 1) and d + 2
+//      scale of (row, dims 32 half ..): half word 256 + 16 half + row
+//   V  byte 8 (16 (row / 4) + i) + 4 p + {0, 2, 1, 3}[row % 4]: dims 32 p + i and 32 p + i + 16
+//      scale: half word 256 + 8 (row / 4) + 4 half + row % 4
+// value = (code - 8) * scale.  A scale has 7 significant bits and is 0 or at
+// least 2^-14, so that a value is exact in fp16 (4 + 7 bits), and so is a
+// sixteenth of its scale.
+struct q4_t {};
+constexpr int kQ4Block = 576;
+
+// Byte geometry of pages: from row to row of a head, of a page, and of head h in its page.
+template <typename T>
+struct PageFmt {
+    __device__ static size_t row(int kv) { return (size_t)kv * CacheFmt<T>::kHeadBytes; }
+    __device__ static size_t page(int kv) { return kPageRows * row(kv); }
+    __device__ static size_t head(int h) { return (size_t)h * CacheFmt<T>::kHeadBytes; }
+};
+template <>
+struct PageFmt<q4_t> {
+    __device__ static size_t row(int) { return 0; }
+    __device__ static size_t page(int kv) { return (size_t)kv * kQ4Block; }
+    __device__ static size_t head(int h) { return (size_t)h * kQ4Block; }
+};
+
 // This lane's 8 dims of a cache head row as loaded (raw words): fp32 8
 // floats, 16-bit 4 words, Q8_0 the two 4-byte runs plus the scale word.
 // Prefetch buffers hold raw rows and are widened where they are used, so the

@@ -6,6 +6,8 @@
 // heads per kv head at run time; a kernel is built per cache element type.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "attn_args.h"
 #include "attn_device.h"
 
@@ -908,8 +910,9 @@ struct Own {
         }
     }
     // Keys lo[u] .. hi[u] - 1 of page u take part.
+    template <typename Score>
     __device__ static void attend(State& st, const Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles],
-                                  Lds& lds, int lane) {
+                                  Lds& lds, int lane, Score score) {
         using KO = typename Parts<T>::KOps;
         const int i = lane & 15, g = lane >> 4;
         const u32x4 zero = {0, 0, 0, 0};
@@ -959,6 +962,8 @@ struct Own {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) w[u][r] = 4 * g + r >= lo[u] && 4 * g + r < hi[u] ? w[u][r] : kNegInf;
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) score(u, w[u] + st.base);
         softmax_step<S>(st.m, st.l, st.base, st.o, w);
         values_step<T, S>(st, w[0], w[1], &lds.v[0][0], 0, lds.vd[0], lds.vd[Q8 ? 1 : 0], lane);
     }
@@ -1015,8 +1020,9 @@ struct Own<float> {
 #pragma unroll
         for (int r = 0; r < 4; ++r) t.v[r] = *reinterpret_cast<const f32x4*>(vp + (4 * g + r) * stride + 16 * i);
     }
+    template <typename Score>
     __device__ static void attend(State& st, const Tile (&tiles)[1], const int (&lo)[1], const int (&hi)[1], Lds&,
-                                  int lane) {
+                                  int lane, Score score) {
         const Tile& t = tiles[0];
         const int g = lane >> 4;
         const bool full = lo[0] <= 0 && hi[0] >= kPageRows;
@@ -1034,6 +1040,7 @@ struct Own<float> {
 #pragma unroll
             for (int r = 0; r < 4; ++r) w[0][r] = in(r) ? w[0][r] : kNegInf;
         }
+        score(0, w[0] + st.base);
         softmax_step<S>(st.m, st.l, st.base, st.o, w);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -1058,18 +1065,23 @@ union OwnLds {
     __device__ OwnLds() {}
 };
 
+// No use for the scores themselves.
+struct NoScores {
+    __device__ __forceinline__ void operator()(int, f32x4) const {}
+};
+
 // A run of pages.  look(e, logical, page) gives entry e (0 <= e < n) its page of
 // the pool (checked, in range) and its logical page index (-1: skipped); rows
 // row_lo .. row_hi - 1 of the sequence take part.  The NW waves take the
 // entries in turn, kTiles at once; a wave looks up 64 of its entries at a time,
-// one a lane.
-template <typename T, int NW, typename Look>
+// one a lane.  score(logical, x): this lane's four scores of that page, log2 units.
+template <typename T, int NW, typename Look, typename Score = NoScores>
 __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const PagedAttnArgs& a, int h, int n,
                                            int64_t row_lo, int64_t row_hi, typename Own<T>::Lds& lds, int wave,
-                                           int lane, Look look) {
+                                           int lane, Look look, Score score = Score()) {
     using O = Own<T>;
-    constexpr int HB = CacheFmt<T>::kHeadBytes, KT = O::kTiles;
-    const size_t stride = (size_t)a.n_kv_head * HB, page_bytes = kPageRows * stride;
+    constexpr int KT = O::kTiles;
+    const size_t stride = PageFmt<T>::row(a.n_kv_head), page_bytes = PageFmt<T>::page(a.n_kv_head);
     const int steps = ((n + KT - 1) / KT - wave + NW - 1) / NW;  // this wave's
     for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
         const int cnt = min(64 / KT, steps - s0);
@@ -1080,7 +1092,7 @@ __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const Pag
         auto fetch = [&](typename O::Tile (&x)[KT], int step) {
 #pragma unroll
             for (int u = 0; u < KT; ++u) {
-                const size_t at = (size_t)__builtin_amdgcn_readlane(page, KT * step + u) * page_bytes + (size_t)h * HB;
+                const size_t at = (size_t)__builtin_amdgcn_readlane(page, KT * step + u) * page_bytes + PageFmt<T>::head(h);
                 O::fetch(x[u], a.k_pages + at, a.v_pages + at, stride, lane);
             }
         };
@@ -1090,16 +1102,17 @@ __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const Pag
             for (int d = 0; d < 2; ++d) {
                 if (step + d < cnt) {
                     if (step + d + 1 < cnt) fetch(t[1 - d], step + d + 1);
-                    int lo[KT], hi[KT], any = 0;
+                    int lo[KT], hi[KT], at[KT], any = 0;
 #pragma unroll
                     for (int u = 0; u < KT; ++u) {
                         const int j = __builtin_amdgcn_readlane(logical, KT * (step + d) + u);
                         const int64_t r0 = (int64_t)j * kPageRows;
+                        at[u] = j;
                         lo[u] = (int)max((int64_t)0, min(row_lo - r0, (int64_t)kPageRows));
                         hi[u] = j < 0 ? 0 : (int)max((int64_t)0, min(row_hi - r0, (int64_t)kPageRows));
                         any |= hi[u] > lo[u];
                     }
-                    if (any) O::attend(st, t[d], lo, hi, lds, lane);
+                    if (any) O::attend(st, t[d], lo, hi, lds, lane, [&](int u, f32x4 x) { score(at[u], x); });
                 }
             }
         }
@@ -1789,6 +1802,8 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     *reinterpret_cast<f32x4*>(a.out + row * kHeadDim + 4 * lane) = y;
 }
 
+#include "budget_kernels.h"
+
 }  // namespace
 
 #define TMAC_PAGED_KERNELS(NAME, T)                                                                                    \
@@ -1812,6 +1827,23 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_tail_finish_wide_##NAME(PagedAttnArgs a) {    \
         tail_body<T, kSharedWaves, true>(a);                                                                           \
     }
+#define TMAC_BUDGET_KERNELS(NAME, T)                                                                                  \
+    extern "C" __global__ __launch_bounds__(256) void tmac_append_axes_##NAME(AppendAxesArgs a) {                     \
+        append_axes_body<T>(a);                                                                                       \
+    }                                                                                                                 \
+    extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_rows_##NAME(PagedAttnArgs a) {                \
+        rows_body<T, kPagedWaves>(a);                                                                                 \
+    }                                                                                                                 \
+    extern "C" __global__ __launch_bounds__(256) void tmac_compact_##NAME(CompactArgs a) { compact_body<T>(a); }      \
+    extern "C" __global__ __launch_bounds__(256) void tmac_widen_##NAME(WidenArgs a) { widen_body<T>(a); }
+TMAC_BUDGET_KERNELS(f32, float)
+TMAC_BUDGET_KERNELS(bf16, __bf16)
+TMAC_BUDGET_KERNELS(f16, _Float16)
+TMAC_BUDGET_KERNELS(q8, q8_0_t)
+TMAC_BUDGET_KERNELS(q4, q4_t)
+extern "C" __global__ __launch_bounds__(256) void tmac_row_weights(PagedAttnArgs a) { row_weights_body(a); }
+extern "C" __global__ __launch_bounds__(1024) void tmac_select_rows(SelectRowsArgs a) { select_rows_body(a); }
+
 TMAC_PAGED_KERNELS(f32, float)
 TMAC_PAGED_KERNELS(bf16, __bf16)
 TMAC_PAGED_KERNELS(f16, _Float16)

@@ -38,7 +38,9 @@ extern "C" const uint64_t tmac_attn_code_object_sizes[kCodeParts];
 extern "C" int tmac_scratch_setup(int device, void** ptr);
 
 using tmac::AppendArgs;
+using tmac::AppendAxesArgs;
 using tmac::BoundsArgs;
+using tmac::CompactArgs;
 using tmac::CopyArgs;
 using tmac::CvtArgs;
 using tmac::DecodeArgs;
@@ -52,6 +54,8 @@ using tmac::PosArgs;
 using tmac::KqArgs;
 using tmac::PagedAttnArgs;
 using tmac::SelectArgs;
+using tmac::SelectRowsArgs;
+using tmac::WidenArgs;
 using tmac::QkvArgs;
 using tmac::kQkvWaves;
 using tmac::RopeArgs;
@@ -77,7 +81,8 @@ constexpr int kShapes[][2] = {{7, 2}, {1, 1}, {1, 2}, {2, 2}, {4, 2}, {4, 4}, {8
 enum { kModeUniform = 0, kModeRagged = 1, kModeLayer = 2 };
 enum { kPagedDecode = 0, kPagedLayer = 1 };
 constexpr int kNarrowTypes = 3;  // TMAC_KV_BF16, TMAC_KV_F16, TMAC_KV_Q8_0 (index kv_dtype - 1)
-const char* const kTypeName[4] = {"f32", "bf16", "f16", "q8"};  // by kv_dtype
+const char* const kTypeName[5] = {"f32", "bf16", "f16", "q8", "q4"};  // by kv_dtype; kQ4: TMAC_KV_Q4_PAGES
+constexpr int kQ4 = 4;
 
 
 struct RopeTable {
@@ -142,6 +147,9 @@ struct tmac_context {
     hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[2][4] = {}, k_scores[2] = {}, k_select_short[2] = {};
     hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[2][4] = {};  // shared prefixes, own rows
     hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
+    // the same, long contexts in a small cache: by cache type, 4-bit pages last
+    hipFunction_t k_append_axes[5] = {}, k_rows[5] = {}, k_compact[5] = {}, k_widen[5] = {};
+    hipFunction_t k_row_weights = nullptr, k_select_rows = nullptr;
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
     float* ws = nullptr;
@@ -1073,6 +1081,19 @@ int tmac_init(tmac_context** out, int device) {
                 if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
             }
         }
+        for (int dt = 0; dt < 5; dt++) {
+            const std::pair<const char*, hipFunction_t*> by_type[] = {{"tmac_append_axes", &ctx->k_append_axes[dt]},
+                                                                      {"tmac_rows", &ctx->k_rows[dt]},
+                                                                      {"tmac_compact", &ctx->k_compact[dt]},
+                                                                      {"tmac_widen", &ctx->k_widen[dt]}};
+            for (auto& k : by_type) {
+                std::snprintf(name, sizeof(name), "%s_%s", k.first, kTypeName[dt]);
+                if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
+            }
+        }
+        if ((e = get_function(ctx, &ctx->k_row_weights, "tmac_row_weights")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_select_rows, "tmac_select_rows")) != hipSuccess)
+            return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
         if ((e = get_function(ctx, &ctx->k_scores[0], "tmac_page_scores_h4")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_scores[1], "tmac_page_scores_h8")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_select_short[0], "tmac_select_short_h4")) != hipSuccess ||
@@ -1850,6 +1871,287 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
                                       tail_threads, (hipStream_t)stream, &a, (unsigned)n_seq)))
         return rc;
     return launch_paged_merge(ctx, stream, ctx->k_shared_merge, &a);
+}
+
+// ---- long contexts in a small cache ----
+
+// Index of a cache type of these calls (4-bit pages beside the row types), or -1.
+static int budget_type(int kv_dtype) {
+    return kv_dtype >= TMAC_KV_F32 && kv_dtype <= TMAC_KV_Q8_0 ? kv_dtype : kv_dtype == TMAC_KV_Q4_PAGES ? kQ4 : -1;
+}
+static int check_budget(tmac_context* ctx, const char* what, int kv_dtype, int n_pages, const int32_t* block_table,
+                        int max_pages, int n_seq, int n_head, int n_kv_head, int head_dim) {
+    if (budget_type(kv_dtype) < 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG,
+                    std::string(what) + ": kv_dtype must be TMAC_KV_F32, _BF16, _F16, _Q8_0 or _Q4_PAGES");
+    return check_serving(ctx, what, TMAC_KV_F32, n_pages, block_table, max_pages, n_seq, n_head, n_kv_head, head_dim);
+}
+
+// Bytes from the first to the last of n rows of `row` floats, `stride` floats apart (as many as there can be if more).
+static size_t extent_bytes(int64_t n, int64_t stride, int64_t row) {
+    int64_t x = 0;
+    if (n < 1 || stride < 0) return n < 1 ? 0 : (size_t)row * sizeof(float);
+    if (__builtin_mul_overflow(n - 1, stride, &x) || __builtin_add_overflow(x, row, &x) ||
+        __builtin_mul_overflow(x, (int64_t)sizeof(float), &x))
+        return SIZE_MAX;
+    return (size_t)x;
+}
+// Whether two ranges of bytes share one.
+static bool ranges_meet(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return na && nb && (x < y ? y - x < na : x - y < nb);
+}
+
+int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q, int64_t q_stride,
+                              float* q_out, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                              void* k_pages, void* v_pages, int n_pages, const int32_t* block_table, int max_pages,
+                              const int32_t* row_starts, const int32_t* first_rows, const int32_t* positions, int n_axes,
+                              const uint8_t* pair_axis, int n_seq, int n_rows, int n_head, int n_kv_head, int head_dim,
+                              int max_pos, float base) {
+    const char* what = "kv_append_axes_paged";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    AppendAxesArgs x{};
+    AppendArgs& a = x.a;
+    if (!k || !v || !k_pages || !v_pages || !row_starts || !first_rows || !positions || !q != !q_out)
+        return fail(ctx, TMAC_ERR_NULL_POINTER, "kv_append_axes_paged: null buffer");
+    if (n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: n_head must be a positive multiple of n_kv_head");
+    if ((rc = check_budget(ctx, what, kv_dtype, n_pages, block_table, max_pages, n_seq, n_kv_head, n_kv_head, head_dim)))
+        return rc;
+    if (!aligned16(q) || !aligned16(q_out) || !aligned16(k) || !aligned16(v) || !aligned16(k_pages) ||
+        !aligned16(v_pages) || q_stride % 4 || k_stride % 4 || v_stride % 4 || (uintptr_t)row_starts % 4 ||
+        (uintptr_t)first_rows % 4 || (uintptr_t)positions % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "kv_append_axes_paged: rows and pools must be 16-byte aligned");
+    if (n_rows < 0 || max_pos < 1)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: need n_rows >= 0 and max_pos >= 1");
+    if (n_axes < 1 || n_axes > 4)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: 1 to 4 axes");
+    for (int i = 0; pair_axis && i < kHeadDim / 2; i++) {
+        if (pair_axis[i] >= n_axes)
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: a pair's axis is not below n_axes");
+        x.pair_axis |= (uint64_t)pair_axis[i] << (2 * i);
+    }
+    const int64_t q_row = (int64_t)n_head * kHeadDim, kv_row = (int64_t)n_kv_head * kHeadDim;
+    if (n_rows > 1 && ((q && q_stride < q_row) || k_stride < kv_row || v_stride < kv_row))
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: a row stride is shorter than its row");
+    if (!(base > 0.f) || !std::isfinite(base))
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: bad base");
+    if (n_seq == 0 || n_rows == 0) return TMAC_OK;
+    if (q) {  // as tmac_kv_append_paged
+        const size_t out_bytes = extent_bytes(n_rows, q_row, q_row);
+        if (!(q == q_out && (q_stride == q_row || n_rows == 1)) &&
+            ranges_meet(q_out, out_bytes, q, extent_bytes(n_rows, q_stride, q_row)))
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: q_out overlaps q without being it");
+        if (ranges_meet(q_out, out_bytes, k, extent_bytes(n_rows, k_stride, kv_row)) ||
+            ranges_meet(q_out, out_bytes, v, extent_bytes(n_rows, v_stride, kv_row)))
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_append_axes_paged: q_out overlaps k or v");
+    }
+    if ((rc = set_device(ctx))) return rc;
+    const RopeTable* rt = nullptr;
+    if ((rc = rope_table(ctx, (hipStream_t)stream, head_dim, base, max_pos, &rt))) return rc;
+    a.q = q;
+    a.q_out = q_out;
+    a.k = k;
+    a.v = v;
+    a.k_pages = static_cast<char*>(k_pages);
+    a.v_pages = static_cast<char*>(v_pages);
+    a.block_table = block_table;
+    a.row_starts = row_starts;
+    a.positions = first_rows;
+    a.rope_cs = rt->dev;
+    a.err = ctx->err;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.n_pages = n_pages;
+    a.max_pages = max_pages;
+    a.n_seq = n_seq;
+    a.n_rows = n_rows;
+    a.n_head = n_head;
+    a.n_kv_head = n_kv_head;
+    a.capacity = (int)std::min<int64_t>((int64_t)max_pages * kPageRows, INT_MAX);
+    x.pos = positions;
+    x.n_axes = n_axes;
+    x.max_pos = max_pos;
+    a.rows_per_group = (int)std::min<int64_t>(tmac::kAppendRows, std::max<int64_t>(1, n_rows / (8 * ctx->n_cu)));
+    const int64_t blocks = cdiv(n_rows, a.rows_per_group);
+    const int64_t heads = a.rows_per_group * (2 * (int64_t)n_kv_head + (q ? n_head : 0));
+    if ((rc = check_units(ctx, what, blocks, 256)) || (rc = check_units(ctx, what, heads + 32))) return rc;
+    return launch(ctx, ctx->k_append_axes[budget_type(kv_dtype)], (unsigned)blocks, 1, 256, (hipStream_t)stream, &x);
+}
+
+int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
+                                   const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
+                                   int max_pages, const int32_t* lengths, const float* weights_in, float* weights_out,
+                                   int64_t weight_stride, float* out, int n_seq, int n_head, int n_kv_head, int head_dim,
+                                   int max_len) {
+    const char* what = "decode_weighted";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    const int dt = budget_type(kv_dtype);
+    if (dt < 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG,
+                    "decode_weighted: kv_dtype must be TMAC_KV_F32, _BF16, _F16, _Q8_0 or _Q4_PAGES");
+    PagedAttnArgs a{};
+    if ((rc = paged_attn_args(ctx, what, TMAC_KV_F32, q, k_pages, v_pages, n_pages, block_table, max_pages, lengths, out,
+                              n_seq, n_head, n_kv_head, head_dim, &a)))
+        return rc;
+    if (max_len < 1 || max_len > (int64_t)max_pages * kPageRows)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: 1 <= max_len <= 16 * max_pages");
+    if (weights_in && !weights_out) return fail(ctx, TMAC_ERR_NULL_POINTER, "decode_weighted: weights_in alone");
+    if ((uintptr_t)weights_in % 4 || (uintptr_t)weights_out % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "decode_weighted: weights");
+    if (weights_out && weight_stride < max_len)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: weight_stride below max_len");
+    if (n_seq == 0) return TMAC_OK;
+    const int64_t n_sk = (int64_t)n_seq * n_kv_head;
+    if (weights_out) {
+        const size_t bytes = extent_bytes(n_sk, weight_stride, max_len);
+        if (weights_in && weights_in != weights_out && ranges_meet(weights_in, bytes, weights_out, bytes))
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: weights_out overlaps weights_in without being it");
+    }
+    a.max_len = max_len;
+    const int64_t pages = cdiv(max_len, kPageRows);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({4 * ctx->n_cu / n_sk, cdiv(pages, 2 * tmac::kPagedWaves),
+                                                             (int64_t)kMaxSplits}));
+    a.slot_rows = (int)(cdiv(pages, splits) * kPageRows);
+    a.n_slots = (int)cdiv(max_len, a.slot_rows);
+    if ((rc = check_units(ctx, what, n_sk * a.n_slots, 64 * tmac::kPagedWaves))) return rc;
+    const size_t n_rows = (size_t)n_seq * n_head, part = n_rows * a.n_slots * (kHeadDim + 2);
+    if (weights_out) {
+        if (n_sk > kMaxGridYZ)
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: more than 65535 sequences times kv heads with weights");
+        a.score_stride = pages * kPageRows;
+        a.weights_in = weights_in;
+        a.weights_out = weights_out;
+        a.weight_stride = weight_stride;
+    }
+    if ((rc = set_device(ctx))) return rc;
+    const size_t scores_at = (part + 3) / 4 * 4;  // the scores behind the partials, 16-byte aligned
+    const size_t floats = weights_out ? scores_at + n_rows * (size_t)a.score_stride : part;
+    if (weights_out || a.n_slots > 1) {
+        if ((rc = ensure_workspace(ctx, (hipStream_t)stream, floats))) return rc;
+        a.ws = workspace(ctx);
+        if (weights_out) a.scores = a.ws + scores_at;
+    }
+    if ((rc = launch(ctx, ctx->k_rows[dt], (unsigned)(n_sk * a.n_slots), 1, 64 * tmac::kPagedWaves, (hipStream_t)stream,
+                     &a)))
+        return rc;
+    if (a.n_slots > 1 && (rc = launch_paged_merge(ctx, stream, ctx->k_selected_merge, &a))) return rc;
+    if (!weights_out) return TMAC_OK;
+    return launch(ctx, ctx->k_row_weights, (unsigned)cdiv(max_len, 1024), (unsigned)n_sk, 256, (hipStream_t)stream, &a);
+}
+
+int tmac_select_rows(tmac_context* ctx, tmac_stream stream, const float* weights, int64_t weight_stride,
+                     const int32_t* lengths, int32_t* kept, int n_seq, int n_kv_head, int max_len, int keep, int first,
+                     int last) {
+    const char* what = "select_rows";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    if (!weights || !lengths || !kept) return fail(ctx, TMAC_ERR_NULL_POINTER, "select_rows: null buffer");
+    if ((uintptr_t)weights % 4 || (uintptr_t)lengths % 4 || (uintptr_t)kept % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "select_rows: buffers must be 4-byte aligned");
+    if (n_seq < 0 || n_kv_head <= 0 || max_len < 1 || weight_stride < max_len)
+        return fail(ctx, TMAC_ERR_INVALID_ARG,
+                    "select_rows: need n_seq >= 0, n_kv_head >= 1 and 1 <= max_len <= weight_stride");
+    if (keep < 1 || first < 0 || last < 0 || (int64_t)first + last > keep)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "select_rows: need keep >= 1, first, last >= 0 and first + last <= keep");
+    if (n_seq == 0) return TMAC_OK;
+    const int64_t n_sk = (int64_t)n_seq * n_kv_head;
+    if ((rc = check_units(ctx, what, n_sk, 1024)) || (rc = set_device(ctx))) return rc;
+    SelectRowsArgs a{};
+    a.weights = weights;
+    a.lengths = lengths;
+    a.kept = kept;
+    a.err = ctx->err;
+    a.weight_stride = weight_stride;
+    a.n_seq = n_seq;
+    a.n_kv_head = n_kv_head;
+    a.max_len = max_len;
+    a.keep = keep;
+    a.first = first;
+    a.last = last;
+    return launch(ctx, ctx->k_select_rows, (unsigned)n_sk, 1, 1024, (hipStream_t)stream, &a);
+}
+
+int tmac_kv_compact_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, void* k_pages, void* v_pages, int n_pages,
+                          const int32_t* block_table, int max_pages, const int32_t* lengths, const int32_t* kept,
+                          int keep, const int32_t* to_table, int to_pages, const float* weights_in, float* weights_out,
+                          int64_t weight_stride, int n_seq, int n_kv_head, int head_dim) {
+    const char* what = "kv_compact_paged";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    if (!k_pages || !v_pages || !lengths || !kept || !to_table || !weights_in != !weights_out)
+        return fail(ctx, TMAC_ERR_NULL_POINTER, "kv_compact_paged: null buffer");
+    if ((rc = check_budget(ctx, what, kv_dtype, n_pages, block_table, max_pages, n_seq, n_kv_head, n_kv_head, head_dim)))
+        return rc;
+    if (!aligned16(k_pages) || !aligned16(v_pages) || (uintptr_t)lengths % 4 || (uintptr_t)kept % 4 ||
+        (uintptr_t)to_table % 4 || (uintptr_t)weights_in % 4 || (uintptr_t)weights_out % 4)
+        return fail(ctx, TMAC_ERR_MISALIGNED, "kv_compact_paged: pools must be 16-byte aligned");
+    if (keep < 1 || to_pages < cdiv(keep, kPageRows))
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: 1 <= keep <= 16 * to_pages");
+    if (weights_out && weight_stride < keep)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: weight_stride below keep");
+    if (n_seq == 0) return TMAC_OK;
+    const int64_t n_sk = (int64_t)n_seq * n_kv_head;
+    CompactArgs a{};
+    a.n_grid = (int)cdiv(keep, kPageRows);
+    if (n_sk > INT_MAX / a.n_grid || (rc = check_units(ctx, what, n_sk * a.n_grid, 256)))
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: too many units of work");
+    if (weights_out) {
+        const size_t bytes = extent_bytes(n_sk, weight_stride, weight_stride);
+        if (ranges_meet(weights_in, bytes, weights_out, bytes))
+            return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: weights_out overlaps weights_in");
+    }
+    if ((rc = set_device(ctx))) return rc;
+    a.k_pages = static_cast<char*>(k_pages);
+    a.v_pages = static_cast<char*>(v_pages);
+    a.block_table = block_table;
+    a.lengths = lengths;
+    a.kept = kept;
+    a.to_table = to_table;
+    a.weights_in = weights_in;
+    a.weights_out = weights_out;
+    a.err = ctx->err;
+    a.weight_stride = weight_stride;
+    a.n_pages = n_pages;
+    a.max_pages = max_pages;
+    a.to_pages = to_pages;
+    a.n_seq = n_seq;
+    a.n_kv_head = n_kv_head;
+    a.keep = keep;
+    return launch(ctx, ctx->k_compact[budget_type(kv_dtype)], (unsigned)(n_sk * a.n_grid), 1, 256, (hipStream_t)stream,
+                  &a);
+}
+
+int tmac_kv_widen_pages(tmac_context* ctx, tmac_stream stream, int kv_dtype, const void* k_pages, const void* v_pages,
+                        float* k_out, float* v_out, int n_pages, int n_kv_head, int head_dim) {
+    const char* what = "kv_widen_pages";
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    if (!k_pages != !k_out || !v_pages != !v_out || (!k_pages && !v_pages))
+        return fail(ctx, TMAC_ERR_NULL_POINTER, "kv_widen_pages: null buffer");
+    const int dt = budget_type(kv_dtype);
+    if (dt < 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG,
+                    "kv_widen_pages: kv_dtype must be TMAC_KV_F32, _BF16, _F16, _Q8_0 or _Q4_PAGES");
+    if (head_dim != kHeadDim) return fail(ctx, TMAC_ERR_UNSUPPORTED, "kv_widen_pages: head_dim must be 64");
+    if (n_pages < 0 || n_kv_head <= 0)
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_widen_pages: n_pages >= 0, n_kv_head >= 1");
+    if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(k_out) || !aligned16(v_out))
+        return fail(ctx, TMAC_ERR_MISALIGNED, "kv_widen_pages: pools and outputs must be 16-byte aligned");
+    if (n_pages == 0) return TMAC_OK;
+    const int64_t units = (int64_t)n_pages * n_kv_head;
+    if ((rc = check_units(ctx, what, units, 256)) || (rc = set_device(ctx))) return rc;
+    WidenArgs a{};
+    a.pages[0] = static_cast<const char*>(k_pages);
+    a.pages[1] = static_cast<const char*>(v_pages);
+    a.out[0] = k_out;
+    a.out[1] = v_out;
+    a.n_pages = n_pages;
+    a.n_kv_head = n_kv_head;
+    return launch(ctx, ctx->k_widen[dt], (unsigned)units, 1, 256, (hipStream_t)stream, &a);
 }
 
 int tmac_kv_convert(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* src, void* dst, int64_t n) {

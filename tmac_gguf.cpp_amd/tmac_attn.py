@@ -44,7 +44,9 @@ TMAC_KV_F32 = 0
 TMAC_KV_BF16 = 1
 TMAC_KV_F16 = 2
 TMAC_KV_Q8_0 = 3
+TMAC_KV_Q4_PAGES = 16    # 4-bit pages: [kv head][Q4_BLOCK_BYTES] each
 PAGE_ROWS = 16           # rows per page of a paged cache
+Q4_BLOCK_BYTES = 576     # 4-bit pages: bytes per (page, kv head): 16 rows x 64 codes, 32 fp16 scales
 Q8_HEAD_BYTES = 68       # Q8_0 cache: bytes per (row, kv head): int8 q[64], fp16 d0, d1
 TMAC_OPT_SPLIT_LEN = 1
 TMAC_OPT_TARGET_GROUPS = 2
@@ -98,6 +100,14 @@ SIGNATURES = {
                                             _i]),
     "tmac_attention_decode_shared": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i,
                                           _i, _i, _i]),
+    "tmac_kv_append_axes_paged": (_i, [_vp, _vp, _i, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp, _i, _vp,
+                                       _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f]),
+    "tmac_attention_decode_weighted": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i64, _vp, _i, _i,
+                                            _i, _i, _i]),
+    "tmac_select_rows": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i]),
+    "tmac_kv_compact_paged": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i64, _i, _i,
+                                   _i]),
+    "tmac_kv_widen_pages": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i]),
     "tmac_matmul_q8_0": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp]),
     "tmac_matmul_q5_0": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp]),
     "tmac_matmul_add": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
@@ -594,6 +604,68 @@ class Context:
                                                    head_dim, max_prefix, max_tail)
         if check:
             self._check(rc, "decode_shared")
+        return rc
+
+    def kv_append_axes_paged(self, q, q_stride, q_out, k, k_stride, v, v_stride, k_pages, v_pages, n_pages, block_table,
+                             max_pages, row_starts, first_rows, positions, n_axes, pair_axis, n_seq, n_rows, n_head,
+                             n_kv_head, head_dim, max_pos, base=1e6, stream=None, check=True,
+                             kv_dtype=TMAC_KV_F32) -> int:
+        """kv_append_paged at cache rows first_rows[s] + i, turned by positions [n_axes][n_rows] of the axes that
+        pair_axis (None, or 32 values on the host: bytes or an array) deals to the pairs."""
+        if pair_axis is not None and type(pair_axis) is not bytes:
+            pair_axis = bytes(bytearray(pair_axis))
+        if pair_axis is not None and len(pair_axis) != 32:
+            raise ValueError("pair_axis: 32 pairs")
+        rc = self.lib.tmac_kv_append_axes_paged(self.handle, stream, kv_dtype, _p(q), q_stride, _p(q_out), _p(k),
+                                                k_stride, _p(v), v_stride, _p(k_pages), _p(v_pages), n_pages,
+                                                _p(block_table), max_pages, _p(row_starts), _p(first_rows),
+                                                _p(positions), n_axes, pair_axis, n_seq, n_rows, n_head, n_kv_head,
+                                                head_dim, max_pos, base)
+        if check:
+            self._check(rc, "kv_append_axes_paged")
+        return rc
+
+    def decode_weighted(self, q, k_pages, v_pages, n_pages, block_table, max_pages, lengths, weights_in, weights_out,
+                        weight_stride, out, n_seq, n_head, n_kv_head, head_dim, max_len, stream=None, check=True,
+                        kv_dtype=TMAC_KV_F32) -> int:
+        """decode_paged that adds the softmax weight of every row to weights_in (None: zeros), into weights_out (None:
+        not wanted) [n_seq][n_kv_head][weight_stride]."""
+        rc = self.lib.tmac_attention_decode_weighted(self.handle, stream, kv_dtype, _p(q), _p(k_pages), _p(v_pages),
+                                                     n_pages, _p(block_table), max_pages, _p(lengths), _p(weights_in),
+                                                     _p(weights_out), weight_stride, _p(out), n_seq, n_head, n_kv_head,
+                                                     head_dim, max_len)
+        if check:
+            self._check(rc, "decode_weighted")
+        return rc
+
+    def select_rows(self, weights, weight_stride, lengths, kept, n_seq, n_kv_head, max_len, keep, first=4, last=64,
+                    stream=None, check=True) -> int:
+        """kept [n_seq][n_kv_head][keep]: the first, the last and the heaviest rows, ascending, then -1."""
+        rc = self.lib.tmac_select_rows(self.handle, stream, _p(weights), weight_stride, _p(lengths), _p(kept), n_seq,
+                                       n_kv_head, max_len, keep, first, last)
+        if check:
+            self._check(rc, "select_rows")
+        return rc
+
+    def kv_compact_paged(self, k_pages, v_pages, n_pages, block_table, max_pages, lengths, kept, keep, to_table, to_pages,
+                         weights_in, weights_out, weight_stride, n_seq, n_kv_head, head_dim, stream=None, check=True,
+                         kv_dtype=TMAC_KV_F32) -> int:
+        """Rows kept[s][h][j] of k, v and the weights to row j of the pages to_table[s]."""
+        rc = self.lib.tmac_kv_compact_paged(self.handle, stream, kv_dtype, _p(k_pages), _p(v_pages), n_pages,
+                                            _p(block_table), max_pages, _p(lengths), _p(kept), keep, _p(to_table),
+                                            to_pages, _p(weights_in), _p(weights_out), weight_stride, n_seq, n_kv_head,
+                                            head_dim)
+        if check:
+            self._check(rc, "kv_compact_paged")
+        return rc
+
+    def kv_widen_pages(self, k_pages, v_pages, k_out, v_out, n_pages, n_kv_head, head_dim, stream=None, check=True,
+                       kv_dtype=TMAC_KV_F32) -> int:
+        """Pool pages as fp32 rows [n_pages][16][n_kv_head][64]."""
+        rc = self.lib.tmac_kv_widen_pages(self.handle, stream, kv_dtype, _p(k_pages), _p(v_pages), _p(k_out), _p(v_out),
+                                          n_pages, n_kv_head, head_dim)
+        if check:
+            self._check(rc, "kv_widen_pages")
         return rc
 
     def prefill(self, q, k, v, out, n_seq, n_q, prefix_len, seq_stride, n_head, n_kv_head, head_dim,
