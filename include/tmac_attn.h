@@ -466,8 +466,8 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
  * weights_out (null: not wanted) [n_seq][n_kv_head][weight_stride]: for r < lengths[s], weights_in of row r
  * (null: 0) plus the softmax weights that the kv head's query heads gave row r, summed; other entries are
  * left as they were, those of sequences that are too long among them.  weights_in may be weights_out;
- * another overlap is refused.  weight_stride >= max_len.  At most 65,535 sequences times kv heads with
- * weights.  The scores wait in the context's workspace, 4 bytes a row and query head of max_len.
+ * another overlap is refused.  weight_stride >= max_len.  The scores wait in the context's workspace, 4
+ * bytes a row and query head of max_len.
  *
  * Rows to keep: kept [n_seq][n_kv_head][keep]: the sequence's first `first` and last `last` rows and, up to
  * keep in all, those with the largest weights (ties: the lower row; a NaN as +infinity), ascending, then -1;

@@ -262,13 +262,6 @@ struct PagedAttnArgs {
     int prefix_groups;       // workgroups of the prefix kernel that share its units
     int prefix_blocks;       // blocks of kSharedCols (sequence, query head) columns, at most
     int tail_splits, tail_rows;  // slots behind them: runs of tail_rows own rows (of all, if it reads the prefix itself)
-    // whole sequences (rows kernel): slot i holds rows i * slot_rows ..
-    int max_len, slot_rows;
-    float* scores;           // [n_seq][n_head][score_stride] in log2 units; null: no weights are wanted
-    int64_t score_stride;    // a multiple of kPageRows
-    const float* weights_in;  // [n_seq][n_kv_head][weight_stride]; null: zeros
-    float* weights_out;
-    int64_t weight_stride;
 };
 constexpr int kPagedWaves = 4;    // waves per workgroup
 constexpr int kSharedWaves = 8;   // the same, shared prefixes
@@ -286,6 +279,38 @@ struct AppendAxesArgs {
     int n_axes;
     uint64_t pair_axis;      // 2 bits a pair: its axis
 };
+
+// Attention of every (sequence, kv head) over all of its rows, with the weights of
+// the rows if they are wanted.  Dealt: the batch's steps of kRowsStep rows in one
+// row, cut into equal runs, a wave each, of which every stretch inside a (sequence,
+// kv head) leaves a partial, number run + (sequence, kv head) of all.  Whole: a
+// workgroup a (sequence, kv head).
+struct RowsArgs {
+    const float* q;          // [n_seq][n_head][64]
+    const char* k_pages;
+    const char* v_pages;
+    const int32_t* block_table;
+    const int32_t* lengths;
+    float* out;
+    float* part;             // partials: acc [group][64] each
+    float* ml;               // and their (m, l) [group]; whole: of every (sequence, kv head), if weights are wanted
+    int* meta;               // dealt: first partial and number of them, of every (sequence, kv head)
+    float* scores;           // [n_seq][n_head][score_stride] in log2 units; null: no weights are wanted
+    const float* weights_in;  // [n_seq][n_kv_head][weight_stride]; null: zeros
+    float* weights_out;
+    int* err;
+    int64_t score_stride;    // a multiple of kRowsStep
+    int64_t weight_stride;
+    int n_pages, max_pages, n_seq, n_head, n_kv_head;
+    int group;               // n_head / n_kv_head
+    int max_len;
+    int runs;                // waves that the steps are dealt to, at most; 0: whole
+    int merge_blocks;        // finish kernel: workgroups a (sequence, kv head) that merge; the others take its weights
+    int weight_blocks;       // the same, weights: 1,024 rows each
+    float qscale;
+};
+constexpr int kRowsStep = 32;
+constexpr int kRowsSeqs = 256;  // sequences whose steps can be dealt, at most
 
 // The rows to keep of every (sequence, kv head): all up to keep, else the first and
 // last ones and those of the largest weights.

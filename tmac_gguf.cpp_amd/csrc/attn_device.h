@@ -178,12 +178,15 @@ struct PageFmt {
     __device__ static size_t page(int kv) { return kPageRows * row(kv); }
     __device__ static size_t head(int h) { return (size_t)h * CacheFmt<T>::kHeadBytes; }
 };
+struct q4_pair_t {};  // the same pages, for at most 8 query heads a kv head (Own<q4_pair_t>)
 template <>
 struct PageFmt<q4_t> {
     __device__ static size_t row(int) { return 0; }
     __device__ static size_t page(int kv) { return (size_t)kv * kQ4Block; }
     __device__ static size_t head(int h) { return (size_t)h * kQ4Block; }
 };
+template <>
+struct PageFmt<q4_pair_t> : PageFmt<q4_t> {};
 
 // This lane's 8 dims of a cache head row as loaded (raw words): fp32 8
 // floats, 16-bit 4 words, Q8_0 the two 4-byte runs plus the scale word.

@@ -201,20 +201,86 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
 // n the fp16 pair 1024 + n (codes in the high half of a byte: 1024 + 16 n), a
 // subtraction and a product with the scale (a sixteenth of it) the pair of
 // values, all exact.
-template <>
-struct Own<q4_t> {
-    using S = Mfma16;
-    using State = Cols<_Float16, S>;
-    using RawQuery = RawQ<_Float16, S>;
-    static constexpr int kTiles = 2;
+struct Codes {
+    using M = MMath<_Float16>;
     struct Tile {
         u32x2 k, v;
-        unsigned kd;  // scale of row lane % 16, dims 16 (lane / 16) ..
+        unsigned kd;  // scales of rows lane % 16 & ~1, | 1, dims 16 (lane / 16) .. (16 bits alone are widened where
+                      // the loop waits for them)
         u32x4 vd;     // scales of rows 4 (lane / 16) .. of dims 0 .. 31, then 32 .. 63
     };
-    struct Lds {};
-    // Dims 16 g + 8 m + 0..7: the operand of product m.
-    __device__ static void query(RawQuery& q, const float* p, int lane) {
+    __device__ static void fetch(Tile& t, const char* kp, const char* vp, int lane) {
+        // Through descriptors of one block each: offsets of 32 bits beside a scalar base.
+        auto block = [](const char* p) {
+            return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, kQ4Block, 0x00020000);
+        };
+        const auto kb = block(kp), vb = block(vp);
+        t.k = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(kb, 8 * lane, 0, 0));
+        t.v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vb, 8 * lane, 0, 0));
+        t.kd = __builtin_amdgcn_raw_buffer_load_b32(kb, 32 * (lane >> 5) + 4 * ((lane & 15) >> 1), 512, 0);
+        t.vd = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vb, 16 * (lane >> 4), 512, 0));
+    }
+    // Weights come up to 2^15, so that their low parts stay in fp16's normal range without a product of their own.
+    static constexpr int kGain = 7;
+    static constexpr _Float16 kSixteenth = (_Float16)0.0625f;
+    // Masks in scalar registers and the ones in a vector register make mask and or one instruction (as plain constants
+    // two, 32 more a step); minus one makes x - (float)half one mixed fma (as a constant a conversion and a difference).
+    unsigned low_mask = 0x000F000Fu, high_mask = 0x00F000F0u, one = 0x64006400u;
+    float minus = -1.f;
+    __device__ Codes() { asm("" : "+s"(low_mask), "+s"(high_mask), "+v"(one), "+s"(minus)); }
+    __device__ f16x2 low(unsigned w) const {
+        const f16x2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
+        return __builtin_bit_cast(f16x2, (w & low_mask) | one) - bias;
+    }
+    __device__ f16x2 high(unsigned w) const {
+        const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+        return __builtin_bit_cast(f16x2, (w & high_mask) | one) - bias;
+    }
+    // The K operand of depth block m: dims 16 g + 8 m + 0..7 of row lane % 16.
+    __device__ f16x2 key_scale(const Tile& t, int lane) const {
+        const _Float16 d = __builtin_bit_cast(_Float16, (unsigned short)(t.kd >> (16 * (lane & 1))));
+        return f16x2{d, d};
+    }
+    __device__ M::v8 key(const Tile& t, int m, f16x2 d0) const {
+        const f16x2 d1 = d0 * f16x2{kSixteenth, kSixteenth};
+        const unsigned x = t.k[m], y = x >> 8;
+        const f16x2 e[4] = {low(x) * d0, high(x) * d1, low(y) * d0, high(y) * d1};
+        return __builtin_bit_cast(M::v8, e);
+    }
+    // The V operands of dims 32 p + i, 32 p + 16 + i: rows 4 g + 0..3 of both pages.
+    __device__ void values(M::v8 (&x)[2], const Tile (&t)[2], const u32x4 (&vd)[2], int p) const {
+        f16x2 e[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned w = t[u].v[p], y = w >> 8;
+            // (a copy first: the bit cast of a vector's element reads the vector's first one)
+            const unsigned a0 = vd[u][2 * p], b0 = vd[u][2 * p + 1];
+            const f16x2 a = __builtin_bit_cast(f16x2, a0), b = __builtin_bit_cast(f16x2, b0);
+            const f16x2 s = {kSixteenth, kSixteenth};
+            e[0][2 * u] = low(w) * a;
+            e[0][2 * u + 1] = low(y) * b;
+            e[1][2 * u] = high(w) * (a * s);
+            e[1][2 * u + 1] = high(y) * (b * s);
+        }
+        x[0] = __builtin_bit_cast(M::v8, e[0]);
+        x[1] = __builtin_bit_cast(M::v8, e[1]);
+    }
+    // Two weights as their two parts.
+    __device__ void parts(float x, float y, unsigned& top, unsigned& rest) const {
+        top = M::pack2(x, y);
+        asm("" : "+v"(top));  // (one conversion of the pair, not one more of each)
+        const f16x2 t = __builtin_bit_cast(f16x2, top);
+        rest = M::pack2(__builtin_fmaf((float)t[0], minus, x), __builtin_fmaf((float)t[1], minus, y));
+    }
+    // Scales of V with those of the rows outside lo .. hi - 1 as zeros (a row outside may hold any).
+    __device__ static u32x4 rows_in(u32x4 vd, int lo, int hi, int g) {
+        auto in = [&](int r) { return 4 * g + r >= lo && 4 * g + r < hi; };
+        const unsigned m0 = (in(0) ? 0xFFFFu : 0u) | (in(1) ? 0xFFFF0000u : 0u);
+        const unsigned m1 = (in(2) ? 0xFFFFu : 0u) | (in(3) ? 0xFFFF0000u : 0u);
+        return u32x4{vd[0] & m0, vd[1] & m1, vd[2] & m0, vd[3] & m1};
+    }
+    // Dims 16 g + 8 m + 0..7 of a query.
+    __device__ static void query(RawQ<_Float16, Mfma16>& q, const float* p, int lane) {
         const int g = lane >> 4;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -224,165 +290,482 @@ struct Own<q4_t> {
                 if (p) q.x[m][i] = *reinterpret_cast<const f32x4*>(p + 16 * g + 8 * m + 4 * i);
             }
     }
+};
+
+// Up to 16 query heads a kv head: a column each, the parts as products of their own, 16 a step.
+template <>
+struct Own<q4_t> {
+    using S = Mfma16;
+    using State = Cols<_Float16, S>;
+    using RawQuery = RawQ<_Float16, S>;
+    using Tile = Codes::Tile;
+    static constexpr int kTiles = 2;
+    struct Lds {};
+    __device__ static int column(int lane) { return lane & 15; }
+    __device__ static void query(RawQuery& q, const float* p, int lane) { Codes::query(q, p, lane); }
     __device__ static void init(State& st, const RawQuery& q, float scale) { cols_init<_Float16, S>(st, q, scale); }
-    __device__ static void fetch(Tile& t, const char* kp, const char* vp, size_t, int lane) {
-        const int i = lane & 15, g = lane >> 4;
-        t.k = *reinterpret_cast<const u32x2*>(kp + 8 * lane);
-        t.v = *reinterpret_cast<const u32x2*>(vp + 8 * lane);
-        t.kd = *reinterpret_cast<const uint16_t*>(kp + 512 + 32 * (g >> 1) + 2 * i);
-        t.vd = *reinterpret_cast<const u32x4*>(vp + 512 + 16 * g);
-    }
-    __device__ static f16x2 low(unsigned w) {
-        const f16x2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
-        return __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) - bias;
-    }
-    __device__ static f16x2 high(unsigned w) {
-        const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-        return __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u) - bias;
-    }
-    static constexpr _Float16 kSixteenth = (_Float16)0.0625f;
+    __device__ static void fetch(Tile& t, const char* kp, const char* vp, size_t, int lane) { Codes::fetch(t, kp, vp, lane); }
     // Keys lo[u] .. hi[u] - 1 of page u take part.
     template <typename Score>
     __device__ static void attend(State& st, const Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles],
                                   Lds&, int lane, Score score) {
         using M = MMath<_Float16>;
+        const Codes k;
         const int g = lane >> 4;
-        const bool full = lo[0] <= 0 && lo[1] <= 0 && hi[0] >= kPageRows && hi[1] >= kPageRows;
         f32x4 w[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const _Float16 d = __builtin_bit_cast(_Float16, (unsigned short)t[u].kd);
-            const f16x2 d0 = {d, d}, d1 = d0 * f16x2{kSixteenth, kSixteenth};
-            w[u] = score_tile<_Float16, S>(st, nullptr, nullptr, g, [&](int m, int) {
-                const unsigned x = t[u].k[m], y = x >> 8;
-                const f16x2 e[4] = {low(x) * d0, high(x) * d1, low(y) * d0, high(y) * d1};
-                return __builtin_bit_cast(M::v8, e);
-            });
+            const f16x2 d = k.key_scale(t[u], lane);
+            w[u] = score_tile<_Float16, S>(st, nullptr, nullptr, g, [&](int m, int) { return k.key(t[u], m, d); });
         }
         u32x4 vd[2] = {t[0].vd, t[1].vd};
-        if (!full) {
+        if (!(lo[0] <= 0 && lo[1] <= 0 && hi[0] >= kPageRows && hi[1] >= kPageRows)) {
             asm volatile("");  // a branch, not selects
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                auto in = [&](int r) { return 4 * g + r >= lo[u] && 4 * g + r < hi[u]; };
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w[u][r] = in(r) ? w[u][r] : kNegInf;
-                // a row outside may hold any scale
-                const unsigned m0 = (in(0) ? 0xFFFFu : 0u) | (in(1) ? 0xFFFF0000u : 0u);
-                const unsigned m1 = (in(2) ? 0xFFFFu : 0u) | (in(3) ? 0xFFFF0000u : 0u);
-                vd[u] = u32x4{vd[u][0] & m0, vd[u][1] & m1, vd[u][2] & m0, vd[u][3] & m1};
+                for (int r = 0; r < 4; ++r) w[u][r] = 4 * g + r >= lo[u] && 4 * g + r < hi[u] ? w[u][r] : kNegInf;
+                vd[u] = Codes::rows_in(vd[u], lo[u], hi[u], g);
             }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) score(u, w[u] + st.base);
-        softmax_step<S>(st.m, st.l, st.base, st.o, w);
-        M::v8 px[2];
-        {
-            u32x4 p[2];
+        softmax_step<S, Codes::kGain>(st.m, st.l, st.base, st.o, w);
+        u32x4 p[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    unsigned z[3] = {0, 0, 0};
-                    split<M, 2>(w[u][2 * r] * M::kPScale, w[u][2 * r + 1] * M::kPScale, z);
-                    p[0][2 * u + r] = z[0];
-                    p[1][2 * u + r] = z[1];
-                }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) px[i] = __builtin_bit_cast(M::v8, p[i]);
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {  // dims 32 p + i, then 32 p + 16 + i
-            f16x2 e[2][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const unsigned x = t[u].v[p], y = x >> 8;
-                // (a copy first: the bit cast of a vector's element reads the vector's first one)
-                const unsigned a0 = vd[u][2 * p], b0 = vd[u][2 * p + 1];
-                const f16x2 a = __builtin_bit_cast(f16x2, a0), b = __builtin_bit_cast(f16x2, b0);
-                const f16x2 s = {kSixteenth, kSixteenth};
-                e[0][2 * u] = low(x) * a;
-                e[0][2 * u + 1] = low(y) * b;
-                e[1][2 * u] = high(x) * (a * s);
-                e[1][2 * u + 1] = high(y) * (b * s);
+            for (int r = 0; r < 2; ++r) {
+                unsigned top, rest;
+                k.parts(w[u][2 * r], w[u][2 * r + 1], top, rest);
+                p[0][2 * u + r] = top;
+                p[1][2 * u + r] = rest;
             }
+        const M::v8 px[2] = {__builtin_bit_cast(M::v8, p[0]), __builtin_bit_cast(M::v8, p[1])};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            M::v8 x[2];
+            k.values(x, t, vd, h);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    st.o[2 * p + b] = M::mfma32(__builtin_bit_cast(M::v8, e[b]), px[i], st.o[2 * p + b]);
+                for (int i = 0; i < 2; ++i) st.o[2 * h + b] = M::mfma32(x[b], px[i], st.o[2 * h + b]);
         }
     }
+    __device__ static void finish(State& st) { st.l *= 1.0f / (1 << Codes::kGain); }
     static constexpr int dim(int b, int g) { return 16 * b + 4 * g; }
-    __device__ static f32x4 sums(const State& st, int b) { return st.o[b] * (1.0f / MMath<_Float16>::kPScale); }
+    __device__ static f32x4 sums(const State& st, int b) { return st.o[b] * (1.0f / (1 << Codes::kGain)); }
 };
 
+// Up to 8 query heads a kv head: column c < 8 holds the first part of head c, column
+// c + 8 the second, of q and of the weights, so that a product takes both (8 a step
+// instead of 16, which cost the SIMD 16 cycles each beside the other instructions, not
+// under them).  A score is the sum of two columns; lane c goes on with page 0 and
+// lane c + 8 with page 1 of the step, half the exponentials each.
+template <>
+struct Own<q4_pair_t> {
+    using S = Mfma16;
+    using M = MMath<_Float16>;
+    using RawQuery = RawQ<_Float16, S>;
+    using Tile = Codes::Tile;
+    static constexpr int kTiles = 2;
+    struct State {
+        M::v8 q[2];
+        f32x4 o[4];
+        float unscale, m, l, base;
+    };
+    struct Lds {};
+    __device__ static int column(int lane) { return lane & 7; }
+    __device__ static float across(float x) { return dpp<0x128>(x); }  // of lane ^ 8
+    __device__ static unsigned across(unsigned x) { return dpp_u<0x128>(x); }
+    __device__ static void query(RawQuery& q, const float* p, int lane) { Codes::query(q, p, lane); }
+    __device__ static void init(State& st, const RawQuery& q, float scale) {
+        Cols<_Float16, S> c;
+        cols_init<_Float16, S>(c, q, scale);
+        const bool first = !(threadIdx.x & 8);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const u32x4 a = __builtin_bit_cast(u32x4, c.q[m][0]), b = __builtin_bit_cast(u32x4, c.q[m][1]);
+            u32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = first ? a[i] : b[i];
+            st.q[m] = __builtin_bit_cast(M::v8, x);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) st.o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        st.unscale = c.unscale;
+        st.m = kNoMax;
+        st.l = st.base = 0.f;
+    }
+    __device__ static void fetch(Tile& t, const char* kp, const char* vp, size_t, int lane) { Codes::fetch(t, kp, vp, lane); }
+    template <typename Score>
+    __device__ static void attend(State& st, const Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles],
+                                  Lds&, int lane, Score score) {
+        const Codes k;
+        const int g = lane >> 4;
+        const bool first = !(lane & 8);
+        f32x4 acc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const f16x2 d = k.key_scale(t[u], lane);
+            acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int m = 0; m < 2; ++m) acc[u] = M::mfma32(k.key(t[u], m, d), st.q[m], acc[u]);
+        }
+        f32x4 w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float a = acc[0][r] + across(acc[0][r]), b = acc[1][r] + across(acc[1][r]);
+            w[r] = __builtin_fmaf(first ? a : b, st.unscale, -st.base);
+        }
+        u32x4 vd[2] = {t[0].vd, t[1].vd};
+        if (!(lo[0] <= 0 && lo[1] <= 0 && hi[0] >= kPageRows && hi[1] >= kPageRows)) {
+            asm volatile("");  // a branch, not selects
+            const int from = first ? lo[0] : lo[1], to = first ? hi[0] : hi[1];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[r] = 4 * g + r >= from && 4 * g + r < to ? w[r] : kNegInf;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) vd[u] = Codes::rows_in(vd[u], lo[u], hi[u], g);
+        }
+        score(first ? 0 : 1, w + st.base);
+        // as softmax_step, a column's maximum over its lanes of both pages
+        const int over = max(max((int)__float_as_uint(w[0]), (int)__float_as_uint(w[1])),
+                             max((int)__float_as_uint(w[2]), (int)__float_as_uint(w[3])));
+        if (__any(over > (int)__float_as_uint(kTau + Codes::kGain) || st.m == kNoMax)) {
+            float top = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+            top = max4_rows(top);
+            top = fmaxf(top, across(top));
+            const float m1 = fmaxf(st.m, st.base + top);
+            const float b1 = m1 == kNoMax ? 0.f : m1 - Codes::kGain, shift = b1 - st.base;
+            const float f = fast_exp2(st.m - m1);
+            st.m = m1;
+            st.base = b1;
+            st.l *= f;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) st.o[b] *= f;
+            w -= shift;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = fast_exp2(w[r]);
+        st.l += (w[0] + w[1]) + (w[2] + w[3]);
+        unsigned p[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            unsigned top, rest;
+            k.parts(w[2 * r], w[2 * r + 1], top, rest);
+            const unsigned got = across(first ? rest : top);  // the other page's part that this column holds
+            p[r] = first ? top : got;
+            p[2 + r] = first ? got : rest;
+        }
+        const M::v8 px = __builtin_bit_cast(M::v8, u32x4{p[0], p[1], p[2], p[3]});
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            M::v8 x[2];
+            k.values(x, t, vd, h);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) st.o[2 * h + b] = M::mfma32(x[b], px, st.o[2 * h + b]);
+        }
+    }
+    // Both columns of a head get its sums.
+    __device__ static void finish(State& st) {
+        st.l = (st.l + across(st.l)) * (1.0f / (1 << Codes::kGain));
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st.o[b][r] += across(st.o[b][r]);
+    }
+    static constexpr int dim(int b, int g) { return 16 * b + 4 * g; }
+    __device__ static f32x4 sums(const State& st, int b) { return st.o[b] * (1.0f / (1 << Codes::kGain)); }
+};
+
+template <typename T>
+constexpr bool kPages4 = __is_same(T, q4_t) || __is_same(T, q4_pair_t);
+// The query head that this lane's column is of.
+template <typename T>
+__device__ __forceinline__ int column_of(int lane) {
+    if constexpr (kPages4<T>)
+        return Own<T>::column(lane);
+    else
+        return lane & 15;
+}
+
 // ---------------------------------------------------------------------------
-// Attention over whole sequences: workgroup (slot of slot_rows rows, kv head,
-// sequence).  With a.scores set it leaves every score, and the slot's (m, l)
-// also where it is the only one, for the weights.
+// Attention over whole sequences.  A sequence's length in rows, -1 where it is
+// longer than the launch covers.
+__device__ __forceinline__ int rows_of(const RowsArgs& a, int s) {
+    const int len = max(a.lengths[s], 0);
+    return len > a.max_len ? -1 : len;
+}
+
+// Rows lo .. hi - 1 (lo at a step's start) of one (sequence, kv head): this wave's
+// steps of kTiles pages, every BY-th from step `wave` on.  It looks up 64 pages at
+// a time, and holds one step while the next AHEAD are in flight.
+template <typename T, int BY, int AHEAD>
+__device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::State& st, typename Own<T>::Lds& lds, int s,
+                                            int h, int lo, int hi, int wave, int lane) {
+    using O = Own<T>;
+    constexpr int KT = O::kTiles;
+    const int G = a.group, col = column_of<T>(lane);
+    const int64_t row0 = (int64_t)s * a.n_head + h * G;
+    typename O::RawQuery raw;
+    O::query(raw, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, lane);
+    const size_t stride = PageFmt<T>::row(a.n_kv_head), page_bytes = PageFmt<T>::page(a.n_kv_head), head = PageFmt<T>::head(h);
+    const int32_t* table = a.block_table + (size_t)s * a.max_pages + (lo >> kPageShift);
+    float* scores = a.scores && col < G ? a.scores + (row0 + col) * a.score_stride + lo + 4 * (lane >> 4) : nullptr;
+    const int rows = hi - lo, n = (rows + kPageRows - 1) >> kPageShift;
+    const int steps = ((n + KT - 1) / KT - wave + BY - 1) / BY;  // this wave's
+    for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
+        const int cnt = min(64 / KT, steps - s0);
+        int page = 0;
+        const int e = ((s0 + lane / KT) * BY + wave) * KT + lane % KT;
+        if (lane < cnt * KT && e < n) {
+            page = table[e];
+            if (page < 0 || page >= a.n_pages) {
+                atomicOr(a.err, 4);
+                page = min(max(page, 0), a.n_pages - 1);
+            }
+        }
+        typename O::Tile t[AHEAD + 1][KT];
+        auto fetch = [&](typename O::Tile (&x)[KT], int step) {
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
+                const size_t at = (size_t)(unsigned)__builtin_amdgcn_readlane(page, KT * step + u) * page_bytes + head;
+                O::fetch(x[u], a.k_pages + at, a.v_pages + at, stride, lane);
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) fetch(t[d], min(d, cnt - 1));
+        if (s0 == 0) O::init(st, raw, a.qscale);
+        for (int step = 0; step < cnt; step += AHEAD + 1) {
+#pragma unroll
+            for (int d = 0; d <= AHEAD; ++d) {
+                if (step + d < cnt) {
+                    // The last steps fetch the last one again: under a condition, the wait for this step's rows would be
+                    // one for all loads, the next steps' among them.
+                    fetch(t[(d + AHEAD) % (AHEAD + 1)], min(step + d + AHEAD, cnt - 1));
+                    const int r0 = ((s0 + step + d) * BY + wave) * KT * kPageRows, left = rows - r0;
+                    int from[KT], to[KT];
+#pragma unroll
+                    for (int u = 0; u < KT; ++u) {
+                        from[u] = 0;
+                        to[u] = max(0, min(left - u * kPageRows, kPageRows));
+                    }
+                    O::attend(st, t[d], from, to, lds, lane, [&](int u, f32x4 x) {
+                        if (scores) *reinterpret_cast<f32x4*>(scores + r0 + u * kPageRows) = x;
+                    });
+                }
+            }
+        }
+    }
+    if (steps <= 0) O::init(st, raw, a.qscale);
+    if constexpr (kPages4<T>) O::finish(st);
+}
+
+// Whole: a workgroup a (sequence, kv head).
 template <typename T, int NW>
-__device__ __forceinline__ void rows_body(const PagedAttnArgs& a) {
+__device__ __forceinline__ void rows_whole_body(const RowsArgs& a) {
     __shared__ OwnLds<T, NW> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv = a.n_kv_head, G = a.group;
-    const int split = blockIdx.x % a.n_slots, sk = blockIdx.x / a.n_slots, s = sk / kv, h = sk - s * kv;
-    const int len = max(a.lengths[s], 0);
-    const bool bad = len > a.max_len;
-    const int64_t lo = (int64_t)split * a.slot_rows, hi = bad ? lo : min((int64_t)len, lo + a.slot_rows);
-    const int64_t row0 = (int64_t)s * a.n_head + h * G;
-    const int col = lane & 15;
-    typename Own<T>::RawQuery raw;
-    typename Own<T>::State st;
-    Own<T>::query(raw, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, lane);
-    Own<T>::init(st, raw, a.qscale);
-    if (lo < hi) {
-        const int j0 = (int)(lo >> kPageShift), n = (int)((hi - 1) >> kPageShift) - j0 + 1;
-        const int32_t* table = a.block_table + (size_t)s * a.max_pages;
-        float* scores = a.scores && col < G ? a.scores + (row0 + col) * a.score_stride + 4 * (lane >> 4) : nullptr;
-        attend_run<T, NW>(
-            st, a, h, n, lo, hi, lds.own[wave], wave, lane,
-            [&](int e, int& logical, int& page) {
-                logical = j0 + e;
-                page = table[logical];
-                if (page < 0 || page >= a.n_pages) {
-                    atomicOr(a.err, 4);
-                    page = min(max(page, 0), a.n_pages - 1);
-                }
-            },
-            [&](int j, f32x4 x) {
-                if (scores && j >= 0) *reinterpret_cast<f32x4*>(scores + (int64_t)j * kPageRows) = x;
-            });
+    const int sk = blockIdx.x, s = sk / a.n_kv_head, h = sk - s * a.n_kv_head, G = a.group, len = rows_of(a, s);
+    float* out = a.out + (int64_t)sk * G * kHeadDim;
+    if (len <= 0) {  // zeros, or NaN for a length that the launch does not cover
+        if (len < 0 && threadIdx.x == 0) atomicOr(a.err, 2);
+        for (int i = threadIdx.x; i < G * kHeadDim; i += 64 * NW) out[i] = len < 0 ? __builtin_nanf("") : 0.f;
+        return;
     }
+    typename Own<T>::State st;
+    rows_attend<T, NW, 1>(a, st, lds.own[wave], s, h, 0, len, wave, lane);
     merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
-        if (bad) {
-            if (split == 0 && c == 0 && d == 0) atomicOr(a.err, 2);
-            const float nan = __builtin_nanf("");
-            L = nan;
-            A = f32x4{nan, nan, nan, nan};
-        }
-        if (a.n_slots == 1) *reinterpret_cast<f32x4*>(a.out + (row0 + c) * kHeadDim + d) = finish_row(A, L);
-        if (a.n_slots > 1 || a.scores) put_partial(a, row0 + c, split, d, M, L, A);
+        *reinterpret_cast<f32x4*>(out + c * kHeadDim + d) = finish_row(A, L);
+        if (d == 0 && a.scores) *reinterpret_cast<float2*>(a.ml + 2 * ((size_t)sk * G + c)) = make_float2(M, L);
     });
 }
 
-// Weights of the rows: workgroup (1,024 rows, (sequence, kv head)).  A head's
-// maximum and sum come from the slots' partials, 16 lanes a head; then a thread
-// takes four rows and adds their weights over the heads.
-__device__ __forceinline__ void row_weights_body(const PagedAttnArgs& a) {
+// Inclusive sum over the lanes of a wave, in registers (row shifts, then each row's last lane to the next rows).
+__device__ __forceinline__ int lane_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+}
+
+#ifndef TMAC_AHEAD
+#define TMAC_AHEAD 1
+#endif
+#ifndef TMAC_WPE
+#define TMAC_WPE 3
+#endif
+// Waves a SIMD, and steps in flight: 256 sequences of up to 4,096 4-bit rows (2 kv heads, 7 heads each) in 32.3 us with 3
+// and 1, 36.0 with 4 (128 registers spill), 33.6 with 2 and 2, 33.4 with 3 and 2.
+template <typename T>
+constexpr int kRowsAhead = kPages4<T> ? TMAC_AHEAD : 1;
+template <typename T>
+constexpr int kRowsPerSimd = kPages4<T> ? TMAC_WPE : 2;
+
+// Dealt: a run of steps a wave, which leaves one partial for every (sequence, kv
+// head) that it touches and waits for no other wave.  (A run a workgroup, merged
+// over its waves in LDS, spent a third of its instructions on starts and merges.)
+// What bounds the start is the issue of the scan, which all waves of a SIMD do at
+// once: in 64 bits and over the LDS crossbar it took 1,200 instructions of a
+// wave's 3,300 (256 sequences of 2,048 to 4,096 4-bit rows, 2 kv heads).
+template <typename T>
+__device__ __forceinline__ void rows_dealt_body(const RowsArgs& a) {
+    __shared__ typename Own<T>::Lds lds[kPagedWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned kv = a.n_kv_head;
+    // Lane l of chunk c holds sequence l + 64 c.  The products below fit 32 bits (the host deals no more).
+    constexpr int C = kRowsSeqs / 64;
+    int len[C];
+    unsigned incl[C], all = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int i = lane + 64 * c;
+        len[c] = i < a.n_seq ? max(rows_of(a, i), 0) : 0;
+    }
+    auto steps_of = [](int rows) { return ((unsigned)rows + kRowsStep - 1) / kRowsStep; };
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        incl[c] = all;
+        if (64 * c >= a.n_seq) continue;
+        incl[c] += (unsigned)lane_scan((int)(steps_of(len[c]) * kv));
+        all = (unsigned)__builtin_amdgcn_readlane((int)incl[c], 63);
+    }
+    auto len_of = [&](unsigned s) {  // (from the lanes: loaded again, every segment would wait for it)
+        int x = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (s / 64 == (unsigned)c) x = __builtin_amdgcn_readlane(len[c], s % 64);
+        return x;
+    };
+    const unsigned runs = max(1u, min((unsigned)a.runs, all)), w = blockIdx.x * kPagedWaves + wave;
+    if (w >= runs) return;
+    const unsigned first = __builtin_amdgcn_readfirstlane(all * w / runs);
+    unsigned left = __builtin_amdgcn_readfirstlane(all * (w + 1) / runs) - first;
+    unsigned s = 0, before = 0;  // the sequence that holds the first step, and the steps of those before it
+#pragma unroll
+    for (int c = C - 1; c >= 0; --c) {
+        const uint64_t b = __ballot(incl[c] > first);
+        if (b) {
+            const int l = __builtin_ctzll(b);
+            s = 64 * c + l;
+            before = (unsigned)__builtin_amdgcn_readlane((int)incl[c], l) - steps_of(__builtin_amdgcn_readlane(len[c], l)) * kv;
+        }
+    }
+    unsigned at = first - before;  // step of its heads
+    while (left > 0) {
+        const int rows = len_of(s);
+        const unsigned m = steps_of(rows);  // steps per kv head
+        if (at >= m * kv) {
+            before += m * kv;
+            at = 0;
+            ++s;
+            continue;
+        }
+        const unsigned h = __builtin_amdgcn_readfirstlane(at / m), g0 = at - h * m, g1 = min(m, g0 + left), sk = s * kv + h;
+        if (g0 == 0 && lane == 0) {
+            a.meta[2 * (size_t)sk] = w + sk;
+            a.meta[2 * (size_t)sk + 1] = ((before + at + m) * runs - 1) / all - w + 1;  // up to the last step's run
+        }
+        typename Own<T>::State st;
+        rows_attend<T, 1, kRowsAhead<T>>(a, st, lds[wave], s, h, g0 * kRowsStep, min(rows, (int)(g1 * kRowsStep)), 0, lane);
+        const int c = lane & 15, g = lane >> 4;
+        const float l = sum4_rows(st.l);
+        if (c < a.group) {
+            const size_t p = (size_t)(w + sk) * a.group + c;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                *reinterpret_cast<f32x4*>(a.part + p * kHeadDim + Own<T>::dim(b, g)) = Own<T>::sums(st, b);
+            if (g == 0) *reinterpret_cast<float2*>(a.ml + 2 * p) = make_float2(st.m, l);
+        }
+        at += g1 - g0;
+        left -= g1 - g0;
+    }
+}
+
+// What follows: of every (sequence, kv head) merge_blocks workgroups merge its
+// partials, a head a wave or, where there are as many workgroups as heads, a head
+// all four; the others take the weights of 1,024 rows each: a head's maximum and sum from the partials, 16 lanes
+// a head, then four rows a thread, summed over the heads.
+template <int WPR>
+__device__ __forceinline__ void merge_parts(const RowsArgs& a, int64_t row, int c, int p0, int n, int w, int lane) {
+    constexpr int kRound = 16 * WPR;
+    const int sub = lane >> 4, G = a.group;
+    const float* acc = a.part + ((size_t)p0 * G + c) * kHeadDim + 4 * (lane & 15);
+    const float2* ml = reinterpret_cast<const float2*>(a.ml) + (size_t)p0 * G + c;
+    float M = kNoMax, L = 0.f;
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+    for (int c0 = 0; c0 < n; c0 += kRound) {
+        f32x4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = c0 + 4 * (WPR * i + w) + sub;
+            v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (e < n) v[i] = *reinterpret_cast<const f32x4*>(acc + (size_t)e * G * kHeadDim);
+        }
+        float2 x = make_float2(kNoMax, 0.f);
+        if (lane < kRound && c0 + lane < n) x = ml[(size_t)(c0 + lane) * G];
+        const float m1 = fmaxf(M, xor_max<1>(x.x));
+        const float f = fast_exp2(M - m1), y = fast_exp2(x.x - m1);
+        L = L * f + xor_sum<1>(x.y * y);
+        A *= f;
+        M = m1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A += __shfl(y, (4 * (WPR * i + w) + sub) & 63) * v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) A[i] = xor_sum<16>(A[i]);
+    if constexpr (WPR > 1) {
+        __shared__ f32x4 s_a[WPR][16];
+        if (lane < 16) s_a[w][lane] = A;
+        __syncthreads();
+        if (lane < 16) {
+            A = s_a[0][lane];
+#pragma unroll
+            for (int i = 1; i < WPR; ++i) A += s_a[i][lane];
+        }
+    }
+    if (w == 0 && lane < 16) *reinterpret_cast<f32x4*>(a.out + row * kHeadDim + 4 * lane) = finish_row(A, L);
+}
+
+__device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
     __shared__ float s_m[kMaxGroupHeads], s_r[kMaxGroupHeads];
-    const int tid = threadIdx.x, sk = blockIdx.y, s = sk / a.n_kv_head, h = sk - s * a.n_kv_head, G = a.group;
-    const int len = max(a.lengths[s], 0);
-    const int64_t row = 4 * ((int64_t)blockIdx.x * 256 + tid);
-    if ((int64_t)blockIdx.x * 1024 >= len || len > a.max_len) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.group;
+    const int per = a.merge_blocks + a.weight_blocks;
+    const int sk = blockIdx.x / per, i0 = blockIdx.x - sk * per, s = sk / a.n_kv_head, h = sk - s * a.n_kv_head;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
-    const float2* ml = reinterpret_cast<const float2*>(a.ws + (size_t)a.n_seq * a.n_head * a.n_slots * kHeadDim);
+    const int len = rows_of(a, s);
+    const bool dealt = a.runs != 0;
+    int p0 = sk, n = 1;
+    if (dealt && len > 0) {
+        p0 = a.meta[2 * (size_t)sk];
+        n = a.meta[2 * (size_t)sk + 1];
+    }
+    if (i0 < a.merge_blocks) {
+        if (len <= 0) {  // no partials: zeros, or NaN for a length that the launch does not cover
+            if (len < 0 && tid == 0) atomicOr(a.err, 2);
+            const float x = len < 0 ? __builtin_nanf("") : 0.f;
+            for (int i = i0 * 256 + tid; i < G * kHeadDim; i += 256 * a.merge_blocks) a.out[row0 * kHeadDim + i] = x;
+        } else {
+            if (a.merge_blocks == G) {
+                merge_parts<kPagedWaves>(a, row0 + i0, i0, p0, n, wave, lane);
+            } else {
+                for (int c = i0 * kPagedWaves + wave; c < G; c += kPagedWaves * a.merge_blocks)
+                    merge_parts<1>(a, row0 + c, c, p0, n, 0, lane);
+            }
+        }
+        return;
+    }
+    const int64_t block0 = (int64_t)(i0 - a.merge_blocks) * 1024, row = block0 + 4 * tid;
+    if (block0 >= len) return;
+    const float2* ml = reinterpret_cast<const float2*>(a.ml) + (size_t)p0 * G;
     const int c = tid >> 4, sub = tid & 15;
     if (c < G) {
         float m = kNoMax, l = 0.f;
-        for (int i = sub; i < a.n_slots; i += 16) {
-            const float2 x = ml[(row0 + c) * a.n_slots + i];
+        for (int i = sub; i < n; i += 16) {
+            const float2 x = ml[(size_t)i * G + c];
             const float m1 = fmaxf(m, x.x);
             l = l * fast_exp2(m - m1) + x.y * fast_exp2(x.x - m1);
             m = m1;

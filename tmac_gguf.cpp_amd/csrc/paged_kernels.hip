@@ -6,6 +6,7 @@
 // heads per kv head at run time; a kernel is built per cache element type.
 #include <hip/hip_runtime.h>
 
+#include <climits>
 #include <type_traits>
 
 #include "attn_args.h"
@@ -762,8 +763,9 @@ __device__ __forceinline__ typename S::Acc score_tile(const Cols<T, S>& c, const
 }
 
 // Scores minus base of NT tiles -> weights, online: the base is raised only
-// when a score exceeds it by more than kTau.
-template <typename S, int NB, int NT>
+// when a score exceeds it by more than kTau.  GAIN: the base lies that far below
+// the maximum, so that weights (and their sums) come 2^GAIN times as large.
+template <typename S, int GAIN = 0, int NB, int NT>
 __device__ __forceinline__ void softmax_step(float& m, float& l, float& base, typename S::Acc (&o)[NB],
                                              typename S::Acc (&st)[NT]) {
     // Whether any score is over the base by more than kTau, as integers: their order is that of the floats where it
@@ -773,14 +775,14 @@ __device__ __forceinline__ void softmax_step(float& m, float& l, float& base, ty
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < S::kAcc; ++r) over = max(over, (int)__float_as_uint(st[t][r]));
-    if (__any(over > (int)__float_as_uint(kTau) || m == kNoMax)) {
+    if (__any(over > (int)__float_as_uint(kTau + GAIN) || m == kNoMax)) {
         float top = kNegInf;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < S::kAcc; ++r) top = fmaxf(top, st[t][r]);
         const float m1 = fmaxf(m, base + S::top(top));
-        const float b1 = m1 == kNoMax ? 0.f : m1, shift = b1 - base;
+        const float b1 = m1 == kNoMax ? 0.f : GAIN ? m1 - GAIN : m1, shift = b1 - base;
         const float w = fast_exp2(m - m1);
         m = m1;
         base = b1;
@@ -867,6 +869,11 @@ __device__ __forceinline__ void values_step(Cols<T, S>& c, f32x4 w0, f32x4 w1, c
 // 64 sequences of 128 listed bf16 pages on 2 kv heads: 18.4 us, 3.7 TB/s.
 typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
+
+// What attend() does with the scores themselves, in log2 units: score(u, x) for page u of the step.
+struct NoScores {
+    __device__ __forceinline__ void operator()(int, f32x4) const {}
+};
 
 // 16-bit and Q8_0 rows: two pages a step, 32 keys.  K is read as the MFMA operand
 // it is, V through LDS (a buffer of the wave's own, no barrier), where it comes
@@ -962,8 +969,10 @@ struct Own {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) w[u][r] = 4 * g + r >= lo[u] && 4 * g + r < hi[u] ? w[u][r] : kNegInf;
         }
+        if constexpr (!__is_same(Score, NoScores)) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) score(u, w[u] + st.base);
+            for (int u = 0; u < 2; ++u) score(u, w[u] + st.base);
+        }
         softmax_step<S>(st.m, st.l, st.base, st.o, w);
         values_step<T, S>(st, w[0], w[1], &lds.v[0][0], 0, lds.vd[0], lds.vd[Q8 ? 1 : 0], lane);
     }
@@ -1040,7 +1049,7 @@ struct Own<float> {
 #pragma unroll
             for (int r = 0; r < 4; ++r) w[0][r] = in(r) ? w[0][r] : kNegInf;
         }
-        score(0, w[0] + st.base);
+        if constexpr (!__is_same(Score, NoScores)) score(0, w[0] + st.base);
         softmax_step<S>(st.m, st.l, st.base, st.o, w);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -1065,23 +1074,18 @@ union OwnLds {
     __device__ OwnLds() {}
 };
 
-// No use for the scores themselves.
-struct NoScores {
-    __device__ __forceinline__ void operator()(int, f32x4) const {}
-};
-
 // A run of pages.  look(e, logical, page) gives entry e (0 <= e < n) its page of
 // the pool (checked, in range) and its logical page index (-1: skipped); rows
 // row_lo .. row_hi - 1 of the sequence take part.  The NW waves take the
 // entries in turn, kTiles at once; a wave looks up 64 of its entries at a time,
-// one a lane.  score(logical, x): this lane's four scores of that page, log2 units.
-template <typename T, int NW, typename Look, typename Score = NoScores>
+// one a lane.
+template <typename T, int NW, typename Look>
 __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const PagedAttnArgs& a, int h, int n,
                                            int64_t row_lo, int64_t row_hi, typename Own<T>::Lds& lds, int wave,
-                                           int lane, Look look, Score score = Score()) {
+                                           int lane, Look look) {
     using O = Own<T>;
-    constexpr int KT = O::kTiles;
-    const size_t stride = PageFmt<T>::row(a.n_kv_head), page_bytes = PageFmt<T>::page(a.n_kv_head);
+    constexpr int HB = CacheFmt<T>::kHeadBytes, KT = O::kTiles;
+    const size_t stride = (size_t)a.n_kv_head * HB, page_bytes = kPageRows * stride;
     const int steps = ((n + KT - 1) / KT - wave + NW - 1) / NW;  // this wave's
     for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
         const int cnt = min(64 / KT, steps - s0);
@@ -1092,7 +1096,7 @@ __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const Pag
         auto fetch = [&](typename O::Tile (&x)[KT], int step) {
 #pragma unroll
             for (int u = 0; u < KT; ++u) {
-                const size_t at = (size_t)__builtin_amdgcn_readlane(page, KT * step + u) * page_bytes + PageFmt<T>::head(h);
+                const size_t at = (size_t)__builtin_amdgcn_readlane(page, KT * step + u) * page_bytes + (size_t)h * HB;
                 O::fetch(x[u], a.k_pages + at, a.v_pages + at, stride, lane);
             }
         };
@@ -1102,17 +1106,16 @@ __device__ __forceinline__ void attend_run(typename Own<T>::State& st, const Pag
             for (int d = 0; d < 2; ++d) {
                 if (step + d < cnt) {
                     if (step + d + 1 < cnt) fetch(t[1 - d], step + d + 1);
-                    int lo[KT], hi[KT], at[KT], any = 0;
+                    int lo[KT], hi[KT], any = 0;
 #pragma unroll
                     for (int u = 0; u < KT; ++u) {
                         const int j = __builtin_amdgcn_readlane(logical, KT * (step + d) + u);
                         const int64_t r0 = (int64_t)j * kPageRows;
-                        at[u] = j;
                         lo[u] = (int)max((int64_t)0, min(row_lo - r0, (int64_t)kPageRows));
                         hi[u] = j < 0 ? 0 : (int)max((int64_t)0, min(row_hi - r0, (int64_t)kPageRows));
                         any |= hi[u] > lo[u];
                     }
-                    if (any) O::attend(st, t[d], lo, hi, lds, lane, [&](int u, f32x4 x) { score(at[u], x); });
+                    if (any) O::attend(st, t[d], lo, hi, lds, lane, NoScores());
                 }
             }
         }
@@ -1827,21 +1830,28 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
     extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_tail_finish_wide_##NAME(PagedAttnArgs a) {    \
         tail_body<T, kSharedWaves, true>(a);                                                                           \
     }
+#define TMAC_ROWS_KERNELS(NAME, T)                                                                                    \
+    extern "C" __global__ __launch_bounds__(64 * kPagedWaves, kRowsPerSimd<T>) void tmac_rows_##NAME(                \
+        RowsArgs a) {                                                                                                 \
+        rows_dealt_body<T>(a);                                                                                        \
+    }                                                                                                                 \
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_rows_whole_##NAME(RowsArgs a) {              \
+        rows_whole_body<T, kSharedWaves>(a);                                                                          \
+    }
 #define TMAC_BUDGET_KERNELS(NAME, T)                                                                                  \
     extern "C" __global__ __launch_bounds__(256) void tmac_append_axes_##NAME(AppendAxesArgs a) {                     \
         append_axes_body<T>(a);                                                                                       \
     }                                                                                                                 \
-    extern "C" __global__ __launch_bounds__(64 * kPagedWaves) void tmac_rows_##NAME(PagedAttnArgs a) {                \
-        rows_body<T, kPagedWaves>(a);                                                                                 \
-    }                                                                                                                 \
     extern "C" __global__ __launch_bounds__(256) void tmac_compact_##NAME(CompactArgs a) { compact_body<T>(a); }      \
-    extern "C" __global__ __launch_bounds__(256) void tmac_widen_##NAME(WidenArgs a) { widen_body<T>(a); }
+    extern "C" __global__ __launch_bounds__(256) void tmac_widen_##NAME(WidenArgs a) { widen_body<T>(a); }            \
+    TMAC_ROWS_KERNELS(NAME, T)
 TMAC_BUDGET_KERNELS(f32, float)
 TMAC_BUDGET_KERNELS(bf16, __bf16)
 TMAC_BUDGET_KERNELS(f16, _Float16)
 TMAC_BUDGET_KERNELS(q8, q8_0_t)
 TMAC_BUDGET_KERNELS(q4, q4_t)
-extern "C" __global__ __launch_bounds__(256) void tmac_row_weights(PagedAttnArgs a) { row_weights_body(a); }
+TMAC_ROWS_KERNELS(q4_pair, q4_pair_t)
+extern "C" __global__ __launch_bounds__(256) void tmac_rows_finish(RowsArgs a) { rows_finish_body(a); }
 extern "C" __global__ __launch_bounds__(1024) void tmac_select_rows(SelectRowsArgs a) { select_rows_body(a); }
 
 TMAC_PAGED_KERNELS(f32, float)

@@ -57,6 +57,7 @@ using tmac::SelectArgs;
 using tmac::SelectRowsArgs;
 using tmac::WidenArgs;
 using tmac::QkvArgs;
+using tmac::RowsArgs;
 using tmac::kQkvWaves;
 using tmac::RopeArgs;
 using tmac::kHeadDim;
@@ -147,9 +148,9 @@ struct tmac_context {
     hipFunction_t k_append[4] = {}, k_bounds[4] = {}, k_selected[2][4] = {}, k_scores[2] = {}, k_select_short[2] = {};
     hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[2][4] = {};  // shared prefixes, own rows
     hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
-    // the same, long contexts in a small cache: by cache type, 4-bit pages last
-    hipFunction_t k_append_axes[5] = {}, k_rows[5] = {}, k_compact[5] = {}, k_widen[5] = {};
-    hipFunction_t k_row_weights = nullptr, k_select_rows = nullptr;
+    // the same, long contexts in a small cache: by cache type, 4-bit pages last (and of few query heads a kv head)
+    hipFunction_t k_append_axes[5] = {}, k_rows[6] = {}, k_rows_whole[6] = {}, k_compact[5] = {}, k_widen[5] = {};
+    hipFunction_t k_rows_finish = nullptr, k_select_rows = nullptr;
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
     float* ws = nullptr;
@@ -1083,7 +1084,6 @@ int tmac_init(tmac_context** out, int device) {
         }
         for (int dt = 0; dt < 5; dt++) {
             const std::pair<const char*, hipFunction_t*> by_type[] = {{"tmac_append_axes", &ctx->k_append_axes[dt]},
-                                                                      {"tmac_rows", &ctx->k_rows[dt]},
                                                                       {"tmac_compact", &ctx->k_compact[dt]},
                                                                       {"tmac_widen", &ctx->k_widen[dt]}};
             for (auto& k : by_type) {
@@ -1091,7 +1091,13 @@ int tmac_init(tmac_context** out, int device) {
                 if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
             }
         }
-        if ((e = get_function(ctx, &ctx->k_row_weights, "tmac_row_weights")) != hipSuccess ||
+        for (int i = 0; i < 6; i++)
+            for (int whole = 0; whole < 2; whole++) {
+                std::snprintf(name, sizeof(name), "tmac_rows_%s%s", whole ? "whole_" : "", i == 5 ? "q4_pair" : kTypeName[i]);
+                if ((e = get_function(ctx, whole ? &ctx->k_rows_whole[i] : &ctx->k_rows[i], name)) != hipSuccess)
+                    return bail(hip_fail(ctx, e, name));
+            }
+        if ((e = get_function(ctx, &ctx->k_rows_finish, "tmac_rows_finish")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_select_rows, "tmac_select_rows")) != hipSuccess)
             return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
         if ((e = get_function(ctx, &ctx->k_scores[0], "tmac_page_scores_h4")) != hipSuccess ||
@@ -1981,6 +1987,9 @@ int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtyp
     return launch(ctx, ctx->k_append_axes[budget_type(kv_dtype)], (unsigned)blocks, 1, 256, (hipStream_t)stream, &x);
 }
 
+constexpr int kRowsRunsPerCu = 12;   // waves that the steps of a batch are dealt to
+constexpr int kRowsWholeSteps = 32;  // steps up to which one workgroup takes a (sequence, kv head)
+constexpr int kRowsMergeWide = 16;   // partials a row from which four waves merge one
 int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                    const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                    int max_pages, const int32_t* lengths, const float* weights_in, float* weights_out,
@@ -1993,9 +2002,9 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     if (dt < 0)
         return fail(ctx, TMAC_ERR_INVALID_ARG,
                     "decode_weighted: kv_dtype must be TMAC_KV_F32, _BF16, _F16, _Q8_0 or _Q4_PAGES");
-    PagedAttnArgs a{};
+    PagedAttnArgs c{};
     if ((rc = paged_attn_args(ctx, what, TMAC_KV_F32, q, k_pages, v_pages, n_pages, block_table, max_pages, lengths, out,
-                              n_seq, n_head, n_kv_head, head_dim, &a)))
+                              n_seq, n_head, n_kv_head, head_dim, &c)))
         return rc;
     if (max_len < 1 || max_len > (int64_t)max_pages * kPageRows)
         return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: 1 <= max_len <= 16 * max_pages");
@@ -2011,36 +2020,57 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
         if (weights_in && weights_in != weights_out && ranges_meet(weights_in, bytes, weights_out, bytes))
             return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: weights_out overlaps weights_in without being it");
     }
+    RowsArgs a{};
+    a.q = q;
+    a.k_pages = c.k_pages;
+    a.v_pages = c.v_pages;
+    a.block_table = block_table;
+    a.lengths = lengths;
+    a.out = out;
+    a.err = ctx->err;
+    a.n_pages = n_pages;
+    a.max_pages = max_pages;
+    a.n_seq = n_seq;
+    a.n_head = n_head;
+    a.n_kv_head = n_kv_head;
+    a.group = c.group;
     a.max_len = max_len;
-    const int64_t pages = cdiv(max_len, kPageRows);
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({4 * ctx->n_cu / n_sk, cdiv(pages, 2 * tmac::kPagedWaves),
-                                                             (int64_t)kMaxSplits}));
-    a.slot_rows = (int)(cdiv(pages, splits) * kPageRows);
-    a.n_slots = (int)cdiv(max_len, a.slot_rows);
-    if ((rc = check_units(ctx, what, n_sk * a.n_slots, 64 * tmac::kPagedWaves))) return rc;
-    const size_t n_rows = (size_t)n_seq * n_head, part = n_rows * a.n_slots * (kHeadDim + 2);
+    a.qscale = kQScale;
+    const int64_t group = a.group, steps = cdiv(max_len, tmac::kRowsStep);  // per (sequence, kv head), at most
+    // (dealt in 32 bits: steps times runs)
+    const int64_t most = (int64_t)kRowsRunsPerCu * ctx->n_cu;
+    if (n_seq <= tmac::kRowsSeqs && steps > kRowsWholeSteps && n_sk * steps < INT_MAX / most)
+        a.runs = (int)std::min<int64_t>(most, n_sk * steps);
+    const int64_t blocks = a.runs ? cdiv(a.runs, tmac::kPagedWaves) : n_sk, parts = a.runs ? a.runs + n_sk : weights_out ? n_sk : 0;
+    const unsigned threads = 64 * (a.runs ? tmac::kPagedWaves : tmac::kSharedWaves);
+    if ((rc = check_units(ctx, what, blocks, threads))) return rc;
+    if (a.runs) a.merge_blocks = (int)(a.runs > kRowsMergeWide * n_sk ? group : cdiv(group, tmac::kPagedWaves));
     if (weights_out) {
-        if (n_sk > kMaxGridYZ)
-            return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: more than 65535 sequences times kv heads with weights");
-        a.score_stride = pages * kPageRows;
+        a.score_stride = steps * tmac::kRowsStep;
+        a.weight_blocks = (int)cdiv(max_len, 1024);
         a.weights_in = weights_in;
         a.weights_out = weights_out;
         a.weight_stride = weight_stride;
     }
+    const int64_t finish = a.merge_blocks + a.weight_blocks;
+    if (finish && (n_sk > INT_MAX / finish || check_units(ctx, what, n_sk * finish, 256)))
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: too many units of work");
     if ((rc = set_device(ctx))) return rc;
-    const size_t scores_at = (part + 3) / 4 * 4;  // the scores behind the partials, 16-byte aligned
-    const size_t floats = weights_out ? scores_at + n_rows * (size_t)a.score_stride : part;
-    if (weights_out || a.n_slots > 1) {
-        if ((rc = ensure_workspace(ctx, (hipStream_t)stream, floats))) return rc;
-        a.ws = workspace(ctx);
-        if (weights_out) a.scores = a.ws + scores_at;
+    if (finish) {
+        // partials, their (m, l), the scores (16-byte aligned), what every (sequence, kv head) left
+        const size_t part = (size_t)(a.runs ? parts : 0) * group * kHeadDim, ml = (size_t)cdiv(2 * parts * group, 4) * 4;
+        const size_t scores = weights_out ? (size_t)n_seq * n_head * (size_t)a.score_stride : 0;
+        if ((rc = ensure_workspace(ctx, (hipStream_t)stream, part + ml + scores + 2 * (size_t)n_sk))) return rc;
+        a.part = workspace(ctx);
+        a.ml = a.part + part;
+        if (weights_out) a.scores = a.ml + ml;
+        a.meta = reinterpret_cast<int*>(a.ml + ml + scores);
     }
-    if ((rc = launch(ctx, ctx->k_rows[dt], (unsigned)(n_sk * a.n_slots), 1, 64 * tmac::kPagedWaves, (hipStream_t)stream,
-                     &a)))
+    const int kernel = dt == kQ4 && group <= 8 ? kQ4 + 1 : dt;
+    if ((rc = launch(ctx, (a.runs ? ctx->k_rows : ctx->k_rows_whole)[kernel], (unsigned)blocks, 1, threads, (hipStream_t)stream, &a)) ||
+        !finish)
         return rc;
-    if (a.n_slots > 1 && (rc = launch_paged_merge(ctx, stream, ctx->k_selected_merge, &a))) return rc;
-    if (!weights_out) return TMAC_OK;
-    return launch(ctx, ctx->k_row_weights, (unsigned)cdiv(max_len, 1024), (unsigned)n_sk, 256, (hipStream_t)stream, &a);
+    return launch(ctx, ctx->k_rows_finish, (unsigned)(n_sk * finish), 1, 256, (hipStream_t)stream, &a);
 }
 
 int tmac_select_rows(tmac_context* ctx, tmac_stream stream, const float* weights, int64_t weight_stride,
