@@ -281,10 +281,8 @@ struct AppendAxesArgs {
 };
 
 // Attention of every (sequence, kv head) over all of its rows, with the weights of
-// the rows if they are wanted.  Dealt: the batch's steps of kRowsStep rows in one
-// row, cut into equal runs, a wave each, of which every stretch inside a (sequence,
-// kv head) leaves a partial, number run + (sequence, kv head) of all.  Whole: a
-// workgroup a (sequence, kv head).
+// the rows if they are wanted: a workgroup each, or as many as its share of the
+// batch's steps of kRowsStep rows makes, whose partials are merged.
 struct RowsArgs {
     const float* q;          // [n_seq][n_head][64]
     const char* k_pages;
@@ -292,9 +290,9 @@ struct RowsArgs {
     const int32_t* block_table;
     const int32_t* lengths;
     float* out;
-    float* part;             // partials: acc [group][64] each
-    float* ml;               // and their (m, l) [group]; whole: of every (sequence, kv head), if weights are wanted
-    int* meta;               // dealt: first partial and number of them, of every (sequence, kv head)
+    float* part;             // partials, by workgroup: acc [group][64] each
+    float* ml;               // and (m, l) [group] each
+    int* meta;               // first workgroup and number of them, of every (sequence, kv head); not if it is one each
     float* scores;           // [n_seq][n_head][score_stride] in log2 units; null: no weights are wanted
     const float* weights_in;  // [n_seq][n_kv_head][weight_stride]; null: zeros
     float* weights_out;
@@ -304,13 +302,14 @@ struct RowsArgs {
     int n_pages, max_pages, n_seq, n_head, n_kv_head;
     int group;               // n_head / n_kv_head
     int max_len;
-    int runs;                // waves that the steps are dealt to, at most; 0: whole
+    int workgroups;          // more than n_seq * n_kv_head; 0: one each
     int merge_blocks;        // finish kernel: workgroups a (sequence, kv head) that merge; the others take its weights
     int weight_blocks;       // the same, weights: 1,024 rows each
     float qscale;
 };
 constexpr int kRowsStep = 32;
-constexpr int kRowsSeqs = 256;  // sequences whose steps can be dealt, at most
+constexpr int kRowsShare = 8;   // steps that make another workgroup, at least: one a wave (one sequence of 4,096 4-bit rows,
+                                // 2 kv heads: 8.8 us, with 16 9.4; 32 of 2,000 11.5 and 10.1)
 
 // The rows to keep of every (sequence, kv head): all up to keep, else the first and
 // last ones and those of the largest weights.

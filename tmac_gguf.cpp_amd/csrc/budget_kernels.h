@@ -199,8 +199,8 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
 // fp16 rows (two parts of q and of the weights).  Both operands come from memory
 // in their lanes.  A word of 8 codes: a mask and an or make each pair of codes
 // n the fp16 pair 1024 + n (codes in the high half of a byte: 1024 + 16 n), a
-// subtraction and a product with the scale (a sixteenth of it) the pair of
-// values, all exact.
+// subtraction (a fma: a sixteenth, minus 72) n - 8, and a product with the scale
+// the pair of values, all exact.
 struct Codes {
     using M = MMath<_Float16>;
     struct Tile {
@@ -222,7 +222,6 @@ struct Codes {
     }
     // Weights come up to 2^15, so that their low parts stay in fp16's normal range without a product of their own.
     static constexpr int kGain = 7;
-    static constexpr _Float16 kSixteenth = (_Float16)0.0625f;
     // Masks in scalar registers and the ones in a vector register make mask and or one instruction (as plain constants
     // two, 32 more a step); minus one makes x - (float)half one mixed fma (as a constant a conversion and a difference).
     unsigned low_mask = 0x000F000Fu, high_mask = 0x00F000F0u, one = 0x64006400u;
@@ -233,8 +232,8 @@ struct Codes {
         return __builtin_bit_cast(f16x2, (w & low_mask) | one) - bias;
     }
     __device__ f16x2 high(unsigned w) const {
-        const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-        return __builtin_bit_cast(f16x2, (w & high_mask) | one) - bias;
+        const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, bias = {(_Float16)-72.0f, (_Float16)-72.0f};
+        return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & high_mask) | one), sixteenth, bias);
     }
     // The K operand of depth block m: dims 16 g + 8 m + 0..7 of row lane % 16.
     __device__ f16x2 key_scale(const Tile& t, int lane) const {
@@ -242,25 +241,23 @@ struct Codes {
         return f16x2{d, d};
     }
     __device__ M::v8 key(const Tile& t, int m, f16x2 d0) const {
-        const f16x2 d1 = d0 * f16x2{kSixteenth, kSixteenth};
         const unsigned x = t.k[m], y = x >> 8;
-        const f16x2 e[4] = {low(x) * d0, high(x) * d1, low(y) * d0, high(y) * d1};
+        const f16x2 e[4] = {low(x) * d0, high(x) * d0, low(y) * d0, high(y) * d0};
         return __builtin_bit_cast(M::v8, e);
     }
     // The V operands of dims 32 p + i, 32 p + 16 + i: rows 4 g + 0..3 of both pages.
-    __device__ void values(M::v8 (&x)[2], const Tile (&t)[2], const u32x4 (&vd)[2], int p) const {
+    __device__ void values(M::v8 (&x)[2], const Tile (&t)[2], int p) const {
         f16x2 e[2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const unsigned w = t[u].v[p], y = w >> 8;
             // (a copy first: the bit cast of a vector's element reads the vector's first one)
-            const unsigned a0 = vd[u][2 * p], b0 = vd[u][2 * p + 1];
+            const unsigned a0 = t[u].vd[2 * p], b0 = t[u].vd[2 * p + 1];
             const f16x2 a = __builtin_bit_cast(f16x2, a0), b = __builtin_bit_cast(f16x2, b0);
-            const f16x2 s = {kSixteenth, kSixteenth};
             e[0][2 * u] = low(w) * a;
             e[0][2 * u + 1] = low(y) * b;
-            e[1][2 * u] = high(w) * (a * s);
-            e[1][2 * u + 1] = high(y) * (b * s);
+            e[1][2 * u] = high(w) * a;
+            e[1][2 * u + 1] = high(y) * b;
         }
         x[0] = __builtin_bit_cast(M::v8, e[0]);
         x[1] = __builtin_bit_cast(M::v8, e[1]);
@@ -307,8 +304,8 @@ struct Own<q4_t> {
     __device__ static void fetch(Tile& t, const char* kp, const char* vp, size_t, int lane) { Codes::fetch(t, kp, vp, lane); }
     // Keys lo[u] .. hi[u] - 1 of page u take part.
     template <typename Score>
-    __device__ static void attend(State& st, const Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles],
-                                  Lds&, int lane, Score score) {
+    __device__ static void attend(State& st, Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles], Lds&,
+                                  int lane, Score score) {
         using M = MMath<_Float16>;
         const Codes k;
         const int g = lane >> 4;
@@ -318,14 +315,13 @@ struct Own<q4_t> {
             const f16x2 d = k.key_scale(t[u], lane);
             w[u] = score_tile<_Float16, S>(st, nullptr, nullptr, g, [&](int m, int) { return k.key(t[u], m, d); });
         }
-        u32x4 vd[2] = {t[0].vd, t[1].vd};
         if (!(lo[0] <= 0 && lo[1] <= 0 && hi[0] >= kPageRows && hi[1] >= kPageRows)) {
             asm volatile("");  // a branch, not selects
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) w[u][r] = 4 * g + r >= lo[u] && 4 * g + r < hi[u] ? w[u][r] : kNegInf;
-                vd[u] = Codes::rows_in(vd[u], lo[u], hi[u], g);
+                t[u].vd = Codes::rows_in(t[u].vd, lo[u], hi[u], g);
             }
         }
 #pragma unroll
@@ -345,7 +341,7 @@ struct Own<q4_t> {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             M::v8 x[2];
-            k.values(x, t, vd, h);
+            k.values(x, t, h);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -399,8 +395,8 @@ struct Own<q4_pair_t> {
     }
     __device__ static void fetch(Tile& t, const char* kp, const char* vp, size_t, int lane) { Codes::fetch(t, kp, vp, lane); }
     template <typename Score>
-    __device__ static void attend(State& st, const Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles],
-                                  Lds&, int lane, Score score) {
+    __device__ static void attend(State& st, Tile (&t)[kTiles], const int (&lo)[kTiles], const int (&hi)[kTiles], Lds&,
+                                  int lane, Score score) {
         const Codes k;
         const int g = lane >> 4;
         const bool first = !(lane & 8);
@@ -418,14 +414,13 @@ struct Own<q4_pair_t> {
             const float a = acc[0][r] + across(acc[0][r]), b = acc[1][r] + across(acc[1][r]);
             w[r] = __builtin_fmaf(first ? a : b, st.unscale, -st.base);
         }
-        u32x4 vd[2] = {t[0].vd, t[1].vd};
         if (!(lo[0] <= 0 && lo[1] <= 0 && hi[0] >= kPageRows && hi[1] >= kPageRows)) {
             asm volatile("");  // a branch, not selects
             const int from = first ? lo[0] : lo[1], to = first ? hi[0] : hi[1];
 #pragma unroll
             for (int r = 0; r < 4; ++r) w[r] = 4 * g + r >= from && 4 * g + r < to ? w[r] : kNegInf;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) vd[u] = Codes::rows_in(vd[u], lo[u], hi[u], g);
+            for (int u = 0; u < 2; ++u) t[u].vd = Codes::rows_in(t[u].vd, lo[u], hi[u], g);
         }
         score(first ? 0 : 1, w + st.base);
         // as softmax_step, a column's maximum over its lanes of both pages
@@ -461,7 +456,7 @@ struct Own<q4_pair_t> {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             M::v8 x[2];
-            k.values(x, t, vd, h);
+            k.values(x, t, h);
 #pragma unroll
             for (int b = 0; b < 2; ++b) st.o[2 * h + b] = M::mfma32(x[b], px, st.o[2 * h + b]);
         }
@@ -561,133 +556,132 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
     if constexpr (kPages4<T>) O::finish(st);
 }
 
-// Whole: a workgroup a (sequence, kv head).
-template <typename T, int NW>
-__device__ __forceinline__ void rows_whole_body(const RowsArgs& a) {
-    __shared__ OwnLds<T, NW> lds;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sk = blockIdx.x, s = sk / a.n_kv_head, h = sk - s * a.n_kv_head, G = a.group, len = rows_of(a, s);
-    float* out = a.out + (int64_t)sk * G * kHeadDim;
-    if (len <= 0) {  // zeros, or NaN for a length that the launch does not cover
-        if (len < 0 && threadIdx.x == 0) atomicOr(a.err, 2);
-        for (int i = threadIdx.x; i < G * kHeadDim; i += 64 * NW) out[i] = len < 0 ? __builtin_nanf("") : 0.f;
-        return;
-    }
-    typename Own<T>::State st;
-    rows_attend<T, NW, 1>(a, st, lds.own[wave], s, h, 0, len, wave, lane);
-    merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
-        if (c >= G) return;
-        *reinterpret_cast<f32x4*>(out + c * kHeadDim + d) = finish_row(A, L);
-        if (d == 0 && a.scores) *reinterpret_cast<float2*>(a.ml + 2 * ((size_t)sk * G + c)) = make_float2(M, L);
-    });
-}
-
 // Inclusive sum over the lanes of a wave, in registers (row shifts, then each row's last lane to the next rows).
-__device__ __forceinline__ int lane_scan(int x) {
+__device__ __forceinline__ unsigned lane_scan(unsigned y) {
+    int x = (int)y;
     x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
     x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
     x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
     x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
-    return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return (unsigned)(x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));
 }
 
-#ifndef TMAC_AHEAD
-#define TMAC_AHEAD 1
-#endif
-#ifndef TMAC_WPE
-#define TMAC_WPE 3
-#endif
-// Waves a SIMD, and steps in flight: 256 sequences of up to 4,096 4-bit rows (2 kv heads, 7 heads each) in 32.3 us with 3
-// and 1, 36.0 with 4 (128 registers spill), 33.6 with 2 and 2, 33.4 with 3 and 2.
-template <typename T>
-constexpr int kRowsAhead = kPages4<T> ? TMAC_AHEAD : 1;
-template <typename T>
-constexpr int kRowsPerSimd = kPages4<T> ? TMAC_WPE : 2;
+// A workgroup's stretch: part `part` of `parts` of one (sequence, kv head).
+struct Stretch {
+    int s, h, len;  // len: rows_of
+    unsigned part, parts;
+};
 
-// Dealt: a run of steps a wave, which leaves one partial for every (sequence, kv
-// head) that it touches and waits for no other wave.  (A run a workgroup, merged
-// over its waves in LDS, spent a third of its instructions on starts and merges.)
-// What bounds the start is the issue of the scan, which all waves of a SIMD do at
-// once: in 64 bits and over the LDS crossbar it took 1,200 instructions of a
-// wave's 3,300 (256 sequences of 2,048 to 4,096 4-bit rows, 2 kv heads).
-template <typename T>
-__device__ __forceinline__ void rows_dealt_body(const RowsArgs& a) {
-    __shared__ typename Own<T>::Lds lds[kPagedWaves];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// The stretch of workgroup w where the lengths decide: every (sequence, kv head)
+// gets a workgroup for each `share` of its steps, the share being such that the
+// workgroups there are suffice.  64 sequences at a time, one a lane; s < 0: no work.
+// (Even runs over all steps, whatever sequence they lie in, cost a start and a merge
+// more in many workgroups: 128 sequences of 1,024 4-bit rows 17 us instead of 8.)
+__device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int lane) {
+    constexpr int C = 4;  // chunks whose lengths are loaded together
     const unsigned kv = a.n_kv_head;
-    // Lane l of chunk c holds sequence l + 64 c.  The products below fit 32 bits (the host deals no more).
-    constexpr int C = kRowsSeqs / 64;
     int len[C];
-    unsigned incl[C], all = 0;
+    auto load = [&](int s0) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int i = lane + 64 * c;
-        len[c] = i < a.n_seq ? max(rows_of(a, i), 0) : 0;
-    }
-    auto steps_of = [](int rows) { return ((unsigned)rows + kRowsStep - 1) / kRowsStep; };
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        incl[c] = all;
-        if (64 * c >= a.n_seq) continue;
-        incl[c] += (unsigned)lane_scan((int)(steps_of(len[c]) * kv));
-        all = (unsigned)__builtin_amdgcn_readlane((int)incl[c], 63);
-    }
-    auto len_of = [&](unsigned s) {  // (from the lanes: loaded again, every segment would wait for it)
-        int x = 0;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (s / 64 == (unsigned)c) x = __builtin_amdgcn_readlane(len[c], s % 64);
-        return x;
+        for (int c = 0; c < C; ++c) {
+            const int i = s0 + 64 * c + lane;
+            len[c] = i < a.n_seq ? rows_of(a, i) : 0;
+        }
     };
-    const unsigned runs = max(1u, min((unsigned)a.runs, all)), w = blockIdx.x * kPagedWaves + wave;
-    if (w >= runs) return;
-    const unsigned first = __builtin_amdgcn_readfirstlane(all * w / runs);
-    unsigned left = __builtin_amdgcn_readfirstlane(all * (w + 1) / runs) - first;
-    unsigned s = 0, before = 0;  // the sequence that holds the first step, and the steps of those before it
+    auto steps_of = [](int rows) { return ((unsigned)max(rows, 0) + kRowsStep - 1) / kRowsStep; };
+    unsigned all = 0;
+    load(0);
+    for (int s0 = 0;;) {
+        unsigned x = 0;
 #pragma unroll
-    for (int c = C - 1; c >= 0; --c) {
-        const uint64_t b = __ballot(incl[c] > first);
-        if (b) {
-            const int l = __builtin_ctzll(b);
-            s = 64 * c + l;
-            before = (unsigned)__builtin_amdgcn_readlane((int)incl[c], l) - steps_of(__builtin_amdgcn_readlane(len[c], l)) * kv;
-        }
+        for (int c = 0; c < C; ++c) x += steps_of(len[c]);
+        all += (unsigned)__builtin_amdgcn_readlane((int)lane_scan(x), 63);
+        s0 += 64 * C;
+        if (s0 >= a.n_seq) break;
+        load(s0);
     }
-    unsigned at = first - before;  // step of its heads
-    while (left > 0) {
-        const int rows = len_of(s);
-        const unsigned m = steps_of(rows);  // steps per kv head
-        if (at >= m * kv) {
-            before += m * kv;
-            at = 0;
-            ++s;
-            continue;
-        }
-        const unsigned h = __builtin_amdgcn_readfirstlane(at / m), g0 = at - h * m, g1 = min(m, g0 + left), sk = s * kv + h;
-        if (g0 == 0 && lane == 0) {
-            a.meta[2 * (size_t)sk] = w + sk;
-            a.meta[2 * (size_t)sk + 1] = ((before + at + m) * runs - 1) / all - w + 1;  // up to the last step's run
-        }
-        typename Own<T>::State st;
-        rows_attend<T, 1, kRowsAhead<T>>(a, st, lds[wave], s, h, g0 * kRowsStep, min(rows, (int)(g1 * kRowsStep)), 0, lane);
-        const int c = lane & 15, g = lane >> 4;
-        const float l = sum4_rows(st.l);
-        if (c < a.group) {
-            const size_t p = (size_t)(w + sk) * a.group + c;
+    const unsigned spare = a.workgroups - (unsigned)a.n_seq * kv;
+    const unsigned share = max((unsigned)kRowsShare, (all * kv + spare - 1) / spare);
+    if (a.n_seq > 64 * C) load(0);
+    unsigned before = 0;
+    for (int s0 = 0;;) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-                *reinterpret_cast<f32x4*>(a.part + p * kHeadDim + Own<T>::dim(b, g)) = Own<T>::sums(st, b);
-            if (g == 0) *reinterpret_cast<float2*>(a.ml + 2 * p) = make_float2(st.m, l);
+        for (int c = 0; c < C; ++c) {
+            if (s0 + 64 * c >= a.n_seq) break;
+            const int i = s0 + 64 * c + lane;
+            const unsigned parts = max(1u, (steps_of(len[c]) + share - 1) / share), n = i < a.n_seq ? parts * kv : 0;
+            const unsigned incl = before + lane_scan(n);
+            const uint64_t b = __ballot(incl > w);
+            if (b) {
+                const int l = __builtin_ctzll(b);
+                Stretch r;
+                r.s = s0 + 64 * c + l;
+                r.len = __builtin_amdgcn_readlane(len[c], l);
+                r.parts = (unsigned)__builtin_amdgcn_readlane((int)parts, l);
+                const unsigned at = w - (unsigned)__builtin_amdgcn_readlane((int)(incl - n), l);
+                r.h = (int)(unsigned)__builtin_amdgcn_readfirstlane((int)(at / r.parts));
+                r.part = at - (unsigned)r.h * r.parts;
+                return r;
+            }
+            before = (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
         }
-        at += g1 - g0;
-        left -= g1 - g0;
+        s0 += 64 * C;
+        if (s0 >= a.n_seq) return Stretch{-1, 0, 0, 0, 0};
+        load(s0);
     }
+}
+
+template <typename T, int NW>
+__device__ __forceinline__ void rows_body(const RowsArgs& a) {
+    __shared__ OwnLds<T, NW> lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = blockIdx.x, G = a.group;
+    Stretch r;
+    if (a.workgroups) {
+        r = rows_deal(a, (unsigned)w, lane);
+        if (r.s < 0) return;
+    } else {
+        r.s = w / a.n_kv_head;
+        r.h = w - r.s * a.n_kv_head;
+        r.len = rows_of(a, r.s);
+        r.part = 0;
+        r.parts = 1;
+    }
+    const int sk = r.s * a.n_kv_head + r.h;
+    float* out = a.out + (int64_t)sk * G * kHeadDim;
+    if (a.workgroups && r.part == 0 && threadIdx.x == 0) {
+        a.meta[2 * (size_t)sk] = w;
+        a.meta[2 * (size_t)sk + 1] = (int)r.parts;
+    }
+    if (r.len <= 0) {  // zeros, or NaN for a length that the launch does not cover
+        if (r.len < 0 && threadIdx.x == 0) atomicOr(a.err, 2);
+        for (int i = threadIdx.x; i < G * kHeadDim; i += 64 * NW) out[i] = r.len < 0 ? __builtin_nanf("") : 0.f;
+        return;
+    }
+    const bool whole = r.parts == 1;
+    int lo = 0, hi = r.len;
+    if (!whole) {  // (the last parts may be shorter, or empty)
+        const unsigned per = (((unsigned)r.len + kRowsStep - 1) / kRowsStep + r.parts - 1) / r.parts * kRowsStep;
+        lo = (int)min((unsigned)r.len, r.part * per);
+        hi = (int)min((unsigned)r.len, lo + per);
+    }
+    typename Own<T>::State st;
+    rows_attend<T, NW, 1>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane);
+    merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
+        if (c >= G) return;
+        const size_t p = (size_t)w * G + c;
+        if (whole)
+            *reinterpret_cast<f32x4*>(out + c * kHeadDim + d) = finish_row(A, L);
+        else
+            *reinterpret_cast<f32x4*>(a.part + p * kHeadDim + d) = A;
+        if (d == 0 && (!whole || a.scores)) *reinterpret_cast<float2*>(a.ml + 2 * p) = make_float2(M, L);
+    });
 }
 
 // What follows: of every (sequence, kv head) merge_blocks workgroups merge its
-// partials, a head a wave or, where there are as many workgroups as heads, a head
-// all four; the others take the weights of 1,024 rows each: a head's maximum and sum from the partials, 16 lanes
+// partials (if it had several workgroups), a head a wave or, where there are as many
+// workgroups as heads, a head all four; the others take the weights of 1,024 rows each: a head's maximum and sum from the partials, 16 lanes
 // a head, then four rows a thread, summed over the heads.
 template <int WPR>
 __device__ __forceinline__ void merge_parts(const RowsArgs& a, int64_t row, int c, int p0, int n, int w, int lane) {
@@ -737,24 +731,18 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
     const int sk = blockIdx.x / per, i0 = blockIdx.x - sk * per, s = sk / a.n_kv_head, h = sk - s * a.n_kv_head;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
     const int len = rows_of(a, s);
-    const bool dealt = a.runs != 0;
     int p0 = sk, n = 1;
-    if (dealt && len > 0) {
+    if (a.workgroups && len > 0) {
         p0 = a.meta[2 * (size_t)sk];
         n = a.meta[2 * (size_t)sk + 1];
     }
     if (i0 < a.merge_blocks) {
-        if (len <= 0) {  // no partials: zeros, or NaN for a length that the launch does not cover
-            if (len < 0 && tid == 0) atomicOr(a.err, 2);
-            const float x = len < 0 ? __builtin_nanf("") : 0.f;
-            for (int i = i0 * 256 + tid; i < G * kHeadDim; i += 256 * a.merge_blocks) a.out[row0 * kHeadDim + i] = x;
+        if (n == 1) return;  // the output is there
+        if (a.merge_blocks == G) {
+            merge_parts<kPagedWaves>(a, row0 + i0, i0, p0, n, wave, lane);
         } else {
-            if (a.merge_blocks == G) {
-                merge_parts<kPagedWaves>(a, row0 + i0, i0, p0, n, wave, lane);
-            } else {
-                for (int c = i0 * kPagedWaves + wave; c < G; c += kPagedWaves * a.merge_blocks)
-                    merge_parts<1>(a, row0 + c, c, p0, n, 0, lane);
-            }
+            for (int c = i0 * kPagedWaves + wave; c < G; c += kPagedWaves * a.merge_blocks)
+                merge_parts<1>(a, row0 + c, c, p0, n, 0, lane);
         }
         return;
     }

@@ -1831,12 +1831,8 @@ __device__ __forceinline__ void shared_merge_body(const PagedAttnArgs& a) {
         tail_body<T, kSharedWaves, true>(a);                                                                           \
     }
 #define TMAC_ROWS_KERNELS(NAME, T)                                                                                    \
-    extern "C" __global__ __launch_bounds__(64 * kPagedWaves, kRowsPerSimd<T>) void tmac_rows_##NAME(                \
-        RowsArgs a) {                                                                                                 \
-        rows_dealt_body<T>(a);                                                                                        \
-    }                                                                                                                 \
-    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_rows_whole_##NAME(RowsArgs a) {              \
-        rows_whole_body<T, kSharedWaves>(a);                                                                          \
+    extern "C" __global__ __launch_bounds__(64 * kSharedWaves) void tmac_rows_##NAME(RowsArgs a) {                    \
+        rows_body<T, kSharedWaves>(a);                                                                                \
     }
 #define TMAC_BUDGET_KERNELS(NAME, T)                                                                                  \
     extern "C" __global__ __launch_bounds__(256) void tmac_append_axes_##NAME(AppendAxesArgs a) {                     \

@@ -149,7 +149,7 @@ struct tmac_context {
     hipFunction_t k_prefix[4] = {}, k_tail[4] = {}, k_tail_finish[2][4] = {};  // shared prefixes, own rows
     hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // the same, long contexts in a small cache: by cache type, 4-bit pages last (and of few query heads a kv head)
-    hipFunction_t k_append_axes[5] = {}, k_rows[6] = {}, k_rows_whole[6] = {}, k_compact[5] = {}, k_widen[5] = {};
+    hipFunction_t k_append_axes[5] = {}, k_rows[6] = {}, k_compact[5] = {}, k_widen[5] = {};
     hipFunction_t k_rows_finish = nullptr, k_select_rows = nullptr;
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
@@ -1091,12 +1091,10 @@ int tmac_init(tmac_context** out, int device) {
                 if ((e = get_function(ctx, k.second, name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
             }
         }
-        for (int i = 0; i < 6; i++)
-            for (int whole = 0; whole < 2; whole++) {
-                std::snprintf(name, sizeof(name), "tmac_rows_%s%s", whole ? "whole_" : "", i == 5 ? "q4_pair" : kTypeName[i]);
-                if ((e = get_function(ctx, whole ? &ctx->k_rows_whole[i] : &ctx->k_rows[i], name)) != hipSuccess)
-                    return bail(hip_fail(ctx, e, name));
-            }
+        for (int i = 0; i < 6; i++) {
+            std::snprintf(name, sizeof(name), "tmac_rows_%s", i == 5 ? "q4_pair" : kTypeName[i]);
+            if ((e = get_function(ctx, &ctx->k_rows[i], name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
+        }
         if ((e = get_function(ctx, &ctx->k_rows_finish, "tmac_rows_finish")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_select_rows, "tmac_select_rows")) != hipSuccess)
             return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
@@ -1987,8 +1985,25 @@ int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtyp
     return launch(ctx, ctx->k_append_axes[budget_type(kv_dtype)], (unsigned)blocks, 1, 256, (hipStream_t)stream, &x);
 }
 
-constexpr int kRowsRunsPerCu = 12;   // waves that the steps of a batch are dealt to
-constexpr int kRowsWholeSteps = 32;  // steps up to which one workgroup takes a (sequence, kv head)
+// Steps of 32 rows up to which one workgroup takes a (sequence, kv head), n_sk of them in all: a launch and partials less
+// (2.2 us) against CUs that stay idle, the longer the more workgroups there are anyway.  Past 2/3 of two a CU, more only for
+// sequences of over twice the average: up to 128 steps even one such beside short ones costs less than what all others
+// would pay.  Captured calls of 14 heads on 2, lengths of half to all the rows, us, whole / by their share:
+//   4-bit  2: 1,024 rows 7.1 / 8.7, 2,048 9.2 / 8.8;  32: 1,024 7.8 / 9.2, 2,048 10.8 / 10.0;  90: 2,048 10.8 / 12.7, 3,000
+//          13.8 / 12.8, 8,192 29.5 / 18.6;  128: 3,000 14.0 / 14.4, 4,096 17.4 / 16.0;  512: 4,096 30.0 / 32.3
+//   bf16   2: 1,024 8.3 / 9.4, 2,048 11.5 / 9.4;  32: 1,024 9.5 / 10.9, 1,536 11.7 / 11.1;  90: 3,000 19.1 / 20.6, 4,096 23.4
+//          / 23.6, 8,192 41.0 / 33.6;  128: 4,096 24.4 / 27.6, 8,192 41.8 / 42.2
+//   Q8_0   2: 1,024 10.2 / 10.0, 1,536 12.2 / 10.1;  90: 2,048 19.2 / 21.5, 3,000 25.8 / 23.7;  128: 3,000 26.0 / 27.6, 4,096
+//          32.9 / 31.7
+//   fp32   2: 512 8.2 / 9.9, 1,024 11.9 / 10.3;  32: 512 9.7 / 11.9, 1,024 14.7 / 13.4;  90: 1,536 21.3 / 17.8;  128: 2,048 26.0
+//          / 27.5, 3,000 34.8 / 33.8
+static int64_t rows_whole_steps(const tmac_context* ctx, int dt, int64_t n_sk) {
+    if (3 * n_sk > 2 * ctx->n_cu) return 128;
+    const int64_t sq = n_sk * n_sk;
+    if (dt == kQ4) return 54 + sq / 300;
+    if (dt == TMAC_KV_F32) return 25 + sq / 300;
+    return dt == TMAC_KV_Q8_0 ? 32 + sq / 190 : 38 + sq / 90;
+}
 constexpr int kRowsMergeWide = 16;   // partials a row from which four waves merge one
 int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                    const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
@@ -2037,14 +2052,15 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     a.max_len = max_len;
     a.qscale = kQScale;
     const int64_t group = a.group, steps = cdiv(max_len, tmac::kRowsStep);  // per (sequence, kv head), at most
-    // (dealt in 32 bits: steps times runs)
-    const int64_t most = (int64_t)kRowsRunsPerCu * ctx->n_cu;
-    if (n_seq <= tmac::kRowsSeqs && steps > kRowsWholeSteps && n_sk * steps < INT_MAX / most)
-        a.runs = (int)std::min<int64_t>(most, n_sk * steps);
-    const int64_t blocks = a.runs ? cdiv(a.runs, tmac::kPagedWaves) : n_sk, parts = a.runs ? a.runs + n_sk : weights_out ? n_sk : 0;
-    const unsigned threads = 64 * (a.runs ? tmac::kPagedWaves : tmac::kSharedWaves);
+    // (the kernel counts the batch's steps in 32 bits)
+    if (steps > rows_whole_steps(ctx, dt, n_sk) && n_sk * steps <= INT_MAX) {
+        const int64_t most = n_sk + n_sk * cdiv(steps, tmac::kRowsShare);  // (there are no more to deal)
+        a.workgroups = (int)(3 * n_sk <= 2 * ctx->n_cu ? std::min<int64_t>(2 * ctx->n_cu, most) : n_sk + n_sk / 2 + 1);
+    }
+    const int64_t blocks = a.workgroups ? a.workgroups : n_sk, parts = a.workgroups || weights_out ? blocks : 0;
+    const unsigned threads = 64 * tmac::kSharedWaves;
     if ((rc = check_units(ctx, what, blocks, threads))) return rc;
-    if (a.runs) a.merge_blocks = (int)(a.runs > kRowsMergeWide * n_sk ? group : cdiv(group, tmac::kPagedWaves));
+    if (a.workgroups) a.merge_blocks = (int)(a.workgroups > kRowsMergeWide * n_sk ? group : cdiv(group, tmac::kPagedWaves));
     if (weights_out) {
         a.score_stride = steps * tmac::kRowsStep;
         a.weight_blocks = (int)cdiv(max_len, 1024);
@@ -2058,7 +2074,7 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     if ((rc = set_device(ctx))) return rc;
     if (finish) {
         // partials, their (m, l), the scores (16-byte aligned), what every (sequence, kv head) left
-        const size_t part = (size_t)(a.runs ? parts : 0) * group * kHeadDim, ml = (size_t)cdiv(2 * parts * group, 4) * 4;
+        const size_t part = (size_t)(a.workgroups ? parts : 0) * group * kHeadDim, ml = (size_t)cdiv(2 * parts * group, 4) * 4;
         const size_t scores = weights_out ? (size_t)n_seq * n_head * (size_t)a.score_stride : 0;
         if ((rc = ensure_workspace(ctx, (hipStream_t)stream, part + ml + scores + 2 * (size_t)n_sk))) return rc;
         a.part = workspace(ctx);
@@ -2066,10 +2082,8 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
         if (weights_out) a.scores = a.ml + ml;
         a.meta = reinterpret_cast<int*>(a.ml + ml + scores);
     }
-    const int kernel = dt == kQ4 && group <= 8 ? kQ4 + 1 : dt;
-    if ((rc = launch(ctx, (a.runs ? ctx->k_rows : ctx->k_rows_whole)[kernel], (unsigned)blocks, 1, threads, (hipStream_t)stream, &a)) ||
-        !finish)
-        return rc;
+    const bool pair = dt == kQ4 && group <= 8;
+    if ((rc = launch(ctx, ctx->k_rows[dt + pair], (unsigned)blocks, 1, threads, (hipStream_t)stream, &a)) || !finish) return rc;
     return launch(ctx, ctx->k_rows_finish, (unsigned)(n_sk * finish), 1, 256, (hipStream_t)stream, &a);
 }
 
