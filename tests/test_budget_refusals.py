@@ -117,8 +117,6 @@ BIG = 2 ** 31 - 1
     ("tmac_attention_decode_weighted", dict(weights_out=6 * P + 4)),  # over weights_in, not it
     ("tmac_attention_decode_weighted", dict(weights_out=6 * P + (5 * 640 + 639) * 4)),
     ("tmac_attention_decode_weighted", dict(n_seq=BIG)),
-    ("tmac_attention_decode_weighted", dict(n_seq=2 ** 20, max_pages=2 ** 17, max_len=2 ** 21, weight_stride=2 ** 21,
-                                            weights_in=None)),  # 2 * 2^20 lists of 2,048 blocks of rows
     ("tmac_select_rows", dict(max_len=0)),
     ("tmac_select_rows", dict(max_len=641)),
     ("tmac_select_rows", dict(keep=0, first=0, last=0)),

@@ -100,15 +100,21 @@ __device__ __forceinline__ void load_row4(float (&x)[8], const char* p, int r, i
 template <typename T>
 __device__ __forceinline__ void widen_body(const WidenArgs& a) {
     const int c = threadIdx.x & 7, r = threadIdx.x >> 3 & 15, v = threadIdx.x >> 7;
-    if (!a.pages[v]) return;
     const int64_t unit = blockIdx.x;
     const int page = (int)(unit / a.n_kv_head), h = (int)(unit - (int64_t)page * a.n_kv_head);
-    const char* p = a.pages[v] + (size_t)page * PageFmt<T>::page(a.n_kv_head) + PageFmt<T>::head(h);
+    const size_t at = (size_t)page * PageFmt<T>::page(a.n_kv_head) + PageFmt<T>::head(h);
     float x[8];
-    if constexpr (__is_same(T, q4_t))
-        load_row4(x, p, r, c, v == 0);
-    else
-        load_row<T, false>(x, p + r * PageFmt<T>::row(a.n_kv_head) + 4 * c * CacheFmt<T>::kDimBytes, c);
+    if constexpr (__is_same(T, q4_t)) {
+        __shared__ u32x4 s_block[2][kQ4Block / 16];  // (bytes one by one from memory: 7.3 us instead of 5.4 for 2 x 996 pages)
+        const int i = threadIdx.x & 127;
+        if (a.pages[v] && i < kQ4Block / 16) s_block[v][i] = *reinterpret_cast<const u32x4*>(a.pages[v] + at + 16 * i);
+        __syncthreads();
+        if (!a.pages[v]) return;
+        load_row4(x, reinterpret_cast<const char*>(s_block[v]), r, c, v == 0);
+    } else {
+        if (!a.pages[v]) return;
+        load_row<T, false>(x, a.pages[v] + at + r * PageFmt<T>::row(a.n_kv_head) + 4 * c * CacheFmt<T>::kDimBytes, c);
+    }
     store8(a.out[v] + (((size_t)page * kPageRows + r) * a.n_kv_head + h) * kHeadDim + 4 * c, x);
 }
 
@@ -122,6 +128,7 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
     __shared__ int s_seq[kAppendRows];
     __shared__ int64_t s_page[kAppendRows];  // pool page, -1: not stored
     __shared__ int s_at[kAppendRows];        // row in the page, -1: the row is skipped
+    __shared__ int s_pos[4][kAppendRows];    // position on each axis
     const int R = a.rows_per_group;
     const int t0 = blockIdx.x * R, n = min(R, a.n_rows - t0);
     const int tid = threadIdx.x;
@@ -142,8 +149,11 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
         int64_t page = -1;
         if (s >= 0 && s < a.n_seq) {  // entry n_seq: rows behind the last sequence
             bool ok = true;
-            for (int i = 0; i < x_args.n_axes; ++i)
-                ok &= (unsigned)x_args.pos[(size_t)i * a.n_rows + t0 + tid] < (unsigned)x_args.max_pos;
+            for (int i = 0; i < x_args.n_axes; ++i) {
+                const int p = x_args.pos[(size_t)i * a.n_rows + t0 + tid];
+                ok &= (unsigned)p < (unsigned)x_args.max_pos;
+                s_pos[i][tid] = p;
+            }
             const int64_t row = (int64_t)a.positions[s] + (t0 + tid - a.row_starts[s]);
             if (ok && row >= 0 && row < a.capacity) {
                 at = (int)row & (kPageRows - 1);
@@ -172,7 +182,7 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
             for (int i = 0; i < 4; ++i) {
                 const int pair = (i < 2 ? 0 : 16) + 2 * c + (i & 1);
                 const int axis = (int)(x_args.pair_axis >> (2 * pair)) & 3;
-                const float2 cs = a.rope_cs[(size_t)x_args.pos[(size_t)axis * a.n_rows + t] * (kHeadDim / 2) + pair];
+                const float2 cs = a.rope_cs[(size_t)s_pos[axis][r] * (kHeadDim / 2) + pair];
                 rotate_pair(x[2 * i], x[2 * i + 1], cs.x, cs.y);
             }
         };
@@ -632,9 +642,26 @@ __device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int 
     }
 }
 
+// The weights of four rows, summed over the heads; head g's maximum and one over
+// its sum in m and r.
+__device__ __forceinline__ void row_weights(const RowsArgs& a, int sk, int64_t row, int len, const float* m, const float* r) {
+    const int64_t row0 = (int64_t)sk * a.group;
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < a.group; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.scores + (row0 + g) * a.score_stride + row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(x[i] - m[g]) * r[g];
+    }
+    const int64_t at = (int64_t)sk * a.weight_stride + row;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (row + i < len) a.weights_out[at + i] = (a.weights_in ? a.weights_in[at + i] : 0.f) + w[i];
+}
+
 template <typename T, int NW>
 __device__ __forceinline__ void rows_body(const RowsArgs& a) {
     __shared__ OwnLds<T, NW> lds;
+    __shared__ float s_m[kMaxGroupHeads], s_r[kMaxGroupHeads];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w = blockIdx.x, G = a.group;
     Stretch r;
@@ -675,8 +702,15 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
             *reinterpret_cast<f32x4*>(out + c * kHeadDim + d) = finish_row(A, L);
         else
             *reinterpret_cast<f32x4*>(a.part + p * kHeadDim + d) = A;
-        if (d == 0 && (!whole || a.scores)) *reinterpret_cast<float2*>(a.ml + 2 * p) = make_float2(M, L);
+        if (d == 0 && !whole) *reinterpret_cast<float2*>(a.ml + 2 * p) = make_float2(M, L);
+        if (d == 0 && whole) {
+            s_m[c] = M;
+            s_r[c] = 1.0f / L;
+        }
     });
+    if (!whole || !a.scores) return;
+    __syncthreads();  // all scores and sums are there
+    for (int64_t row = 4 * (int)threadIdx.x; row < r.len; row += 4 * 64 * NW) row_weights(a, sk, row, r.len, s_m, s_r);
 }
 
 // What follows: of every (sequence, kv head) merge_blocks workgroups merge its
@@ -731,13 +765,10 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
     const int sk = blockIdx.x / per, i0 = blockIdx.x - sk * per, s = sk / a.n_kv_head, h = sk - s * a.n_kv_head;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
     const int len = rows_of(a, s);
-    int p0 = sk, n = 1;
-    if (a.workgroups && len > 0) {
-        p0 = a.meta[2 * (size_t)sk];
-        n = a.meta[2 * (size_t)sk + 1];
-    }
+    if (len <= 0) return;
+    const int p0 = a.meta[2 * (size_t)sk], n = a.meta[2 * (size_t)sk + 1];
+    if (n == 1) return;  // its workgroup did it all
     if (i0 < a.merge_blocks) {
-        if (n == 1) return;  // the output is there
         if (a.merge_blocks == G) {
             merge_parts<kPagedWaves>(a, row0 + i0, i0, p0, n, wave, lane);
         } else {
@@ -770,17 +801,7 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
         }
     }
     __syncthreads();
-    if (row >= len) return;
-    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < G; ++g) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.scores + (row0 + g) * a.score_stride + row);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(x[i] - s_m[g]) * s_r[g];
-    }
-    const int64_t at = (int64_t)sk * a.weight_stride + row;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (row + i < len) a.weights_out[at + i] = (a.weights_in ? a.weights_in[at + i] : 0.f) + w[i];
+    if (row < len) row_weights(a, sk, row, len, s_m, s_r);
 }
 
 // ---------------------------------------------------------------------------
@@ -788,98 +809,116 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
 // (the weights' bits in order, the first and last rows above all) is found
 // eleven bits at a time: a histogram in LDS of the digits of the keys that agree
 // with the bits found so far, and the digit at which its sum from the top passes
-// what is left.  Then every wave counts, and places, the rows of its own run: those
-// above the key, and the first of those equal to it.
-constexpr int kRowsWaves = 16, kRowsThreads = 64 * kRowsWaves, kRowsBins = 2048;
-constexpr int kRowsRegs = 16;  // keys a thread holds; of longer lists it reads the rest again
+// what is left; a digit all of whose keys are kept ends the search.  Then every
+// wave counts, and places, the rows of its own run: those above the key, and the
+// first of those equal to it.
+constexpr int kRowsBins = 2048;
+template <int NT, int REGS>  // threads; keys a thread holds, of longer lists it reads the rest again
 __device__ __forceinline__ void select_rows_body(const SelectRowsArgs& a) {
+    constexpr int NW = NT / 64, PER = kRowsBins / NT;
     __shared__ unsigned s_bin[kRowsBins];
-    __shared__ unsigned s_sum[kRowsWaves], s_eq[kRowsWaves];
-    __shared__ unsigned s_found[2];  // digit, keys above it
+    __shared__ unsigned s_sum[16], s_eq[16];
+    __shared__ unsigned s_found[3];  // digit, keys above it, keys of it
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sk = blockIdx.x, s = sk / a.n_kv_head;
     const int len = max(a.lengths[s], 0), n = len > a.max_len ? 0 : len;
     int32_t* out = a.kept + (size_t)sk * a.keep;
     if (len > a.max_len && tid == 0) atomicOr(a.err, 2);
     if (n <= a.keep) {
-        for (int i = tid; i < a.keep; i += kRowsThreads) out[i] = i < n ? i : -1;
+        for (int i = tid; i < a.keep; i += NT) out[i] = i < n ? i : -1;
         return;
     }
     const float* w = a.weights + sk * a.weight_stride;
-    const int rounds = (n + kRowsThreads - 1) / kRowsThreads, j0 = wave * rounds * 64 + lane;  // this lane's: j0 + 64 r
+    const int rounds = (n + NT - 1) / NT, j0 = wave * rounds * 64 + lane;  // this lane's: j0 + 64 r
     auto key_at = [&](int r) {  // 0: behind the last row (no weight has that key)
         const int64_t j = (int64_t)j0 + 64 * (int64_t)r;
         return j >= n ? 0u : j < a.first || j >= n - a.last ? 0xFFFFFFFFu : order_key(w[j]);
     };
-    unsigned k[kRowsRegs];
+    unsigned k[REGS];
 #pragma unroll
-    for (int r = 0; r < kRowsRegs; ++r) k[r] = r < rounds ? key_at(r) : 0u;
+    for (int r = 0; r < REGS; ++r) k[r] = r < rounds ? key_at(r) : 0u;
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+            if (r < rounds) f(k[r], r);
+        for (int r = REGS; r < rounds; ++r) f(key_at(r), r);
+    };
+    // what the waves before this one left in sums, and this lane's place in its wave
+    auto of_waves_before = [&](const unsigned* sums) {
+        const unsigned x = lane_scan(lane < NW ? sums[lane & 15] : 0u);
+        return wave ? (unsigned)__builtin_amdgcn_readlane((int)x, wave - 1) : 0u;
+    };
+    auto lanes_before = [](uint64_t b) {
+        return __builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)b, 0u));
+    };
     unsigned prefix = 0, mask = 0, left = (unsigned)a.keep;  // of the keys with key & mask == prefix the left largest are kept
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-        for (int i = tid; i < kRowsBins; i += kRowsThreads) s_bin[i] = 0;
-        __syncthreads();
-        auto count = [&](unsigned x) {
-            if (x && (x & mask) == prefix) atomicAdd(&s_bin[x >> shift & (unsigned)(bins - 1)], 1u);
-        };
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const unsigned digits = pass == 2 ? 1023u : 2047u;
 #pragma unroll
-        for (int r = 0; r < kRowsRegs; ++r) {
-            if (r < rounds) count(k[r]);
-        }
-        for (int r = kRowsRegs; r < rounds; ++r) count(key_at(r));
+        for (int i = 0; i < PER; ++i) s_bin[tid + i * NT] = 0;
         __syncthreads();
-        // two bins a thread, from the top
-        const int b1 = kRowsBins - 1 - 2 * tid;
-        const unsigned c1 = s_bin[b1], c0 = s_bin[b1 - 1];
-        const unsigned incl = (unsigned)wave_scan((int)(c0 + c1), lane);
+        each([&](unsigned x, int) {
+            if (x && (x & mask) == prefix) atomicAdd(&s_bin[x >> shift & digits], 1u);
+        });
+        __syncthreads();
+        // PER bins a thread, from the top
+        unsigned c[PER], sum = 0;
+        const int top = kRowsBins - 1 - PER * tid;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum += c[i] = s_bin[top - i];
+        const unsigned incl = lane_scan(sum);
         if (lane == 63) s_sum[wave] = incl;
         __syncthreads();
-        unsigned before = incl - c0 - c1;
-        for (int i = 0; i < wave; ++i) before += s_sum[i];
-        if (before < left && before + c0 + c1 >= left) {
-            const bool upper = before + c1 >= left;
-            s_found[0] = (unsigned)(upper ? b1 : b1 - 1);
-            s_found[1] = upper ? before : before + c1;
+        unsigned before = of_waves_before(s_sum) + incl - sum;
+        if (before < left && before + sum >= left) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (before < left && before + c[i] >= left) {
+                    s_found[0] = (unsigned)(top - i);
+                    s_found[1] = before;
+                    s_found[2] = c[i];
+                }
+                before += c[i];
+            }
         }
         __syncthreads();
         prefix |= s_found[0] << shift;
         left -= s_found[1];
-        mask |= (unsigned)(bins - 1) << shift;
+        mask |= digits << shift;
+        if (left == s_found[2] && prefix) {  // all of them: the keys above the one below
+            --prefix;
+            left = 0;
+            break;
+        }
     }
     // keys above prefix are kept, and the first `left` of those equal to it
     unsigned gt = 0, eq = 0;
-    auto tally = [&](unsigned x) {
+    each([&](unsigned x, int) {
         gt += __popcll(__ballot(x > prefix));
         eq += __popcll(__ballot(x == prefix));
-    };
-#pragma unroll
-    for (int r = 0; r < kRowsRegs; ++r) {
-        if (r < rounds) tally(k[r]);
-    }
-    for (int r = kRowsRegs; r < rounds; ++r) tally(key_at(r));
+    });
     if (lane == 0) {
         s_sum[wave] = gt;
         s_eq[wave] = eq;
     }
     __syncthreads();
-    gt = eq = 0;
-    for (int i = 0; i < wave; ++i) {
-        gt += s_sum[i];
-        eq += s_eq[i];
-    }
-    auto place = [&](unsigned x, int r) {
-        const uint64_t bg = __ballot(x > prefix), be = __ballot(x == prefix), below = (1ull << lane) - 1;
-        const unsigned g = gt + __popcll(bg & below), e = eq + __popcll(be & below);
-        if (x > prefix || (x == prefix && e < left)) out[g + min(e, left)] = j0 + 64 * r;
-        gt += __popcll(bg);
-        eq += __popcll(be);
-    };
-#pragma unroll
-    for (int r = 0; r < kRowsRegs; ++r) {
-        if (r < rounds) place(k[r], r);
-    }
-    for (int r = kRowsRegs; r < rounds; ++r) place(key_at(r), r);
+    gt = of_waves_before(s_sum);
+    eq = of_waves_before(s_eq);
+    int32_t* o = out + gt + min(eq, left);  // the next row's place
+    each([&](unsigned x, int r) {
+        uint64_t b = __ballot(x > prefix);
+        if (eq < left) {
+            const uint64_t be = __ballot(x == prefix);
+            if (be) {
+                b |= __ballot(x == prefix && eq + lanes_before(be) < left);
+                eq += __popcll(be);
+            }
+        }
+        if (b >> lane & 1) o[lanes_before(b)] = j0 + 64 * r;
+        o += __popcll(b);
+    });
 }
 
 // ---------------------------------------------------------------------------

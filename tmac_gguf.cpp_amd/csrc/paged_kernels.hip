@@ -1848,7 +1848,8 @@ TMAC_BUDGET_KERNELS(q8, q8_0_t)
 TMAC_BUDGET_KERNELS(q4, q4_t)
 TMAC_ROWS_KERNELS(q4_pair, q4_pair_t)
 extern "C" __global__ __launch_bounds__(256) void tmac_rows_finish(RowsArgs a) { rows_finish_body(a); }
-extern "C" __global__ __launch_bounds__(1024) void tmac_select_rows(SelectRowsArgs a) { select_rows_body(a); }
+extern "C" __global__ __launch_bounds__(256) void tmac_select_rows_256(SelectRowsArgs a) { select_rows_body<256, 16>(a); }
+extern "C" __global__ __launch_bounds__(1024) void tmac_select_rows_1024(SelectRowsArgs a) { select_rows_body<1024, 32>(a); }
 
 TMAC_PAGED_KERNELS(f32, float)
 TMAC_PAGED_KERNELS(bf16, __bf16)

@@ -150,7 +150,7 @@ struct tmac_context {
     hipFunction_t k_select[2] = {}, k_selected_merge[2] = {}, k_shared_merge[2] = {};  // merges: 1, 4 waves a row
     // the same, long contexts in a small cache: by cache type, 4-bit pages last (and of few query heads a kv head)
     hipFunction_t k_append_axes[5] = {}, k_rows[6] = {}, k_compact[5] = {}, k_widen[5] = {};
-    hipFunction_t k_rows_finish = nullptr, k_select_rows = nullptr;
+    hipFunction_t k_rows_finish = nullptr, k_select_rows[2] = {};
     // quantized GEMV of a large matrix; K-quants: [Q6_K][large matrix]
     hipFunction_t k_gemv_q8 = nullptr, k_gemv_q5 = nullptr, k_kq[2][2] = {};
     float* ws = nullptr;
@@ -1096,7 +1096,8 @@ int tmac_init(tmac_context** out, int device) {
             if ((e = get_function(ctx, &ctx->k_rows[i], name)) != hipSuccess) return bail(hip_fail(ctx, e, name));
         }
         if ((e = get_function(ctx, &ctx->k_rows_finish, "tmac_rows_finish")) != hipSuccess ||
-            (e = get_function(ctx, &ctx->k_select_rows, "tmac_select_rows")) != hipSuccess)
+            (e = get_function(ctx, &ctx->k_select_rows[0], "tmac_select_rows_256")) != hipSuccess ||
+            (e = get_function(ctx, &ctx->k_select_rows[1], "tmac_select_rows_1024")) != hipSuccess)
             return bail(hip_fail(ctx, e, "hipModuleGetFunction"));
         if ((e = get_function(ctx, &ctx->k_scores[0], "tmac_page_scores_h4")) != hipSuccess ||
             (e = get_function(ctx, &ctx->k_scores[1], "tmac_page_scores_h8")) != hipSuccess ||
@@ -2057,28 +2058,30 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
         const int64_t most = n_sk + n_sk * cdiv(steps, tmac::kRowsShare);  // (there are no more to deal)
         a.workgroups = (int)(3 * n_sk <= 2 * ctx->n_cu ? std::min<int64_t>(2 * ctx->n_cu, most) : n_sk + n_sk / 2 + 1);
     }
-    const int64_t blocks = a.workgroups ? a.workgroups : n_sk, parts = a.workgroups || weights_out ? blocks : 0;
+    const int64_t blocks = a.workgroups ? a.workgroups : n_sk;
     const unsigned threads = 64 * tmac::kSharedWaves;
     if ((rc = check_units(ctx, what, blocks, threads))) return rc;
-    if (a.workgroups) a.merge_blocks = (int)(a.workgroups > kRowsMergeWide * n_sk ? group : cdiv(group, tmac::kPagedWaves));
     if (weights_out) {
         a.score_stride = steps * tmac::kRowsStep;
-        a.weight_blocks = (int)cdiv(max_len, 1024);
         a.weights_in = weights_in;
         a.weights_out = weights_out;
         a.weight_stride = weight_stride;
+    }
+    if (a.workgroups) {
+        a.merge_blocks = (int)(a.workgroups > kRowsMergeWide * n_sk ? group : cdiv(group, tmac::kPagedWaves));
+        if (weights_out) a.weight_blocks = (int)cdiv(max_len, 1024);
     }
     const int64_t finish = a.merge_blocks + a.weight_blocks;
     if (finish && (n_sk > INT_MAX / finish || check_units(ctx, what, n_sk * finish, 256)))
         return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: too many units of work");
     if ((rc = set_device(ctx))) return rc;
-    if (finish) {
+    if (a.workgroups || weights_out) {
         // partials, their (m, l), the scores (16-byte aligned), what every (sequence, kv head) left
-        const size_t part = (size_t)(a.workgroups ? parts : 0) * group * kHeadDim, ml = (size_t)cdiv(2 * parts * group, 4) * 4;
+        const size_t parts = (size_t)a.workgroups * group, ml = (size_t)cdiv(2 * (int64_t)parts, 4) * 4;
         const size_t scores = weights_out ? (size_t)n_seq * n_head * (size_t)a.score_stride : 0;
-        if ((rc = ensure_workspace(ctx, (hipStream_t)stream, part + ml + scores + 2 * (size_t)n_sk))) return rc;
+        if ((rc = ensure_workspace(ctx, (hipStream_t)stream, parts * kHeadDim + ml + scores + 2 * (size_t)n_sk))) return rc;
         a.part = workspace(ctx);
-        a.ml = a.part + part;
+        a.ml = a.part + parts * kHeadDim;
         if (weights_out) a.scores = a.ml + ml;
         a.meta = reinterpret_cast<int*>(a.ml + ml + scores);
     }
@@ -2087,6 +2090,7 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     return launch(ctx, ctx->k_rows_finish, (unsigned)(n_sk * finish), 1, 256, (hipStream_t)stream, &a);
 }
 
+constexpr int kSelectRowsNarrow = 4096;  // rows up to which 256 threads choose
 int tmac_select_rows(tmac_context* ctx, tmac_stream stream, const float* weights, int64_t weight_stride,
                      const int32_t* lengths, int32_t* kept, int n_seq, int n_kv_head, int max_len, int keep, int first,
                      int last) {
@@ -2116,7 +2120,8 @@ int tmac_select_rows(tmac_context* ctx, tmac_stream stream, const float* weights
     a.keep = keep;
     a.first = first;
     a.last = last;
-    return launch(ctx, ctx->k_select_rows, (unsigned)n_sk, 1, 1024, (hipStream_t)stream, &a);
+    const bool wide = max_len > kSelectRowsNarrow;
+    return launch(ctx, ctx->k_select_rows[wide], (unsigned)n_sk, 1, wide ? 1024 : 256, (hipStream_t)stream, &a);
 }
 
 int tmac_kv_compact_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, void* k_pages, void* v_pages, int n_pages,
