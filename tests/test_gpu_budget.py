@@ -725,3 +725,107 @@ def test_two_streams_of_two_contexts(ctx):
             same_bits(out.numpy(), a, "out")
             same_bits(w.numpy(), b, "weights")
             c.destroy_stream(s)
+
+
+# ---- workgroups by share of the batch's steps ------------------------------------------------
+
+@pytest.mark.parametrize("n,nkv,group", [(3, 2, 7), (70, 1, 1), (60, 3, 2), (257, 1, 9), (300, 1, 2), (1030, 1, 1)])
+@pytest.mark.parametrize("dt", [F32, Q4], ids=["f32", "q4"])
+def test_weighted_uneven_batches(ctx, dt, n, nkv, group):
+    """A few long sequences among short and empty ones, more sequences than a round of the lengths holds: some have
+    many workgroups, most one, and the lengths alone decide."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 41, n)
+    for i, x in zip((0, n // 2, n - 1), (5003, 4100, 6000)):
+        lens[i] = x
+    run_weighted(ctx, dt, nkv * group, nkv, lens, 1800 + n, max_len=6016)
+    run_weighted(ctx, dt, nkv * group, nkv, lens, 1801 + n, weights=False, max_len=6016)
+    no_fault(ctx)
+
+
+@by_type
+def test_weighted_long_bound_short_rows(ctx, dt):
+    """max_len far above every length, no rows at all, one row."""
+    for lens in ([0, 0, 0], [1, 0, 5], [300, 299, 31]):
+        run_weighted(ctx, dt, 14, 2, lens, 1810, max_len=9000)
+    no_fault(ctx)
+
+
+def test_weighted_errors_of_long_batches(ctx):
+    """As test_weighted_errors where a batch's steps are dealt: too long a sequence gets NaN, the others their result."""
+    rng = np.random.default_rng(16)
+    lens = np.array([4500, 6000, 30], np.int32)
+    table, n_pages = tables(rng, lens)
+    pools = [make_pool(1820 + i, n_pages, 2, Q4, i == 0) for i in (0, 1)]
+    q = oracle.normal(1822, (3, 14, 64))
+    w, out = ctx.upload(np.full((3, 2, 5000), 7.5, np.float32)), ctx.empty((3, 14, 64))
+    ctx.decode_weighted(ctx.upload(q), ctx.upload(pools[0][0]), ctx.upload(pools[1][0]), n_pages, ctx.upload(table),
+                        table.shape[1], ctx.upload(lens), None, w, 5000, out, 3, 14, 2, 64, 5000, kv_dtype=Q4)
+    faults(ctx)
+    got, gw = out.numpy(), w.numpy()
+    assert np.isnan(got[1]).all() and (gw[1] == 7.5).all()
+    keep = [0, 2]
+    ref, rw, tol, w_tol = budget.attend64(q[keep], pools[0][1], pools[1][1], table[keep], lens[keep], 2)
+    assert (np.abs(got[keep] - ref) <= tol).all()
+    for i, s in enumerate(keep):
+        m = lens[s]
+        assert (np.abs(gw[s, :, :m] - rw[i, :, :m]) <= w_tol[i, :, :m] + 2.0 ** -23 * gw[s, :, :m]).all()
+        assert (gw[s, :, m:] == 7.5).all()
+
+
+def test_captured_long_batch_replays_with_other_lengths(ctx):
+    """The lengths on the device deal the work anew on every replay; eager calls on the same workspace between."""
+    nh, nkv, n, L = 14, 2, 5, 7000
+    rng = np.random.default_rng(52)
+    table, n_pages = tables(rng, [L] * n)
+    pools = [make_pool(1830 + i, n_pages, nkv, Q4, i == 0)[0] for i in (0, 1)]
+    s = ctx.stream()
+    dk, dv, dtab, dlen = ctx.upload(pools[0]), ctx.upload(pools[1]), ctx.upload(table), ctx.empty(n, np.int32)
+    dq, out, w = ctx.upload(oracle.normal(1832, (n, nh, 64))), ctx.empty((n, nh, 64)), ctx.empty((n, nkv, L))
+    w.copy_from(np.zeros((n, nkv, L), np.float32), s)
+
+    def step():
+        ctx.decode_weighted(dq, dk, dv, n_pages, dtab, table.shape[1], dlen, None, w, L, out, n, nh, nkv, 64, L, stream=s,
+                            kv_dtype=Q4)
+
+    batches = [np.array(x, np.int32) for x in ([7000, 1, 0, 333, 5000], [0, 0, 0, 0, 0], [64, 6999, 7000, 7000, 31], [7000] * 5)]
+    eager = []
+    for lens in batches:
+        dlen.copy_from(lens, s)
+        w.copy_from(np.zeros((n, nkv, L), np.float32), s)
+        step()
+        ctx.synchronize(s)
+        eager.append((out.numpy(), w.numpy()))
+    ctx.step_begin(s)
+    step()
+    graph = ctx.step_end(s)
+    try:
+        for i, lens in enumerate(batches * 2):
+            dlen.copy_from(lens, s)
+            w.copy_from(np.zeros((n, nkv, L), np.float32), s)
+            ctx.graph_launch(graph, s)
+            ctx.synchronize(s)
+            for a, b in zip((out.numpy(), w.numpy()), eager[i % len(batches)]):
+                same_bits(a, b, f"replay {i}")
+            run_weighted(ctx, BF16, 8, 8, [200 + 900 * i, 50], 1840 + i)
+    finally:
+        ctx.graph_destroy(graph)
+        ctx.destroy_stream(s)
+    no_fault(ctx)
+
+
+@pytest.mark.parametrize("nh,nkv", [(8, 1), (9, 1), (16, 2), (18, 2)])
+def test_weighted_4_bit_scales_of_all_sizes(ctx, nh, nkv):
+    """Rows whose scales go from 2^-14 to 2^9, values and keys: both forms of the 4-bit products (up to 8 query heads a kv
+    head, and more) hold the bounds."""
+    rng = np.random.default_rng(53)
+    lens = np.array([400, 77], np.int32)
+    table, n_pages = tables(rng, lens)
+    pools = []
+    for i in (0, 1):
+        x = oracle.normal(1850 + i, (n_pages, PR, nkv, 64))
+        x *= np.exp2(rng.uniform(-11, 1 if i == 0 else 9, (n_pages, PR, nkv, 1))).astype(np.float32)
+        st = budget.pack4(x, i == 0)
+        pools.append((st, budget.widen4(st, i == 0)))
+    run_weighted(ctx, Q4, nh, nkv, lens, 1852, pools=pools, table=table, n_pages=n_pages)
+    no_fault(ctx)
