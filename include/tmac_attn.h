@@ -476,7 +476,8 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
  *
  * Compaction: kv head h of row kept[s][h][j] becomes row j of the pages to_table[s] (to_pages of them a
  * sequence), k and v, bit for bit; the row stays where it was too.  An entry of -1 leaves its row of the
- * destination as it was; another entry outside [0, lengths[s]) does too, and sets bit 2.  A block-table
+ * destination as it was; another entry outside [0, lengths[s]) does too, and sets bit 2 (so does one at
+ * weight_stride or above, with weights).  A block-table
  * entry outside the pool is clamped (bit 2), a to_table entry outside it leaves its page out (bit 2).  The
  * destination pages are pages of the same pools that hold no row of the call's sequences, each named once;
  * once the call has run, the pages of block_table that nobody else shares are free.  weights_out (both

@@ -643,19 +643,34 @@ __device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int 
 }
 
 // The weights of four rows, summed over the heads; head g's maximum and one over
-// its sum in m and r.
+// its sum in m and r.  The scores of kWeightHeads heads are read at once.
+#ifndef WH
+#define WH 4
+#endif
+constexpr int kWeightHeads = WH;
 __device__ __forceinline__ void row_weights(const RowsArgs& a, int sk, int64_t row, int len, const float* m, const float* r) {
-    const int64_t row0 = (int64_t)sk * a.group;
-    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < a.group; ++g) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.scores + (row0 + g) * a.score_stride + row);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(x[i] - m[g]) * r[g];
-    }
+    const float* const x = a.scores + (int64_t)sk * a.group * a.score_stride + row;
     const int64_t at = (int64_t)sk * a.weight_stride + row;
+    f32x4 w = {0.f, 0.f, 0.f, 0.f}, before = {0.f, 0.f, 0.f, 0.f};
+    if (a.weights_in) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) before[i] = a.weights_in[at + min(i, (int)(len - 1 - row))];
+    }
+    for (int g0 = 0; g0 < a.group; g0 += kWeightHeads) {
+        f32x4 y[kWeightHeads];
+#pragma unroll
+        for (int g = 0; g < kWeightHeads; ++g)
+            y[g] = *reinterpret_cast<const f32x4*>(x + min(g0 + g, a.group - 1) * a.score_stride);
+#pragma unroll
+        for (int g = 0; g < kWeightHeads; ++g) {
+            if (g0 + g >= a.group) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] += fast_exp2(y[g][i] - m[g0 + g]) * r[g0 + g];
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (row + i < len) a.weights_out[at + i] = (a.weights_in ? a.weights_in[at + i] : 0.f) + w[i];
+        if (row + i < len) a.weights_out[at + i] = before[i] + w[i];
 }
 
 template <typename T, int NW>
@@ -922,86 +937,122 @@ __device__ __forceinline__ void select_rows_body(const SelectRowsArgs& a) {
 }
 
 // ---------------------------------------------------------------------------
-// Compaction.  A workgroup takes 16 kept rows of one (sequence, kv head), the
-// rows of one destination page.
+// Compaction: a copy through a list, bound by memory.  A wave takes 16 kept rows
+// of one (sequence, kv head), the rows of one destination page.  The chain list
+// -> table -> row is three loads deep, so a wave has all of its page's rows in
+// flight at once, two to eight 16-byte loads a lane, and no barrier.  Loads are
+// unconditional (a place without a row reads another's row), stores are not.
 template <typename T>
 __device__ __forceinline__ void compact_body(const CompactArgs& a) {
-    __shared__ int64_t s_src[kPageRows];  // source page of the pool * 16 + row in it, -1: no row
-    __shared__ int s_to;
-    const int tid = threadIdx.x, kv = a.n_kv_head;
-    const int64_t unit = blockIdx.x, sk = unit / a.n_grid;
-    const int jp = (int)(unit - sk * a.n_grid), s = (int)(sk / kv), h = (int)(sk - (int64_t)s * kv);
-    const int len = max(a.lengths[s], 0);
-    if (tid < kPageRows) {
-        const int j = jp * kPageRows + tid;
-        const int row = j < a.keep ? a.kept[sk * a.keep + j] : -1;
-        int64_t src = -1;
-        if (row >= 0 && row < len && row < (int64_t)a.max_pages * kPageRows) {
-            const int page = a.block_table[(size_t)s * a.max_pages + (row >> kPageShift)];
-            if (page < 0 || page >= a.n_pages) atomicOr(a.err, 4);
-            src = (int64_t)min(max(page, 0), a.n_pages - 1) * kPageRows + (row & (kPageRows - 1));
-        } else if (row != -1) {
-            atomicOr(a.err, 4);
-        }
-        const uint64_t any = __ballot(src >= 0);
-        if (tid == 0) {
-            int to = -1;
-            if (any) {
-                to = a.to_table[(size_t)s * a.to_pages + jp];
-                if (to < 0 || to >= a.n_pages) {
-                    atomicOr(a.err, 4);
-                    to = -1;
-                }
-            }
-            s_to = to;
-        }
-        s_src[tid] = src;
-        if (a.weights_out && j < a.keep)
-            a.weights_out[sk * a.weight_stride + j] = src >= 0 ? a.weights_in[sk * a.weight_stride + row] : 0.f;
-    }
-    __syncthreads();
-    if (a.weights_out && jp == a.n_grid - 1)  // what follows the last kept row
-        for (int64_t j = a.keep + tid; j < a.weight_stride; j += 256) a.weights_out[sk * a.weight_stride + j] = 0.f;
-    const int to = s_to;
-    if (to < 0) return;
-    const size_t page_bytes = PageFmt<T>::page(kv), head = PageFmt<T>::head(h), row_bytes = PageFmt<T>::row(kv);
-    if constexpr (__is_same(T, q4_t)) {
-        for (int i = tid; i < 2 * 16 * 8; i += 256) {  // a slot of 8 lanes moves a row
-            const int v = i >> 7, r = i >> 3 & 15, c = i & 7;
-            const int64_t src = s_src[r];
-            if (src < 0) continue;
-            char* pool = v ? a.v_pages : a.k_pages;
-            const char* from = pool + (src >> kPageShift) * page_bytes + head;
-            char* dst = pool + (size_t)to * page_bytes + head;
-            const int r1 = (int)src & (kPageRows - 1);
-            if (v) {
-                const int p0 = (r & 3) == 1 ? 2 : (r & 3) == 2 ? 1 : r & 3, p1 = (r1 & 3) == 1 ? 2 : (r1 & 3) == 2 ? 1 : r1 & 3;
-                for (int k = c; k < 32; k += 8)  // byte k of the row
-                    dst[8 * (16 * (r >> 2) + (k & 15)) + 4 * (k >> 4) + p0] =
-                        from[8 * (16 * (r1 >> 2) + (k & 15)) + 4 * (k >> 4) + p1];
-                if (c < 2)
-                    reinterpret_cast<uint16_t*>(dst)[256 + 8 * (r >> 2) + 4 * c + (r & 3)] =
-                        reinterpret_cast<const uint16_t*>(from)[256 + 8 * (r1 >> 2) + 4 * c + (r1 & 3)];
-            } else {
-                const int g = c >> 1, m = c & 1;
-                *reinterpret_cast<unsigned*>(dst + 8 * (16 * g + r) + 4 * m) =
-                    *reinterpret_cast<const unsigned*>(from + 8 * (16 * g + r1) + 4 * m);
-                if (c < 2)
-                    reinterpret_cast<uint16_t*>(dst)[256 + 16 * c + r] =
-                        reinterpret_cast<const uint16_t*>(from)[256 + 16 * c + r1];
-            }
-        }
+    const int lane = threadIdx.x & 63, kv = a.n_kv_head;
+    // kv heads next to each other: the ends of their rows share lines
+    const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sp = unit / kv, h = unit - sp * kv, s = sp / a.n_grid, jp = sp - s * a.n_grid;
+    if (s >= a.n_seq) return;
+    const int64_t sk = (int64_t)s * kv + h;
+    // Lanes 0..15 (and their copies): source page of the pool * 16 + row in it, -1: no row.
+    const int j = jp * kPageRows + (lane & 15);
+    const int row = j < a.keep ? a.kept[sk * a.keep + j] : -1;
+    const int to = a.to_table[(size_t)s * a.to_pages + jp], len = a.lengths[s];
+    int64_t src = -1;
+    float weight = 0.f;
+    bool bad = false;
+    if (row >= 0 && row < len && row < (int64_t)a.max_pages * kPageRows && (!a.weights_out || row < a.weight_stride)) {
+        const int page = a.block_table[(size_t)s * a.max_pages + (row >> kPageShift)];
+        if (a.weights_out) weight = a.weights_in[sk * a.weight_stride + row];
+        bad = page < 0 || page >= a.n_pages;
+        src = (int64_t)min(max(page, 0), a.n_pages - 1) * kPageRows + (row & (kPageRows - 1));
     } else {
-        constexpr int HB = CacheFmt<T>::kHeadBytes, CH = HB % 16 ? 4 : 16, PER = HB / CH;
-        using Word = std::conditional_t<CH == 16, u32x4, unsigned>;
-        for (int i = tid; i < 2 * kPageRows * PER; i += 256) {
-            const int v = i / (kPageRows * PER), k = i - v * kPageRows * PER, r = k / PER, c = k - r * PER;
-            const int64_t src = s_src[r];
-            if (src < 0) continue;
-            char* pool = v ? a.v_pages : a.k_pages;
-            *reinterpret_cast<Word*>(pool + (size_t)to * page_bytes + r * row_bytes + head + c * CH) =
-                *reinterpret_cast<const Word*>(pool + (src >> kPageShift) * page_bytes +
-                                               (src & (kPageRows - 1)) * row_bytes + head + c * CH);
+        bad = row != -1;
+    }
+    const unsigned rows = (unsigned)__ballot(src >= 0) & 0xffff;
+    const bool to_bad = to < 0 || to >= a.n_pages;
+    if ((__any(bad) || (rows && to_bad)) && lane == 0) atomicOr(a.err, 4);
+    const auto weights = [&]() {  // behind the rows' loads
+        if (!a.weights_out) return;
+        float* const out = a.weights_out + sk * a.weight_stride;
+        if (lane < 16 && j < a.keep) out[j] = weight;
+        // what follows the last kept row, shared out among the pages' waves
+        const int64_t part = (a.weight_stride - a.keep + a.n_grid - 1) / a.n_grid, b = a.keep + jp * part;
+        const int64_t e = min(b + part, a.weight_stride);
+        for (int64_t i = b + lane; i < e; i += 64) out[i] = 0.f;
+    };
+    if (!rows || to_bad) return weights();
+    const int64_t other = __shfl(src, __builtin_ctz(rows));
+    src = src < 0 ? other : src;
+    const size_t page_bytes = PageFmt<T>::page(kv), head = PageFmt<T>::head(h);
+    char* const pools[2] = {a.k_pages, a.v_pages};
+    if constexpr (__is_same(T, q4_t)) {
+        // Of k, lane (g, r) moves the 8 bytes of row r's dims 16 g ..  Of v, 16 lanes a quad of rows: lane i has the
+        // quad's dims i + 16 d, a byte of 8 for each row, taken from the byte of each source row that is its place there.
+        const int r = lane & 15, g = lane >> 4;
+        const int r1 = (int)src & (kPageRows - 1);
+        const char* from = a.k_pages + (src >> kPageShift) * page_bytes + head;
+        const u32x2 k = *reinterpret_cast<const u32x2*>(from + 8 * (16 * g + r1));
+        const uint16_t kd = reinterpret_cast<const uint16_t*>(from)[256 + 16 * (g & 1) + r1];
+        const auto place = [](int x) { return (x & 3) == 1 ? 2 : (x & 3) == 2 ? 1 : x & 3; };
+        u32x2 v[4];
+        uint16_t vd[4];
+        int at[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t sq = __shfl(src, 4 * g + q);
+            at[q] = (int)sq & (kPageRows - 1);
+            const char* vf = a.v_pages + (sq >> kPageShift) * page_bytes + head;
+            v[q] = *reinterpret_cast<const u32x2*>(vf + 8 * (16 * (at[q] >> 2) + r));
+            vd[q] = reinterpret_cast<const uint16_t*>(vf)[256 + 8 * (at[q] >> 2) + 4 * (r & 1) + (at[q] & 3)];
+        }
+        weights();
+        char* const kt = a.k_pages + (size_t)to * page_bytes + head;
+        char* const vt = a.v_pages + (size_t)to * page_bytes + head;
+        if (rows >> r & 1) {
+            *reinterpret_cast<u32x2*>(kt + 8 * (16 * g + r)) = k;
+            if (g < 2) reinterpret_cast<uint16_t*>(kt)[256 + 16 * g + r] = kd;
+        }
+        const unsigned quad = rows >> (4 * g) & 15;
+        u32x2* const vo = reinterpret_cast<u32x2*>(vt + 8 * (16 * g + r));
+        u32x2 w = {0, 0};
+        if (quad && quad != 15) w = *vo;  // rows without a source stay
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (!(quad >> q & 1)) continue;
+            const int to8 = 8 * place(q), at8 = 8 * place(at[q]);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) w[p] = (w[p] & ~(0xffu << to8)) | ((v[q][p] >> at8 & 0xff) << to8);
+            if (r < 2) reinterpret_cast<uint16_t*>(vt)[256 + 8 * g + 4 * r + q] = vd[q];
+        }
+        if (quad) *vo = w;
+    } else {
+        // LANES lanes a row, 16 bytes each; rows of 68 bytes have another four.
+        constexpr int HB = CacheFmt<T>::kHeadBytes, LANES = HB / 16, STEPS = kPageRows * LANES / 64;
+        constexpr bool TAIL = HB % 16 != 0;
+        static_assert(HB == 16 * LANES + 4 * TAIL && (LANES == 4 || !TAIL), "whole steps");
+        const size_t row_bytes = PageFmt<T>::row(kv);
+        const int r0 = lane / LANES, c = lane % LANES;
+        u32x4_a4 x[2][STEPS];
+        unsigned tail[2];
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+            const int64_t sr = __shfl(src, r0 + t * (64 / LANES));
+            const size_t off = (sr >> kPageShift) * page_bytes + (sr & (kPageRows - 1)) * row_bytes + head;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                x[v][t] = *reinterpret_cast<const u32x4_a4*>(pools[v] + off + 16 * c);
+                if constexpr (TAIL) tail[v] = *reinterpret_cast<const unsigned*>(pools[v] + off + 16 * LANES);
+            }
+        }
+        weights();
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+            const int r = r0 + t * (64 / LANES);
+            if (!(rows >> r & 1)) continue;
+            const size_t off = (size_t)to * page_bytes + r * row_bytes + head;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                *reinterpret_cast<u32x4_a4*>(pools[v] + off + 16 * c) = x[v][t];
+                if constexpr (TAIL)
+                    if (c == 0) *reinterpret_cast<unsigned*>(pools[v] + off + 16 * LANES) = tail[v];
+            }
         }
     }
 }

@@ -2146,7 +2146,7 @@ int tmac_kv_compact_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, v
     const int64_t n_sk = (int64_t)n_seq * n_kv_head;
     CompactArgs a{};
     a.n_grid = (int)cdiv(keep, kPageRows);
-    if (n_sk > INT_MAX / a.n_grid || (rc = check_units(ctx, what, n_sk * a.n_grid, 256)))
+    if (n_sk > (INT_MAX - 3) / a.n_grid || (rc = check_units(ctx, what, n_sk * a.n_grid, 64)))
         return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: too many units of work");
     if (weights_out) {
         const size_t bytes = extent_bytes(n_sk, weight_stride, weight_stride);
@@ -2170,8 +2170,8 @@ int tmac_kv_compact_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, v
     a.n_seq = n_seq;
     a.n_kv_head = n_kv_head;
     a.keep = keep;
-    return launch(ctx, ctx->k_compact[budget_type(kv_dtype)], (unsigned)(n_sk * a.n_grid), 1, 256, (hipStream_t)stream,
-                  &a);
+    return launch(ctx, ctx->k_compact[budget_type(kv_dtype)], (unsigned)cdiv(n_sk * a.n_grid, 4), 1, 256,
+                  (hipStream_t)stream, &a);
 }
 
 int tmac_kv_widen_pages(tmac_context* ctx, tmac_stream stream, int kv_dtype, const void* k_pages, const void* v_pages,
