@@ -293,7 +293,7 @@ struct RowsArgs {
     float* part;             // partials, by workgroup: acc [group][64] each
     float* ml;               // and (m, l) [group] each
     int* meta;               // first workgroup and number of them, of every (sequence, kv head); not if it is one each
-    float* scores;           // [n_seq][n_head][score_stride] in log2 units; null: no weights are wanted
+    float* scores;           // [n_seq][n_kv_head][score_stride / 16][group][16] in log2 units; null: no weights are wanted
     const float* weights_in;  // [n_seq][n_kv_head][weight_stride]; null: zeros
     float* weights_out;
     int* err;

@@ -516,7 +516,9 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
     O::query(raw, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, lane);
     const size_t stride = PageFmt<T>::row(a.n_kv_head), page_bytes = PageFmt<T>::page(a.n_kv_head), head = PageFmt<T>::head(h);
     const int32_t* table = a.block_table + (size_t)s * a.max_pages + (lo >> kPageShift);
-    float* scores = a.scores && col < G ? a.scores + (row0 + col) * a.score_stride + lo + 4 * (lane >> 4) : nullptr;
+    float* scores = a.scores && col < G
+                        ? a.scores + row0 * a.score_stride + (int64_t)lo * G + kPageRows * col + 4 * (lane >> 4)
+                        : nullptr;
     const int rows = hi - lo, n = (rows + kPageRows - 1) >> kPageShift;
     const int steps = ((n + KT - 1) / KT - wave + BY - 1) / BY;  // this wave's
     for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
@@ -556,7 +558,7 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
                         to[u] = max(0, min(left - u * kPageRows, kPageRows));
                     }
                     O::attend(st, t[d], from, to, lds, lane, [&](int u, f32x4 x) {
-                        if (scores) *reinterpret_cast<f32x4*>(scores + r0 + u * kPageRows) = x;
+                        if (scores) *reinterpret_cast<f32x4*>(scores + (int64_t)(r0 + u * kPageRows) * G) = x;
                     });
                 }
             }
@@ -643,34 +645,20 @@ __device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int 
 }
 
 // The weights of four rows, summed over the heads; head g's maximum and one over
-// its sum in m and r.  The scores of kWeightHeads heads are read at once.
-#ifndef WH
-#define WH 4
-#endif
-constexpr int kWeightHeads = WH;
+// its sum in m and r.
 __device__ __forceinline__ void row_weights(const RowsArgs& a, int sk, int64_t row, int len, const float* m, const float* r) {
-    const float* const x = a.scores + (int64_t)sk * a.group * a.score_stride + row;
+    const float* scores = a.scores + (int64_t)sk * a.group * a.score_stride + (row & -kPageRows) * a.group +
+                          (row & (kPageRows - 1));
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < a.group; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(scores + kPageRows * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(x[i] - m[g]) * r[g];
+    }
     const int64_t at = (int64_t)sk * a.weight_stride + row;
-    f32x4 w = {0.f, 0.f, 0.f, 0.f}, before = {0.f, 0.f, 0.f, 0.f};
-    if (a.weights_in) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) before[i] = a.weights_in[at + min(i, (int)(len - 1 - row))];
-    }
-    for (int g0 = 0; g0 < a.group; g0 += kWeightHeads) {
-        f32x4 y[kWeightHeads];
-#pragma unroll
-        for (int g = 0; g < kWeightHeads; ++g)
-            y[g] = *reinterpret_cast<const f32x4*>(x + min(g0 + g, a.group - 1) * a.score_stride);
-#pragma unroll
-        for (int g = 0; g < kWeightHeads; ++g) {
-            if (g0 + g >= a.group) break;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] += fast_exp2(y[g][i] - m[g0 + g]) * r[g0 + g];
-        }
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (row + i < len) a.weights_out[at + i] = before[i] + w[i];
+        if (row + i < len) a.weights_out[at + i] = (a.weights_in ? a.weights_in[at + i] : 0.f) + w[i];
 }
 
 template <typename T, int NW>
