@@ -505,7 +505,7 @@ __device__ __forceinline__ int rows_of(const RowsArgs& a, int s) {
 // Rows lo .. hi - 1 (lo at a step's start) of one (sequence, kv head): this wave's
 // steps of kTiles pages, every BY-th from step `wave` on.  It looks up 64 pages at
 // a time, and holds one step while the next AHEAD are in flight.
-template <typename T, int BY, int AHEAD>
+template <typename T, int BY, int AHEAD, bool SCORES>
 __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::State& st, typename Own<T>::Lds& lds, int s,
                                             int h, int lo, int hi, int wave, int lane) {
     using O = Own<T>;
@@ -516,9 +516,8 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
     O::query(raw, col < G ? a.q + (row0 + col) * kHeadDim : nullptr, lane);
     const size_t stride = PageFmt<T>::row(a.n_kv_head), page_bytes = PageFmt<T>::page(a.n_kv_head), head = PageFmt<T>::head(h);
     const int32_t* table = a.block_table + (size_t)s * a.max_pages + (lo >> kPageShift);
-    float* scores = a.scores && col < G
-                        ? a.scores + row0 * a.score_stride + (int64_t)lo * G + kPageRows * col + 4 * (lane >> 4)
-                        : nullptr;
+    float* const scores = a.scores + row0 * a.score_stride + (int64_t)lo * G;
+    const int score_at = col < G ? 4 * (kPageRows * col + 4 * (lane >> 4)) : 1 << 30;  // (behind the range: dropped)
     const int rows = hi - lo, n = (rows + kPageRows - 1) >> kPageShift;
     const int steps = ((n + KT - 1) / KT - wave + BY - 1) / BY;  // this wave's
     for (int s0 = 0; s0 < steps; s0 += 64 / KT) {
@@ -557,9 +556,18 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
                         from[u] = 0;
                         to[u] = max(0, min(left - u * kPageRows, kPageRows));
                     }
-                    O::attend(st, t[d], from, to, lds, lane, [&](int u, f32x4 x) {
-                        if (scores) *reinterpret_cast<f32x4*>(scores + (int64_t)(r0 + u * kPageRows) * G) = x;
-                    });
+                    if constexpr (SCORES) {
+                        const auto page_scores = __builtin_amdgcn_make_buffer_rsrc(
+                            scores + (int64_t)r0 * G, 0, KT * kPageRows * G * (int)sizeof(float), 0x00020000);
+                        O::attend(st, t[d], from, to, lds, lane, [&](int u, f32x4 x) {
+                            // (The page's offset not as the scalar one: with a register there, the instruction behind the
+                            // store may overwrite the data before they are read.)
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), page_scores,
+                                                                   score_at + u * kPageRows * G * (int)sizeof(float), 0, 0);
+                        });
+                    } else {
+                        O::attend(st, t[d], from, to, lds, lane, NoScores());
+                    }
                 }
             }
         }
@@ -697,7 +705,10 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
         hi = (int)min((unsigned)r.len, lo + per);
     }
     typename Own<T>::State st;
-    rows_attend<T, NW, 1>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane);
+    if (a.scores)
+        rows_attend<T, NW, 1, true>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane);
+    else
+        rows_attend<T, NW, 1, false>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane);
     merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         const size_t p = (size_t)w * G + c;
