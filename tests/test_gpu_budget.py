@@ -829,3 +829,14 @@ def test_weighted_4_bit_scales_of_all_sizes(ctx, nh, nkv):
         pools.append((st, budget.widen4(st, i == 0)))
     run_weighted(ctx, Q4, nh, nkv, lens, 1852, pools=pools, table=table, n_pages=n_pages)
     no_fault(ctx)
+
+
+@pytest.mark.parametrize("dt,nh,nkv,n,max_len", [(BF16, 14, 2, 85, 4384), (BF16, 14, 2, 85, 4385), (BF16, 16, 1, 160, 1920),
+                                                 (Q4, 16, 1, 160, 1921), (Q4, 14, 2, 86, 4096), (F32, 16, 1, 172, 1921),
+                                                 (Q8, 30, 2, 84, 2049)])
+def test_weights_on_both_sides_of_the_scores_in_lds(ctx, dt, nh, nkv, n, max_len):
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 70, n)
+    lens[[1, n // 2, n - 1]] = max_len, max_len - 33, max_len // 2
+    run_weighted(ctx, dt, nh, nkv, lens, 1860, max_len=max_len)
+    no_fault(ctx)

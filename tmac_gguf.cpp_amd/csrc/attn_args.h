@@ -293,7 +293,7 @@ struct RowsArgs {
     float* part;             // partials, by workgroup: acc [group][64] each
     float* ml;               // and (m, l) [group] each
     int* meta;               // first workgroup and number of them, of every (sequence, kv head); not if it is one each
-    float* scores;           // [n_seq][n_kv_head][score_stride / 16][group][16] in log2 units; null: no weights are wanted
+    float* scores;           // [n_seq][n_kv_head][score_stride / 16][group][16] in log2 units; null: none, or in LDS
     const float* weights_in;  // [n_seq][n_kv_head][weight_stride]; null: zeros
     float* weights_out;
     int* err;
@@ -305,9 +305,11 @@ struct RowsArgs {
     int workgroups;          // more than n_seq * n_kv_head; 0: one each
     int merge_blocks;        // finish kernel: workgroups a (sequence, kv head) that merge; the others take its weights
     int weight_blocks;       // the same, weights: 1,024 rows each
+    int near;                // the scores wait in LDS (of launches without workgroups to deal)
     float qscale;
 };
 constexpr int kRowsStep = 32;
+constexpr int kRowsNear = 120 << 10;  // bytes of LDS for scores, at most, beside up to 37 KB
 constexpr int kRowsShare = 8;   // steps that make another workgroup, at least: one a wave (one sequence of 4,096 4-bit rows,
                                 // 2 kv heads: 8.8 us, with 16 9.4; 32 of 2,000 11.5 and 10.1)
 

@@ -502,12 +502,14 @@ __device__ __forceinline__ int rows_of(const RowsArgs& a, int s) {
     return len > a.max_len ? -1 : len;
 }
 
+enum class Scores { kNone, kFar, kNear };  // where they go: memory, LDS (near)
+
 // Rows lo .. hi - 1 (lo at a step's start) of one (sequence, kv head): this wave's
 // steps of kTiles pages, every BY-th from step `wave` on.  It looks up 64 pages at
 // a time, and holds one step while the next AHEAD are in flight.
-template <typename T, int BY, int AHEAD, bool SCORES>
+template <typename T, int BY, int AHEAD, Scores SCORES>
 __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::State& st, typename Own<T>::Lds& lds, int s,
-                                            int h, int lo, int hi, int wave, int lane) {
+                                            int h, int lo, int hi, int wave, int lane, float* near) {
     using O = Own<T>;
     constexpr int KT = O::kTiles;
     const int G = a.group, col = column_of<T>(lane);
@@ -556,7 +558,12 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
                         from[u] = 0;
                         to[u] = max(0, min(left - u * kPageRows, kPageRows));
                     }
-                    if constexpr (SCORES) {
+                    if constexpr (SCORES == Scores::kNear) {
+                        float* const to_scores = near + r0 * G + kPageRows * col + 4 * (lane >> 4);
+                        O::attend(st, t[d], from, to, lds, lane, [&](int u, f32x4 x) {
+                            if (col < G) *reinterpret_cast<f32x4*>(to_scores + u * kPageRows * G) = x;
+                        });
+                    } else if constexpr (SCORES == Scores::kFar) {
                         const auto page_scores = __builtin_amdgcn_make_buffer_rsrc(
                             scores + (int64_t)r0 * G, 0, KT * kPageRows * G * (int)sizeof(float), 0x00020000);
                         O::attend(st, t[d], from, to, lds, lane, [&](int u, f32x4 x) {
@@ -654,9 +661,9 @@ __device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int 
 
 // The weights of four rows, summed over the heads; head g's maximum and one over
 // its sum in m and r.
-__device__ __forceinline__ void row_weights(const RowsArgs& a, int sk, int64_t row, int len, const float* m, const float* r) {
-    const float* scores = a.scores + (int64_t)sk * a.group * a.score_stride + (row & -kPageRows) * a.group +
-                          (row & (kPageRows - 1));
+__device__ __forceinline__ void row_weights(const RowsArgs& a, const float* scores, int sk, int64_t row, int len,
+                                            const float* m, const float* r) {
+    scores += (row & -kPageRows) * a.group + (row & (kPageRows - 1));
     f32x4 w = {0.f, 0.f, 0.f, 0.f};
     for (int g = 0; g < a.group; ++g) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(scores + kPageRows * g);
@@ -705,10 +712,14 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
         hi = (int)min((unsigned)r.len, lo + per);
     }
     typename Own<T>::State st;
-    if (a.scores)
-        rows_attend<T, NW, 1, true>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane);
+    extern __shared__ f32x4 near4[];
+    float* const near = reinterpret_cast<float*>(near4);
+    if (a.near)
+        rows_attend<T, NW, 1, Scores::kNear>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
+    else if (a.scores)
+        rows_attend<T, NW, 1, Scores::kFar>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
     else
-        rows_attend<T, NW, 1, false>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane);
+        rows_attend<T, NW, 1, Scores::kNone>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
     merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         const size_t p = (size_t)w * G + c;
@@ -722,9 +733,16 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
             s_r[c] = 1.0f / L;
         }
     });
-    if (!whole || !a.scores) return;
+    if (!whole || !a.weights_out) return;
     __syncthreads();  // all scores and sums are there
-    for (int64_t row = 4 * (int)threadIdx.x; row < r.len; row += 4 * 64 * NW) row_weights(a, sk, row, r.len, s_m, s_r);
+    if (a.near) {
+        for (int row = 4 * (int)threadIdx.x; row < r.len; row += 4 * 64 * NW)
+            row_weights(a, near, sk, row, r.len, s_m, s_r);
+    } else {
+        const float* scores = a.scores + (int64_t)sk * G * a.score_stride;
+        for (int64_t row = 4 * (int)threadIdx.x; row < r.len; row += 4 * 64 * NW)
+            row_weights(a, scores, sk, row, r.len, s_m, s_r);
+    }
 }
 
 // What follows: of every (sequence, kv head) merge_blocks workgroups merge its
@@ -815,7 +833,7 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
         }
     }
     __syncthreads();
-    if (row < len) row_weights(a, sk, row, len, s_m, s_r);
+    if (row < len) row_weights(a, a.scores + (int64_t)sk * G * a.score_stride, sk, row, len, s_m, s_r);
 }
 
 // ---------------------------------------------------------------------------

@@ -618,9 +618,9 @@ int rope_table(tmac_context* ctx, hipStream_t stream, int head_dim, float base, 
 }
 
 int launch(tmac_context* ctx, hipFunction_t f, unsigned gx, unsigned gy, unsigned block, hipStream_t stream,
-           void* args, unsigned gz = 1) {
+           void* args, unsigned gz = 1, unsigned lds = 0) {
     void* params[] = {args};
-    HIP_TRY(ctx, hipModuleLaunchKernel(f, gx, gy, gz, block, 1, 1, 0, stream, params, nullptr));
+    HIP_TRY(ctx, hipModuleLaunchKernel(f, gx, gy, gz, block, 1, 1, lds, stream, params, nullptr));
     return TMAC_OK;
 }
 
@@ -2061,8 +2061,12 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     const int64_t blocks = a.workgroups ? a.workgroups : n_sk;
     const unsigned threads = 64 * tmac::kSharedWaves;
     if ((rc = check_units(ctx, what, blocks, threads))) return rc;
+    unsigned near = 0;
     if (weights_out) {
         a.score_stride = steps * tmac::kRowsStep;
+        const int64_t bytes = 4 * group * a.score_stride;
+        if (!a.workgroups && bytes <= tmac::kRowsNear) near = (unsigned)bytes;
+        a.near = near != 0;
         a.weights_in = weights_in;
         a.weights_out = weights_out;
         a.weight_stride = weight_stride;
@@ -2075,7 +2079,7 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     if (finish && (n_sk > INT_MAX / finish || check_units(ctx, what, n_sk * finish, 256)))
         return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: too many units of work");
     if ((rc = set_device(ctx))) return rc;
-    if (a.workgroups || weights_out) {
+    if (a.workgroups || (weights_out && !near)) {
         // partials, their (m, l), the scores (16-byte aligned), what every (sequence, kv head) left
         const size_t parts = (size_t)a.workgroups * group, ml = (size_t)cdiv(2 * (int64_t)parts, 4) * 4;
         const size_t scores = weights_out ? (size_t)n_seq * n_head * (size_t)a.score_stride : 0;
@@ -2086,7 +2090,8 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
         a.meta = reinterpret_cast<int*>(a.ml + ml + scores);
     }
     const bool pair = dt == kQ4 && group <= 8;
-    if ((rc = launch(ctx, ctx->k_rows[dt + pair], (unsigned)blocks, 1, threads, (hipStream_t)stream, &a)) || !finish) return rc;
+    if ((rc = launch(ctx, ctx->k_rows[dt + pair], (unsigned)blocks, 1, threads, (hipStream_t)stream, &a, 1, near)) || !finish)
+        return rc;
     return launch(ctx, ctx->k_rows_finish, (unsigned)(n_sk * finish), 1, 256, (hipStream_t)stream, &a);
 }
 
