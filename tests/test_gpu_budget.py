@@ -840,3 +840,27 @@ def test_weights_on_both_sides_of_the_scores_in_lds(ctx, dt, nh, nkv, n, max_len
     lens[[1, n // 2, n - 1]] = max_len, max_len - 33, max_len // 2
     run_weighted(ctx, dt, nh, nkv, lens, 1860, max_len=max_len)
     no_fault(ctx)
+
+
+@by_type
+def test_compact_rows_behind_the_weights(ctx, dt):
+    """With weights, an entry at weight_stride or above has none: it is skipped and reported, and nothing behind the last
+    row of weights is read (the weights end with their allocation)."""
+    rng = np.random.default_rng(33)
+    lens = np.array([90, 90], np.int32)
+    kept = np.sort(rng.integers(0, 90, (2, 3, 40)).astype(np.int32), -1)
+    table, n_pages = tables(rng, lens, extra_pages=6)
+    to = np.setdiff1d(np.arange(n_pages), table)[:6].reshape(2, 3).astype(np.int32)
+    kp, vp = (make_pool(1870 + i, n_pages, 3, dt, i == 0)[0] for i in (0, 1))
+    w = rng.random((2, 3, 50), dtype=np.float32)
+    got = []
+    for lst in (kept, np.where(kept < 50, kept, -1).astype(np.int32)):
+        dk, dv, dw = ctx.upload(kp), ctx.upload(vp), ctx.upload(np.full_like(w, 7.5))
+        ctx.kv_compact_paged(dk, dv, n_pages, ctx.upload(table), table.shape[1], ctx.upload(lens), ctx.upload(lst), 40,
+                             ctx.upload(to), 3, ctx.upload(w), dw, 50, 2, 3, 64, kv_dtype=dt)
+        (faults if lst is kept else no_fault)(ctx)
+        got.append((dk.numpy(), dv.numpy(), dw.numpy()))
+    for a, b in zip(*got):
+        same_bits(a, b, "skipped")
+    for a, b in zip(got[1], compact_ref(kp, vp, dt, table, lens, np.where(kept < 50, kept, -1), to, w, w)):
+        same_bits(a, b, "the others")
