@@ -445,8 +445,8 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
  * significant bits, so that values are exact in fp16; below 2^-14 it is 0 and the block's values are 0,
  * above 8,128 it is infinity, and a NaN makes it NaN.  Codes are the nearest (x / scale + 8, ties to even,
  * 0 .. 15).  Codes lie in the order in which the products read them; tmac_kv_widen_pages gives the rows
- * back.  In a (page, kv head) block (row r of the page, dim d, c = d % 8; the low half of a byte holds the
- * lower of its two dims):
+ * back, as the fp32 pool that the calls without this type take.  In a (page, kv head) block (row r of the
+ * page, dim d, c = d % 8; the low half of a byte holds the lower of its two dims):
  *   K code:  byte 8 (16 (d / 16) + r) + 4 (d / 8 % 2) + c / 4 + 2 (c % 2), its high half if c / 2 is odd
  *   V code:  byte 8 (16 (r / 4) + d % 16) + 4 (d / 32) + {0, 2, 1, 3}[r % 4], its high half if d / 16 is odd
  *   K scale of dims 32 b ..: half word 256 + 16 b + r;  V: half word 256 + 8 (r / 4) + 4 b + r % 4
@@ -466,8 +466,8 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
  * weights_out (null: not wanted) [n_seq][n_kv_head][weight_stride]: for r < lengths[s], weights_in of row r
  * (null: 0) plus the softmax weights that the kv head's query heads gave row r, summed; other entries are
  * left as they were, those of sequences that are too long among them.  weights_in may be weights_out;
- * another overlap is refused.  weight_stride >= max_len.  The scores wait in the context's workspace, 4
- * bytes a row and query head of max_len.
+ * another overlap is refused.  weight_stride >= max_len.  Where sequences are cut, or the scores of one
+ * exceed a workgroup's memory, they wait in the context's workspace, 4 bytes a row and query head of max_len.
  *
  * Rows to keep: kept [n_seq][n_kv_head][keep]: the sequence's first `first` and last `last` rows and, up to
  * keep in all, those with the largest weights (ties: the lower row; a NaN as +infinity), ascending, then -1;

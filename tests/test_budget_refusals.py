@@ -214,3 +214,21 @@ def test_blocks_at_the_ends_of_the_scale():
     assert d[4, 0] == -np.inf and np.isnan(d[5, 0]) and d[6].tolist() == [0, -np.inf]
     assert (q[0] == 8).all() and (q[1] == 8).all() and q[2, 5] == 0
     assert q[3, 5] == 0
+
+
+def test_workgroups_by_length_and_number(fake):  # noqa: F811
+    """The splits that the rules give on a card of 256 CUs: whole sequences in one launch, long ones dealt, then joined."""
+    d = "tmac_attention_decode_weighted"
+    long = dict(max_len=6400, max_pages=400, weight_stride=6400, weights_out=6 * P)
+    assert call(fake, d) == (TMAC_OK, [("tmac_rows_q4_pair", 6)])
+    assert call(fake, d, n_head=18) == (TMAC_OK, [("tmac_rows_q4", 6)])
+    assert call(fake, d, weights_in=None, weights_out=None) == (TMAC_OK, [("tmac_rows_q4_pair", 6)])
+    assert call(fake, d, **long) == (TMAC_OK, [("tmac_rows_q4_pair", 156), ("tmac_rows_finish", 6 * (7 + 7))])
+    assert call(fake, d, **{**long, "weights_in": None, "weights_out": None}) == (
+        TMAC_OK, [("tmac_rows_q4_pair", 156), ("tmac_rows_finish", 6 * 7)])
+    assert call(fake, d, **long, n_seq=100) == (TMAC_OK, [("tmac_rows_q4_pair", 301), ("tmac_rows_finish", 200 * (2 + 7))])
+    assert call(fake, d, **{**long, "max_len": 4096}, n_seq=100) == (TMAC_OK, [("tmac_rows_q4_pair", 200)])
+    wide = dict(max_len=4097, weight_stride=4097)
+    assert call(fake, "tmac_select_rows", **{**wide, "max_len": 4096}) == (TMAC_OK, [("tmac_select_rows_256", 6)])
+    assert call(fake, "tmac_select_rows", **wide) == (TMAC_OK, [("tmac_select_rows_1024", 6)])
+    assert call(fake, "tmac_kv_compact_paged") == (TMAC_OK, [("tmac_compact_q4", 11)])

@@ -2031,6 +2031,8 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
         return fail(ctx, TMAC_ERR_INVALID_ARG, "decode_weighted: weight_stride below max_len");
     if (n_seq == 0) return TMAC_OK;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head;
+    const unsigned threads = 64 * tmac::kSharedWaves;
+    if ((rc = check_units(ctx, what, n_sk, threads))) return rc;
     if (weights_out) {
         const size_t bytes = extent_bytes(n_sk, weight_stride, max_len);
         if (weights_in && weights_in != weights_out && ranges_meet(weights_in, bytes, weights_out, bytes))
@@ -2059,7 +2061,6 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
         a.workgroups = (int)(3 * n_sk <= 2 * ctx->n_cu ? std::min<int64_t>(2 * ctx->n_cu, most) : n_sk + n_sk / 2 + 1);
     }
     const int64_t blocks = a.workgroups ? a.workgroups : n_sk;
-    const unsigned threads = 64 * tmac::kSharedWaves;
     if ((rc = check_units(ctx, what, blocks, threads))) return rc;
     unsigned near = 0;
     if (weights_out) {
