@@ -96,7 +96,9 @@ __device__ __forceinline__ void load_row4(float (&x)[8], const char* p, int r, i
 
 // ---------------------------------------------------------------------------
 // Pages widened to fp32.  A workgroup takes a page's head, a slot of 8 lanes a
-// row of K (first half of the slots) or V.
+// row of K (first half of the slots) or V; 4-bit blocks come through LDS.  Bound by
+// the fp32 rows it writes: 2 x 996 pages of 2 heads, 18 MB, 5.7 us of which 2 are
+// the launch; 2 x 24,750 pages, 460 MB, 94 us = 4.9 TB/s, a large copy's rate.
 template <typename T>
 __device__ __forceinline__ void widen_body(const WidenArgs& a) {
     const int c = threadIdx.x & 7, r = threadIdx.x >> 3 & 15, v = threadIdx.x >> 7;
@@ -105,7 +107,7 @@ __device__ __forceinline__ void widen_body(const WidenArgs& a) {
     const size_t at = (size_t)page * PageFmt<T>::page(a.n_kv_head) + PageFmt<T>::head(h);
     float x[8];
     if constexpr (__is_same(T, q4_t)) {
-        __shared__ u32x4 s_block[2][kQ4Block / 16];  // (bytes one by one from memory: 7.3 us instead of 5.4 for 2 x 996 pages)
+        __shared__ u32x4 s_block[2][kQ4Block / 16];  // (bytes one by one from memory: 7.3 us instead of 5.7)
         const int i = threadIdx.x & 127;
         if (a.pages[v] && i < kQ4Block / 16) s_block[v][i] = *reinterpret_cast<const u32x4*>(a.pages[v] + at + 16 * i);
         __syncthreads();
@@ -121,7 +123,11 @@ __device__ __forceinline__ void widen_body(const WidenArgs& a) {
 // ---------------------------------------------------------------------------
 // Append at given rows.  The rows' sequences are found as in append_body; a
 // pair (d, d + 1) turns by the position on its axis, so a lane reads the four
-// (cos, sin) of its pairs from up to four table rows.
+// (cos, sin) of its pairs from up to four table rows.  A 4-bit row is rounded by the
+// 8 lanes that hold it.  Bound by memory: 18,096 rows of 14 + 2 + 2 heads into 4-bit
+// pages, 136 MB, 27.3 us where they come again from the last-level cache (5.0 TB/s),
+// 38.8 from memory; a large copy takes 27.8.  (Two head rows a slot under way before
+// the places are known: 40.3.)  A single row is all latency: 4.3 us.
 template <typename T>
 __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
     const AppendArgs& a = x_args.a;
@@ -211,6 +217,10 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
 // n the fp16 pair 1024 + n (codes in the high half of a byte: 1024 + 16 n), a
 // subtraction (a fma: a sixteenth, minus 72) n - 8, and a product with the scale
 // the pair of values, all exact.
+// A step of 7 heads is 188 vector instructions and 8 products, which do not overlap:
+// some 930 cycles of a SIMD.  256 sequences of up to 4,096 rows (14 heads on 2,
+// 117 MB) take 29.4 us, 4.0 TB/s where a large copy reaches 4.9; instructions fill
+// two thirds of that time.
 struct Codes {
     using M = MMath<_Float16>;
     struct Tile {
@@ -367,7 +377,8 @@ struct Own<q4_t> {
 // c + 8 the second, of q and of the weights, so that a product takes both (8 a step
 // instead of 16, which cost the SIMD 16 cycles each beside the other instructions, not
 // under them).  A score is the sum of two columns; lane c goes on with page 0 and
-// lane c + 8 with page 1 of the step, half the exponentials each.
+// lane c + 8 with page 1 of the step, half the exponentials each.  (256 sequences as
+// above: 29.2 us instead of 33.8 by the form for 16 heads; one of 700 rows 6.1, both.)
 template <>
 struct Own<q4_pair_t> {
     using S = Mfma16;
@@ -495,8 +506,15 @@ __device__ __forceinline__ int column_of(int lane) {
 }
 
 // ---------------------------------------------------------------------------
-// Attention over whole sequences.  A sequence's length in rows, -1 where it is
-// longer than the launch covers.
+// Attention over whole sequences, and the weights that rows get: w_r = sum over the
+// heads of exp(s_r - M) / L, for which a row's scores wait until M and L are known.
+// A workgroup of 8 waves takes a (sequence, kv head) whole, in one launch, or a share
+// of it, and a second launch joins.  Read once, rows cost what memory gives: 256
+// sequences of up to 4,096 rows, 14 heads on 2: bf16 81 us (5.0 TB/s), fp32 157 (5.2);
+// Q8_0 and 4-bit rows the unpacking, 77 (2.9) and 29.4 (4.0).  One of 700 4-bit rows
+// 6.0, a launch being 3.
+
+// A sequence's length in rows, -1 where it is longer than the launch covers.
 __device__ __forceinline__ int rows_of(const RowsArgs& a, int s) {
     const int len = max(a.lengths[s], 0);
     return len > a.max_len ? -1 : len;
@@ -506,8 +524,9 @@ enum class Scores { kNone, kFar, kNear };  // where they go: memory, LDS (near)
 
 // Rows lo .. hi - 1 (lo at a step's start) of one (sequence, kv head): this wave's
 // steps of kTiles pages, every BY-th from step `wave` on.  It looks up 64 pages at
-// a time, and holds one step while the next AHEAD are in flight.
-template <typename T, int BY, int AHEAD, Scores SCORES>
+// a time, and holds one step while the next is in flight (two in flight, or 16 waves,
+// took as long).
+template <typename T, int BY, Scores SCORES>
 __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::State& st, typename Own<T>::Lds& lds, int s,
                                             int h, int lo, int hi, int wave, int lane, float* near) {
     using O = Own<T>;
@@ -533,7 +552,7 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
                 page = min(max(page, 0), a.n_pages - 1);
             }
         }
-        typename O::Tile t[AHEAD + 1][KT];
+        typename O::Tile t[2][KT];
         auto fetch = [&](typename O::Tile (&x)[KT], int step) {
 #pragma unroll
             for (int u = 0; u < KT; ++u) {
@@ -541,16 +560,15 @@ __device__ __forceinline__ void rows_attend(const RowsArgs& a, typename Own<T>::
                 O::fetch(x[u], a.k_pages + at, a.v_pages + at, stride, lane);
             }
         };
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d) fetch(t[d], min(d, cnt - 1));
+        fetch(t[0], 0);
         if (s0 == 0) O::init(st, raw, a.qscale);
-        for (int step = 0; step < cnt; step += AHEAD + 1) {
+        for (int step = 0; step < cnt; step += 2) {
 #pragma unroll
-            for (int d = 0; d <= AHEAD; ++d) {
+            for (int d = 0; d < 2; ++d) {
                 if (step + d < cnt) {
-                    // The last steps fetch the last one again: under a condition, the wait for this step's rows would be
-                    // one for all loads, the next steps' among them.
-                    fetch(t[(d + AHEAD) % (AHEAD + 1)], min(step + d + AHEAD, cnt - 1));
+                    // The last step is fetched again behind itself: under a condition, the wait for this step's rows would
+                    // be one for all loads, the next step's among them.
+                    fetch(t[1 - d], min(step + d + 1, cnt - 1));
                     const int r0 = ((s0 + step + d) * BY + wave) * KT * kPageRows, left = rows - r0;
                     int from[KT], to[KT];
 #pragma unroll
@@ -660,7 +678,10 @@ __device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int 
 }
 
 // The weights of four rows, summed over the heads; head g's maximum and one over
-// its sum in m and r.
+// its sum in m and r.  Scores lie by page, head and row: what a step writes and a
+// thread reads is close together (by head and row, power-of-two strides apart, 128
+// sequences of 8,192 bf16 rows 130 us instead of 125).  Four heads' scores read at
+// once took up to 3% longer.
 __device__ __forceinline__ void row_weights(const RowsArgs& a, const float* scores, int sk, int64_t row, int len,
                                             const float* m, const float* r) {
     scores += (row & -kPageRows) * a.group + (row & (kPageRows - 1));
@@ -715,11 +736,11 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
     extern __shared__ f32x4 near4[];
     float* const near = reinterpret_cast<float*>(near4);
     if (a.near)
-        rows_attend<T, NW, 1, Scores::kNear>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
+        rows_attend<T, NW, Scores::kNear>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
     else if (a.scores)
-        rows_attend<T, NW, 1, Scores::kFar>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
+        rows_attend<T, NW, Scores::kFar>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
     else
-        rows_attend<T, NW, 1, Scores::kNone>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
+        rows_attend<T, NW, Scores::kNone>(a, st, lds.own[wave], r.s, r.h, lo, hi, wave, lane, near);
     merge_waves<T, NW>(st, lds.merge, wave, lane, [&](int c, int d, float M, float L, f32x4 A) {
         if (c >= G) return;
         const size_t p = (size_t)w * G + c;
@@ -745,10 +766,13 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
     }
 }
 
-// What follows: of every (sequence, kv head) merge_blocks workgroups merge its
-// partials (if it had several workgroups), a head a wave or, where there are as many
-// workgroups as heads, a head all four; the others take the weights of 1,024 rows each: a head's maximum and sum from the partials, 16 lanes
-// a head, then four rows a thread, summed over the heads.
+// What follows where sequences are cut: of every (sequence, kv head) of several
+// workgroups, merge_blocks workgroups merge the partials, a head a wave or, where there
+// are as many workgroups as heads, a head all four; the others take the weights of
+// 1,024 rows each: a head's maximum and sum from the partials, 16 lanes a head, then
+// four rows a thread, summed over the heads.  A launch and the chain partials ->
+// maximum -> scores: 3.2 us without weights, 6 with those of 64 sequences of up to
+// 4,096 rows (18 MB).
 template <int WPR>
 __device__ __forceinline__ void merge_parts(const RowsArgs& a, int64_t row, int c, int p0, int n, int w, int lane) {
     constexpr int kRound = 16 * WPR;
@@ -843,7 +867,10 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
 // with the bits found so far, and the digit at which its sum from the top passes
 // what is left; a digit all of whose keys are kept ends the search.  Then every
 // wave counts, and places, the rows of its own run: those above the key, and the
-// first of those equal to it.
+// first of those equal to it.  Up to three rounds over the keys in registers, each a
+// chain of counts and barriers, bound it, not the bytes: 2 lists of 2,048 take 5.7 us
+// (3 of them the launch), 128 of 8,192 to 16,384 14.7, on half the CUs.  (The
+// first form, 1,024 threads and no early end: 8.1 and 17.9.)
 constexpr int kRowsBins = 2048;
 template <int NT, int REGS>  // threads; keys a thread holds, of longer lists it reads the rest again
 __device__ __forceinline__ void select_rows_body(const SelectRowsArgs& a) {
@@ -959,6 +986,10 @@ __device__ __forceinline__ void select_rows_body(const SelectRowsArgs& a) {
 // -> table -> row is three loads deep, so a wave has all of its page's rows in
 // flight at once, two to eight 16-byte loads a lane, and no barrier.  Loads are
 // unconditional (a place without a row reads another's row), stores are not.
+// 40 sequences of up to 8,001 rows kept to 4,001, 2 kv heads, from memory: bf16
+// 168 MB 40.6 us (4.1 TB/s), fp32 74, Q8_0 41, 4-bit 28 (rows of 68 and 36 bytes lie
+// across lines of 128).  Four lanes' worth of loads less a wave and barriers: 50, 77,
+// 69 and 55.
 template <typename T>
 __device__ __forceinline__ void compact_body(const CompactArgs& a) {
     const int lane = threadIdx.x & 63, kv = a.n_kv_head;

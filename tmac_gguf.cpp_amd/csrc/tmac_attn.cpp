@@ -1987,7 +1987,7 @@ int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtyp
 }
 
 // Steps of 32 rows up to which one workgroup takes a (sequence, kv head), n_sk of them in all: a launch and partials less
-// (2.2 us) against CUs that stay idle, the longer the more workgroups there are anyway.  Past 2/3 of two a CU, more only for
+// (2.2 us) against CUs that stay idle, the longer the more workgroups there are anyway.  Past 2/3 of a CU each, more only for
 // sequences of over twice the average: up to 128 steps even one such beside short ones costs less than what all others
 // would pay.  Captured calls of 14 heads on 2, lengths of half to all the rows, us, whole / by their share:
 //   4-bit  2: 1,024 rows 7.1 / 8.7, 2,048 9.2 / 8.8;  32: 1,024 7.8 / 9.2, 2,048 10.8 / 10.0;  90: 2,048 10.8 / 12.7, 3,000
@@ -2005,7 +2005,9 @@ static int64_t rows_whole_steps(const tmac_context* ctx, int dt, int64_t n_sk) {
     if (dt == TMAC_KV_F32) return 25 + sq / 300;
     return dt == TMAC_KV_Q8_0 ? 32 + sq / 190 : 38 + sq / 90;
 }
-constexpr int kRowsMergeWide = 16;   // partials a row from which four waves merge one
+// Partials a row beyond which four waves merge one, and not one.  14 heads on 2, 4-bit, us, four / one: 1 sequence of 4,096
+// rows 9.2 / 8.8, of 16,384 9.4 / 10.4; 4 of 16,384 11.5 / 13.2; 16 of 4,096 11.6 / 11.4; 45 of 9,001 19.7 / 19.3.
+constexpr int kRowsMergeWide = 16;
 int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                    const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                    int max_pages, const int32_t* lengths, const float* weights_in, float* weights_out,
@@ -2066,6 +2068,9 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     if (weights_out) {
         a.score_stride = steps * tmac::kRowsStep;
         const int64_t bytes = 4 * group * a.score_stride;
+        // In LDS whenever they fit, even where a CU then holds one workgroup and not two (in memory / in LDS, 14 heads on 2,
+        // us: 256 sequences of up to 4,096 rows 42.7 / 40.1 in 4 bits, 113 / 91 in bf16; 128 of 2,000 26.2 / 23.8 in bf16;
+        // 64 of 1,000 10.0 / 9.5 in 4 bits; but 256 of 2,000 in 4 bits 23.6 / 24.6).
         if (!a.workgroups && bytes <= tmac::kRowsNear) near = (unsigned)bytes;
         a.near = near != 0;
         a.weights_in = weights_in;
@@ -2096,7 +2101,10 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     return launch(ctx, ctx->k_rows_finish, (unsigned)(n_sk * finish), 1, 256, (hipStream_t)stream, &a);
 }
 
-constexpr int kSelectRowsNarrow = 4096;  // rows up to which 256 threads choose
+// Rows up to which 256 threads choose the rows to keep, of lists that they hold in registers; beyond, 1,024.  Two lists (one
+// sequence), half of them kept, captured, us, 256 / 1,024: 1,000 rows 5.3 / 7.2, 4,096 7.8 / 8.1, 8,192 14.8 / 9.4; 128
+// lists: 2,048 7.0 / 8.8, 4,096 9.0 / 9.3, 8,192 22.2 / 11.6.
+constexpr int kSelectRowsNarrow = 4096;
 int tmac_select_rows(tmac_context* ctx, tmac_stream stream, const float* weights, int64_t weight_stride,
                      const int32_t* lengths, int32_t* kept, int n_seq, int n_kv_head, int max_len, int keep, int first,
                      int last) {
