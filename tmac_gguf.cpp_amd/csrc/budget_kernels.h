@@ -124,10 +124,12 @@ __device__ __forceinline__ void widen_body(const WidenArgs& a) {
 // Append at given rows.  The rows' sequences are found as in append_body; a
 // pair (d, d + 1) turns by the position on its axis, so a lane reads the four
 // (cos, sin) of its pairs from up to four table rows.  A 4-bit row is rounded by the
-// 8 lanes that hold it.  Bound by memory: 18,096 rows of 14 + 2 + 2 heads into 4-bit
-// pages, 136 MB, 27.3 us where they come again from the last-level cache (5.0 TB/s),
-// 38.8 from memory; a large copy takes 27.8.  (Two head rows a slot under way before
-// the places are known: 40.3.)  A single row is all latency: 4.3 us.
+// 8 lanes that hold it.  Bound by memory: 18,000 rows of 14 + 2 + 2 heads into 4-bit
+// pages, 136 MB, 25 us where they come again from the last-level cache (5.4 TB/s),
+// 34.6 from memory (3.9; a large copy takes 27.8).  A wave has head rows of one kind:
+// with q, k and v mixed every wave went through the rounding, 38.8.  Loads one or two
+// head rows ahead, and (cos, sin) through LDS, took as long.  A single row is all
+// latency, 3.2 us.
 template <typename T>
 __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
     const AppendArgs& a = x_args.a;
@@ -177,9 +179,13 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
     }
     __syncthreads();
     const int c = tid & 7, slot = tid >> 3;
-    const int nh = a.q ? a.n_head : 0, kv = a.n_kv_head, per = nh + 2 * kv;
-    for (int it = slot; it < n * per; it += 32) {
-        const int r = it / per, h = it - r * per, at = s_at[r];
+    // Head rows of q, then of k, then of v, each from a wave's first slot on: a wave has one kind.
+    const int nh = a.q ? a.n_head : 0, kv = a.n_kv_head, nq = n * nh, nk = n * kv, q8 = (nq + 7) & ~7, k8 = (nk + 7) & ~7;
+    for (int it = slot; it < q8 + 2 * k8; it += 32) {
+        const bool query = it < q8, key = it < q8 + k8;
+        const int i = query ? it : key ? it - q8 : it - q8 - k8, heads = query ? nh : kv;
+        if (i >= (query ? nq : nk)) continue;
+        const int r = i / heads, h = i - r * heads, at = s_at[r];
         if (at < 0) continue;
         const int64_t t = t0 + r, page = s_page[r];
         float x[8];
@@ -192,16 +198,14 @@ __device__ __forceinline__ void append_axes_body(const AppendAxesArgs& x_args) {
                 rotate_pair(x[2 * i], x[2 * i + 1], cs.x, cs.y);
             }
         };
-        if (h < nh) {
+        if (query) {
             load8(x, a.q + t * a.q_stride + (int64_t)h * kHeadDim + 4 * c);
             turn();
             store8(a.q_out + (t * nh + h) * kHeadDim + 4 * c, x);
         } else if (page >= 0) {
-            const bool key = h < nh + kv;
-            const int hk = key ? h - nh : h - nh - kv;
-            load8(x, (key ? a.k + t * a.k_stride : a.v + t * a.v_stride) + (int64_t)hk * kHeadDim + 4 * c);
+            load8(x, (key ? a.k + t * a.k_stride : a.v + t * a.v_stride) + (int64_t)h * kHeadDim + 4 * c);
             if (key) turn();
-            char* p = (key ? a.k_pages : a.v_pages) + (size_t)page * PageFmt<T>::page(kv) + PageFmt<T>::head(hk);
+            char* p = (key ? a.k_pages : a.v_pages) + (size_t)page * PageFmt<T>::page(kv) + PageFmt<T>::head(h);
             if constexpr (__is_same(T, q4_t))
                 put_row4(x, p, at, c, key);
             else
