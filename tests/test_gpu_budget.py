@@ -833,7 +833,8 @@ def test_weighted_4_bit_scales_of_all_sizes(ctx, nh, nkv):
 
 @pytest.mark.parametrize("dt,nh,nkv,n,max_len", [(BF16, 14, 2, 85, 4384), (BF16, 14, 2, 85, 4385), (BF16, 16, 1, 160, 1920),
                                                  (Q4, 16, 1, 160, 1921), (Q4, 14, 2, 86, 4096), (F32, 16, 1, 172, 1921),
-                                                 (Q8, 30, 2, 84, 2049)])
+                                                 (Q8, 30, 2, 84, 2049), (Q4, 14, 2, 130, 1600), (Q4, 14, 2, 130, 1601),
+                                                 (Q4, 14, 2, 130, 2640)])
 def test_weights_on_both_sides_of_the_scores_in_lds(ctx, dt, nh, nkv, n, max_len):
     rng = np.random.default_rng(n)
     lens = rng.integers(0, 70, n)

@@ -681,6 +681,18 @@ __device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int 
     }
 }
 
+// Adds a head's weights of four rows: its scores x, its maximum, one over its sum.
+__device__ __forceinline__ void add_weights(f32x4& w, f32x4 x, float m, float r) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] += fast_exp2(x[i] - m) * r;
+}
+__device__ __forceinline__ void put_weights(const RowsArgs& a, int sk, int64_t row, int len, f32x4 w) {
+    const int64_t at = (int64_t)sk * a.weight_stride + row;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (row + i < len) a.weights_out[at + i] = (a.weights_in ? a.weights_in[at + i] : 0.f) + w[i];
+}
+
 // The weights of four rows, summed over the heads; head g's maximum and one over
 // its sum in m and r.  Scores lie by page, head and row: what a step writes and a
 // thread reads is close together (by head and row, power-of-two strides apart, 128
@@ -690,15 +702,8 @@ __device__ __forceinline__ void row_weights(const RowsArgs& a, const float* scor
                                             const float* m, const float* r) {
     scores += (row & -kPageRows) * a.group + (row & (kPageRows - 1));
     f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < a.group; ++g) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(scores + kPageRows * g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(x[i] - m[g]) * r[g];
-    }
-    const int64_t at = (int64_t)sk * a.weight_stride + row;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (row + i < len) a.weights_out[at + i] = (a.weights_in ? a.weights_in[at + i] : 0.f) + w[i];
+    for (int g = 0; g < a.group; ++g) add_weights(w, *reinterpret_cast<const f32x4*>(scores + kPageRows * g), m[g], r[g]);
+    put_weights(a, sk, row, len, w);
 }
 
 template <typename T, int NW>
@@ -774,9 +779,10 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
 // workgroups, merge_blocks workgroups merge the partials, a head a wave or, where there
 // are as many workgroups as heads, a head all four; the others take the weights of
 // 1,024 rows each: a head's maximum and sum from the partials, 16 lanes a head, then
-// four rows a thread, summed over the heads.  A launch and the chain partials ->
-// maximum -> scores: 3.2 us without weights, 6 with those of 64 sequences of up to
-// 4,096 rows (18 MB).
+// four rows a thread, summed over the heads, whose scores are under way before that.
+// A launch and the chain partials -> maximum: 3.2 us without weights, 6 with those of
+// 64 sequences of up to 4,096 rows (18 MB; scores read after the maxima: 0.3 more, 0.5
+// at one of 2,000).
 template <int WPR>
 __device__ __forceinline__ void merge_parts(const RowsArgs& a, int64_t row, int c, int p0, int n, int w, int lane) {
     constexpr int kRound = 16 * WPR;
@@ -824,10 +830,8 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
     const int per = a.merge_blocks + a.weight_blocks;
     const int sk = blockIdx.x / per, i0 = blockIdx.x - sk * per, s = sk / a.n_kv_head, h = sk - s * a.n_kv_head;
     const int64_t row0 = (int64_t)s * a.n_head + h * G;
-    const int len = rows_of(a, s);
-    if (len <= 0) return;
-    const int p0 = a.meta[2 * (size_t)sk], n = a.meta[2 * (size_t)sk + 1];
-    if (n == 1) return;  // its workgroup did it all
+    const int len = rows_of(a, s), p0 = a.meta[2 * (size_t)sk], n = a.meta[2 * (size_t)sk + 1];
+    if (len <= 0 || n == 1) return;  // its workgroup did it all
     if (i0 < a.merge_blocks) {
         if (a.merge_blocks == G) {
             merge_parts<kPagedWaves>(a, row0 + i0, i0, p0, n, wave, lane);
@@ -839,6 +843,13 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
     }
     const int64_t block0 = (int64_t)(i0 - a.merge_blocks) * 1024, row = block0 + 4 * tid;
     if (block0 >= len) return;
+    // The first heads' scores are on their way while the maxima are joined.
+    constexpr int kFirst = 8;
+    const int64_t at = min(row, (int64_t)(len - 1) & -4);
+    const float* const scores = a.scores + (int64_t)sk * G * a.score_stride + (at & -kPageRows) * G + (at & (kPageRows - 1));
+    f32x4 y[kFirst];
+#pragma unroll
+    for (int g = 0; g < kFirst; ++g) y[g] = *reinterpret_cast<const f32x4*>(scores + kPageRows * min(g, G - 1));
     const float2* ml = reinterpret_cast<const float2*>(a.ml) + (size_t)p0 * G;
     const int c = tid >> 4, sub = tid & 15;
     if (c < G) {
@@ -861,7 +872,16 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
         }
     }
     __syncthreads();
-    if (row < len) row_weights(a, a.scores + (int64_t)sk * G * a.score_stride, sk, row, len, s_m, s_r);
+    if (row >= len) return;
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < kFirst; ++g) {
+        if (g >= G) break;
+        add_weights(w, y[g], s_m[g], s_r[g]);
+    }
+    for (int g = kFirst; g < G; ++g)
+        add_weights(w, *reinterpret_cast<const f32x4*>(scores + kPageRows * g), s_m[g], s_r[g]);
+    put_weights(a, sk, row, len, w);
 }
 
 // ---------------------------------------------------------------------------

@@ -2008,6 +2008,7 @@ static int64_t rows_whole_steps(const tmac_context* ctx, int dt, int64_t n_sk) {
 // Partials a row beyond which four waves merge one, and not one.  14 heads on 2, 4-bit, us, four / one: 1 sequence of 4,096
 // rows 9.2 / 8.8, of 16,384 9.4 / 10.4; 4 of 16,384 11.5 / 13.2; 16 of 4,096 11.6 / 11.4; 45 of 9,001 19.7 / 19.3.
 constexpr int kRowsMergeWide = 16;
+constexpr int64_t kRowsNearTwo = 44 << 10, kRowsNearOne = 72 << 10;  // scores beside which two workgroups fit; see below
 int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q,
                                    const void* k_pages, const void* v_pages, int n_pages, const int32_t* block_table,
                                    int max_pages, const int32_t* lengths, const float* weights_in, float* weights_out,
@@ -2064,14 +2065,17 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     }
     const int64_t blocks = a.workgroups ? a.workgroups : n_sk;
     if ((rc = check_units(ctx, what, blocks, threads))) return rc;
+    const bool pair = dt == kQ4 && group <= 8;
     unsigned near = 0;
     if (weights_out) {
         a.score_stride = steps * tmac::kRowsStep;
         const int64_t bytes = 4 * group * a.score_stride;
-        // In LDS whenever they fit, even where a CU then holds one workgroup and not two (in memory / in LDS, 14 heads on 2,
-        // us: 256 sequences of up to 4,096 rows 42.7 / 40.1 in 4 bits, 113 / 91 in bf16; 128 of 2,000 26.2 / 23.8 in bf16;
-        // 64 of 1,000 10.0 / 9.5 in 4 bits; but 256 of 2,000 in 4 bits 23.6 / 24.6).
-        if (!a.workgroups && bytes <= tmac::kRowsNear) near = (unsigned)bytes;
+        // In LDS where they fit (in memory / in LDS, 14 heads on 2, us: 128 4-bit sequences of up to 2,048 rows 15.3 / 13.3,
+        // 600 of 1,600 41.5 / 34.6, 256 of 4,096 42.7 / 40.4; bf16 113 / 91, fp32 256 of 1,600 80 / 65), but not where a
+        // CU with other work to do would hold one workgroup of the 4-bit form instead of two (256 of 2,048 24.1 / 24.8, 600
+        // 48.5 / 54.2), unless they are so many that the caches do not hold them (from 2,600 rows on both take as long).
+        const bool two = pair && n_sk > ctx->n_cu && bytes > kRowsNearTwo && bytes < kRowsNearOne;
+        if (!a.workgroups && bytes <= tmac::kRowsNear && !two) near = (unsigned)bytes;
         a.near = near != 0;
         a.weights_in = weights_in;
         a.weights_out = weights_out;
@@ -2095,7 +2099,6 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
         if (weights_out) a.scores = a.ml + ml;
         a.meta = reinterpret_cast<int*>(a.ml + ml + scores);
     }
-    const bool pair = dt == kQ4 && group <= 8;
     if ((rc = launch(ctx, ctx->k_rows[dt + pair], (unsigned)blocks, 1, threads, (hipStream_t)stream, &a, 1, near)) || !finish)
         return rc;
     return launch(ctx, ctx->k_rows_finish, (unsigned)(n_sk * finish), 1, 256, (hipStream_t)stream, &a);
