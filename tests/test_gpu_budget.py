@@ -865,3 +865,48 @@ def test_compact_rows_behind_the_weights(ctx, dt):
         same_bits(a, b, "skipped")
     for a, b in zip(got[1], compact_ref(kp, vp, dt, table, lens, np.where(kept < 50, kept, -1), to, w, w)):
         same_bits(a, b, "the others")
+
+
+def test_two_graphs_share_the_workspace(ctx):
+    """Two captured calls of different shapes, both with parts and scores in the workspace, replayed in turn, weights added
+    up in place: as often as that the eager call gives."""
+    s = ctx.stream()
+    sides = []
+    for i, (dt, nh, nkv, lens) in enumerate([(Q4, 14, 2, [7000, 3]), (BF16, 16, 4, [3000, 2999, 0, 1500])]):
+        rng = np.random.default_rng(70 + i)
+        lens = np.array(lens, np.int32)
+        n, L = len(lens), int(lens.max())
+        table, n_pages = tables(rng, lens)
+        pools = [make_pool(1880 + 2 * i + j, n_pages, nkv, dt, j == 0)[0] for j in (0, 1)]
+        q, out, w = ctx.upload(oracle.normal(1890 + i, (n, nh, 64))), ctx.empty((n, nh, 64)), ctx.empty((n, nkv, L))
+        args = (q, ctx.upload(pools[0]), ctx.upload(pools[1]), n_pages, ctx.upload(table), table.shape[1], ctx.upload(lens), w, w, L,
+                out, n, nh, nkv, 64, L)
+        zeros = np.zeros((n, nkv, L), np.float32)
+        w.copy_from(zeros, s)
+        eager = []
+        for _ in range(3):
+            ctx.decode_weighted(*args, stream=s, kv_dtype=dt)
+            ctx.synchronize(s)
+            eager.append((out.numpy(), w.numpy()))
+        sides.append((args, dt, out, w, zeros, eager))
+    graphs = []
+    for args, dt, out, w, zeros, _ in sides:
+        w.copy_from(zeros, s)
+        out.copy_from(np.zeros(out.shape, np.float32), s)
+        ctx.step_begin(s)
+        ctx.decode_weighted(*args, stream=s, kv_dtype=dt)
+        graphs.append(ctx.step_end(s))
+    try:
+        for turn in range(3):
+            for g in graphs:
+                ctx.graph_launch(g, s)
+            ctx.synchronize(s)
+            for _, _, out, w, _, eager in sides:
+                same_bits(out.numpy(), eager[turn][0], f"turn {turn}")
+                same_bits(w.numpy(), eager[turn][1], f"turn {turn}")
+            run_weighted(ctx, F32, 8, 2, [4000 + turn, 77], 1895 + turn)
+    finally:
+        for g in graphs:
+            ctx.graph_destroy(g)
+        ctx.destroy_stream(s)
+    no_fault(ctx)
