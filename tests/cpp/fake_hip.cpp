@@ -3,10 +3,17 @@
 // memory, streams are always idle (or capturing, fake_set_capturing), and a launch
 // is only written down: fake_launch_name(i) and fake_launch_grid(i, d) give its
 // kernel and grid, fake_launch_prefix(i, field) how a prefix kernel's work is cut.
+// fake_syncs_in_capture() counts the synchronizations of the device that met a capture;
+// a capture begun takes fake_set_capture_us to return.
 #include <hip/hip_runtime_api.h>
 
+#include <atomic>
+#include <chrono>
 #include <cstdint>
 #include <cstdlib>
+#include <mutex>
+#include <set>
+#include <thread>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -22,6 +29,9 @@ struct Launch {
 std::vector<Launch> g_launches;
 std::vector<std::string*> g_names;  // hipFunction_t values
 bool g_capturing = false;
+std::mutex g_streams_lock;
+std::set<hipStream_t> g_streams;  // captured ones
+std::atomic<int> g_syncs_in_capture{0}, g_capture_us{0};
 char g_handle[8];
 }  // namespace
 
@@ -45,8 +55,14 @@ unsigned fake_launch_grid(int i, int d) { return g_launches[(size_t)i].grid[d]; 
 int fake_launch_prefix(int i, int field) { return g_launches[(size_t)i].prefix[field]; }
 unsigned fake_launch_block(int i) { return g_launches[(size_t)i].block; }
 void fake_set_capturing(int on) { g_capturing = on != 0; }
+void fake_set_capture_us(int us) { g_capture_us = us; }
+int fake_syncs_in_capture() { return g_syncs_in_capture; }
 
-hipError_t hipDeviceSynchronize() { return hipSuccess; }
+hipError_t hipDeviceSynchronize() {
+    std::lock_guard<std::mutex> lock(g_streams_lock);
+    if (!g_streams.empty()) ++g_syncs_in_capture;
+    return hipSuccess;
+}
 hipError_t hipEventCreate(hipEvent_t* e) { *e = (hipEvent_t)g_handle; return hipSuccess; }
 hipError_t hipEventDestroy(hipEvent_t) { return hipSuccess; }
 hipError_t hipEventElapsedTime(float* ms, hipEvent_t, hipEvent_t) { *ms = 0; return hipSuccess; }
@@ -98,10 +114,23 @@ hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned gx, unsigned gy, unsi
     return hipSuccess;
 }
 hipError_t hipSetDevice(int) { return hipSuccess; }
-hipError_t hipStreamBeginCapture(hipStream_t, hipStreamCaptureMode) { return hipSuccess; }
-hipError_t hipStreamEndCapture(hipStream_t, hipGraph_t* g) { *g = (hipGraph_t)g_handle; return hipSuccess; }
-hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* s) {
-    *s = g_capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
+hipError_t hipStreamBeginCapture(hipStream_t s, hipStreamCaptureMode) {
+    {
+        std::lock_guard<std::mutex> lock(g_streams_lock);
+        g_streams.insert(s);
+    }
+    std::this_thread::sleep_for(std::chrono::microseconds(g_capture_us));
+    return hipSuccess;
+}
+hipError_t hipStreamEndCapture(hipStream_t s, hipGraph_t* g) {
+    std::lock_guard<std::mutex> lock(g_streams_lock);
+    g_streams.erase(s);
+    *g = (hipGraph_t)g_handle;
+    return hipSuccess;
+}
+hipError_t hipStreamIsCapturing(hipStream_t stream, hipStreamCaptureStatus* s) {
+    std::lock_guard<std::mutex> lock(g_streams_lock);
+    *s = g_capturing || g_streams.count(stream) ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
     return hipSuccess;
 }
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) { *s = (hipStream_t)g_handle; return hipSuccess; }

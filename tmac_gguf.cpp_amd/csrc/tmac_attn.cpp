@@ -22,6 +22,7 @@
 #include <exception>
 #include <map>
 #include <memory>
+#include <mutex>
 #include <numeric>
 #include <string>
 #include <unordered_map>
@@ -255,10 +256,14 @@ bool capturing(hipStream_t s) {
 // buffers a growth replaces are retired instead of freed after a synchronize,
 // and the error check reads the error word without one.
 std::atomic<int> g_captures{0};
+// Held while a capture begins and is counted, and while the count is looked at and the device synchronized: a capture
+// that began between the look and the synchronize, or before it was counted, was ended by it.
+std::mutex g_capture_gate;
 
 // Synchronizes the context's device when no step capture is in progress;
 // true when the device is then idle.
 bool quiesce(tmac_context* ctx) {
+    std::lock_guard<std::mutex> gate(g_capture_gate);
     if (g_captures.load() != 0) return false;
     (void)hipSetDevice(ctx->device);
     return hipDeviceSynchronize() == hipSuccess;
@@ -2716,6 +2721,7 @@ int tmac_step_begin(tmac_context* ctx, tmac_stream stream) {
     if (rc) return rc;
     if (!stream) return fail(ctx, TMAC_ERR_INVALID_ARG, "step_begin: capture needs a created stream, not NULL");
     if ((rc = set_device(ctx))) return rc;
+    std::lock_guard<std::mutex> gate(g_capture_gate);
     HIP_TRY(ctx, hipStreamBeginCapture((hipStream_t)stream, hipStreamCaptureModeThreadLocal));
     g_captures.fetch_add(1);
     return TMAC_OK;
@@ -2854,6 +2860,7 @@ int tmac_device_synchronize(tmac_context* ctx) {
     int rc = check_ctx(ctx);
     if (rc) return rc;
     if ((rc = set_device(ctx))) return rc;
+    std::lock_guard<std::mutex> gate(g_capture_gate);
     if (g_captures.load() != 0)
         return fail(ctx, TMAC_ERR_CAPTURE,
                     "device_synchronize: a step capture is in progress (a device-wide synchronize would end it); "
