@@ -476,14 +476,17 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
  *
  * Compaction: kv head h of row kept[s][h][j] becomes row j of the pages to_table[s] (to_pages of them a
  * sequence), k and v, bit for bit; the row stays where it was too.  An entry of -1 leaves its row of the
- * destination as it was; another entry outside [0, lengths[s]) does too, and sets bit 2 (so does one at
- * weight_stride or above, with weights).  A block-table
- * entry outside the pool is clamped (bit 2), a to_table entry outside it leaves its page out (bit 2).  The
+ * destination as it was; another entry outside [0, lengths[s]) does too, and sets bit 2 (with weights, so does
+ * one whose row or place j is weight_stride or above).  A block-table entry outside the pool is clamped (bit 2), a
+ * to_table entry outside it leaves its page out (bit 2), as do entries at places past to_pages.  The
  * destination pages are pages of the same pools that hold no row of the call's sequences, each named once;
  * once the call has run, the pages of block_table that nobody else shares are free.  weights_out (both
  * null: not wanted; strides alike; no overlap) gets the weight of every kept row at j, and 0 where there is
  * none, up to weight_stride: the next rows start from nothing.  The sequence goes on with length
- * min(lengths[s], keep), where appended rows keep counting their positions from the old length. */
+ * min(lengths[s], keep), where appended rows keep counting their positions from the old length.  `keep` is the
+ * width of the lists and may be above every length: sizes go by what a list can hold, to_pages >= pages of the
+ * smaller of keep and 16 * max_pages rows, weight_stride >= the smaller of keep and 16 * max_pages - 15 (a block
+ * table as wide as its longest sequence needs). */
 int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q, int64_t q_stride,
                               float* q_out, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                               void* k_pages, void* v_pages, int n_pages, const int32_t* block_table, int max_pages,

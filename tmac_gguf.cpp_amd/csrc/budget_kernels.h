@@ -1025,11 +1025,12 @@ __device__ __forceinline__ void compact_body(const CompactArgs& a) {
     // Lanes 0..15 (and their copies): source page of the pool * 16 + row in it, -1: no row.
     const int j = jp * kPageRows + (lane & 15);
     const int row = j < a.keep ? a.kept[sk * a.keep + j] : -1;
-    const int to = a.to_table[(size_t)s * a.to_pages + jp], len = a.lengths[s];
+    // (a list may be wider than its destination: its places past to_pages have no page)
+    const int to = jp < a.to_pages ? a.to_table[(size_t)s * a.to_pages + jp] : -1, len = a.lengths[s];
     int64_t src = -1;
     float weight = 0.f;
     bool bad = false;
-    if (row >= 0 && row < len && row < (int64_t)a.max_pages * kPageRows && (!a.weights_out || row < a.weight_stride)) {
+    if (row >= 0 && row < len && row < (int64_t)a.max_pages * kPageRows && (!a.weights_out || max(row, j) < a.weight_stride)) {
         const int page = a.block_table[(size_t)s * a.max_pages + (row >> kPageShift)];
         if (a.weights_out) weight = a.weights_in[sk * a.weight_stride + row];
         bad = page < 0 || page >= a.n_pages;
@@ -1043,9 +1044,10 @@ __device__ __forceinline__ void compact_body(const CompactArgs& a) {
     const auto weights = [&]() {  // behind the rows' loads
         if (!a.weights_out) return;
         float* const out = a.weights_out + sk * a.weight_stride;
-        if (lane < 16 && j < a.keep) out[j] = weight;
+        const int64_t listed = min((int64_t)a.keep, a.weight_stride);
+        if (lane < 16 && j < listed) out[j] = weight;
         // what follows the last kept row, shared out among the pages' waves
-        const int64_t part = (a.weight_stride - a.keep + a.n_grid - 1) / a.n_grid, b = a.keep + jp * part;
+        const int64_t part = (a.weight_stride - listed + a.n_grid - 1) / a.n_grid, b = listed + jp * part;
         const int64_t e = min(b + part, a.weight_stride);
         for (int64_t i = b + lane; i < e; i += 64) out[i] = 0.f;
     };

@@ -2160,10 +2160,13 @@ int tmac_kv_compact_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, v
     if (!aligned16(k_pages) || !aligned16(v_pages) || (uintptr_t)lengths % 4 || (uintptr_t)kept % 4 ||
         (uintptr_t)to_table % 4 || (uintptr_t)weights_in % 4 || (uintptr_t)weights_out % 4)
         return fail(ctx, TMAC_ERR_MISALIGNED, "kv_compact_paged: pools must be 16-byte aligned");
-    if (keep < 1 || to_pages < cdiv(keep, kPageRows))
-        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: 1 <= keep <= 16 * to_pages");
-    if (weights_out && weight_stride < keep)
-        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: weight_stride below keep");
+    // A list has no more rows than the block table, whatever its width; the last of its pages may hold one row alone.
+    const int64_t rows = (int64_t)max_pages * kPageRows;
+    if (keep < 1 || to_pages < cdiv(std::min<int64_t>(keep, rows), kPageRows))
+        return fail(ctx, TMAC_ERR_INVALID_ARG,
+                    "kv_compact_paged: keep >= 1, and to_pages of 16 rows for keep or what max_pages hold");
+    if (weights_out && weight_stride < std::min<int64_t>(keep, rows - kPageRows + 1))
+        return fail(ctx, TMAC_ERR_INVALID_ARG, "kv_compact_paged: weight_stride below keep and the block table's rows");
     if (n_seq == 0) return TMAC_OK;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head;
     CompactArgs a{};
