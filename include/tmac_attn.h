@@ -465,8 +465,9 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
  * tmac_attention_decode_paged (max_len as there; a longer sequence gives NaN and bit 1, length 0 zeros).
  * weights_out (null: not wanted) [n_seq][n_kv_head][weight_stride]: for r < lengths[s], weights_in of row r
  * (null: 0) plus the softmax weights that the kv head's query heads gave row r, summed; other entries are
- * left as they were, those of sequences that are too long among them.  weights_in may be weights_out;
- * another overlap is refused.  weight_stride >= max_len.  Where sequences are cut, or the scores of one
+ * left as they were, those of sequences that are too long among them.  A query head none of whose rows takes
+ * part (every score -infinity: output 0) gives none, one whose output is NaN for its scores' sake gives NaN.
+ * weights_in may be weights_out; another overlap is refused.  weight_stride >= max_len.  Where sequences are cut, or the scores of one
  * exceed a workgroup's memory, they wait in the context's workspace, 4 bytes a row and query head of max_len.
  *
  * Rows to keep: kept [n_seq][n_kv_head][keep]: the sequence's first `first` and last `last` rows and, up to

@@ -681,6 +681,8 @@ __device__ __forceinline__ Stretch rows_deal(const RowsArgs& a, unsigned w, int 
     }
 }
 
+// One over a head's sum; without a row that takes part (all scores -infinity) the head gives none, as its output.
+__device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 // Adds a head's weights of four rows: its scores x, its maximum, one over its sum.
 __device__ __forceinline__ void add_weights(f32x4& w, f32x4 x, float m, float r) {
 #pragma unroll
@@ -760,7 +762,7 @@ __device__ __forceinline__ void rows_body(const RowsArgs& a) {
         if (d == 0 && !whole) *reinterpret_cast<float2*>(a.ml + 2 * p) = make_float2(M, L);
         if (d == 0 && whole) {
             s_m[c] = M;
-            s_r[c] = 1.0f / L;
+            s_r[c] = over_sum(L);
         }
     });
     if (!whole || !a.weights_out) return;
@@ -868,7 +870,7 @@ __device__ __forceinline__ void rows_finish_body(const RowsArgs& a) {
         }
         if (sub == 0) {
             s_m[c] = m;
-            s_r[c] = 1.0f / l;
+            s_r[c] = over_sum(l);
         }
     }
     __syncthreads();
