@@ -47,3 +47,40 @@ def test_host_objects_are_no_addresses(ctx, name):
         for bad in (b"\x00" * 16, "text", bytearray(16), np.zeros(4, np.float32), [P], 1.5j):
             with pytest.raises((TypeError, ValueError)):
                 getattr(ctx, name)(*good[:i], bad, *good[i + 1:])
+
+
+@pytest.mark.parametrize("make", [list, tuple, bytes, bytearray, lambda x: np.array(x, np.uint8), lambda x: np.array(x, np.int8),
+                                  lambda x: np.array(x, np.int32), lambda x: np.array(x, np.int64), iter,
+                                  lambda x: np.repeat(np.array(x, np.uint8), 2)[::2]],
+                         ids=["list", "tuple", "bytes", "bytearray", "uint8", "int8", "int32", "int64", "iterator", "strided"])
+def test_axes_of_the_pairs_in_every_form(ctx, monkeypatch, make):
+    """32 values, whatever holds them, reach the library as 32 bytes."""
+    seen, lib, axes = [], ctx.lib, [0] * 8 + [1] * 12 + [2] * 12
+
+    class Library:
+        def __getattr__(self, name):
+            fn = getattr(lib, name)
+            return lambda *a: seen.append(a[19]) or fn(*a)
+
+    ctx.lib = Library()
+    good = list(CALLS["kv_append_axes_paged"][1])
+    good[16] = make(axes)
+    assert ctx.kv_append_axes_paged(*good) == 0
+    assert seen == [bytes(axes)]
+
+
+@pytest.mark.parametrize("bad", [[0] * 31, [0] * 33, b"\x00" * 31, np.zeros(4, np.int64), np.zeros(8, np.int32),
+                                 np.zeros(128, np.uint8), [0.5] * 32, [-1] * 32, [300] * 32, np.zeros(32, np.float32)])
+def test_axes_that_are_not_32_bytes(ctx, bad):
+    good = list(CALLS["kv_append_axes_paged"][1])
+    good[16] = bad
+    with pytest.raises((TypeError, ValueError)):
+        ctx.kv_append_axes_paged(*good)
+
+
+@pytest.mark.parametrize("bad", [[3] * 32, np.full(32, -1, np.int8), np.full(32, 255, np.uint8)])
+def test_axes_beyond_n_axes(ctx, bad):
+    good = list(CALLS["kv_append_axes_paged"][1])
+    good[16] = bad
+    with pytest.raises(tmac_attn.TmacError):
+        ctx.kv_append_axes_paged(*good)
