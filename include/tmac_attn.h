@@ -351,7 +351,8 @@ int tmac_layer_attention_paged(tmac_context* ctx, tmac_stream stream, int kv_dty
  * Pools, pages, block tables and kv_dtype as above; head_dim 64, any n_kv_head, at most 16 query
  * heads per kv head (more: TMAC_ERR_UNSUPPORTED).  tmac_select_pages and tmac_attention_decode_shared
  * take at most 65,535 sequences, the latter as many kv heads, and every call as much work as a grid of
- * 2^32 threads holds (more: TMAC_ERR_INVALID_ARG).  Row, length and position arrays are DEVICE arrays,
+ * 2^32 threads holds (more: TMAC_ERR_INVALID_ARG; so are sequences of an append, max_len and keep above
+ * 2^31 - 1024 in those calls that loop over them).  Row, length and position arrays are DEVICE arrays,
  * so a captured call replays with new ones.  n_seq = 0 does nothing.  Which workgroup sums what
  * depends on the call's host arguments and, for shared prefixes, on the groups: the same call gives
  * the same bits.  Rows that no sequence reads may hold anything.  Of those that are read, a NaN key or

@@ -81,3 +81,21 @@ def test_every_drawn_case_is_accepted(fake, monkeypatch):  # noqa: F811
         assert fake.lib.fake_launches() >= 1, case
         kinds[kind] = kinds.get(kind, 0) + 1
     assert set(kinds) == {"append", "attend", "weigh", "rows", "compact"} and wide > 5, (kinds, wide)
+
+
+@pytest.mark.parametrize("name,arg,most,more", [
+    ("tmac_select_rows", "max_len", 2 ** 31 - 1024, dict(weight_stride=2 ** 31)),
+    ("tmac_select_rows", "keep", 2 ** 31 - 1024, {}),
+    ("tmac_attention_decode_weighted", "max_len", 2 ** 31 - 1024, dict(max_pages=2 ** 27, weights_in=None, weights_out=None, n_seq=1)),
+    ("tmac_kv_append_axes_paged", "n_seq", 2 ** 31 - 1024, {}),
+    ("tmac_kv_append_paged", "n_seq", 2 ** 31 - 1024, {})])
+def test_counts_that_loops_pass_by_their_steps(fake, name, arg, most, more):  # noqa: F811
+    """A kernel's loop adds up to 1,024 to a count behind its end: counts are refused where that would leave 32 bits."""
+    def go(n):
+        if name == "tmac_kv_append_paged":
+            return fake.call(name, **{**more, arg: n})
+        return call(fake, name, **{**more, arg: n})
+    rc, launches = go(most)
+    assert rc == TMAC_OK and launches
+    for n in (most + 1, 2 ** 31 - 1):
+        assert go(n) == (TMAC_ERR_INVALID_ARG, [])

@@ -1504,6 +1504,9 @@ static int check_units(tmac_context* ctx, const char* what, int64_t units, int64
     return TMAC_OK;
 }
 
+// A count that a kernel's loop passes by up to its step, the threads of a workgroup.
+static int check_count(tmac_context* ctx, const char* what, int64_t count) { return check_units(ctx, what, count + 1023); }
+
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, const float* q, int64_t q_stride,
@@ -1573,7 +1576,9 @@ int tmac_kv_append_paged(tmac_context* ctx, tmac_stream stream, int kv_dtype, co
     const int64_t blocks = cdiv(n_rows, a.rows_per_group);
     // a workgroup numbers the heads of its rows in 32 bits, and counts past the last by its 32 slots
     const int64_t heads = a.rows_per_group * (2 * (int64_t)n_kv_head + (q ? n_head : 0));
-    if ((rc = check_units(ctx, what, blocks, 256)) || (rc = check_units(ctx, what, heads + 32))) return rc;
+    if ((rc = check_units(ctx, what, blocks, 256)) || (rc = check_units(ctx, what, heads + 32)) ||
+        (rc = check_count(ctx, what, n_seq)))
+        return rc;
     return launch(ctx, ctx->k_append[kv_dtype], (unsigned)blocks, 1, 256, (hipStream_t)stream, &a);
 }
 
@@ -1987,7 +1992,9 @@ int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtyp
     a.rows_per_group = (int)std::min<int64_t>(tmac::kAppendRows, std::max<int64_t>(1, n_rows / (8 * ctx->n_cu)));
     const int64_t blocks = cdiv(n_rows, a.rows_per_group);
     const int64_t heads = a.rows_per_group * (2 * (int64_t)n_kv_head + (q ? n_head : 0));
-    if ((rc = check_units(ctx, what, blocks, 256)) || (rc = check_units(ctx, what, heads + 48))) return rc;
+    if ((rc = check_units(ctx, what, blocks, 256)) || (rc = check_units(ctx, what, heads + 48)) ||
+        (rc = check_count(ctx, what, n_seq)))
+        return rc;
     return launch(ctx, ctx->k_append_axes[budget_type(kv_dtype)], (unsigned)blocks, 1, 256, (hipStream_t)stream, &x);
 }
 
@@ -2040,7 +2047,7 @@ int tmac_attention_decode_weighted(tmac_context* ctx, tmac_stream stream, int kv
     if (n_seq == 0) return TMAC_OK;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head;
     const unsigned threads = 64 * tmac::kSharedWaves;
-    if ((rc = check_units(ctx, what, n_sk, threads))) return rc;
+    if ((rc = check_units(ctx, what, n_sk, threads)) || (rc = check_count(ctx, what, max_len))) return rc;
     if (weights_out) {
         const size_t bytes = extent_bytes(n_sk, weight_stride, max_len);
         if (weights_in && weights_in != weights_out && ranges_meet(weights_in, bytes, weights_out, bytes))
@@ -2129,7 +2136,9 @@ int tmac_select_rows(tmac_context* ctx, tmac_stream stream, const float* weights
         return fail(ctx, TMAC_ERR_INVALID_ARG, "select_rows: need keep >= 1, first, last >= 0 and first + last <= keep");
     if (n_seq == 0) return TMAC_OK;
     const int64_t n_sk = (int64_t)n_seq * n_kv_head;
-    if ((rc = check_units(ctx, what, n_sk, 1024)) || (rc = set_device(ctx))) return rc;
+    if ((rc = check_units(ctx, what, n_sk, 1024)) || (rc = check_count(ctx, what, max_len)) ||
+        (rc = check_count(ctx, what, keep)) || (rc = set_device(ctx)))
+        return rc;
     SelectRowsArgs a{};
     a.weights = weights;
     a.lengths = lengths;
