@@ -437,8 +437,8 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
 /* ---- long contexts in a small cache (extensions; no counterpart in the reference): a cache held in
  *      4 bits, the eviction of rows by the attention that they got, and rows whose place in the cache
  *      is not their position ----
- * Limits, pools and arrays as under "serving on paged caches"; kv_dtype is any tmac_kv_dtype,
- * TMAC_KV_Q4_PAGES among them.
+ * Limits, pools, arrays and what stored values that are not finite do (a 4-bit scale as a Q8_0 one) as under
+ * "serving on paged caches"; kv_dtype is any tmac_kv_dtype, TMAC_KV_Q4_PAGES among them.
  *
  * 4-bit pages: a page is [n_kv_head][576 bytes], K and V pools alike: the codes of 16 rows of 64 dims,
  * then fp16 scales, one a row and block of 32 dims; value = (code - 8) * scale, 4.5 bits a value.  The
@@ -468,13 +468,17 @@ int tmac_attention_decode_shared(tmac_context* ctx, tmac_stream stream, int kv_d
  * (null: 0) plus the softmax weights that the kv head's query heads gave row r, summed; other entries are
  * left as they were, those of sequences that are too long among them.  A query head none of whose rows takes
  * part (every score -infinity: output 0) gives none, one whose output is NaN for its scores' sake gives NaN.
- * weights_in may be weights_out; another overlap is refused.  weight_stride >= max_len.  Where sequences are cut, or the scores of one
- * exceed a workgroup's memory, they wait in the context's workspace, 4 bytes a row and query head of max_len.
+ * weights_in may be weights_out; another overlap is refused.  weight_stride >= max_len.  The context's workspace
+ * holds the sums of cut sequences (264 bytes a part and query head, up to two parts a CU or 3/2 a (sequence, kv
+ * head)) and, where they do not wait in a workgroup's memory, the scores (4 bytes a query head and row of max_len,
+ * rounded up to 32 rows, for every sequence).  Sequences may be cut, and scores lie there, whatever their lengths:
+ * the host arguments decide, so a call that is to be captured runs once before with the same ones.
  *
  * Rows to keep: kept [n_seq][n_kv_head][keep]: the sequence's first `first` and last `last` rows and, up to
- * keep in all, those with the largest weights (ties: the lower row; a NaN as +infinity), ascending, then -1;
- * all rows where there are no more than keep.  first + last <= keep.  A length above max_len gives an empty
- * list (all -1) and sets bit 1.  The weights of the first and last rows may hold anything.
+ * keep in all, those with the largest weights (ties: the lower row; a NaN counts as +infinity, and -0, which
+ * no sum of weights is, as below +0), ascending, then -1; all rows where there are no more than keep.
+ * first + last <= keep.  A length above max_len gives an empty list (all -1) and sets bit 1.  The weights of the
+ * first and last rows may hold anything.
  *
  * Compaction: kv head h of row kept[s][h][j] becomes row j of the pages to_table[s] (to_pages of them a
  * sequence), k and v, bit for bit; the row stays where it was too.  An entry of -1 leaves its row of the
