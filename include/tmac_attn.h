@@ -100,7 +100,8 @@ int tmac_init(tmac_context** ctx, int device);
  * at the same time from different host threads (one thread per context at a time).  The library's own
  * copies and fills run on a stream of the context, and it synchronizes the whole device only while no
  * step capture of any context is in progress, so a call on one context never ends another thread's
- * capture (on this runtime a legacy-stream copy or a device-wide synchronize from any thread would). */
+ * capture (on this runtime a legacy-stream copy or a device-wide synchronize from any thread would):
+ * tmac_step_begin waits for a synchronize that is under way, until that device is idle. */
 int tmac_shutdown(tmac_context* ctx);
 
 /* ---- the reference's three per-layer dispatches ---- */

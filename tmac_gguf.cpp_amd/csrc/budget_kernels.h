@@ -124,7 +124,7 @@ __device__ __forceinline__ void widen_body(const WidenArgs& a) {
 // Append at given rows.  The rows' sequences are found as in append_body; a
 // pair (d, d + 1) turns by the position on its axis, so a lane reads the four
 // (cos, sin) of its pairs from up to four table rows.  A 4-bit row is rounded by the
-// 8 lanes that hold it.  Bound by memory: 18,000 rows of 14 + 2 + 2 heads into 4-bit
+// 8 lanes that hold it.  Bound by memory: 15,829 rows of 14 + 2 + 2 heads into 4-bit
 // pages, 136 MB, 25 us where they come again from the last-level cache (5.4 TB/s),
 // 34.6 from memory (3.9; a large copy takes 27.8).  A wave has head rows of one kind:
 // with q, k and v mixed every wave went through the rounding, 38.8.  Loads one or two

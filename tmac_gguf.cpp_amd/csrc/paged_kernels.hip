@@ -6,9 +6,6 @@
 // heads per kv head at run time; a kernel is built per cache element type.
 #include <hip/hip_runtime.h>
 
-#include <climits>
-#include <type_traits>
-
 #include "attn_args.h"
 #include "attn_device.h"
 

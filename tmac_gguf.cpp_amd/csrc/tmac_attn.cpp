@@ -1999,17 +1999,23 @@ int tmac_kv_append_axes_paged(tmac_context* ctx, tmac_stream stream, int kv_dtyp
 }
 
 // Steps of 32 rows up to which one workgroup takes a (sequence, kv head), n_sk of them in all: a launch and partials less
-// (2.2 us) against CUs that stay idle, the longer the more workgroups there are anyway.  Past 2/3 of a CU each, more only for
-// sequences of over twice the average: up to 128 steps even one such beside short ones costs less than what all others
-// would pay.  Captured calls of 14 heads on 2, lengths of half to all the rows, us, whole / by their share:
-//   4-bit  2: 1,024 rows 7.1 / 8.7, 2,048 9.2 / 8.8;  32: 1,024 7.8 / 9.2, 2,048 10.8 / 10.0;  90: 2,048 10.8 / 12.7, 3,000
-//          13.8 / 12.8, 8,192 29.5 / 18.6;  128: 3,000 14.0 / 14.4, 4,096 17.4 / 16.0;  512: 4,096 30.0 / 32.3
-//   bf16   2: 1,024 8.3 / 9.4, 2,048 11.5 / 9.4;  32: 1,024 9.5 / 10.9, 1,536 11.7 / 11.1;  90: 3,000 19.1 / 20.6, 4,096 23.4
-//          / 23.6, 8,192 41.0 / 33.6;  128: 4,096 24.4 / 27.6, 8,192 41.8 / 42.2
-//   Q8_0   2: 1,024 10.2 / 10.0, 1,536 12.2 / 10.1;  90: 2,048 19.2 / 21.5, 3,000 25.8 / 23.7;  128: 3,000 26.0 / 27.6, 4,096
-//          32.9 / 31.7
-//   fp32   2: 512 8.2 / 9.9, 1,024 11.9 / 10.3;  32: 512 9.7 / 11.9, 1,024 14.7 / 13.4;  90: 1,536 21.3 / 17.8;  128: 2,048 26.0
-//          / 27.5, 3,000 34.8 / 33.8
+// (2.2 us) against CUs that stay idle, the longer the more workgroups there are anyway.  Captured calls of 14 heads on 2,
+// lengths of half to all the rows, us, whole / by their share, at n_sk:
+//   4-bit  2: 1,024 rows 6.9 / 8.9, 2,048 9.1 / 8.9;  32: 1,536 9.2 / 9.4, 2,048 10.6 / 9.4;  90: 2,048 10.7 / 11.8, 3,000
+//          13.5 / 12.9;  128: 3,000 13.8 / 14.1, 4,096 17.1 / 15.9
+//   bf16   2: 1,024 8.0 / 9.3, 1,536 9.4 / 9.1;  32: 1,024 9.3 / 9.8, 1,536 11.4 / 9.9;  90: 3,000 18.8 / 20.8, 4,096 23.2
+//          / 23.8, 8,192 40.6 / 33.5;  128: 4,096 23.9 / 27.3, 8,192 42.0 / 42.0
+//   Q8_0   2: 512 7.3 / 9.8, 1,024 10.0 / 10.0;  90: 2,048 19.2 / 19.5, 3,000 25.7 / 23.6;  128: 3,000 25.8 / 27.5, 4,096
+//          32.7 / 31.5
+//   fp32   2: 512 8.2 / 9.6, 1,024 12.0 / 10.5;  32: 512 9.7 / 10.9, 1,024 15.0 / 10.8;  90: 1,536 20.9 / 20.8, 2,048 25.7 /
+//          23.4;  128: 2,048 25.9 / 27.6, 3,000 34.7 / 33.8
+// Past 2/3 of a CU each no batch of such lengths gains by shares (4,096 rows, n_sk 180 to 512: 4-bit loses 2 to 3 us, bf16 2
+// to 4, Q8_0 2 to 5, fp32 3 to 4, and 4 to 43 where weights are wanted, whose scores no longer wait in LDS).  What gains is one
+// long sequence among short ones, which the bound alone does not show.  Among 99 of 300 rows one of 4,096: 4-bit 16.7 / 10.0,
+// bf16 22.6 / 11.2, Q8_0 31.7 / 12.4, fp32 45.0 / 14.0; of 8,192: 28.5 / 10.4, 40.1 / 11.3, 58.2 / 12.8, 85.1 / 15.2; of 32,768:
+// 100 / 12.6 (4-bit) to 325 / 23.0 (fp32).  Up to 128 steps what one side loses where the other is right is alike, beyond it is
+// a few us against a multiple.  A bound far above all lengths pays for that (256 of 300 rows, bound 32,768: 4-bit 8.8 / 11.6,
+// bf16 12.5 / 18.4, Q8_0 14.8 / 20.3, fp32 18.0 / 22.3; with weights 10.7 / 19.6, 16.9 / 29.0, 18.9 / 30.8, 20.8 / 31.0).
 static int64_t rows_whole_steps(const tmac_context* ctx, int dt, int64_t n_sk) {
     if (3 * n_sk > 2 * ctx->n_cu) return 128;
     const int64_t sq = n_sk * n_sk;
