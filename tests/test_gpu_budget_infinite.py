@@ -126,3 +126,31 @@ def test_a_row_that_is_not_finite(ctx, dt, n, nh, nkv, length, max_len, value):
             assert not np.isfinite(rows).any()
     assert np.isfinite(got[1:]).all() and np.isfinite(w[1:, :, :length]).all()
     no_fault(ctx)
+
+
+@by_type
+@PATHS
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf], ids=["nan", "inf", "minus_inf"])
+def test_a_query_that_is_not_finite(ctx, dt, n, nh, nkv, length, max_len, value):
+    """One dim of one query head: that head's output and its kv head's weights are not finite, all others are held to their
+    bounds.  (Not to the bits of the call without: a step raises the base of all of a wave's heads when one asks for it, and
+    NaN asks at every step, which rounds sums elsewhere.  Each call's results are within budget.attend64's bounds, which do
+    not depend on where the base stands.)"""
+    rng = np.random.default_rng(6)
+    lens = np.full(n, length, np.int32)
+    table, n_pages = tables(rng, lens, width=-(-max_len // PR))
+    (kp, kw), (vp, vw) = (make_pool(2230 + i, n_pages, nkv, dt, i == 0) for i in (0, 1))
+    q = oracle.normal(2233, (n, nh, 64))
+    out, rw, tol, w_tol = budget.attend64(q, kw, vw, table, lens, nkv)
+    q[n - 1, 1, 5] = value
+    got, w, w0 = run(ctx, dt, n, nh, nkv, length, max_len, q, kp, vp, table, n_pages, lens, max_len, False)
+    w = w[:, :, :length]
+    assert not np.isfinite(got[n - 1, 1]).any() and not np.isfinite(w[n - 1, 0]).any()
+    others = np.ones((n, nh), bool)
+    others[n - 1, 1] = False
+    assert (np.abs(got - out) <= tol)[others].all()
+    others = np.ones((n, nkv), bool)
+    others[n - 1, 0] = False
+    ref = w0[:, :, :length] + rw
+    assert (np.abs(w - ref) <= w_tol + 2.0 ** -24 * 1.01 * ref)[others].all()
+    no_fault(ctx)
